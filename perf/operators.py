@@ -244,7 +244,7 @@ def _encode(x, top, draw):
     e = (a.amax(1).view(torch.int32) + 0xFFFFF) >> 23
     y = (a.double() * _power(top - e)[:, None]).float().view(-1)
     code = ((y.view(torch.int32) + (draw << 4)) >> 20).clamp(max=(top + 1) * 8 - 1)
-    code = torch.where(x < 0, code + 128, code) if top == 15 else torch.where(y > 0, code.clamp(min=1), code)
+    code = torch.where(x < 0, code + 128, code) if top == 15 else torch.where(x > 0, code.clamp(min=1), code)
     return code.to(torch.uint8), e.to(torch.uint8)
 
 
