@@ -1,5 +1,6 @@
 """Loads libd1hip.so (built in-tree by build.py) and declares its C ABI (include/d1hip.h) and the
-entry points only this package calls (csrc/d1_internal.h).
+entry points only this package calls (csrc/d1_internal.h); likewise libd1ops.so (include/d1ops.h)
+and the learning task's libraries.
 
 There is no fallback: without the built library every entry point raises."""
 import ctypes as C
@@ -18,7 +19,10 @@ SYMBOLS = ('d1_state_bytes', 'd1_obs_bytes', 'd1_action_size', 'd1_out_size', 'd
 LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', 'learn_obs_size',
                  'learn_action_size', 'learn_out_size', 'learn_config_bytes', 'learn_init', 'learn_step',
                  'learn_step_active', 'learn_heuristic')
+OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
+               'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read')
 _LEARN = {}
+_OPS = None
 
 
 class D1PPOStep(C.Structure):
@@ -77,6 +81,45 @@ def load():
         L.d1_policy_fwd_sample_ar.argtypes = [p, i, p, p, p, p, p, C.c_uint64, p, C.c_uint32, p, p, p, p, p, p, p, p]
         _LIB = L
     return _LIB
+
+
+class D1AdamWTensor(C.Structure):
+    """The D1AdamWTensor struct of include/d1ops.h (one tensor of an AdamW step)."""
+    _fields_ = [('p', C.c_void_p), ('g', C.c_void_p), ('m', C.c_void_p), ('v', C.c_void_p), ('m_exp', C.c_void_p),
+                ('v_exp', C.c_void_p), ('copy', C.c_void_p), ('n', C.c_int64), ('counter', C.c_int64),
+                ('lr', C.c_double), ('weight_decay', C.c_double), ('lag', C.c_int32), ('ptype', C.c_uint8),
+                ('gtype', C.c_uint8), ('pad', C.c_uint8 * 2)]
+
+
+class D1AdamW(C.Structure):
+    """The D1AdamW struct of include/d1ops.h."""
+    _fields_ = [('beta1', C.c_double), ('beta2', C.c_double), ('eps', C.c_double), ('max_norm', C.c_double),
+                ('seed', C.c_uint64), ('bits', C.c_int32), ('pad', C.c_int32)]
+
+
+def load_ops():
+    """libd1ops.so: the operators of a policy update beside the fused step (include/d1ops.h)."""
+    global _OPS
+    if _OPS is None:
+        path = HERE / 'libd1ops.so'
+        if not path.exists():
+            raise RuntimeError(f'{path} is missing: build it with __graft_entry__.build() '
+                               '(the operators have no CPU fallback)')
+        L = C.CDLL(str(path))
+        p, i, n, f = C.c_void_p, C.c_int, C.c_int64, C.c_float
+        L.d1_tokens_work_bytes.argtypes = [n, i, i]
+        L.d1_tokens_fwd.argtypes = [p, i, n, i, n, p, p, n, i, p, p, p, p, p, p, n, p]
+        L.d1_tokens_bwd.argtypes = [p, i, n, i, n, p, p, n, p, p, p, p, p, p]
+        L.d1_norm_fwd.argtypes = [p, i, n, i, n, p, p, i, f, p, p, p, p]
+        L.d1_norm_work_bytes.argtypes = [n, i, i]
+        L.d1_norm_bwd.argtypes = [p, n, p, i, n, i, n, p, i, p, p, p, p, p, p, n, p]
+        L.d1_adamw_work_bytes.argtypes = [p, i, p]
+        L.d1_adamw_step.argtypes = [p, i, p, p, p, n, p]
+        L.d1_adamw_read.argtypes = [p, p, n, i, p, p]
+        for name in ('d1_tokens_work_bytes', 'd1_norm_work_bytes', 'd1_adamw_work_bytes'):
+            getattr(L, name).restype = C.c_int64
+        _OPS = L
+    return _OPS
 
 
 def load_learn(clump=0):

@@ -1,6 +1,7 @@
 """In-tree build of the gfx950 libraries (hipcc, no CUDA, no JIT cache).
 
 libd1hip.so          environment, wait workload, LOS compiler, MFMA trunk layer, sampling, GAE, PPO step
+libd1ops.so          token log probabilities, layer norm, the AdamW step over many tensors (include/d1ops.h)
 libd1learn_clump0.so the d1-stairs-v2 learning task (learn_* ABI), CLUMP_MODE 0
 libd1learn_clump1.so the same task with clumped placement in a third of resets
 """
@@ -14,6 +15,7 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-ffp
 TARGETS = {
     'libd1hip.so': ([CSRC / 'd1_env.hip', CSRC / 'd1_policy.hip', CSRC / 'd1_forward.hip', CSRC / 'd1_ppo.hip',
                      CSRC / 'd1_maps.hip'], []),
+    'libd1ops.so': ([CSRC / 'd1_tokens.hip', CSRC / 'd1_norm.hip', CSRC / 'd1_optim.hip'], []),
     'libd1learn_clump0.so': ([CSRC / 'd1_learn.hip'], ['-DD1_CLUMP_MODE=0']),
     'libd1learn_clump1.so': ([CSRC / 'd1_learn.hip'], ['-DD1_CLUMP_MODE=1']),
 }

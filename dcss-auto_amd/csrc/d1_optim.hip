@@ -1,0 +1,380 @@
+// d1ops: one AdamW step over many tensors, moments in 32 or 8 bits, gfx950.
+//
+//   g' = c g;  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2
+//   p = p (1 - lr wd) - (lr / (1-b1^t)) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+// A launch carries the addresses of up to MAX_TENSORS tensors in its arguments (nothing is uploaded);
+// a workgroup of 256 takes CHUNK adjacent elements of one of them, four at a time a lane, so each
+// operand is one 16-byte access. k_adamw_begin, one workgroup before the step, advances the step
+// count on the device, forms the two bias corrections in fp64 and, for a clip, adds the partial
+// sums of squares of k_adamw_norm (fp64, a fixed order: the same bits each time).
+//
+// 8-bit moments. 256 adjacent elements (a wave's four a lane) share one power of two, the exponent
+// e of their largest magnitude. An element is scaled by 2^(top-e) so that its fp32 exponent field
+// is at most `top` (15 for m, 31 for v): the field and 3 bits of mantissa are the code, and what
+// lies below the field's range is an fp32 denormal, which is the code's own linear range. Rounding
+// adds a 16-bit draw below the code's last bit and cuts. Its expectation is the value: a moment that
+// moves by less than a step an update (v moves by a thousandth, a step is an eighth) still follows
+// its mean, where rounding to the nearest would leave it where it is.
+#include "d1_rows.h"
+
+namespace d1o {
+
+constexpr int CHUNK = 4096, MAX_TENSORS = 40, NORM_GRID = 2048;
+// of ctl
+constexpr int STEP = 0, SKIPPED = 1, COEF = 2, INV_BC1 = 3, INV_BC2 = 4, NORM = 5, GO = 6;
+
+struct Tensors {
+    void *p[MAX_TENSORS];
+    const void *g[MAX_TENSORS];
+    void *m[MAX_TENSORS], *v[MAX_TENSORS];
+    uint8_t *m_exp[MAX_TENSORS], *v_exp[MAX_TENSORS];
+    void *copy[MAX_TENSORS];
+    int64_t n[MAX_TENSORS], counter[MAX_TENSORS];
+    float lr[MAX_TENSORS], keep[MAX_TENSORS];            // keep = 1 - lr wd
+    int32_t lag[MAX_TENSORS], last_chunk[MAX_TENSORS];   // last_chunk: chunks of this and all tensors before
+    uint8_t types[MAX_TENSORS];                          // bit 0: p is bf16, bit 1: g is bf16
+    int32_t count, chunks;
+};
+struct Rates {
+    float b1, omb1, b2, omb2, eps;                       // omb = 1 - b
+    double log_b1, log_b2;
+    uint64_t seed;
+};
+
+// the tensor of a chunk, and the chunk's number within it
+__device__ __forceinline__ int tensor_of(const Tensors &t, int chunk, int &within) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (chunk < t.last_chunk[mid])
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    within = chunk - (lo ? t.last_chunk[lo - 1] : 0);
+    return lo;
+}
+
+template <class T>
+__device__ __forceinline__ void add_squares(double &sum, const T *g, int64_t n, int64_t i) {
+    const Pack<T, 4> a = load_part<T, 4>(g + i, n - i < 4 ? (int)(n - i) : 4, (T)0.f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const double d = (double)(float)a.v[j];
+        sum = __builtin_fma(d, d, sum);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_adamw_norm(const Tensors t, double *__restrict__ parts) {
+    __shared__ double s[256];
+    double sum = 0.0;
+    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+        int within;
+        const int k = tensor_of(t, chunk, within);
+        const int64_t begin = (int64_t)within * CHUNK, n = t.n[k];
+#pragma unroll
+        for (int u = 0; u < CHUNK / 1024; u++) {
+            const int64_t i = begin + u * 1024 + threadIdx.x * 4;
+            if (i < n) {
+                if (t.types[k] & 2)
+                    add_squares(sum, (const __bf16 *)t.g[k], n, i);
+                else
+                    add_squares(sum, (const float *)t.g[k], n, i);
+            }
+        }
+    }
+    s[threadIdx.x] = sum;
+    __syncthreads();
+    for (int d = 128; d; d >>= 1) {
+        if ((int)threadIdx.x < d) s[threadIdx.x] += s[threadIdx.x + d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) parts[blockIdx.x] = s[0];
+}
+
+__device__ __forceinline__ void corrections(double log_b1, double log_b2, int step, float &inv1, float &inv2) {
+    inv1 = (float)(1.0 / -expm1((double)step * log_b1));
+    inv2 = (float)(1.0 / sqrt(-expm1((double)step * log_b2)));
+}
+
+__global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl, const double *__restrict__ parts, int nparts,
+                                                      double max_norm, double log_b1, double log_b2) {
+    __shared__ double s[1024];
+    double coef = 1.0;
+    bool go = true;
+    if (parts) {
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < nparts; i += 1024) sum += parts[i];
+        s[threadIdx.x] = sum;
+        __syncthreads();
+        for (int d = 512; d; d >>= 1) {
+            if ((int)threadIdx.x < d) s[threadIdx.x] += s[threadIdx.x + d];
+            __syncthreads();
+        }
+        const double norm = sqrt(s[0]);
+        go = isfinite(norm);
+        coef = max_norm / (norm + 1e-6);
+        if (!(coef < 1.0)) coef = 1.0;
+        if (threadIdx.x == 0) ctl[NORM] = __float_as_int((float)norm);
+    }
+    if (threadIdx.x) return;
+    ctl[GO] = go;
+    if (!go) {
+        ctl[SKIPPED]++;
+        return;
+    }
+    const int step = ++ctl[STEP];
+    float inv1, inv2;
+    corrections(log_b1, log_b2, step, inv1, inv2);
+    ctl[COEF] = __float_as_int((float)coef);
+    ctl[INV_BC1] = __float_as_int(inv1);
+    ctl[INV_BC2] = __float_as_int(inv2);
+}
+
+// ---- 8-bit moments
+
+// a 32-bit word through two multiplications and three shifts
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x9E3779B1u;
+    x ^= x >> 15;
+    x *= 0xB7E15163u;
+    return x ^ (x >> 16);
+}
+__device__ __forceinline__ uint32_t draw_key(uint64_t seed, uint32_t step, uint32_t counter_high) {
+    return mix(mix(mix(mix((uint32_t)seed) ^ (uint32_t)(seed >> 32)) ^ step) ^ counter_high);
+}
+// the block's exponent field: one more where rounding up could pass the largest code
+__device__ __forceinline__ int block_exp(float largest) { return (int)((__float_as_uint(largest) + 0xFFFFFu) >> 23); }
+template <int TOP>
+__device__ __forceinline__ uint32_t encode(float a, int e, uint32_t draw16) {
+    const uint32_t c = (__float_as_uint(__builtin_ldexpf(a, TOP - e)) + (draw16 << 4)) >> 20;
+    return c < (TOP + 1) * 8 ? c : (TOP + 1) * 8 - 1;
+}
+template <int TOP>
+__device__ __forceinline__ float decode(uint32_t code, int e) {
+    return __builtin_ldexpf(__uint_as_float((code & ((TOP + 1) * 8 - 1)) << 20), e - TOP);
+}
+__device__ __forceinline__ float decode_m(uint32_t code, int e) {
+    const float a = decode<15>(code, e);
+    return code & 128 ? -a : a;
+}
+
+// ---- the step
+
+template <class P, class G, int BITS>
+__device__ __forceinline__ void step_chunk(const Tensors &t, int k, int within, const Rates &r, float coef, float inv1, float inv2,
+                                           uint32_t step) {
+    const int64_t n = t.n[k];
+    const float size = t.lr[k] * inv1, keep = t.keep[k];
+    P *p = (P *)t.p[k];
+    const G *g = (const G *)t.g[k];
+    __bf16 *copy = (__bf16 *)t.copy[k];
+#pragma unroll
+    for (int u = 0; u < CHUNK / 1024; u++) {
+        const int64_t first = (int64_t)within * CHUNK + u * 1024 + (threadIdx.x & ~63u) * 4;    // of the wave's 256
+        if (first >= n) return;                                                                 // the whole wave
+        const int64_t i = first + (threadIdx.x & 63) * 4;
+        const int have = n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
+        const Pack<P, 4> pp = load_part<P, 4>(p + i, have, (P)0.f);
+        const Pack<G, 4> gg = load_part<G, 4>(g + i, have, (G)0.f);
+        Pack<float, 4> m, v;
+        int me = 0, ve = 0;
+        if (BITS == 8) {
+            const int64_t block = first / D1_ADAMW_BLOCK;
+            const Pack<uint8_t, 4> mc = load_part<uint8_t, 4>((const uint8_t *)t.m[k] + i, have, 0);
+            const Pack<uint8_t, 4> vc = load_part<uint8_t, 4>((const uint8_t *)t.v[k] + i, have, 0);
+            me = t.m_exp[k][block];
+            ve = t.v_exp[k][block];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                m.v[j] = decode_m(mc.v[j], me);
+                v.v[j] = decode<31>(vc.v[j], ve);
+            }
+        } else {
+            m = load_part<float, 4>((const float *)t.m[k] + i, have, 0.f);
+            v = load_part<float, 4>((const float *)t.v[k] + i, have, 0.f);
+        }
+        Pack<P, 4> out;
+        Pack<__bf16, 4> half;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float d = (float)gg.v[j] * coef;
+            m.v[j] = m.v[j] * r.b1 + d * r.omb1;
+            v.v[j] = v.v[j] * r.b2 + (d * d) * r.omb2;
+            const float den = sqrtf(v.v[j]) * inv2 + r.eps;
+            const float q = (float)pp.v[j] * keep - size * (m.v[j] / den);
+            out.v[j] = (P)q;
+            half.v[j] = (__bf16)q;
+        }
+        store_part<P, 4>(p + i, have, out);
+        if (copy) store_part<__bf16, 4>(copy + i, have, half);
+        if (BITS == 8) {
+            float ma = 0.f, va = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j < have) {
+                    ma = fmaxf(ma, fabsf(m.v[j]));
+                    va = fmaxf(va, v.v[j]);
+                }
+            }
+            me = block_exp(lanes_max<64>(ma));
+            ve = block_exp(lanes_max<64>(va));
+            const uint64_t c0 = (uint64_t)t.counter[k] + (uint64_t)i;
+            Pack<uint8_t, 4> mc, vc;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint64_t c = c0 + j;
+                const uint32_t word = mix((uint32_t)c ^ draw_key(r.seed, step, (uint32_t)(c >> 32)));
+                mc.v[j] = (uint8_t)(encode<15>(fabsf(m.v[j]), me, word >> 16) | (m.v[j] < 0.f ? 128u : 0u));
+                const uint32_t code = encode<31>(v.v[j], ve, word & 0xFFFF);
+                vc.v[j] = (uint8_t)(code == 0 && v.v[j] > 0.f ? 1 : code);
+            }
+            store_part<uint8_t, 4>((uint8_t *)t.m[k] + i, have, mc);
+            store_part<uint8_t, 4>((uint8_t *)t.v[k] + i, have, vc);
+            if ((threadIdx.x & 63) == 0) {
+                t.m_exp[k][first / D1_ADAMW_BLOCK] = (uint8_t)me;
+                t.v_exp[k][first / D1_ADAMW_BLOCK] = (uint8_t)ve;
+            }
+        } else {
+            store_part<float, 4>((float *)t.m[k] + i, have, m);
+            store_part<float, 4>((float *)t.v[k] + i, have, v);
+        }
+    }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void k_adamw_step(const Tensors t, const Rates r, const int32_t *__restrict__ ctl) {
+    if (!ctl[GO]) return;
+    int within;
+    const int k = tensor_of(t, blockIdx.x, within);
+    const float coef = __int_as_float(ctl[COEF]);
+    const int step = ctl[STEP];
+    float inv1 = __int_as_float(ctl[INV_BC1]), inv2 = __int_as_float(ctl[INV_BC2]);
+    if (t.lag[k]) corrections(r.log_b1, r.log_b2, step > t.lag[k] ? step - t.lag[k] : 1, inv1, inv2);
+    switch (t.types[k]) {
+    case 0: return step_chunk<float, float, BITS>(t, k, within, r, coef, inv1, inv2, (uint32_t)step);
+    case 1: return step_chunk<__bf16, float, BITS>(t, k, within, r, coef, inv1, inv2, (uint32_t)step);
+    case 2: return step_chunk<float, __bf16, BITS>(t, k, within, r, coef, inv1, inv2, (uint32_t)step);
+    default: return step_chunk<__bf16, __bf16, BITS>(t, k, within, r, coef, inv1, inv2, (uint32_t)step);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_adamw_read(const uint8_t *__restrict__ code, const uint8_t *__restrict__ exp, int64_t n,
+                                                    int is_signed, float *__restrict__ out) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+        const int have = n - i < 4 ? (int)(n - i) : 4;
+        const Pack<uint8_t, 4> c = load_part<uint8_t, 4>(code + i, have, 0);
+        const int e = exp[i / D1_ADAMW_BLOCK];
+        Pack<float, 4> o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o.v[j] = is_signed ? decode_m(c.v[j], e) : decode<31>(c.v[j], e);
+        store_part<float, 4>(out + i, have, o);
+    }
+}
+
+// the next launch's tensors, from t[at]; returns the first tensor it does not hold. Tensors of no
+// elements are left out; a launch holds fewer than 2^31 chunks.
+inline int take(const D1AdamWTensor *t, int count, int at, Tensors &l) {
+    l.count = 0;
+    int64_t chunks = 0;
+    for (; at < count && l.count < MAX_TENSORS; at++) {
+        if (t[at].n == 0) continue;
+        const int64_t more = (t[at].n + CHUNK - 1) / CHUNK;
+        if (chunks + more > (1 << 23)) {          // a grid of 2^31 threads
+            if (l.count) break;
+            return -1;
+        }
+        const int k = l.count++;
+        chunks += more;
+        l.p[k] = t[at].p;
+        l.g[k] = t[at].g;
+        l.m[k] = t[at].m;
+        l.v[k] = t[at].v;
+        l.m_exp[k] = t[at].m_exp;
+        l.v_exp[k] = t[at].v_exp;
+        l.copy[k] = t[at].copy;
+        l.n[k] = t[at].n;
+        l.counter[k] = t[at].counter;
+        l.lr[k] = (float)t[at].lr;
+        l.keep[k] = (float)(1.0 - t[at].lr * t[at].weight_decay);
+        l.lag[k] = t[at].lag;
+        l.last_chunk[k] = (int32_t)chunks;
+        l.types[k] = (uint8_t)((t[at].ptype == D1_BF16) | (t[at].gtype == D1_BF16) << 1);
+    }
+    l.chunks = (int32_t)chunks;
+    return at;
+}
+inline int norm_blocks(const Tensors &l) { return l.chunks < NORM_GRID ? l.chunks : NORM_GRID; }
+
+}  // namespace d1o
+
+using namespace d1o;
+
+static bool adamw_args(const D1AdamWTensor *t, int count, const D1AdamW *h) {
+    if (count < 0 || (count && !t) || !h || (h->bits != 32 && h->bits != 8)) return false;
+    if (!(h->beta1 >= 0 && h->beta1 < 1) || !(h->beta2 >= 0 && h->beta2 < 1) || !(h->eps >= 0) || !(h->max_norm >= 0))
+        return false;
+    for (int i = 0; i < count; i++) {
+        const D1AdamWTensor &a = t[i];
+        if (a.n < 0 || a.n > (int64_t)CHUNK << 23 || a.lag < 0 || !(a.lr >= 0) || !(a.weight_decay >= 0) || (a.ptype != D1_FP32 && a.ptype != D1_BF16) ||
+            (a.gtype != D1_FP32 && a.gtype != D1_BF16))
+            return false;
+        if (a.n && (!a.p || !a.g || !a.m || !a.v || (h->bits == 8 && (!a.m_exp || !a.v_exp)))) return false;
+    }
+    return true;
+}
+
+extern "C" int64_t d1_adamw_work_bytes(const D1AdamWTensor *t, int count, const D1AdamW *h) {
+    if (!adamw_args(t, count, h)) return D1_E_ARG;
+    if (!(h->max_norm > 0)) return 0;
+    int64_t parts = 0;
+    Tensors l;
+    for (int at = 0; at < count;) {
+        at = take(t, count, at, l);
+        parts += norm_blocks(l);
+    }
+    return parts * (int64_t)sizeof(double);
+}
+
+extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, void *work, int64_t work_bytes,
+                             void *stream) {
+    const int64_t need = d1_adamw_work_bytes(t, count, h);
+    if (need < 0 || !ctl || (need && (!work || work_bytes < need || ((uintptr_t)work & 7)))) return D1_E_ARG;
+    hipStream_t s = (hipStream_t)stream;
+    const double log_b1 = h->beta1 > 0 ? log(h->beta1) : -INFINITY, log_b2 = h->beta2 > 0 ? log(h->beta2) : -INFINITY;
+    Tensors l;
+    double *parts = h->max_norm > 0 ? (double *)work : nullptr;
+    int nparts = 0, e;
+    if (parts)
+        for (int at = 0; at < count;) {
+            at = take(t, count, at, l);
+            if (!l.count) break;
+            k_adamw_norm<<<norm_blocks(l), 256, 0, s>>>(l, parts + nparts);
+            if ((e = (int)hipGetLastError())) return e;
+            nparts += norm_blocks(l);
+        }
+    k_adamw_begin<<<1, parts ? 1024 : 64, 0, s>>>(ctl, nparts ? parts : nullptr, nparts, h->max_norm, log_b1, log_b2);
+    if ((e = (int)hipGetLastError())) return e;
+    const Rates r{(float)h->beta1, (float)(1.0 - h->beta1), (float)h->beta2, (float)(1.0 - h->beta2), (float)h->eps,
+                  log_b1, log_b2, h->seed};
+    for (int at = 0; at < count;) {
+        at = take(t, count, at, l);
+        if (!l.count) break;
+        if (h->bits == 8)
+            k_adamw_step<8><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+        else
+            k_adamw_step<32><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+        if ((e = (int)hipGetLastError())) return e;
+    }
+    return 0;
+}
+
+extern "C" int d1_adamw_read(const uint8_t *code, const uint8_t *exp, int64_t n, int is_signed, float *out, void *stream) {
+    if (n < 0 || (is_signed != 0 && is_signed != 1)) return D1_E_ARG;
+    if (n == 0) return 0;
+    if (!code || !exp || !out) return D1_E_ARG;
+    const int64_t need = (n + 1023) / 1024;
+    k_adamw_read<<<(unsigned)(need < (1 << 16) ? need : (1 << 16)), 256, 0, (hipStream_t)stream>>>(code, exp, n, is_signed, out);
+    return (int)hipGetLastError();
+}

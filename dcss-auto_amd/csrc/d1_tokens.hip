@@ -1,0 +1,537 @@
+// d1ops: log probabilities of given tokens with entropy, top alternatives and gradient, gfx950.
+//
+// Of a row's allowed entries x with maximum m:  S = sum e^(x-m),  E = sum e^(x-m) (x-m), then
+//   logp = (x[t] - m) - log S,   entropy = log S - E/S  (both terms are sums of one sign: no
+//   cancellation for a row that is sure of one entry),   p = e^(x-m) / S,
+//   dx = g (1[t] - p) - h p (log p + entropy)  with g, h the gradients of logp and entropy.
+// Each entry is read once: m, S and E run along, rescaled when m grows. The backward pass reads m
+// and S again and no sums.
+//
+// Rows of up to 1,024 entries stay in the registers of 4 to 64 lanes (k_tokens_small). A longer row
+// is cut into segments of one workgroup each, as many as fill the card when rows are few
+// (k_tokens_part), and k_tokens_join adds the segments' m, S, E and merges their best entries.
+//
+// Alternatives are ordered by a 64-bit key: the value's order-preserving bits, then the
+// complemented index, so keys are distinct and the lowest index wins among equal values.
+#include "d1_rows.h"
+
+namespace d1o {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FAR = -1e4f;          // below any difference whose exponential is not 0
+constexpr int SMALL_VOCAB = 1024;
+
+__device__ __forceinline__ float exp_nat(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+// e (x-m) for e = exp(x-m): 0 also for x = -inf, NaN where e is
+__device__ __forceinline__ float weighted(float e, float d) { return e * fmaxf(d, FAR); }
+
+// order-preserving bits: larger value, larger word; -0 as +0, NaN above +inf. No value maps to 0,
+// which stands for none, or to ~0, which is above all.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return x != x ? 0xFFFFFFFEu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);   // NaN's word gives a NaN
+}
+__device__ __forceinline__ uint64_t key_of(float x, int index) { return ((uint64_t)ordered(x) << 32) | (uint32_t)~index; }
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+template <int LANES>
+__device__ __forceinline__ uint64_t lanes_max_key(uint64_t k) {
+    const uint32_t hi = lanes_u<LANES>((uint32_t)(k >> 32), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    const uint32_t lo = lanes_u<LANES>((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    return ((uint64_t)hi << 32) | lo;
+}
+
+// running maximum, sum of exponentials and of exponentials times differences
+struct Sums {
+    float m, s, e;
+};
+__device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.f : m; }
+// a and b over the same base; a part without entries above -inf has s = e = 0
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+    const float m = fmaxf(a.m, b.m), base = finite_base(m);
+    const float da = a.m - base, db = b.m - base;
+    const float ca = exp_nat(da), cb = exp_nat(db);
+    // s and e of a part are about its own maximum: x - m = (x - a.m) + (a.m - m)
+    return {m, ca * a.s + cb * b.s, ca * __builtin_fmaf(a.s, fmaxf(da, FAR), a.e) + cb * __builtin_fmaf(b.s, fmaxf(db, FAR), b.e)};
+}
+template <int LANES>
+__device__ __forceinline__ Sums lanes_joined(Sums a) {
+    const float m = lanes_max<LANES>(a.m), d = a.m - finite_base(m), c = exp_nat(d);
+    return {m, lanes_sum<LANES>(c * a.s), lanes_sum<LANES>(c * __builtin_fmaf(a.s, fmaxf(d, FAR), a.e))};
+}
+
+struct Args {
+    const void *logits;
+    int64_t rows, stride;
+    int vocab, top;
+    const int64_t *tokens;
+    const uint8_t *mask;
+    int64_t mask_stride;
+    float *logp, *entropy, *stats;
+    int64_t *top_ids;
+    float *top_logp;
+};
+
+// what one lane writes of a row once its sums are whole
+template <class T>
+__device__ __forceinline__ void finish(const Args &a, int64_t row, Sums t) {
+    const float base = finite_base(t.m), ls = logf(t.s);
+    const int64_t tok = a.tokens[row];
+    float lp;
+    if (tok < 0)
+        lp = 0.f;
+    else if (tok >= a.vocab)
+        lp = __builtin_nanf("");
+    else if (t.s == 0.f || (a.mask && !a.mask[row * a.mask_stride + tok]))
+        lp = t.s == t.s ? -INFINITY : t.s;
+    else
+        lp = ((float)((const T *)a.logits)[row * a.stride + tok] - base) - ls;
+    a.logp[row] = lp;
+    a.entropy[row] = t.s == 0.f ? 0.f : ls - t.e / t.s;
+    a.stats[2 * row] = base;
+    a.stats[2 * row + 1] = t.s;
+}
+__device__ __forceinline__ void put_top(const Args &a, int64_t row, int k, uint64_t key, float base, float ls, float s) {
+    const bool none = (key >> 32) == 0;
+    a.top_ids[row * a.top + k] = none ? -1 : index_of(key);
+    a.top_logp[row * a.top + k] = none || s == 0.f ? -INFINITY : (value_of((uint32_t)(key >> 32)) - base) - ls;
+}
+
+// ---- rows of up to LANES * CH * 4 entries, one row for LANES lanes, 4 adjacent entries a chunk
+
+template <class T, int LANES, int CH, bool MASK>
+struct SmallRow {
+    float x[CH][4];
+    bool in[CH][4];       // an entry of the row that is allowed
+    __device__ __forceinline__ void read(const T *logits, const uint8_t *mask, int vocab, int lane) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int col = (c * LANES + lane) * 4, n = vocab - col;
+            const Pack<T, 4> p = load_part<T, 4>(logits + col, n, (T)0.f);
+            Pack<uint8_t, 4> q;
+            if (MASK) q = load_part<uint8_t, 4>(mask + col, n, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                in[c][i] = MASK ? q.v[i] != 0 : i < n;
+                x[c][i] = in[c][i] ? (float)p.v[i] : -INFINITY;
+            }
+        }
+    }
+};
+
+template <class T, int LANES, int CH, bool MASK>
+__global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
+    constexpr int GROUPS = 256 / LANES;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows; row += (int64_t)gridDim.x * GROUPS) {
+        SmallRow<T, LANES, CH, MASK> r;
+        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane);
+        float m = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) m = fmaxf(m, r.x[c][i]);
+        m = lanes_max<LANES>(m);
+        const float base = finite_base(m);
+        float s = 0.f, e = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float d = r.x[c][i] - base, w = exp_nat(d);
+                s += w;
+                e += weighted(w, d);
+            }
+        s = lanes_sum<LANES>(s);
+        e = lanes_sum<LANES>(e);
+        if (lane == 0) finish<T>(a, row, {m, s, e});
+        if (a.top) {
+            const float ls = logf(s);
+            uint64_t last = ~0ull;
+            for (int k = 0; k < a.top; k++) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint64_t key = r.in[c][i] ? key_of(r.x[c][i], (c * LANES + lane) * 4 + i) : 0;
+                        if (key < last && key > best) best = key;
+                    }
+                last = lanes_max_key<LANES>(best);
+                if (lane == 0) put_top(a, row, k, last, base, ls, s);
+            }
+        }
+    }
+}
+
+// ---- longer rows: segments
+
+// Threads of a workgroup and the vectors of 16 bytes that a thread takes at once.
+constexpr int PART = 256, AT_ONCE = 4, WAVES = PART / 64, KEEP = 256;
+
+struct Parts {
+    float *sums;              // [rows][splits][4]: m, s, e
+    uint64_t *keys;           // [rows][splits][top]
+    int splits, seg;          // segments a row, entries of one (a multiple of PART * VEC)
+};
+
+// VEC allowed entries of a segment at offset i (n entries in all); what is outside reads -inf
+template <class T, int VEC, bool MASK>
+__device__ __forceinline__ void read_vec(const T *x, const uint8_t *mask, int i, int n, float (&v)[VEC]) {
+    const Pack<T, VEC> p = load_part<T, VEC>(x + i, n - i, (T)-INFINITY);
+    if (MASK) {
+        const Pack<uint8_t, VEC> q = load_part<uint8_t, VEC>(mask + i, n - i, 0);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = q.v[j] ? (float)p.v[j] : -INFINITY;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = (float)p.v[j];
+    }
+}
+
+// what the lanes of a wave wrote to LDS is there for the others after this
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// the `top` largest of up to KEEP keys in `list` (LDS, one wave's), in falling order to out[0..top)
+__device__ __forceinline__ void extract(const uint64_t *list, int count, int top, int lane, uint64_t *out) {
+    uint64_t mine[KEEP / 64];
+#pragma unroll
+    for (int i = 0; i < KEEP / 64; i++) mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
+    uint64_t last = ~0ull;
+    for (int k = 0; k < top; k++) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < KEEP / 64; i++)
+            if (mine[i] < last && mine[i] > best) best = mine[i];
+        last = lanes_max_key<64>(best);
+        if (lane == 0) out[k] = last;
+    }
+}
+
+template <class T, bool MASK, bool TOP>
+__global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts parts) {
+    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
+    __shared__ Sums wave_sums[WAVES];
+    __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? KEEP : 1], best_of[TOP ? WAVES : 1][TOP ? D1_TOKENS_MAX_TOP : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t units = a.rows * parts.splits;
+    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int64_t row = unit / parts.splits;
+        const int split = (int)(unit - row * parts.splits), begin = split * parts.seg;
+        const int n = a.vocab - begin < parts.seg ? a.vocab - begin : parts.seg;     // may be <= 0: nothing to read
+        const T *x = (const T *)a.logits + row * a.stride + begin;
+        const uint8_t *mask = MASK ? a.mask + row * a.mask_stride + begin : nullptr;
+        Sums t = {-INFINITY, 0.f, 0.f};
+        for (int i = threadIdx.x * VEC; i < n; i += STEP * AT_ONCE) {
+            float v[AT_ONCE][VEC];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) read_vec<T, VEC, MASK>(x, mask, i + u * STEP, n, v[u]);
+            float m = t.m;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) m = fmaxf(m, v[u][j]);
+            const float base = finite_base(m), d0 = t.m - base, c = exp_nat(d0);
+            t.e = c * __builtin_fmaf(t.s, fmaxf(d0, FAR), t.e);
+            t.s = c * t.s;
+            t.m = m;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const float d = v[u][j] - base, w = exp_nat(d);
+                    t.s += w;
+                    t.e += weighted(w, d);
+                }
+        }
+        const Sums wave_sum = lanes_joined<64>(t);
+        if (lane == 0) wave_sums[wave] = wave_sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            Sums all = wave_sums[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) all = joined(all, wave_sums[w]);
+            float *o = parts.sums + unit * 4;
+            o[0] = all.m;
+            o[1] = all.s;
+            o[2] = all.e;
+        }
+        if (TOP) {
+            // every entry of the segment against the wave's list: the simplest way that is right
+            uint64_t floor_key = 0;      // keys up to this one are not among the wave's best
+            int count = 0;
+            for (int i0 = 0; i0 < n; i0 += STEP) {
+                const int i = i0 + threadIdx.x * VEC;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const int at = i + j;
+                    uint64_t key = 0;
+                    if (at < n && (!MASK || mask[at])) key = key_of((float)x[at], begin + at);
+                    const uint64_t take = __ballot(key > floor_key);
+                    if (!take) continue;
+                    if (key > floor_key) found[wave][count + __popcll(take & ((1ull << lane) - 1))] = key;
+                    count += __popcll(take);
+                    if (count > KEEP - 64) {      // no room for another 64: keep the best
+                        wave_sync();
+                        extract(found[wave], count, a.top, lane, best_of[wave]);
+                        wave_sync();
+                        if (lane < a.top) found[wave][lane] = best_of[wave][lane];
+                        wave_sync();
+                        count = a.top;
+                        floor_key = best_of[wave][a.top - 1];
+                    }
+                }
+            }
+            wave_sync();
+            extract(found[wave], count, a.top, lane, best_of[wave]);
+            __syncthreads();
+            if (wave == 0) {       // the waves' lists, at most KEEP keys
+                for (int i = lane; i < WAVES * a.top; i += 64) found[0][i] = best_of[i / a.top][i % a.top];
+                wave_sync();
+                extract(found[0], WAVES * a.top, a.top, lane, best_of[0]);
+                wave_sync();
+                if (lane < a.top) parts.keys[unit * a.top + lane] = best_of[0][lane];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// one wave a row: lane l holds segment l (at most 64 segments) and the head of its sorted list
+template <class T>
+__global__ __launch_bounds__(64) void k_tokens_join(const Args a, const Parts parts) {
+    const int lane = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Sums t = {-INFINITY, 0.f, 0.f};
+        if (lane < parts.splits) {
+            const float *p = parts.sums + (row * parts.splits + lane) * 4;
+            t = {p[0], p[1], p[2]};
+        }
+        t = lanes_joined<64>(t);
+        if (lane == 0) finish<T>(a, row, t);
+        if (a.top) {
+            const float base = finite_base(t.m), ls = logf(t.s);
+            const uint64_t *mine = parts.keys + (row * parts.splits + lane) * a.top;
+            int at = 0;
+            uint64_t head = lane < parts.splits ? mine[0] : 0;
+            for (int k = 0; k < a.top; k++) {
+                const uint64_t key = lanes_max_key<64>(head);
+                if (lane == 0) put_top(a, row, k, key, base, ls, t.s);
+                if (key && head == key) head = ++at < a.top ? mine[at] : 0;
+            }
+        }
+    }
+}
+
+// ---- gradient
+
+struct BackArgs {
+    const void *logits;
+    int64_t rows, stride;
+    int vocab;
+    const int64_t *tokens;
+    const uint8_t *mask;
+    int64_t mask_stride;
+    const float *stats, *entropy, *dlogp, *dentropy;
+    void *dlogits;
+};
+// dx = e^d (add + scale d) for d = x - base, and `g` more at the token. e^d is taken as the square
+// of e^(d/2): the hardware's exponential has no denormal results, and p may be small where dx is not.
+struct RowGrad {
+    float base, add, scale, g;
+    int64_t tok;
+};
+__device__ __forceinline__ RowGrad row_grad(const BackArgs &a, int64_t row) {
+    const float s = a.stats[2 * row + 1], inv = s == 0.f ? 0.f : 1.f / s;
+    RowGrad r;
+    r.base = a.stats[2 * row];
+    r.tok = a.tokens[row];
+    const float h = a.dentropy ? a.dentropy[row] : 0.f;
+    r.g = a.dlogp && r.tok >= 0 ? a.dlogp[row] : 0.f;
+    if (a.dlogp && r.tok >= a.vocab) r.g = __builtin_nanf("");
+    const float shift = a.dentropy && s != 0.f ? a.entropy[row] - logf(s) : 0.f;
+    r.add = -inv * __builtin_fmaf(h, shift, r.g);
+    r.scale = -inv * h;
+    if (s == 0.f) r.add = r.scale = r.g = 0.f;
+    return r;
+}
+__device__ __forceinline__ float grad_of(const RowGrad &r, float x) {
+    const float d = x - r.base;
+    const float half = __builtin_amdgcn_exp2f(d * (0.5f * LOG2E));
+    return half * (half * __builtin_fmaf(r.scale, fmaxf(d, FAR), r.add));
+}
+
+template <class T, int LANES, int CH, bool MASK>
+__global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
+    constexpr int GROUPS = 256 / LANES;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows; row += (int64_t)gridDim.x * GROUPS) {
+        SmallRow<T, LANES, CH, MASK> r;
+        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane);
+        const RowGrad q = row_grad(a, row);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int col = (c * LANES + lane) * 4;
+            Pack<T, 4> o;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float d = grad_of(q, r.x[c][i]) + (col + i == q.tok ? q.g : 0.f);
+                o.v[i] = (T)(r.in[c][i] ? d : 0.f);
+            }
+            store_part<T, 4>((T *)a.dlogits + row * a.vocab + col, a.vocab - col, o);
+        }
+    }
+}
+
+template <class T, bool MASK>
+__global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
+    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
+    const int64_t units = a.rows * splits;
+    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int64_t row = unit / splits;
+        const int begin = (int)(unit - row * splits) * seg;
+        const int n = a.vocab - begin < seg ? a.vocab - begin : seg;
+        const T *x = (const T *)a.logits + row * a.stride + begin;
+        const uint8_t *mask = MASK ? a.mask + row * a.mask_stride + begin : nullptr;
+        T *out = (T *)a.dlogits + row * a.vocab + begin;
+        const RowGrad q = row_grad(a, row);
+        for (int i0 = threadIdx.x * VEC; i0 < n; i0 += STEP * AT_ONCE) {
+            Pack<T, VEC> p[AT_ONCE];
+            Pack<uint8_t, VEC> w[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int i = i0 + u * STEP;
+                p[u] = load_part<T, VEC>(x + i, n - i, (T)0.f);
+                if (MASK) w[u] = load_part<uint8_t, VEC>(mask + i, n - i, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int i = i0 + u * STEP;
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const float d = grad_of(q, (float)p[u].v[j]) + (begin + i + j == q.tok ? q.g : 0.f);
+                    o.v[j] = (T)(!MASK || w[u].v[j] ? d : 0.f);
+                }
+                store_part<T, VEC>(out + i, n - i, o);
+            }
+        }
+    }
+}
+
+// Segments of a long row: enough workgroups for the card (4 for each of 256 CUs) where rows are few,
+// none shorter than one vector a thread, at most 64 (the join's lanes).
+inline int splits_of(int64_t rows, int vocab, int type, int &seg) {
+    const int step = PART * (type == D1_FP32 ? 4 : 8);
+    const int most = (vocab + step - 1) / step;
+    int64_t want = (1024 + rows - 1) / rows;
+    if (want > 64) want = 64;
+    int splits = (int)(want < most ? want : most);
+    seg = ((vocab + splits - 1) / splits + step - 1) / step * step;
+    return (vocab + seg - 1) / seg;
+}
+inline unsigned blocks_of(int64_t units) { return (unsigned)(units < (1 << 20) ? units : (1 << 20)); }
+
+#define D1O_SMALL_SHAPES(X) X(4, 1) X(8, 1) X(16, 1) X(64, 1) X(64, 4)
+
+template <class T, bool MASK>
+int small_fwd(const Args &a, hipStream_t s) {
+#define X(L, C)                                                                                                   \
+    if (a.vocab <= L * C * 4) {                                                                                   \
+        k_tokens_small<T, L, C, MASK><<<blocks_of((a.rows + 256 / L - 1) / (256 / L)), 256, 0, s>>>(a);           \
+        return (int)hipGetLastError();                                                                            \
+    }
+    D1O_SMALL_SHAPES(X)
+#undef X
+    return D1_E_ARG;
+}
+template <class T, bool MASK>
+int small_bwd(const BackArgs &a, hipStream_t s) {
+#define X(L, C)                                                                                                   \
+    if (a.vocab <= L * C * 4) {                                                                                   \
+        k_tokens_small_bwd<T, L, C, MASK><<<blocks_of((a.rows + 256 / L - 1) / (256 / L)), 256, 0, s>>>(a);       \
+        return (int)hipGetLastError();                                                                            \
+    }
+    D1O_SMALL_SHAPES(X)
+#undef X
+    return D1_E_ARG;
+}
+
+template <class T, bool MASK>
+int fwd(const Args &a, const Parts &p, hipStream_t s) {
+    if (a.vocab <= SMALL_VOCAB) return small_fwd<T, MASK>(a, s);
+    const unsigned grid = blocks_of(a.rows * p.splits);
+    if (a.top)
+        k_tokens_part<T, MASK, true><<<grid, PART, 0, s>>>(a, p);
+    else
+        k_tokens_part<T, MASK, false><<<grid, PART, 0, s>>>(a, p);
+    const int e = (int)hipGetLastError();
+    if (e) return e;
+    k_tokens_join<T><<<blocks_of(a.rows), 64, 0, s>>>(a, p);
+    return (int)hipGetLastError();
+}
+template <class T, bool MASK>
+int bwd(const BackArgs &a, int splits, int seg, hipStream_t s) {
+    if (a.vocab <= SMALL_VOCAB) return small_bwd<T, MASK>(a, s);
+    k_tokens_bwd<T, MASK><<<blocks_of(a.rows * splits), PART, 0, s>>>(a, splits, seg);
+    return (int)hipGetLastError();
+}
+
+}  // namespace d1o
+
+using namespace d1o;
+
+#define D1O_TOKEN_TYPES(F, ...)                                                              \
+    if (type == D1_FP32) return mask ? F<float, true>(__VA_ARGS__) : F<float, false>(__VA_ARGS__);   \
+    if (type == D1_BF16) return mask ? F<__bf16, true>(__VA_ARGS__) : F<__bf16, false>(__VA_ARGS__); \
+    return mask ? F<_Float16, true>(__VA_ARGS__) : F<_Float16, false>(__VA_ARGS__);
+
+static bool token_args(int type, int64_t rows, int vocab, int64_t stride, int64_t mask_stride) {
+    return is_type(type) && rows >= 0 && vocab >= 1 && vocab <= D1_TOKENS_MAX_VOCAB && stride >= 0 && mask_stride >= 0;
+}
+
+extern "C" int64_t d1_tokens_work_bytes(int64_t rows, int vocab, int top) {
+    if (!token_args(D1_FP32, rows, vocab, 0, 0) || top < 0 || top > D1_TOKENS_MAX_TOP || top > vocab) return D1_E_ARG;
+    if (vocab <= SMALL_VOCAB || rows == 0) return 0;
+    int seg;
+    const int splits = splits_of(rows, vocab, D1_FP32, seg);     // fp32's segments are the shortest
+    return rows * splits * (16 + 8 * (int64_t)top);
+}
+
+extern "C" int d1_tokens_fwd(const void *logits, int type, int64_t rows, int vocab, int64_t stride, const int64_t *tokens,
+                             const uint8_t *mask, int64_t mask_stride, int top, float *logp, float *entropy, float *stats,
+                             int64_t *top_ids, float *top_logp, void *work, int64_t work_bytes, void *stream) {
+    if (!token_args(type, rows, vocab, stride, mask_stride)) return D1_E_ARG;
+    if (top < 0 || top > D1_TOKENS_MAX_TOP || top > vocab) return D1_E_ARG;
+    if (rows == 0) return 0;
+    if (!logits || !tokens || !logp || !entropy || !stats || (top && (!top_ids || !top_logp))) return D1_E_ARG;
+    const int64_t need = d1_tokens_work_bytes(rows, vocab, top);
+    if (need && (!work || work_bytes < need || ((uintptr_t)work & 7))) return D1_E_ARG;
+    Parts p{};
+    if (need) {
+        p.splits = splits_of(rows, vocab, type, p.seg);
+        p.keys = (uint64_t *)work;
+        p.sums = (float *)(p.keys + rows * p.splits * top);
+    }
+    const Args a{logits, rows, stride, vocab, top, tokens, mask, mask_stride, logp, entropy, stats, top_ids, top_logp};
+    D1O_TOKEN_TYPES(fwd, a, p, (hipStream_t)stream)
+}
+
+extern "C" int d1_tokens_bwd(const void *logits, int type, int64_t rows, int vocab, int64_t stride, const int64_t *tokens,
+                             const uint8_t *mask, int64_t mask_stride, const float *stats, const float *entropy,
+                             const float *dlogp, const float *dentropy, void *dlogits, void *stream) {
+    if (!token_args(type, rows, vocab, stride, mask_stride)) return D1_E_ARG;
+    if (rows == 0) return 0;
+    if (!logits || !tokens || !stats || !dlogits || (dentropy && !entropy)) return D1_E_ARG;
+    int seg = 0;
+    const int splits = vocab <= SMALL_VOCAB ? 1 : splits_of(rows, vocab, type, seg);
+    const BackArgs a{logits, rows, stride, vocab, tokens, mask, mask_stride, stats, entropy, dlogp, dentropy, dlogits};
+    D1O_TOKEN_TYPES(bwd, a, splits, seg, (hipStream_t)stream)
+}

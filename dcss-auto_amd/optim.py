@@ -1,0 +1,227 @@
+"""AdamW over many tensors in a few launches, with moments in 32 or 8 bits (csrc/d1_optim.hip).
+
+`AdamW` is the torch optimizer, `adamw_step` the step itself on lists of tensors, `read_moment` what
+an 8-bit moment stands for. The step count, the global norm of a clip and the skip of a step whose
+norm is not finite stay on the device, so a step can be captured in a HIP graph.
+"""
+import ctypes as C
+import struct
+
+import torch
+
+from . import _lib
+from .rows import on_device
+
+BLOCK = 256                         # elements of an 8-bit moment that share an exponent
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_ENTRY = '7Q2q2di2B2x'              # D1AdamWTensor
+
+
+def moment_blocks(numel):
+    """Exponent bytes of an 8-bit moment of `numel` elements."""
+    return -(-numel // BLOCK)
+
+
+def _each(value, count, name):
+    if isinstance(value, (int, float)):
+        return [value] * count
+    if len(value) != count:
+        raise ValueError(f'{name}: {len(value)} values for {count} parameters')
+    return value
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+               max_grad_norm=0.0, copies=None, exps=None, counters=None, seed=0, lags=None):
+    """One AdamW step in place over lists of tensors.
+
+    params: fp32 or bf16, contiguous. grads: fp32 or bf16 of the same sizes. exp_avg, exp_avg_sq:
+    fp32 (32-bit moments), or uint8 codes with exps = (list of exp_avg's, list of exp_avg_sq's)
+    exponents, uint8 of moment_blocks(numel) each, and counters: the first counter of each tensor's
+    rounding draws (a multiple of nothing; ranges that do not overlap draw independently). Zero codes
+    and exponents are zero moments. step: int32 [8] on the device, zeros before the first step; [0]
+    counts the steps made, [1] those skipped. copies: bf16 tensors that get the new fp32 parameters
+    (None in the list: no copy). lr and weight_decay: one value or one for each tensor. lags: steps
+    that each tensor has missed.
+
+    With max_grad_norm > 0 the gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with
+    the norm over all of them, and a step whose norm is not finite changes nothing and is counted."""
+    count = len(params)
+    eight = exps is not None
+    lists = dict(grads=grads, exp_avg=exp_avg, exp_avg_sq=exp_avg_sq)
+    for name, given in (('copies', copies), ('counters', counters), ('lags', lags)):
+        if given is not None:
+            lists[name] = given
+    if eight:
+        lists['exps[0]'], lists['exps[1]'] = exps
+    for name, given in lists.items():
+        if len(given) != count:
+            raise ValueError(f'{name}: {len(given)} for {count} parameters')
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and max_grad_norm >= 0):
+        raise ValueError('betas must be in [0, 1), eps and max_grad_norm not negative')
+    device = step.device
+    if step.dtype != torch.int32 or step.shape != (8,) or not step.is_cuda or not step.is_contiguous():
+        raise ValueError('step must be a contiguous int32 CUDA tensor of 8 elements')
+    moment = torch.uint8 if eight else torch.float32
+    words, held = [], []
+    lr, weight_decay = _each(lr, count, 'lr'), _each(weight_decay, count, 'weight_decay')
+    for i in range(count):
+        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
+        n, copy = p.numel(), None if copies is None else copies[i]
+        if not g.is_contiguous():
+            g = g.contiguous()
+            held.append(g)
+        ptype, gtype = _TYPES.get(p.dtype), _TYPES.get(g.dtype)
+        if ptype is None or gtype is None:
+            raise ValueError(f'tensor {i}: parameter and gradient must be fp32 or bf16, not {p.dtype} and {g.dtype}')
+        if m.dtype != moment or v.dtype != moment or not (g.numel() == m.numel() == v.numel() == n):
+            raise ValueError(f'tensor {i}: the gradient must have the size of the parameter, the moments too, in {moment}')
+        if not (p.device == g.device == m.device == v.device == device):
+            raise ValueError(f'tensor {i}: parameter, gradient and moments must be on {device}')
+        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f'tensor {i}: parameter and moments must be contiguous')
+        if not (lr[i] >= 0 and weight_decay[i] >= 0):
+            raise ValueError(f'tensor {i}: lr and weight_decay must not be negative')
+        if copy is not None and (copy.dtype != torch.bfloat16 or copy.numel() != n or not copy.is_contiguous()
+                                 or copy.device != device or ptype):
+            raise ValueError(f'tensor {i}: a copy is contiguous bf16 of the size of an fp32 parameter')
+        me = ve = 0
+        if eight:
+            for e in (exps[0][i], exps[1][i]):
+                if e.dtype != torch.uint8 or e.numel() != moment_blocks(n) or not e.is_contiguous() or e.device != device:
+                    raise ValueError(f'tensor {i}: exponents are contiguous uint8, one for each {BLOCK} elements')
+            me, ve = exps[0][i].data_ptr(), exps[1][i].data_ptr()
+        words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), me, ve, 0 if copy is None else copy.data_ptr(),
+                  n, 0 if counters is None else counters[i], lr[i], weight_decay[i], 0 if lags is None else lags[i],
+                  ptype, gtype)
+    table = struct.pack('=' + _ENTRY * count, *words)
+    h = _lib.D1AdamW(betas[0], betas[1], eps, max_grad_norm, seed & 0xFFFFFFFFFFFFFFFF, 8 if eight else 32)
+    L = _lib.load_ops()
+    need = L.d1_adamw_work_bytes(table, count, C.byref(h)) if max_grad_norm > 0 else 0
+    _lib.check(min(need, 0), 'd1_adamw_work_bytes')
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with on_device(device) as stream:
+        _lib.check(L.d1_adamw_step(table, count, C.byref(h), step.data_ptr(), work.data_ptr() if need else None, need,
+                                   stream), 'd1_adamw_step')
+
+
+def read_moment(code, exp, signed, out=None):
+    """fp32 values of an 8-bit moment: uint8 codes and their exponents (signed: exp_avg's)."""
+    n = code.numel()
+    if code.dtype != torch.uint8 or exp.dtype != torch.uint8 or not code.is_cuda or exp.device != code.device \
+            or not code.is_contiguous() or not exp.is_contiguous() or exp.numel() != moment_blocks(n):
+        raise ValueError(f'code and exp must be contiguous uint8 CUDA tensors, one exponent for each {BLOCK} codes')
+    if out is None:
+        out = torch.empty(code.shape, dtype=torch.float32, device=code.device)
+    elif out.dtype != torch.float32 or out.numel() != n or not out.is_contiguous() or out.device != code.device:
+        raise ValueError('out must be contiguous fp32 of the size of the codes, on their device')
+    with on_device(code.device) as stream:
+        _lib.check(_lib.load_ops().d1_adamw_read(code.data_ptr(), exp.data_ptr(), n, 1 if signed else 0, out.data_ptr(),
+                                                 stream), 'd1_adamw_read')
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW on the device in a few launches for all tensors of all groups.
+
+    lr and weight_decay may differ between groups; betas, eps, state_bits (32 or 8) and
+    max_grad_norm (the clip by the global norm of all groups' gradients, 0 for none) are the
+    optimizer's. copies: {parameter: bf16 tensor} that a step writes beside fp32 parameters. A
+    parameter without a gradient is left as it is and keeps its own step count. With max_grad_norm a
+    step whose norm is not finite changes nothing; skipped_steps() counts those."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
+                 max_grad_norm=0.0, copies=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError('state_bits is 8 or 32')
+        if not (lr >= 0 and weight_decay >= 0):
+            raise ValueError('lr and weight_decay must not be negative')
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and max_grad_norm >= 0):
+            raise ValueError('betas must be in [0, 1), eps and max_grad_norm not negative')
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+        self.betas, self.eps, self.state_bits, self.max_grad_norm, self.seed = betas, eps, state_bits, max_grad_norm, seed
+        self.copies = copies or {}
+        self.ctl = None                 # the device's step count, skips and norm (adamw_step's `step`)
+        self._calls = self._counter = 0
+
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            s['calls'], s['counter'] = 0, self._counter
+            self._counter += moment_blocks(p.numel()) * BLOCK
+            dtype = torch.uint8 if self.state_bits == 8 else torch.float32
+            for name in ('exp_avg', 'exp_avg_sq'):
+                s[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
+                if self.state_bits == 8:
+                    s[name + '_exp'] = torch.zeros(moment_blocks(p.numel()), dtype=torch.uint8, device=p.device)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, states, lr, decay = [], [], [], []
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.grad is not None:
+                    params.append(p)
+                    states.append(self._state(p))
+                    lr.append(group['lr'])
+                    decay.append(group['weight_decay'])
+        if not params:
+            return loss
+        if self.ctl is None:
+            self.ctl = torch.zeros(8, dtype=torch.int32, device=params[0].device)
+        eight = self.state_bits == 8
+        column = lambda name: [s[name] for s in states]  # noqa: E731
+        adamw_step(params, [p.grad for p in params], column('exp_avg'), column('exp_avg_sq'), self.ctl, lr=lr,
+                   betas=self.betas, eps=self.eps, weight_decay=decay, max_grad_norm=self.max_grad_norm,
+                   copies=[self.copies.get(p) for p in params] if self.copies else None,
+                   exps=(column('exp_avg_exp'), column('exp_avg_sq_exp')) if eight else None,
+                   counters=column('counter') if eight else None, seed=self.seed,
+                   lags=[self._calls - s['calls'] for s in states])
+        self._calls += 1
+        for s in states:
+            s['calls'] += 1
+        return loss
+
+    def skipped_steps(self):
+        """Steps left out because the gradients' norm was not finite (waits for the device)."""
+        return 0 if self.ctl is None else int(self.ctl[1].item())
+
+    def grad_norm(self):
+        """The last step's global gradient norm before the clip, fp32 on the device (max_grad_norm > 0)."""
+        if self.ctl is None:
+            raise RuntimeError('no step was made')
+        return self.ctl[5:6].view(torch.float32)[0]
+
+    def moments(self, p):
+        """fp32 (exp_avg, exp_avg_sq) of a parameter."""
+        s = self.state[p]
+        if self.state_bits == 32:
+            return s['exp_avg'], s['exp_avg_sq']
+        return (read_moment(s['exp_avg'], s['exp_avg_exp'], signed=True),
+                read_moment(s['exp_avg_sq'], s['exp_avg_sq_exp'], signed=False))
+
+    def state_dict(self):
+        d = super().state_dict()
+        d['d1'] = dict(state_bits=self.state_bits, ctl=None if self.ctl is None else self.ctl.clone(), calls=self._calls,
+                       counter=self._counter, seed=self.seed)
+        return d
+
+    def load_state_dict(self, state_dict):
+        own = state_dict['d1']
+        if own['state_bits'] != self.state_bits:
+            raise ValueError(f"the state was saved with {own['state_bits']}-bit moments, this optimizer has {self.state_bits}")
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != 'd1'})
+        # the base class casts tensors to the parameters' type: take the moments as they were saved
+        saved = state_dict['state']
+        ids = [i for group in state_dict['param_groups'] for i in group['params']]
+        for i, p in zip(ids, (p for group in self.param_groups for p in group['params'])):
+            for name, value in saved.get(i, {}).items():
+                if torch.is_tensor(value):
+                    self.state[p][name] = value.to(p.device, copy=True).contiguous()
+        device = self.param_groups[0]['params'][0].device
+        self.ctl = None if own['ctl'] is None else own['ctl'].to(device, copy=True)
+        self._calls, self._counter, self.seed = own['calls'], own['counter'], own['seed']
