@@ -3,7 +3,7 @@
 // With mu and r = 1/sqrt(var + eps) of a row and xh = (x - mu) r:
 //   y = xh w + b;  u = dy w;  dx = r (u - mean(u) - xh mean(u xh));  dw = sum dy xh;  db = sum dy.
 // Both passes read each input once: a row stays in the registers of LANES lanes (4 to 64 of a
-// wave, or a whole workgroup of 256 or 1024), CH chunks of 16 bytes a lane, so the variance is
+// wave, or a workgroup of 128 to 1,024), CH chunks of 16 bytes a lane, so the variance is
 // taken about the mean itself and not from a difference of sums. The backward pass keeps the
 // columns' dw and db sums in registers over all rows that a workgroup walks, writes them once, and
 // k_norm_reduce adds the workgroups' sums in a fixed order (no atomics: the same bits each time).
@@ -12,6 +12,8 @@
 namespace d1o {
 
 constexpr int threads_of(int lanes) { return lanes <= 64 ? 256 : lanes; }
+// waves a SIMD that the forward pass is held to: two workgroups of 1,024 lanes on a CU
+constexpr int fwd_waves(int lanes, int ch) { return lanes == 1024 && ch <= 2 ? 8 : 1; }
 template <class T>
 constexpr int vec_of() { return 16 / (int)sizeof(T); }
 
@@ -26,43 +28,50 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float2 (*scratch)[1
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = make_float2(a, b);
         __syncthreads();
-        a = 0.f, b = 0.f;
-#pragma unroll
-        for (int i = 0; i < LANES / 64; i++) {
-            a += s[i].x;
-            b += s[i].y;
-        }
+        // every lane reads one wave's sums: 16 lanes (8, 4) add them like a row of that many lanes
+        const float2 v = s[threadIdx.x % (LANES / 64)];
+        a = lanes_sum<LANES / 64>(v.x);
+        b = lanes_sum<LANES / 64>(v.y);
     }
 }
 
+// the CH chunks of a lane from a row of `width` elements; `fill` past its end
+template <class T, int LANES, int CH, int VEC>
+__device__ __forceinline__ void read_row(Pack<T, VEC> (&a)[CH], const T *row, int lane, int width, T fill) {
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int col = (c * LANES + lane) * VEC;
+        a[c] = load_part<T, VEC>(row + col, width - col, fill);
+    }
+}
+template <class T, int LANES, int CH, int VEC>
+__device__ __forceinline__ void read_weight(Pack<T, VEC> (&a)[CH], const T *w, int lane, int width, T without) {
+    if (w) return read_row<T, LANES, CH, VEC>(a, w, lane, width, without);
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) a[c].v[i] = without;
+}
+
 template <class T, class W, int LANES, int CH>
-__global__ __launch_bounds__(threads_of(LANES)) void k_norm_fwd(const T *__restrict__ x, int64_t rows, int width, int64_t stride,
+__global__ __launch_bounds__(threads_of(LANES), fwd_waves(LANES, CH)) void k_norm_fwd(const T *__restrict__ x, int64_t rows, int width, int64_t stride,
                                                                 const W *__restrict__ w, const W *__restrict__ b, float eps,
                                                                 T *__restrict__ y, float *__restrict__ mean,
                                                                 float *__restrict__ rstd) {
     constexpr int VEC = vec_of<T>(), GROUPS = threads_of(LANES) / LANES;
     __shared__ float2 scratch[2][16];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
     int turn = 0;
-    float wv[CH][VEC], bv[CH][VEC];
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int col = (c * LANES + lane) * VEC;
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            wv[c][i] = w && col + i < width ? (float)w[col + i] : 1.f;
-            bv[c][i] = b && col + i < width ? (float)b[col + i] : 0.f;
-        }
-    }
+    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+    Pack<W, VEC> wv[CH], bv[CH];
+    read_weight<W, LANES, CH, VEC>(wv, w, lane, width, (W)1.f);
+    read_weight<W, LANES, CH, VEC>(bv, b, lane, width, (W)0.f);
     const float inv = 1.f / (float)width;
-    for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < rows; row += (int64_t)gridDim.x * GROUPS) {
+    for (; row < rows; row += step) {
         Pack<T, VEC> a[CH];
+        read_row<T, LANES, CH, VEC>(a, x + row * stride, lane, width, (T)0.f);
         float sum = 0.f, none = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int col = (c * LANES + lane) * VEC;
-            a[c] = load_part<T, VEC>(x + row * stride + col, width - col, (T)0.f);
-        }
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
@@ -88,7 +97,8 @@ __global__ __launch_bounds__(threads_of(LANES)) void k_norm_fwd(const T *__restr
             const int col = (c * LANES + lane) * VEC;
             Pack<T, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; i++) o.v[i] = (T)__builtin_fmaf(((float)a[c].v[i] - mu) * r, wv[c][i], bv[c][i]);
+            for (int i = 0; i < VEC; i++)
+                o.v[i] = (T)__builtin_fmaf(((float)a[c].v[i] - mu) * r, (float)wv[c].v[i], (float)bv[c].v[i]);
             store_part<T, VEC>(y + row * width + col, width - col, o);
         }
     }
@@ -103,33 +113,24 @@ __global__ __launch_bounds__(threads_of(LANES)) void k_norm_bwd(const T *__restr
     __shared__ float2 scratch[2][16];
     __shared__ float sums[GROUPS > 1 ? GROUPS * COLS : 1];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
     int turn = 0;
-    float wv[CH][VEC], gw[CH][VEC], gb[CH][VEC];
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int col = (c * LANES + lane) * VEC;
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            wv[c][i] = w && col + i < width ? (float)w[col + i] : 1.f;
-            gw[c][i] = gb[c][i] = 0.f;
-        }
-    }
+    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+    Pack<W, VEC> wv[CH];
+    read_weight<W, LANES, CH, VEC>(wv, w, lane, width, (W)1.f);
+    float gw[CH][VEC] = {}, gb[CH][VEC] = {};
     const float inv = 1.f / (float)width;
-    for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < rows; row += (int64_t)gridDim.x * GROUPS) {
+    for (; row < rows; row += step) {
         const float mu = mean[row], r = rstd[row];
         Pack<T, VEC> a[CH], g[CH];
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int col = (c * LANES + lane) * VEC;
-            a[c] = load_part<T, VEC>(x + row * stride + col, width - col, (T)0.f);
-            g[c] = load_part<T, VEC>(dy + row * dy_stride + col, width - col, (T)0.f);
-        }
+        read_row<T, LANES, CH, VEC>(a, x + row * stride, lane, width, (T)0.f);
+        read_row<T, LANES, CH, VEC>(g, dy + row * dy_stride, lane, width, (T)0.f);
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                const float d = (float)g[c].v[i], h = ((float)a[c].v[i] - mu) * r, u = d * wv[c][i];
+                const float d = (float)g[c].v[i], h = ((float)a[c].v[i] - mu) * r, u = d * (float)wv[c].v[i];
                 gw[c][i] = __builtin_fmaf(d, h, gw[c][i]);
                 gb[c][i] += d;
                 c1 += u;
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void k_norm_bwd(const T *__restr
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
                 const float h = ((float)a[c].v[i] - mu) * r;
-                o.v[i] = (T)(r * (__builtin_fmaf((float)g[c].v[i], wv[c][i], -c1) - h * c2));
+                o.v[i] = (T)(r * (__builtin_fmaf((float)g[c].v[i], (float)wv[c].v[i], -c1) - h * c2));
             }
             store_part<T, VEC>(dx + row * width + col, width - col, o);
         }
@@ -156,12 +157,13 @@ __global__ __launch_bounds__(threads_of(LANES)) void k_norm_bwd(const T *__restr
     for (int k = 0; k < 2; k++) {
         if (GROUPS == 1) {
 #pragma unroll
-            for (int c = 0; c < CH; c++)
+            for (int c = 0; c < CH; c++) {
+                const int col = (c * LANES + lane) * VEC;
+                Pack<float, VEC> o;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const int col = (c * LANES + lane) * VEC + i;
-                    if (col < width) out[k * width + col] = k ? gb[c][i] : gw[c][i];
-                }
+                for (int i = 0; i < VEC; i++) o.v[i] = k ? gb[c][i] : gw[c][i];
+                store_part<float, VEC>(out + k * width + col, width - col, o);
+            }
         } else {
             __syncthreads();
 #pragma unroll
@@ -188,8 +190,18 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float *__restrict__ 
     W *out = blockIdx.y ? db : dw;
     if (!out) return;
     float sum = 0.f;
-    if (col < width)
-        for (int p = k; p < nparts; p += 32) sum += parts[((size_t)p * 2 + blockIdx.y) * width + col];
+    if (col < width) {
+        const float *at = parts + (size_t)blockIdx.y * width + col;
+        int p = k;
+        for (; p + 7 * 32 < nparts; p += 8 * 32) {       // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = at[(size_t)(p + j * 32) * 2 * width];
+#pragma unroll
+            for (int j = 0; j < 8; j++) sum += v[j];
+        }
+        for (; p < nparts; p += 32) sum += at[(size_t)p * 2 * width];
+    }
     s[k][c] = sum;
     __syncthreads();
     if (k == 0 && col < width) {
@@ -199,8 +211,13 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float *__restrict__ 
     }
 }
 
-// Row shape for a width: lanes a row and chunks a lane, the fewest that hold it.
-#define D1O_NORM_SHAPES(X) X(4, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(256, 4) X(1024, 2) X(1024, 4)
+// Lanes a row and chunks a lane for a width: the fewest lanes that hold it at one chunk each. Few
+// registers a lane and many waves do more for the bandwidth than many chunks a lane: 16,384 rows of
+// 8,192 bf16 forward 103 us on 1,024 lanes x 1 chunk, 122 on 512 x 2, 136 at best on 256 x 4 (one
+// row ahead in registers); backward 160, 179 and 251. Reading a row ahead costs more
+// waves than it hides (112 and 198 us on 1,024 x 1), so no shape does.
+#define D1O_NORM_SHAPES(X)                                                                                          \
+    X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2) X(1024, 4)
 inline int shape_of(int width, int type, int &lanes) {
     const int vec = type == D1_FP32 ? 4 : 8;
 #define X(L, C)                     \
@@ -213,12 +230,25 @@ inline int shape_of(int width, int type, int &lanes) {
     return 0;
 }
 
-// Workgroups of a pass: at most 4 for each of the 256 CUs, fewer where rows are few.
-inline int grid_of(int64_t rows, int lanes) {
+inline int64_t groups_of_rows(int64_t rows, int lanes) {
     const int groups = threads_of(lanes) / lanes;
-    const int64_t need = (rows + groups - 1) / groups;
-    const int64_t most = lanes == 1024 ? 512 : 1024;
+    return (rows + groups - 1) / groups;
+}
+// Forward: workgroups walk the rows with a stride of the grid; more of them than fit at once even out
+// their ends, up to where reading the weights again costs (65,536 x 256 bf16: 14.2 us at 4,096, 15.0 at 1,024, 15.9
+// at 8,192; 65,536 x 1,024: 88, 52.2 and 52.6 at 1,024, 4,096 and 8,192; 16,384 x 8,192: 103 at 1,024, 109 at 4,096).
+inline int fwd_grid(int64_t rows, int lanes) {
+    const int64_t need = groups_of_rows(rows, lanes), most = lanes == 1024 ? 1024 : lanes == 512 || lanes < 64 ? 4096 : 8192;
     return (int)(need < most ? need : most);
+}
+// Backward: each workgroup writes its columns' sums, which k_norm_reduce reads again, so only about as many
+// as fit at once (65,536 x 1,024 bf16: 118, 83 and 103 us at 1,024, 2,048 and 4,096 of 128 lanes; 16,384 x 8,192: 168,
+// 160 and 173 at 256, 512 and 1,024), and two rows each at least where there are more than 512
+// (8,192 x 256: 7.9 us at 512, 9.1 at 1,024).
+inline int bwd_grid(int64_t rows, int lanes) {
+    const int64_t need = groups_of_rows(rows, lanes), half = (need + 1) / 2, few = need < 512 ? need : half < 512 ? 512 : half;
+    const int threads = threads_of(lanes), most = 256 * (threads == 128 ? 8 : threads == 256 ? 5 : threads == 512 ? 3 : 2);
+    return (int)(few < most ? few : most);
 }
 
 template <class T, class W>
@@ -226,7 +256,7 @@ int fwd(const void *x, int type, int64_t rows, int width, int64_t stride, const 
         float *mean, float *rstd, hipStream_t s) {
     int lanes = 0;
     const int ch = shape_of(width, type, lanes);
-    const dim3 grid(grid_of(rows, lanes));
+    const dim3 grid(fwd_grid(rows, lanes));
 #define X(L, C)                                                                                                            \
     if constexpr (L * C * vec_of<T>() <= D1_NORM_MAX_WIDTH)                                                                \
         if (lanes == L && ch == C)                                                                                         \
@@ -241,7 +271,7 @@ template <class T, class W>
 int bwd(const void *dy, int64_t dy_stride, const void *x, int type, int64_t rows, int width, int64_t stride, const void *w,
         const float *mean, const float *rstd, void *dx, void *dw, void *db, float *parts, hipStream_t s) {
     int lanes = 0;
-    const int ch = shape_of(width, type, lanes), grid = grid_of(rows, lanes);
+    const int ch = shape_of(width, type, lanes), grid = bwd_grid(rows, lanes);
     if (rows > 0) {
 #define X(L, C)                                                                                                          \
     if constexpr (L * C * vec_of<T>() <= D1_NORM_MAX_WIDTH)                                                              \
@@ -287,7 +317,7 @@ extern "C" int64_t d1_norm_work_bytes(int64_t rows, int width, int type) {
     if (!norm_args(type, type, rows, width, 0)) return D1_E_ARG;
     int lanes = 0;
     shape_of(width, type, lanes);
-    return (int64_t)grid_of(rows, lanes) * 2 * width * sizeof(float);
+    return (int64_t)bwd_grid(rows, lanes) * 2 * width * sizeof(float);
 }
 
 extern "C" int d1_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int type, int64_t rows, int width, int64_t stride,
