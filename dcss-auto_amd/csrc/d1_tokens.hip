@@ -37,12 +37,6 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 __device__ __forceinline__ uint64_t key_of(float x, int index) { return ((uint64_t)ordered(x) << 32) | (uint32_t)~index; }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-template <int LANES>
-__device__ __forceinline__ uint64_t lanes_max_key(uint64_t k) {
-    const uint32_t hi = lanes_u<LANES>((uint32_t)(k >> 32), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    const uint32_t lo = lanes_u<LANES>((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    return ((uint64_t)hi << 32) | lo;
-}
 
 // running maximum, sum of exponentials and of exponentials times differences
 struct Sums {
@@ -75,24 +69,29 @@ struct Args {
     float *top_logp;
 };
 
-// what one lane writes of a row once its sums are whole
+// logp of a token whose entry is x (x is -inf where it is masked)
+__device__ __forceinline__ float logp_of(float x, Sums t, float base, float ls) {
+    return t.s == 0.f ? -INFINITY : (x - base) - ls;
+}
+// logp of what is no token: padding, or an index past the row
+__device__ __forceinline__ float logp_of_none(int64_t tok) { return tok < 0 ? 0.f : __builtin_nanf(""); }
+__device__ __forceinline__ void put_row(const Args &a, int64_t row, Sums t, float base, float ls) {
+    a.entropy[row] = t.s == 0.f ? 0.f : ls - t.e / t.s;
+    a.stats[2 * row] = base;
+    a.stats[2 * row + 1] = t.s;
+}
+// what one lane writes of a long row once its sums are whole
 template <class T>
 __device__ __forceinline__ void finish(const Args &a, int64_t row, Sums t) {
     const float base = finite_base(t.m), ls = logf(t.s);
     const int64_t tok = a.tokens[row];
-    float lp;
-    if (tok < 0)
-        lp = 0.f;
-    else if (tok >= a.vocab)
-        lp = __builtin_nanf("");
-    else if (t.s == 0.f || (a.mask && !a.mask[row * a.mask_stride + tok]))
-        lp = t.s == t.s ? -INFINITY : t.s;
-    else
-        lp = ((float)((const T *)a.logits)[row * a.stride + tok] - base) - ls;
-    a.logp[row] = lp;
-    a.entropy[row] = t.s == 0.f ? 0.f : ls - t.e / t.s;
-    a.stats[2 * row] = base;
-    a.stats[2 * row + 1] = t.s;
+    if (tok < 0 || tok >= a.vocab) {
+        a.logp[row] = logp_of_none(tok);
+    } else {
+        const bool in = !a.mask || a.mask[row * a.mask_stride + tok];
+        a.logp[row] = logp_of(in ? (float)((const T *)a.logits)[row * a.stride + tok] : -INFINITY, t, base, ls);
+    }
+    put_row(a, row, t, base, ls);
 }
 __device__ __forceinline__ void put_top(const Args &a, int64_t row, int k, uint64_t key, float base, float ls, float s) {
     const bool none = (key >> 32) == 0;
@@ -129,6 +128,7 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
     for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows; row += (int64_t)gridDim.x * GROUPS) {
         SmallRow<T, LANES, CH, MASK> r;
         r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane);
+        const int64_t tok = a.tokens[row];
         float m = -INFINITY;
 #pragma unroll
         for (int c = 0; c < CH; c++)
@@ -147,21 +147,44 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
             }
         s = lanes_sum<LANES>(s);
         e = lanes_sum<LANES>(e);
-        if (lane == 0) finish<T>(a, row, {m, s, e});
+        const Sums t = {m, s, e};
+        const float ls = logf(s);
+        // the lane that holds the token's entry writes its logp: no second, dependent read of the row
+        if (lane == 0) {
+            put_row(a, row, t, base, ls);
+            if (tok < 0 || tok >= a.vocab) a.logp[row] = logp_of_none(tok);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int64_t at = tok - (c * LANES + lane) * 4;
+            if (at >= 0 && at < 4 && tok < a.vocab) {
+                const float x = at < 2 ? (at ? r.x[c][1] : r.x[c][0]) : (at == 2 ? r.x[c][2] : r.x[c][3]);
+                a.logp[row] = logp_of(x, t, base, ls);
+            }
+        }
         if (a.top) {
-            const float ls = logf(s);
-            uint64_t last = ~0ull;
+            uint32_t word[CH][4];        // 0: not an entry, or taken
+#pragma unroll
+            for (int c = 0; c < CH; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) word[c][i] = r.in[c][i] ? ordered(r.x[c][i]) : 0;
             for (int k = 0; k < a.top; k++) {
-                uint64_t best = 0;
+                uint32_t best = 0, first = 0xFFFFFFFFu;
 #pragma unroll
                 for (int c = 0; c < CH; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint64_t key = r.in[c][i] ? key_of(r.x[c][i], (c * LANES + lane) * 4 + i) : 0;
-                        if (key < last && key > best) best = key;
-                    }
-                last = lanes_max_key<LANES>(best);
-                if (lane == 0) put_top(a, row, k, last, base, ls, s);
+                    for (int i = 0; i < 4; i++) best = best > word[c][i] ? best : word[c][i];
+                best = lanes_u<LANES>(best, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
+#pragma unroll
+                for (int c = CH - 1; c >= 0; c--)
+#pragma unroll
+                    for (int i = 3; i >= 0; i--) first = word[c][i] == best ? (c * LANES + lane) * 4 + i : first;
+                first = lanes_u<LANES>(first, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) word[c][i] = (uint32_t)((c * LANES + lane) * 4 + i) == first ? 0 : word[c][i];
+                if (lane == 0) put_top(a, row, k, ((uint64_t)best << 32) | (uint32_t)~first, base, ls, s);
             }
         }
     }
@@ -199,33 +222,73 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// the `top` largest of up to KEEP keys in `list` (LDS, one wave's), in falling order to out[0..top)
-__device__ __forceinline__ void extract(const uint64_t *list, int count, int top, int lane, uint64_t *out) {
-    uint64_t mine[KEEP / 64];
+// A wave's list of keys in LDS: takes keys in any order, keeps at least the `top` largest seen.
+struct TopList {
+    uint64_t *list, *sorted;     // KEEP and D1_TOKENS_MAX_TOP keys
+    int top, count;
+    uint64_t below;              // keys up to this one are not among the largest
+
+    // the `top` largest to `sorted`, falling; places without a key are 0. A key's place is the number of larger ones.
+    __device__ __forceinline__ void sort(int lane) {
+        uint64_t mine[KEEP / 64];
+        int larger[KEEP / 64] = {};
+        wave_sync();
 #pragma unroll
-    for (int i = 0; i < KEEP / 64; i++) mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; k++) {
-        uint64_t best = 0;
+        for (int i = 0; i < KEEP / 64; i++) mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
+        for (int j = 0; j < count; j++) {
+            const uint64_t key = list[j];
+#pragma unroll
+            for (int i = 0; i < KEEP / 64; i++)
+                if (i * 64 < count) larger[i] += key > mine[i];
+        }
+        if (lane < top) sorted[lane] = 0;
+        wave_sync();
 #pragma unroll
         for (int i = 0; i < KEEP / 64; i++)
-            if (mine[i] < last && mine[i] > best) best = mine[i];
-        last = lanes_max_key<64>(best);
-        if (lane == 0) out[k] = last;
+            if (mine[i] && larger[i] < top) sorted[larger[i]] = mine[i];
+        wave_sync();
     }
+    __device__ __forceinline__ void shrink(int lane) {
+        sort(lane);
+        if (lane < top) list[lane] = sorted[lane];
+        below = sorted[top - 1];
+        count = top;
+        wave_sync();
+    }
+    // one key a lane (0: none); the whole wave calls
+    __device__ __forceinline__ void add(uint64_t key, int lane) {
+        const uint64_t take = __ballot(key > below);
+        if (!take) return;
+        if (key > below) list[count + __popcll(take & ((1ull << lane) - 1))] = key;
+        count += __popcll(take);
+        if (count > KEEP - 64) shrink(lane);
+    }
+};
+
+// the k-th largest (k <= 64) of the lanes' words: bit by bit from the top, as many lanes as k stay above
+__device__ __forceinline__ uint32_t kth_word(uint32_t word, int k) {
+    uint32_t floor = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t at = floor | (1u << bit);
+        if (__popcll(__ballot(word >= at)) >= k) floor = at;
+    }
+    return floor;
 }
 
 template <class T, bool MASK, bool TOP>
 __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts parts) {
     constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
     __shared__ Sums wave_sums[WAVES];
-    __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? KEEP : 1], best_of[TOP ? WAVES : 1][TOP ? D1_TOKENS_MAX_TOP : 1];
+    __shared__ uint32_t wave_floor[WAVES];
+    __shared__ int wave_count[WAVES];
+    __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? KEEP : 1], sorted[TOP ? WAVES : 1][TOP ? D1_TOKENS_MAX_TOP : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t units = a.rows * parts.splits;
     for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int64_t row = unit / parts.splits;
         const int split = (int)(unit - row * parts.splits), begin = split * parts.seg;
-        const int n = a.vocab - begin < parts.seg ? a.vocab - begin : parts.seg;     // may be <= 0: nothing to read
+        const int n = a.vocab - begin < parts.seg ? a.vocab - begin : parts.seg;
         const T *x = (const T *)a.logits + row * a.stride + begin;
         const uint8_t *mask = MASK ? a.mask + row * a.mask_stride + begin : nullptr;
         Sums t = {-INFINITY, 0.f, 0.f};
@@ -252,80 +315,109 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
                 }
         }
         const Sums wave_sum = lanes_joined<64>(t);
-        if (lane == 0) wave_sums[wave] = wave_sum;
+        uint32_t wave_kth = 0, most = 0;     // of TOP: most is a word that no entry of the lane passes
+        if (TOP) {
+            // The maximum leaves NaN out, which is the largest of all; the sum knows of it (or of +inf).
+            // A lane without an entry above -inf may still hold allowed ones there: it counts as one.
+            const bool odd = t.s != t.s;
+            const uint32_t word = (int)threadIdx.x * VEC >= n ? 0 : odd && t.m != INFINITY ? 0xFFFFFFFEu : ordered(t.m);
+            wave_kth = kth_word(word, a.top);
+            most = odd ? 0xFFFFFFFEu : word;
+        }
+        if (lane == 0) {
+            wave_sums[wave] = wave_sum;
+            if (TOP) wave_floor[wave] = wave_kth;
+        }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            Sums all = wave_sums[0];
+        Sums all = wave_sums[0];
 #pragma unroll
-            for (int w = 1; w < WAVES; w++) all = joined(all, wave_sums[w]);
-            float *o = parts.sums + unit * 4;
-            o[0] = all.m;
-            o[1] = all.s;
-            o[2] = all.e;
+        for (int w = 1; w < WAVES; w++) all = joined(all, wave_sums[w]);
+        if (threadIdx.x == 0) {
+            if (parts.splits == 1) {
+                finish<T>(a, row, all);
+            } else {
+                float *o = parts.sums + unit * 4;
+                o[0] = all.m;
+                o[1] = all.s;
+                o[2] = all.e;
+            }
         }
         if (TOP) {
-            // every entry of the segment against the wave's list: the simplest way that is right
-            uint64_t floor_key = 0;      // keys up to this one are not among the wave's best
-            int count = 0;
-            for (int i0 = 0; i0 < n; i0 += STEP) {
-                const int i = i0 + threadIdx.x * VEC;
+            // At least `top` lanes of some wave hold an entry of this word or more, so the segment's best are
+            // no smaller; only lanes that hold such an entry are looked through again, by their whole wave.
+            uint32_t floor = wave_floor[0];
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const int at = i + j;
+            for (int w = 1; w < WAVES; w++) floor = floor > wave_floor[w] ? floor : wave_floor[w];
+            TopList best = {found[wave], sorted[wave], a.top, 0, 0};
+            const int each = ((n + STEP - 1) / STEP) * VEC;      // entries of a lane
+            for (uint64_t left = __ballot(most && most >= floor); left; left &= left - 1) {
+                const int who = wave * 64 + __builtin_ctzll(left);
+                for (int q0 = 0; q0 < each; q0 += 64) {
+                    const int q = q0 + lane, at = (q / VEC * PART + who) * VEC + q % VEC;
                     uint64_t key = 0;
-                    if (at < n && (!MASK || mask[at])) key = key_of((float)x[at], begin + at);
-                    const uint64_t take = __ballot(key > floor_key);
-                    if (!take) continue;
-                    if (key > floor_key) found[wave][count + __popcll(take & ((1ull << lane) - 1))] = key;
-                    count += __popcll(take);
-                    if (count > KEEP - 64) {      // no room for another 64: keep the best
-                        wave_sync();
-                        extract(found[wave], count, a.top, lane, best_of[wave]);
-                        wave_sync();
-                        if (lane < a.top) found[wave][lane] = best_of[wave][lane];
-                        wave_sync();
-                        count = a.top;
-                        floor_key = best_of[wave][a.top - 1];
-                    }
+                    if (q < each && at < n && (!MASK || mask[at])) key = key_of((float)x[at], begin + at);
+                    best.add((uint32_t)(key >> 32) >= floor ? key : 0, lane);
                 }
             }
-            wave_sync();
-            extract(found[wave], count, a.top, lane, best_of[wave]);
+            if (best.count > KEEP / WAVES) best.shrink(lane);
+            if (lane == 0) wave_count[wave] = best.count;
             __syncthreads();
-            if (wave == 0) {       // the waves' lists, at most KEEP keys
-                for (int i = lane; i < WAVES * a.top; i += 64) found[0][i] = best_of[i / a.top][i % a.top];
-                wave_sync();
-                extract(found[0], WAVES * a.top, a.top, lane, best_of[0]);
-                wave_sync();
-                if (lane < a.top) parts.keys[unit * a.top + lane] = best_of[0][lane];
+            if (wave == 0) {       // the waves' lists, KEEP / WAVES keys each at most
+                for (int w = 1; w < WAVES; w++) {
+                    const int more = wave_count[w];
+                    if (lane < more) found[0][best.count + lane] = found[w][lane];
+                    best.count += more;
+                }
+                best.sort(lane);
+                if (parts.splits == 1) {
+                    if (lane < a.top) put_top(a, row, lane, sorted[0][lane], finite_base(all.m), logf(all.s), all.s);
+                } else if (lane < a.top) {
+                    parts.keys[unit * a.top + lane] = sorted[0][lane];
+                }
             }
         }
         __syncthreads();
     }
 }
 
-// one wave a row: lane l holds segment l (at most 64 segments) and the head of its sorted list
+// one wave a row: lane l holds segment l (at most 64 segments) and walks its sorted list
 template <class T>
 __global__ __launch_bounds__(64) void k_tokens_join(const Args a, const Parts parts) {
+    __shared__ uint64_t found[KEEP], sorted[D1_TOKENS_MAX_TOP];
     const int lane = threadIdx.x;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         Sums t = {-INFINITY, 0.f, 0.f};
-        if (lane < parts.splits) {
+        const bool mine = lane < parts.splits;
+        if (mine) {
             const float *p = parts.sums + (row * parts.splits + lane) * 4;
             t = {p[0], p[1], p[2]};
         }
+        const uint64_t *keys = parts.keys + (row * parts.splits + lane) * a.top;
+        const uint64_t head = mine && a.top ? keys[0] : 0;
         t = lanes_joined<64>(t);
         if (lane == 0) finish<T>(a, row, t);
         if (a.top) {
-            const float base = finite_base(t.m), ls = logf(t.s);
-            const uint64_t *mine = parts.keys + (row * parts.splits + lane) * a.top;
-            int at = 0;
-            uint64_t head = lane < parts.splits ? mine[0] : 0;
-            for (int k = 0; k < a.top; k++) {
-                const uint64_t key = lanes_max_key<64>(head);
-                if (lane == 0) put_top(a, row, k, key, base, ls, t.s);
-                if (key && head == key) head = ++at < a.top ? mine[at] : 0;
+            // the top-th largest head bounds the row's best from below
+            const uint32_t floor = kth_word((uint32_t)(head >> 32), a.top);
+            const bool open = head && (uint32_t)(head >> 32) >= floor;
+            TopList best = {found, sorted, a.top, 0, 0};
+            best.add(open ? head : 0, lane);
+            for (int k0 = 1; k0 < a.top; k0 += 4) {
+                uint64_t key[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) key[j] = open && k0 + j < a.top ? keys[k0 + j] : 0;
+                uint64_t some = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if ((uint32_t)(key[j] >> 32) < floor) key[j] = 0;
+                    some |= __ballot(key[j] > best.below);
+                    best.add(key[j], lane);
+                }
+                if (!some) break;        // the lists fall: nothing larger follows
             }
+            best.sort(lane);
+            if (lane < a.top) put_top(a, row, lane, sorted[lane], finite_base(t.m), logf(t.s), t.s);
+            wave_sync();
         }
     }
 }
@@ -473,7 +565,7 @@ int fwd(const Args &a, const Parts &p, hipStream_t s) {
     else
         k_tokens_part<T, MASK, false><<<grid, PART, 0, s>>>(a, p);
     const int e = (int)hipGetLastError();
-    if (e) return e;
+    if (e || p.splits == 1) return e;
     k_tokens_join<T><<<blocks_of(a.rows), 64, 0, s>>>(a, p);
     return (int)hipGetLastError();
 }
