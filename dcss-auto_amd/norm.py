@@ -9,7 +9,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rows import TYPES, as_rows, like, on_device, type_of
+from .rows import TYPES, as_rows, call, like, type_of
 
 MAX_WIDTH = 16384
 
@@ -17,14 +17,18 @@ MAX_WIDTH = 16384
 def _check(x, weight, bias):
     """-> (x's type code, the weights' type code, x as rows, weight, bias)."""
     code = type_of(x, 'x')
-    width = x.shape[-1]
+    width, index, dtype = x.shape[-1], x.get_device(), x.dtype
     if width > MAX_WIDTH:
         raise ValueError(f'x: rows of at most {MAX_WIDTH} elements')
-    dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
-    if dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"weight and bias must be fp32 or of x's type, not {dtype}")
-    weight = None if weight is None else like(weight, (width,), x.device, 'weight', dtype)
-    bias = None if bias is None else like(bias, (width,), x.device, 'bias', dtype)
+    first = bias if weight is None else weight
+    if first is not None:
+        dtype = first.dtype
+        if dtype != x.dtype and dtype != torch.float32:
+            raise ValueError(f"weight and bias must be fp32 or of x's type, not {dtype}")
+        if weight is not None:
+            weight = like(weight, (width,), index, 'weight', dtype)
+        if bias is not None:
+            bias = like(bias, (width,), index, 'bias', dtype)
     return code, TYPES[dtype], as_rows(x), weight, bias
 
 
@@ -37,12 +41,10 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     code, wcode, rows, weight, bias = _check(x, weight, bias)
     n, width = rows.shape
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    with on_device(x.device) as stream:
-        _lib.check(_lib.load_ops().d1_norm_fwd(rows.data_ptr(), code, n, width, rows.stride(0), _ptr(weight), _ptr(bias),
-                                               wcode, eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), stream),
-                   'd1_norm_fwd')
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    call(_lib.load_ops().d1_norm_fwd, x.get_device(), rows.data_ptr(), code, n, width, rows.stride(0), _ptr(weight), _ptr(bias),
+         wcode, eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -50,22 +52,19 @@ def layer_norm_bwd(dy, x, weight, bias, mean, rstd):
     """-> (dx, dweight, dbias) from layer_norm_fwd's arguments and its mean and rstd; dweight and
     dbias are None where the weight or the bias is."""
     code, wcode, rows, weight, bias = _check(x, weight, bias)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    index, shape, (n, width) = x.get_device(), x.shape[:-1], rows.shape
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.get_device() != index:
         raise ValueError(f'dy must be {x.dtype} of shape {tuple(x.shape)} on {x.device}')
     drows = as_rows(dy)
-    mean = like(mean, x.shape[:-1], x.device, 'mean')
-    rstd = like(rstd, x.shape[:-1], x.device, 'rstd')
-    n, width = rows.shape
+    mean, rstd = like(mean, shape, index, 'mean'), like(rstd, shape, index, 'rstd')
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dw = None if weight is None else torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
     L = _lib.load_ops()
-    need = L.d1_norm_work_bytes(n, width, code) if dw is not None or db is not None else 0
+    need = 0 if dw is None and db is None else L.d1_norm_work_bytes(n, width, code)
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with on_device(x.device) as stream:
-        _lib.check(L.d1_norm_bwd(drows.data_ptr(), drows.stride(0), rows.data_ptr(), code, n, width, rows.stride(0),
-                                 _ptr(weight), wcode, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db),
-                                 _ptr(work), need, stream), 'd1_norm_bwd')
+    call(L.d1_norm_bwd, index, drows.data_ptr(), drows.stride(0), rows.data_ptr(), code, n, width, rows.stride(0),
+         _ptr(weight), wcode, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), need)
     return dx, dw, db
 
 

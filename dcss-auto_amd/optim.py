@@ -10,7 +10,7 @@ import struct
 import torch
 
 from . import _lib
-from .rows import on_device
+from .rows import call
 
 BLOCK = 256                         # elements of an 8-bit moment that share an exponent
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -58,39 +58,40 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
             raise ValueError(f'{name}: {len(given)} for {count} parameters')
     if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and max_grad_norm >= 0):
         raise ValueError('betas must be in [0, 1), eps and max_grad_norm not negative')
-    device = step.device
     if step.dtype != torch.int32 or step.shape != (8,) or not step.is_cuda or not step.is_contiguous():
         raise ValueError('step must be a contiguous int32 CUDA tensor of 8 elements')
-    moment = torch.uint8 if eight else torch.float32
+    index, moment = step.get_device(), torch.uint8 if eight else torch.float32
     words, held = [], []
     lr, weight_decay = _each(lr, count, 'lr'), _each(weight_decay, count, 'weight_decay')
     for i in range(count):
         p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
-        n, copy = p.numel(), None if copies is None else copies[i]
+        n = p.numel()
         if not g.is_contiguous():
             g = g.contiguous()
             held.append(g)
         ptype, gtype = _TYPES.get(p.dtype), _TYPES.get(g.dtype)
         if ptype is None or gtype is None:
             raise ValueError(f'tensor {i}: parameter and gradient must be fp32 or bf16, not {p.dtype} and {g.dtype}')
-        if m.dtype != moment or v.dtype != moment or not (g.numel() == m.numel() == v.numel() == n):
+        if m.dtype != moment or v.dtype != moment or not g.numel() == m.numel() == v.numel() == n:
             raise ValueError(f'tensor {i}: the gradient must have the size of the parameter, the moments too, in {moment}')
-        if not (p.device == g.device == m.device == v.device == device):
-            raise ValueError(f'tensor {i}: parameter, gradient and moments must be on {device}')
+        if not p.get_device() == g.get_device() == m.get_device() == v.get_device() == index:
+            raise ValueError(f'tensor {i}: parameter, gradient and moments must be on {step.device}')
         if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
             raise ValueError(f'tensor {i}: parameter and moments must be contiguous')
         if not (lr[i] >= 0 and weight_decay[i] >= 0):
             raise ValueError(f'tensor {i}: lr and weight_decay must not be negative')
-        if copy is not None and (copy.dtype != torch.bfloat16 or copy.numel() != n or not copy.is_contiguous()
-                                 or copy.device != device or ptype):
-            raise ValueError(f'tensor {i}: a copy is contiguous bf16 of the size of an fp32 parameter')
-        me = ve = 0
+        me = ve = copy = 0
+        if copies is not None and (c := copies[i]) is not None:
+            if c.dtype != torch.bfloat16 or c.numel() != n or not c.is_contiguous() or c.get_device() != index or ptype:
+                raise ValueError(f'tensor {i}: a copy is contiguous bf16 of the size of an fp32 parameter')
+            copy = c.data_ptr()
         if eight:
-            for e in (exps[0][i], exps[1][i]):
-                if e.dtype != torch.uint8 or e.numel() != moment_blocks(n) or not e.is_contiguous() or e.device != device:
+            me, ve = exps[0][i], exps[1][i]
+            for e in (me, ve):
+                if e.dtype != torch.uint8 or e.numel() != moment_blocks(n) or not e.is_contiguous() or e.get_device() != index:
                     raise ValueError(f'tensor {i}: exponents are contiguous uint8, one for each {BLOCK} elements')
-            me, ve = exps[0][i].data_ptr(), exps[1][i].data_ptr()
-        words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), me, ve, 0 if copy is None else copy.data_ptr(),
+            me, ve = me.data_ptr(), ve.data_ptr()
+        words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), me, ve, copy,
                   n, 0 if counters is None else counters[i], lr[i], weight_decay[i], 0 if lags is None else lags[i],
                   ptype, gtype)
     table = struct.pack('=' + _ENTRY * count, *words)
@@ -98,10 +99,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     L = _lib.load_ops()
     need = L.d1_adamw_work_bytes(table, count, C.byref(h)) if max_grad_norm > 0 else 0
     _lib.check(min(need, 0), 'd1_adamw_work_bytes')
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with on_device(device) as stream:
-        _lib.check(L.d1_adamw_step(table, count, C.byref(h), step.data_ptr(), work.data_ptr() if need else None, need,
-                                   stream), 'd1_adamw_step')
+    work = torch.empty(need, dtype=torch.uint8, device=step.device) if need else None
+    call(L.d1_adamw_step, index, table, count, C.byref(h), step.data_ptr(), work.data_ptr() if need else None, need)
 
 
 def read_moment(code, exp, signed, out=None):
@@ -114,9 +113,8 @@ def read_moment(code, exp, signed, out=None):
         out = torch.empty(code.shape, dtype=torch.float32, device=code.device)
     elif out.dtype != torch.float32 or out.numel() != n or not out.is_contiguous() or out.device != code.device:
         raise ValueError('out must be contiguous fp32 of the size of the codes, on their device')
-    with on_device(code.device) as stream:
-        _lib.check(_lib.load_ops().d1_adamw_read(code.data_ptr(), exp.data_ptr(), n, 1 if signed else 0, out.data_ptr(),
-                                                 stream), 'd1_adamw_read')
+    call(_lib.load_ops().d1_adamw_read, code.get_device(), code.data_ptr(), exp.data_ptr(), n, 1 if signed else 0,
+         out.data_ptr())
     return out
 
 

@@ -11,9 +11,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rows import as_rows, like, on_device, type_of
+from .rows import as_rows, call, like, type_of
 
 MAX_TOP, MAX_VOCAB = 64, 1 << 24
+REGISTER_VOCAB = 1024      # rows up to this need no scratch memory
 
 
 class TokenLogprobs(NamedTuple):
@@ -30,65 +31,61 @@ class TokenLogprobs(NamedTuple):
 
 
 def _check(logits, tokens, mask):
-    """-> (type code, logits as rows, tokens flat, mask's data pointer or None, mask's row stride, kept tensors)."""
-    code = type_of(logits, 'logits')
-    shape, vocab = logits.shape[:-1], logits.shape[-1]
+    """-> (logits as rows, tokens contiguous, mask as rows, its data pointer, its row stride)."""
+    vocab, index = logits.shape[-1], logits.get_device()
     if vocab > MAX_VOCAB:
         raise ValueError(f'logits: at most {MAX_VOCAB} entries a row')
-    tokens = like(tokens, shape, logits.device, 'tokens', torch.int64)
+    tokens = like(tokens, logits.shape[:-1], index, 'tokens', torch.int64)
     rows = as_rows(logits)
     if mask is None:
-        return code, rows, tokens, None, 0, None
-    if mask.dtype not in (torch.bool, torch.uint8) or mask.device != logits.device:
+        return rows, tokens, None, None, 0
+    if mask.dtype not in (torch.bool, torch.uint8) or mask.get_device() != index:
         raise ValueError('mask must be bool or uint8 on the device of the logits')
+    if mask.shape == logits.shape:
+        mask = as_rows(mask)
+        return rows, tokens, mask, mask.data_ptr(), mask.stride(0)
     if mask.shape == (vocab,):
         mask = mask.contiguous()
-        return code, rows, tokens, mask.data_ptr(), 0, mask
-    if mask.shape != logits.shape:
-        raise ValueError(f'mask must have the shape of the logits or of one row, not {tuple(mask.shape)}')
-    mask = as_rows(mask)
-    return code, rows, tokens, mask.data_ptr(), mask.stride(0), mask
+        return rows, tokens, mask, mask.data_ptr(), 0
+    raise ValueError(f'mask must have the shape of the logits or of one row, not {tuple(mask.shape)}')
 
 
 def _forward(logits, tokens, mask, top):
-    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= MAX_TOP or (logits.dim() and top > logits.shape[-1]):
+    code = type_of(logits, 'logits')
+    if type(top) is not int or not 0 <= top <= MAX_TOP or top > logits.shape[-1]:
         raise ValueError(f'top must be 0 to {MAX_TOP} and at most the number of entries, not {top}')
-    code, rows, tok, mask_ptr, mask_stride, held = _check(logits, tokens, mask)
-    shape, device = logits.shape[:-1], logits.device
-    n, vocab = rows.shape
-    out = torch.empty((4, n), dtype=torch.float32, device=device)   # logp, entropy, stats
-    logp, entropy, stats = out[0].view(shape), out[1].view(shape), out[2:].view(*shape, 2)
-    ids = top_logp = None
+    rows, tok, mask, mask_ptr, mask_stride = _check(logits, tokens, mask)
+    index, (n, vocab) = logits.get_device(), rows.shape
+    logp = torch.empty_like(tok, dtype=torch.float32)
+    entropy = torch.empty_like(logp)
+    stats = logp.new_empty((*logp.shape, 2))
+    ids = top_logp = ids_ptr = top_ptr = work = None
     if top:
-        ids = torch.empty((*shape, top), dtype=torch.int64, device=device)
-        top_logp = torch.empty((*shape, top), dtype=torch.float32, device=device)
+        ids, top_logp = tok.new_empty((*logp.shape, top)), logp.new_empty((*logp.shape, top))
+        ids_ptr, top_ptr = ids.data_ptr(), top_logp.data_ptr()
     L = _lib.load_ops()
-    need = L.d1_tokens_work_bytes(n, vocab, top)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with on_device(device) as stream:
-        _lib.check(L.d1_tokens_fwd(rows.data_ptr(), code, n, vocab, rows.stride(0), tok.data_ptr(), mask_ptr, mask_stride,
-                                   top, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-                                   ids.data_ptr() if top else None, top_logp.data_ptr() if top else None,
-                                   work.data_ptr() if need else None, need, stream), 'd1_tokens_fwd')
+    need = L.d1_tokens_work_bytes(n, vocab, top) if vocab > REGISTER_VOCAB else 0
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    call(L.d1_tokens_fwd, index, rows.data_ptr(), code, n, vocab, rows.stride(0), tok.data_ptr(), mask_ptr, mask_stride, top,
+         logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), ids_ptr, top_ptr, work.data_ptr() if need else None, need)
     return TokenLogprobs(logp, entropy, ids, top_logp, stats)
 
 
 def token_logprobs_bwd(logits, tokens, result, dlogp, dentropy, mask=None):
     """The gradient of the logits (their type, contiguous) from those of logp and entropy (fp32 of
     their shapes; either may be None: zero); `result` is token_logprobs' of the same arguments."""
-    code, rows, tok, mask_ptr, mask_stride, held = _check(logits, tokens, mask)
-    shape, device = logits.shape[:-1], logits.device
-    stats = like(result.stats, (*shape, 2), device, 'result.stats')
-    entropy = like(result.entropy, shape, device, 'result.entropy')
-    dlogp = None if dlogp is None else like(dlogp, shape, device, 'dlogp')
-    dentropy = None if dentropy is None else like(dentropy, shape, device, 'dentropy')
-    n, vocab = rows.shape
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    with on_device(device) as stream:
-        _lib.check(_lib.load_ops().d1_tokens_bwd(
-            rows.data_ptr(), code, n, vocab, rows.stride(0), tok.data_ptr(), mask_ptr, mask_stride, stats.data_ptr(),
-            entropy.data_ptr(), None if dlogp is None else dlogp.data_ptr(),
-            None if dentropy is None else dentropy.data_ptr(), dlogits.data_ptr(), stream), 'd1_tokens_bwd')
+    code = type_of(logits, 'logits')
+    rows, tok, mask, mask_ptr, mask_stride = _check(logits, tokens, mask)
+    shape, index, (n, vocab) = tok.shape, logits.get_device(), rows.shape
+    stats = like(result.stats, (*shape, 2), index, 'result.stats')
+    entropy = like(result.entropy, shape, index, 'result.entropy')
+    dlogp = None if dlogp is None else like(dlogp, shape, index, 'dlogp')
+    dentropy = None if dentropy is None else like(dentropy, shape, index, 'dentropy')
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    call(_lib.load_ops().d1_tokens_bwd, index, rows.data_ptr(), code, n, vocab, rows.stride(0), tok.data_ptr(), mask_ptr,
+         mask_stride, stats.data_ptr(), entropy.data_ptr(), None if dlogp is None else dlogp.data_ptr(),
+         None if dentropy is None else dentropy.data_ptr(), dlogits.data_ptr())
     return dlogits
 
 
