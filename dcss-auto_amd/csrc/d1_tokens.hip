@@ -9,7 +9,7 @@
 //
 // Rows of up to 1,024 entries stay in the registers of 4 to 64 lanes (k_tokens_small). A longer row
 // is cut into segments of one workgroup each, as many as fill the card when rows are few
-// (k_tokens_part), and k_tokens_join adds the segments' m, S, E and merges their best entries.
+// (k_tokens_part), and where there are several k_tokens_join adds their m, S, E and merges their best entries.
 //
 // Alternatives are ordered by a 64-bit key: the value's order-preserving bits, then the
 // complemented index, so keys are distinct and the lowest index wins among equal values.
@@ -80,17 +80,22 @@ __device__ __forceinline__ void put_row(const Args &a, int64_t row, Sums t, floa
     a.stats[2 * row] = base;
     a.stats[2 * row + 1] = t.s;
 }
-// what one lane writes of a long row once its sums are whole
+// A long row's token and its entry, asked for before the row is read (two loads, one after the other).
+struct Given {
+    int64_t tok;
+    float x;
+};
 template <class T>
-__device__ __forceinline__ void finish(const Args &a, int64_t row, Sums t) {
+__device__ __forceinline__ Given given_of(const Args &a, int64_t row) {
+    Given g = {a.tokens[row], -INFINITY};
+    if (g.tok >= 0 && g.tok < a.vocab && (!a.mask || a.mask[row * a.mask_stride + g.tok]))
+        g.x = (float)((const T *)a.logits)[row * a.stride + g.tok];
+    return g;
+}
+// what one lane writes of a long row once its sums are whole
+__device__ __forceinline__ void finish(const Args &a, int64_t row, Sums t, Given g) {
     const float base = finite_base(t.m), ls = logf(t.s);
-    const int64_t tok = a.tokens[row];
-    if (tok < 0 || tok >= a.vocab) {
-        a.logp[row] = logp_of_none(tok);
-    } else {
-        const bool in = !a.mask || a.mask[row * a.mask_stride + tok];
-        a.logp[row] = logp_of(in ? (float)((const T *)a.logits)[row * a.stride + tok] : -INFINITY, t, base, ls);
-    }
+    a.logp[row] = g.tok < 0 || g.tok >= a.vocab ? logp_of_none(g.tok) : logp_of(g.x, t, base, ls);
     put_row(a, row, t, base, ls);
 }
 __device__ __forceinline__ void put_top(const Args &a, int64_t row, int k, uint64_t key, float base, float ls, float s) {
@@ -192,13 +197,14 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
 
 // ---- longer rows: segments
 
-// Threads of a workgroup and the vectors of 16 bytes that a thread takes at once.
-constexpr int PART = 256, AT_ONCE = 4, WAVES = PART / 64, KEEP = 256;
+// Vectors of 16 bytes that a thread takes at once: two; four (512 x 50,001 fp16 31 us against 28, 4,096 x
+// 131,072 bf16 210 against 192) and eight (222) cost more waves than they hide.
+constexpr int AT_ONCE = 2, KEEP = 512, ROUND = 4;
 
 struct Parts {
     float *sums;              // [rows][splits][4]: m, s, e
     uint64_t *keys;           // [rows][splits][top]
-    int splits, seg;          // segments a row, entries of one (a multiple of PART * VEC)
+    int splits, seg;          // segments a row, entries of one (a multiple of a workgroup's vectors)
 };
 
 // VEC allowed entries of a segment at offset i (n entries in all); what is outside reads -inf
@@ -222,6 +228,14 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+template <int PART>
+__device__ __forceinline__ void block_sync() {
+    if (PART == 64)
+        wave_sync();
+    else
+        __syncthreads();
+}
+
 // A wave's list of keys in LDS: takes keys in any order, keeps at least the `top` largest seen.
 struct TopList {
     uint64_t *list, *sorted;     // KEEP and D1_TOKENS_MAX_TOP keys
@@ -230,58 +244,65 @@ struct TopList {
 
     // the `top` largest to `sorted`, falling; places without a key are 0. A key's place is the number of larger ones.
     __device__ __forceinline__ void sort(int lane) {
-        uint64_t mine[KEEP / 64];
-        int larger[KEEP / 64] = {};
         wave_sync();
-#pragma unroll
-        for (int i = 0; i < KEEP / 64; i++) mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
-        for (int j = 0; j < count; j++) {
-            const uint64_t key = list[j];
-#pragma unroll
-            for (int i = 0; i < KEEP / 64; i++)
-                if (i * 64 < count) larger[i] += key > mine[i];
-        }
         if (lane < top) sorted[lane] = 0;
         wave_sync();
+        for (int i0 = 0; i0 < count; i0 += 64) {
+            const uint64_t mine = i0 + lane < count ? list[i0 + lane] : 0;
+            int larger = 0;
+            for (int j0 = 0; j0 < count; j0 += 8) {
+                uint64_t key[8];
 #pragma unroll
-        for (int i = 0; i < KEEP / 64; i++)
-            if (mine[i] && larger[i] < top) sorted[larger[i]] = mine[i];
+                for (int j = 0; j < 8; j++) key[j] = list[j0 + j];     // KEEP is a multiple of 8
+#pragma unroll
+                for (int j = 0; j < 8; j++) larger += j0 + j < count && key[j] > mine;
+            }
+            if (mine && larger < top) sorted[larger] = mine;
+        }
         wave_sync();
     }
     __device__ __forceinline__ void shrink(int lane) {
         sort(lane);
         if (lane < top) list[lane] = sorted[lane];
         below = sorted[top - 1];
-        count = top;
+        count = count < top ? count : top;
         wave_sync();
     }
-    // one key a lane (0: none); the whole wave calls
-    __device__ __forceinline__ void add(uint64_t key, int lane) {
-        const uint64_t take = __ballot(key > below);
-        if (!take) return;
-        if (key > below) list[count + __popcll(take & ((1ull << lane) - 1))] = key;
-        count += __popcll(take);
-        if (count > KEEP - 64) shrink(lane);
+    // ROUND keys a lane (0: none); the whole wave calls
+    __device__ __forceinline__ void add(const uint64_t (&key)[ROUND], int lane) {
+#pragma unroll
+        for (int u = 0; u < ROUND; u++) {
+            const uint64_t take = __ballot(key[u] > below);
+            if (key[u] > below) list[count + __popcll(take & ((1ull << lane) - 1))] = key[u];
+            count += __popcll(take);
+        }
+        if (count > KEEP - 64 * ROUND) shrink(lane);
     }
 };
 
-// the k-th largest (k <= 64) of the lanes' words: bit by bit from the top, as many lanes as k stay above
-__device__ __forceinline__ uint32_t kth_word(uint32_t word, int k) {
+// a bound on the k-th largest of the lanes' words (N a lane) from below, exact in its first 18 bits: bit by bit from the top,
+// as long as k words stay at or above it
+template <int N>
+__device__ __forceinline__ uint32_t kth_word(const uint32_t (&word)[N], int k) {
     uint32_t floor = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 0; bit--) {
+    for (int bit = 31; bit >= 14; bit--) {
         const uint32_t at = floor | (1u << bit);
-        if (__popcll(__ballot(word >= at)) >= k) floor = at;
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) above += __popcll(__ballot(word[i] >= at));
+        if (above >= k) floor = at;
     }
     return floor;
 }
 
-template <class T, bool MASK, bool TOP>
+template <class T, int PART, bool MASK, bool TOP>
 __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts parts) {
-    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
+    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC, WAVES = PART / 64;
     __shared__ Sums wave_sums[WAVES];
-    __shared__ uint32_t wave_floor[WAVES];
+    __shared__ uint32_t words[TOP ? PART : 1];
     __shared__ int wave_count[WAVES];
+    __shared__ uint8_t lanes_of[WAVES][64];
     __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? KEEP : 1], sorted[TOP ? WAVES : 1][TOP ? D1_TOKENS_MAX_TOP : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t units = a.rows * parts.splits;
@@ -292,6 +313,8 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
         const T *x = (const T *)a.logits + row * a.stride + begin;
         const uint8_t *mask = MASK ? a.mask + row * a.mask_stride + begin : nullptr;
         Sums t = {-INFINITY, 0.f, 0.f};
+        Given given = {-1, 0.f};
+        if (parts.splits == 1 && threadIdx.x == 0) given = given_of<T>(a, row);
         for (int i = threadIdx.x * VEC; i < n; i += STEP * AT_ONCE) {
             float v[AT_ONCE][VEC];
 #pragma unroll
@@ -315,26 +338,23 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
                 }
         }
         const Sums wave_sum = lanes_joined<64>(t);
-        uint32_t wave_kth = 0, most = 0;     // of TOP: most is a word that no entry of the lane passes
+        uint32_t most = 0;               // of TOP: a word that no entry of the lane passes
         if (TOP) {
             // The maximum leaves NaN out, which is the largest of all; the sum knows of it (or of +inf).
             // A lane without an entry above -inf may still hold allowed ones there: it counts as one.
             const bool odd = t.s != t.s;
             const uint32_t word = (int)threadIdx.x * VEC >= n ? 0 : odd && t.m != INFINITY ? 0xFFFFFFFEu : ordered(t.m);
-            wave_kth = kth_word(word, a.top);
+            words[threadIdx.x] = word;
             most = odd ? 0xFFFFFFFEu : word;
         }
-        if (lane == 0) {
-            wave_sums[wave] = wave_sum;
-            if (TOP) wave_floor[wave] = wave_kth;
-        }
-        __syncthreads();
+        if (lane == 0) wave_sums[wave] = wave_sum;
+        block_sync<PART>();
         Sums all = wave_sums[0];
 #pragma unroll
         for (int w = 1; w < WAVES; w++) all = joined(all, wave_sums[w]);
         if (threadIdx.x == 0) {
             if (parts.splits == 1) {
-                finish<T>(a, row, all);
+                finish(a, row, all, given);
             } else {
                 float *o = parts.sums + unit * 4;
                 o[0] = all.m;
@@ -343,30 +363,46 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
             }
         }
         if (TOP) {
-            // At least `top` lanes of some wave hold an entry of this word or more, so the segment's best are
-            // no smaller; only lanes that hold such an entry are looked through again, by their whole wave.
-            uint32_t floor = wave_floor[0];
+            // At least `top` lanes hold an entry of this word or more, so the segment's best are no smaller;
+            // only lanes that hold such an entry are looked through again, by their whole wave.
+            uint32_t word[WAVES];
 #pragma unroll
-            for (int w = 1; w < WAVES; w++) floor = floor > wave_floor[w] ? floor : wave_floor[w];
+            for (int w = 0; w < WAVES; w++) word[w] = words[w * 64 + lane];
+            const uint32_t floor = kth_word<WAVES>(word, a.top);
             TopList best = {found[wave], sorted[wave], a.top, 0, 0};
             const int each = ((n + STEP - 1) / STEP) * VEC;      // entries of a lane
-            for (uint64_t left = __ballot(most && most >= floor); left; left &= left - 1) {
-                const int who = wave * 64 + __builtin_ctzll(left);
-                for (int q0 = 0; q0 < each; q0 += 64) {
-                    const int q = q0 + lane, at = (q / VEC * PART + who) * VEC + q % VEC;
-                    uint64_t key = 0;
-                    if (q < each && at < n && (!MASK || mask[at])) key = key_of((float)x[at], begin + at);
-                    best.add((uint32_t)(key >> 32) >= floor ? key : 0, lane);
+            const bool mine = most && most >= floor;
+            const uint64_t open = __ballot(mine);
+            uint8_t *who = lanes_of[wave];                       // the lanes to look through, in order
+            if (mine) who[__popcll(open & ((1ull << lane) - 1))] = (uint8_t)lane;
+            wave_sync();
+            const int total = __popcll(open) * each;
+            for (int q0 = 0; q0 < total; q0 += ROUND * 64) {
+                uint64_t key[ROUND];
+#pragma unroll
+                for (int u = 0; u < ROUND; u++) {                // all loads in flight
+                    const int q = q0 + u * 64 + lane, k = q / each, r = q - k * each;
+                    key[u] = 0;
+                    if (q < total) {
+                        const int at = (r / VEC * PART + wave * 64 + who[k]) * VEC + r % VEC;
+                        if (at < n && (!MASK || mask[at])) key[u] = key_of((float)x[at], begin + at);
+                        if ((uint32_t)(key[u] >> 32) < floor) key[u] = 0;
+                    }
                 }
+                best.add(key, lane);
             }
-            if (best.count > KEEP / WAVES) best.shrink(lane);
-            if (lane == 0) wave_count[wave] = best.count;
-            __syncthreads();
-            if (wave == 0) {       // the waves' lists, KEEP / WAVES keys each at most
-                for (int w = 1; w < WAVES; w++) {
-                    const int more = wave_count[w];
-                    if (lane < more) found[0][best.count + lane] = found[w][lane];
-                    best.count += more;
+            if (WAVES > 1) {
+                if (best.count > 64) best.shrink(lane);
+                if (lane == 0) wave_count[wave] = best.count;
+                block_sync<PART>();
+            }
+            if (wave == 0) {       // the waves' lists, 64 keys each at most
+#pragma unroll
+                for (int w0 = 1; w0 < WAVES; w0 += ROUND) {
+                    uint64_t key[ROUND];
+#pragma unroll
+                    for (int u = 0; u < ROUND; u++) key[u] = w0 + u < WAVES && lane < wave_count[w0 + u] ? found[w0 + u][lane] : 0;
+                    best.add(key, lane);
                 }
                 best.sort(lane);
                 if (parts.splits == 1) {
@@ -376,7 +412,7 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
                 }
             }
         }
-        __syncthreads();
+        block_sync<PART>();
     }
 }
 
@@ -393,27 +429,29 @@ __global__ __launch_bounds__(64) void k_tokens_join(const Args a, const Parts pa
             t = {p[0], p[1], p[2]};
         }
         const uint64_t *keys = parts.keys + (row * parts.splits + lane) * a.top;
-        const uint64_t head = mine && a.top ? keys[0] : 0;
+        constexpr int FIRST = 2 * ROUND;
+        uint64_t key[FIRST];             // the first of the lane's list
+#pragma unroll
+        for (int j = 0; j < FIRST; j++) key[j] = mine && j < a.top ? keys[j] : 0;
+        const Given given = given_of<T>(a, row);
         t = lanes_joined<64>(t);
-        if (lane == 0) finish<T>(a, row, t);
+        if (lane == 0) finish(a, row, t, given);
         if (a.top) {
-            // the top-th largest head bounds the row's best from below
-            const uint32_t floor = kth_word((uint32_t)(head >> 32), a.top);
-            const bool open = head && (uint32_t)(head >> 32) >= floor;
+            // the top-th largest of what is read so far bounds the row's best from below
+            uint32_t word[FIRST];
+#pragma unroll
+            for (int j = 0; j < FIRST; j++) word[j] = (uint32_t)(key[j] >> 32);
+            const uint32_t floor = kth_word<FIRST>(word, a.top);
             TopList best = {found, sorted, a.top, 0, 0};
-            best.add(open ? head : 0, lane);
-            for (int k0 = 1; k0 < a.top; k0 += 4) {
-                uint64_t key[4];
+            uint64_t four[ROUND];
+            for (int k0 = 0; k0 < a.top; k0 += ROUND) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) key[j] = open && k0 + j < a.top ? keys[k0 + j] : 0;
-                uint64_t some = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if ((uint32_t)(key[j] >> 32) < floor) key[j] = 0;
-                    some |= __ballot(key[j] > best.below);
-                    best.add(key[j], lane);
+                for (int j = 0; j < ROUND; j++) {
+                    four[j] = k0 == 0 ? key[j] : k0 == ROUND ? key[ROUND + j] : mine && four[ROUND - 1] && k0 + j < a.top ? keys[k0 + j] : 0;
+                    if ((uint32_t)(four[j] >> 32) < floor) four[j] = 0;
                 }
-                if (!some) break;        // the lists fall: nothing larger follows
+                best.add(four, lane);
+                if (!__ballot(four[ROUND - 1] > best.below)) break;     // the lists fall: nothing larger follows
             }
             best.sort(lane);
             if (lane < a.top) put_top(a, row, lane, sorted[lane], finite_base(t.m), logf(t.s), t.s);
@@ -482,9 +520,17 @@ __global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
     }
 }
 
-template <class T, bool MASK>
-__global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
-    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
+// PAST: written past the caches
+template <class T, int VEC>
+__device__ __forceinline__ void store_past(T *p, const Pack<T, VEC> &a) {
+    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    d1f::u32x4 w;
+    __builtin_memcpy(&w, &a, sizeof a);
+    __builtin_nontemporal_store(w, (u32x4u *)p);
+}
+template <class T, bool MASK, bool PAST>
+__global__ __launch_bounds__(256) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
+    constexpr int VEC = 16 / (int)sizeof(T), STEP = 256 * VEC;
     const int64_t units = a.rows * splits;
     for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int64_t row = unit / splits;
@@ -512,20 +558,27 @@ __global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int split
                     const float d = grad_of(q, (float)p[u].v[j]) + (begin + i + j == q.tok ? q.g : 0.f);
                     o.v[j] = (T)(!MASK || w[u].v[j] ? d : 0.f);
                 }
-                store_part<T, VEC>(out + i, n - i, o);
+                if (PAST && n - i >= VEC)
+                    store_past<T, VEC>(out + i, o);
+                else
+                    store_part<T, VEC>(out + i, n - i, o);
             }
         }
     }
 }
 
-// Segments of a long row: enough workgroups for the card (4 for each of 256 CUs) where rows are few,
-// none shorter than one vector a thread, at most 64 (the join's lanes).
+// Threads of a workgroup for long rows: a wave each where there are rows enough for all CUs and a lane's share of
+// a row is short, since with alternatives a workgroup's search costs as much for few entries as for many
+// (8,192 x 1,500 bf16 with 5 alternatives 14.7 us on 64 threads, 33.7 on 256; none 10.0 and 16.5; 16,384 x 9,000 with
+// 5 80 and 107). Elsewhere 256 (16,384 x 20,000 185 us on 64 and 175 on 256; 1,024 x 9,000 17.0 and 10.4).
+inline int part_of(int64_t rows, int vocab) { return rows >= 2048 && vocab <= 12288 ? 64 : 256; }
+// Segments of a row: as many as make about six workgroups for each of the 256 CUs where rows are fewer than that, none
+// shorter than one vector a thread, at most 64 (the join's lanes). 512 x 50,001 fp16 with 5 alternatives: 28.0 us at
+// 512 workgroups, 25.6 at 1,536, 28.9 at 4,096; 300 x 131,072 bf16 with 20: 82 at 300, 39 at 1,200, 41 at 4,800.
 inline int splits_of(int64_t rows, int vocab, int type, int &seg) {
-    const int step = PART * (type == D1_FP32 ? 4 : 8);
-    const int most = (vocab + step - 1) / step;
-    int64_t want = (1024 + rows - 1) / rows;
-    if (want > 64) want = 64;
-    int splits = (int)(want < most ? want : most);
+    const int step = part_of(rows, vocab) * (type == D1_FP32 ? 4 : 8);
+    const int64_t want = (1536 + rows - 1) / rows, most = (vocab + step - 1) / step, few = want < 64 ? want : 64;
+    const int splits = (int)(few < most ? few : most);
     seg = ((vocab + splits - 1) / splits + step - 1) / step * step;
     return (vocab + seg - 1) / seg;
 }
@@ -560,19 +613,29 @@ template <class T, bool MASK>
 int fwd(const Args &a, const Parts &p, hipStream_t s) {
     if (a.vocab <= SMALL_VOCAB) return small_fwd<T, MASK>(a, s);
     const unsigned grid = blocks_of(a.rows * p.splits);
-    if (a.top)
-        k_tokens_part<T, MASK, true><<<grid, PART, 0, s>>>(a, p);
-    else
-        k_tokens_part<T, MASK, false><<<grid, PART, 0, s>>>(a, p);
+    const int part = part_of(a.rows, a.vocab);
+#define X(P) \
+    if (part == P && a.top) k_tokens_part<T, P, MASK, true><<<grid, P, 0, s>>>(a, p); \
+    if (part == P && !a.top) k_tokens_part<T, P, MASK, false><<<grid, P, 0, s>>>(a, p);
+    X(64) X(256)
+#undef X
     const int e = (int)hipGetLastError();
     if (e || p.splits == 1) return e;
     k_tokens_join<T><<<blocks_of(a.rows), 64, 0, s>>>(a, p);
     return (int)hipGetLastError();
 }
 template <class T, bool MASK>
-int bwd(const BackArgs &a, int splits, int seg, hipStream_t s) {
+int bwd(const BackArgs &a, hipStream_t s) {
     if (a.vocab <= SMALL_VOCAB) return small_bwd<T, MASK>(a, s);
-    k_tokens_bwd<T, MASK><<<blocks_of(a.rows * splits), PART, 0, s>>>(a, splits, seg);
+    // Outputs that no cache of a CU's chiplet can hold (8 x 4 MB) are written past them, and a workgroup takes two rounds of
+    // them (4,096 x 131,072 bf16: 359 us, 391 with one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2)
+    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > (32 << 20);
+    const int seg = (past ? 2 : 1) * AT_ONCE * 256 * (16 / (int)sizeof(T)), splits = (a.vocab + seg - 1) / seg;
+    const unsigned grid = blocks_of(a.rows * splits);
+    if (past)
+        k_tokens_bwd<T, MASK, true><<<grid, 256, 0, s>>>(a, splits, seg);
+    else
+        k_tokens_bwd<T, MASK, false><<<grid, 256, 0, s>>>(a, splits, seg);
     return (int)hipGetLastError();
 }
 
@@ -622,8 +685,6 @@ extern "C" int d1_tokens_bwd(const void *logits, int type, int64_t rows, int voc
     if (!token_args(type, rows, vocab, stride, mask_stride)) return D1_E_ARG;
     if (rows == 0) return 0;
     if (!logits || !tokens || !stats || !dlogits || (dentropy && !entropy)) return D1_E_ARG;
-    int seg = 0;
-    const int splits = vocab <= SMALL_VOCAB ? 1 : splits_of(rows, vocab, type, seg);
     const BackArgs a{logits, rows, stride, vocab, tokens, mask, mask_stride, stats, entropy, dlogp, dentropy, dlogits};
-    D1O_TOKEN_TYPES(bwd, a, splits, seg, (hipStream_t)stream)
+    D1O_TOKEN_TYPES(bwd, a, (hipStream_t)stream)
 }
