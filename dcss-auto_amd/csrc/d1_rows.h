@@ -43,6 +43,30 @@ __device__ __forceinline__ void store_part(T *p, int n, const Pack<T, N> &a) {
         if (i < n) p[i] = a.v[i];
 }
 
+// the same past the caches, for outputs that are larger than the L2s of all chiplets (8 x 4 MB) and so
+// would only push out what is read
+constexpr int64_t PAST_BYTES = 32 << 20;
+template <class T, int N>
+__device__ __forceinline__ void store_past(T *p, const Pack<T, N> &a) {
+    constexpr int WORDS = (int)sizeof(a) / 4;
+    static_assert(WORDS == 1 || WORDS == 2 || WORDS == 4, "one store instruction");
+    if constexpr (WORDS == 1) {
+        typedef uint32_t anywhere __attribute__((aligned(1)));
+        __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, a), (anywhere *)p);
+    } else {
+        typedef uint32_t words __attribute__((ext_vector_type(WORDS)));
+        typedef words anywhere __attribute__((aligned(1)));
+        __builtin_nontemporal_store(__builtin_bit_cast(words, a), (anywhere *)p);
+    }
+}
+template <bool PAST, class T, int N>
+__device__ __forceinline__ void put_part(T *p, int n, const Pack<T, N> &a) {
+    if (PAST && n >= N)
+        store_past<T, N>(p, a);
+    else
+        store_part<T, N>(p, n, a);
+}
+
 // op over aligned groups of LANES lanes (1, 2, 4 ... 64); every lane gets the same result: partners
 // at distance 1, 2, 4, 8 through DPP, 16 and 32 through the lane-swap moves. After the steps before,
 // the lanes of a quad (of a half row) hold equal values, so a mirror reads the other quad's (half's).

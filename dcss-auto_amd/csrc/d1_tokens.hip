@@ -520,14 +520,6 @@ __global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
     }
 }
 
-// PAST: written past the caches
-template <class T, int VEC>
-__device__ __forceinline__ void store_past(T *p, const Pack<T, VEC> &a) {
-    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
-    d1f::u32x4 w;
-    __builtin_memcpy(&w, &a, sizeof a);
-    __builtin_nontemporal_store(w, (u32x4u *)p);
-}
 template <class T, bool MASK, bool PAST>
 __global__ __launch_bounds__(256) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
     constexpr int VEC = 16 / (int)sizeof(T), STEP = 256 * VEC;
@@ -558,10 +550,7 @@ __global__ __launch_bounds__(256) void k_tokens_bwd(const BackArgs a, int splits
                     const float d = grad_of(q, (float)p[u].v[j]) + (begin + i + j == q.tok ? q.g : 0.f);
                     o.v[j] = (T)(!MASK || w[u].v[j] ? d : 0.f);
                 }
-                if (PAST && n - i >= VEC)
-                    store_past<T, VEC>(out + i, o);
-                else
-                    store_part<T, VEC>(out + i, n - i, o);
+                put_part<PAST>(out + i, n - i, o);
             }
         }
     }
@@ -627,9 +616,8 @@ int fwd(const Args &a, const Parts &p, hipStream_t s) {
 template <class T, bool MASK>
 int bwd(const BackArgs &a, hipStream_t s) {
     if (a.vocab <= SMALL_VOCAB) return small_bwd<T, MASK>(a, s);
-    // Outputs that no cache of a CU's chiplet can hold (8 x 4 MB) are written past them, and a workgroup takes two rounds of
-    // them (4,096 x 131,072 bf16: 359 us, 391 with one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2)
-    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > (32 << 20);
+    // Large outputs go past the caches, and a workgroup takes two rounds of them (4,096 x 131,072 bf16: 359 us, 391 with one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2)
+    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > PAST_BYTES;
     const int seg = (past ? 2 : 1) * AT_ONCE * 256 * (16 / (int)sizeof(T)), splits = (a.vocab + seg - 1) / seg;
     const unsigned grid = blocks_of(a.rows * splits);
     if (past)
