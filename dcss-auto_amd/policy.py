@@ -12,6 +12,8 @@ import torch
 from torch import nn
 
 from . import _lib
+from .norm import LayerNorm
+from .tokens import token_logprobs
 
 OBS = 1800
 N_ACTIONS = 16
@@ -61,6 +63,45 @@ class Policy(nn.Module):
             self._packed_val = (pack_weights(w1, w2, w3), b1, b2, b3)
             self._packed_key = key
         return self._packed_val
+
+
+class NormPolicy(nn.Module):
+    """Policy with a layer norm behind each trunk layer, of any width and number of actions; it trains
+    with ModulePPO (ppo.py), through the layer norm and log-probability kernels."""
+
+    def __init__(self, width=256, n_actions=N_ACTIONS, obs=OBS, seed=0):
+        super().__init__()
+        self.l1, self.n1 = nn.Linear(obs, width), LayerNorm(width)
+        self.l2, self.n2 = nn.Linear(width, width), LayerNorm(width)
+        self.head = nn.Linear(width, n_actions + 1)   # logits | value
+        self.n_actions = n_actions
+        g = torch.Generator().manual_seed(seed)
+        for layer in (self.l1, self.l2, self.head):
+            with torch.no_grad():
+                layer.weight.copy_(torch.randn(layer.weight.shape, generator=g) * 0.02)
+                layer.bias.zero_()
+
+    def forward(self, obs_u8):
+        """obs uint8 [B, 15, 15, 8] (or [B, 1800]) -> (fp32 logits [B, A], fp32 value [B])."""
+        dtype = self.l1.weight.dtype
+        if obs_u8.is_cuda and torch.is_autocast_enabled('cuda'):
+            dtype = torch.get_autocast_dtype('cuda')
+        h = torch.relu(self.n1(self.l1(widen(obs_u8.reshape(obs_u8.shape[0], -1), dtype))))
+        h = torch.relu(self.n2(self.l2(h)))
+        out = self.head(h).float()
+        return out[:, :self.n_actions], out[:, self.n_actions]
+
+    def evaluate(self, obs_u8, actions, mask=None):
+        """(log probability, entropy, value), fp32 [B], of the actions that were taken; `mask`: legal actions."""
+        logits, value = self(obs_u8)
+        r = token_logprobs(logits, actions, mask=mask)
+        return r.logp, r.entropy, value
+
+    def act(self, obs_u8, seed, t):
+        """Counter-RNG sample at step t -> (action number, env action, log probability, value)."""
+        logits, value = self(obs_u8)
+        action, logp = sample(logits, seed, t)
+        return action, action, logp, value
 
 
 def pack_weights(w1, w2, w3, out=None):
@@ -229,6 +270,25 @@ class ARPolicy(nn.Module):
         z = torch.tanh(ht[:, None, :] + ev[None])                                       # [B, 8, 64]
         targets = self.t2(z)                                                             # [B, 8, 25]
         return self.verb(h).float(), targets.float(), self.value(h).float().squeeze(-1)
+
+    def evaluate(self, obs_u8, actions):
+        """(log probability, entropy, value), fp32 [B], of actions numbered verb * 25 + target: ARDistribution's
+        sums, one row of token_logprobs for the verb and one for each verb's targets (padding but for the
+        verb that was taken)."""
+        verbs, targets, value = self(obs_u8)
+        verb, target = actions // N_TARGETS, actions % N_TARGETS
+        v = token_logprobs(verbs, verb)
+        taken = torch.arange(N_VERBS, device=verb.device) == verb[:, None]
+        t = token_logprobs(targets, torch.where(taken, target[:, None], -1))
+        p = torch.softmax(verbs, -1)
+        return v.logp + t.logp.sum(-1), v.entropy + (p * t.entropy).sum(-1), value
+
+    def act(self, obs_u8, seed, t):
+        """Two-stage counter-RNG sample at step t -> (action number for evaluate, env action, log
+        probability, value)."""
+        verbs, targets, value = self(obs_u8)
+        verb, target, action, logp = sample_ar(verbs, targets, seed, t)
+        return verb.to(torch.int64) * N_TARGETS + target, action, logp, value
 
     def packed(self, refresh=False):
         """(packed weights, b1, b2, b3, bt) for policy_fwd_sample_ar (bf16 parameters only),

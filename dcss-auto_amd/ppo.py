@@ -11,6 +11,7 @@ autocast while the optimizer keeps fp32 master weights; GAE is the HIP kernel.
 import torch
 
 from . import policy as P
+from .optim import AdamW
 
 OBS = P.OBS
 
@@ -76,6 +77,43 @@ class PPO:
             for inds in perm.split(self.minibatch):
                 last = self.minibatch_step(obs.index_select(0, inds), actions[inds], logp[inds], adv[inds],
                                            ret[inds])
+        return last
+
+
+class ModulePPO(PPO):
+    """PPO for any policy module with evaluate(obs, actions) -> (log probability, entropy, value), such as
+    NormPolicy and ARPolicy: the module's layers by autograd, its log probabilities, layer norms and the
+    update itself by this package's kernels. Interface and loss are PPO's; the optimizer is AdamW over all
+    tensors at once (state_bits: 32 or 8) with the gradient clip in the same call. Nothing waits
+    for the device between minibatches: a minibatch whose gradient norm is not finite changes nothing,
+    and `update` raises at its end."""
+
+    def __init__(self, model, lr=3e-4, eps=1e-5, clip=0.2, vcoef=0.5, ecoef=0.01, max_grad_norm=0.5, epochs=4,
+                 minibatch=8192, gamma=0.99, lam=0.95, autocast=True, weight_decay=0.0, state_bits=32, seed=0):
+        if not max_grad_norm > 0:
+            raise ValueError('ModulePPO needs a gradient clip: its norm is what tells a non-finite loss')
+        super().__init__(model, lr=lr, eps=eps, clip=clip, vcoef=vcoef, ecoef=ecoef, max_grad_norm=max_grad_norm,
+                         epochs=epochs, minibatch=minibatch, gamma=gamma, lam=lam, autocast=autocast)
+        self.opt = AdamW(model.parameters(), lr=lr, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                         max_grad_norm=max_grad_norm, seed=seed)
+
+    def minibatch_step(self, obs, actions, old_logp, adv, ret):
+        with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
+            logp, entropy, value = self.model.evaluate(obs, actions)
+        ratio = torch.exp(logp - old_logp)
+        pg = -torch.minimum(ratio * adv, ratio.clamp(1 - self.clip, 1 + self.clip) * adv).mean()
+        vloss = 0.5 * (value.float() - ret).square().mean()
+        loss = pg + self.vcoef * vloss - self.ecoef * entropy.mean()
+        self.opt.zero_grad(set_to_none=True)
+        loss.backward()
+        self.opt.step()
+        return loss.detach()
+
+    def update(self, buf, generator=None):
+        before = self.opt.skipped_steps()
+        last = super().update(buf, generator)
+        if self.opt.skipped_steps() > before:
+            raise RuntimeError('Non-finite PPO loss')
         return last
 
 

@@ -248,3 +248,45 @@ class Trainer:
         t, r = terminal.cpu(), returns.cpu()
         return dict(clear_rate=t[:, 2].mean().item(), kills=t[:, 3].mean().item(), death_rate=t[:, 6].mean().item(),
                     timeout_rate=t[:, 7].mean().item(), turns=t[:, 5].mean().item(), shaped_return=r.mean().item())
+
+
+class ModuleTrainer:
+    """Rollouts and updates of any policy module with act(obs, seed, t) and evaluate(obs, actions)
+    (NormPolicy, ARPolicy): the module's forward and the sampling kernels for each of T decisions,
+    then ModulePPO over the buffer. Further arguments are ModulePPO's."""
+
+    def __init__(self, env, model, horizon=128, minibatch=8192, sample_seed=7, **ppo):
+        if env.batch * horizon < minibatch:
+            raise ValueError('a rollout must hold at least one minibatch')
+        self.env, self.model, self.T, self.N = env, model, horizon, env.batch
+        self.ppo = ppo_mod.ModulePPO(model, minibatch=minibatch, **ppo)
+        self.buf = ppo_mod.RolloutBuffer(horizon, self.N, device=env.device)
+        self.seed, self.t = sample_seed, 0
+        self.next_obs = env.obs.reshape(self.N, -1).clone()
+        self.gen = torch.Generator(device=env.device).manual_seed(sample_seed)
+
+    @torch.no_grad()
+    def rollout(self):
+        """Fill the buffer with T decisions per world."""
+        buf = self.buf
+        with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.ppo.autocast):
+            for k in range(self.T):
+                buf.obs[k].copy_(self.next_obs)
+                number, action, logp, value = self.model.act(buf.obs[k], self.seed, self.t + k)
+                buf.actions[k].copy_(number)
+                buf.logp[k].copy_(logp)
+                buf.values[k].copy_(value)
+                self.env.step_into(action, self.next_obs, buf.rewards[k], buf.dones[k])
+            buf.bootstrap.copy_(self.model.act(self.next_obs, self.seed, self.t + self.T)[3])
+        self.t += self.T
+        return buf
+
+    def update(self):
+        """One PPO update over the filled buffer; returns the last minibatch's loss."""
+        return self.ppo.update(self.buf, generator=self.gen)
+
+    def train(self, updates):
+        for _ in range(updates):
+            self.rollout()
+            last = self.update()
+        return last
