@@ -12,6 +12,11 @@
 namespace d1o {
 
 constexpr int threads_of(int lanes) { return lanes <= 64 ? 256 : lanes; }
+// Backward: several rows a workgroup, so that few workgroups (and sums to add) fill the card.
+// 5,778 x 861 bf16 with the reduction: 14.1 us on 512 threads, 19.5 on one row's 128; 65,536 x 1,024 78 and 83. On 1,024
+// threads the registers of two workgroups a CU do not hold a row of bf16 (204).
+constexpr int bwd_threads(int lanes) { return lanes > 512 ? lanes : 512; }
+constexpr int bwd_waves(int ch) { return ch == 1 ? 6 : 1; }
 // waves a SIMD that the forward pass is held to: two workgroups of 1,024 lanes on a CU
 constexpr int fwd_waves(int lanes, int ch) { return lanes == 1024 && ch <= 2 ? 8 : 1; }
 template <class T>
@@ -24,14 +29,16 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float2 (*scratch)[1
     a = lanes_sum<(LANES < 64 ? LANES : 64)>(a);
     b = lanes_sum<(LANES < 64 ? LANES : 64)>(b);
     if (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
         float2 *s = scratch[turn];
         turn ^= 1;
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = make_float2(a, b);
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) s[wave] = make_float2(a, b);
         __syncthreads();
-        // every lane reads one wave's sums: 16 lanes (8, 4) add them like a row of that many lanes
-        const float2 v = s[threadIdx.x % (LANES / 64)];
-        a = lanes_sum<LANES / 64>(v.x);
-        b = lanes_sum<LANES / 64>(v.y);
+        // every lane reads the sums of one of its row's waves: WAVES lanes add them like a row of that many lanes
+        const float2 v = s[wave / WAVES * WAVES + threadIdx.x % WAVES];
+        a = lanes_sum<WAVES>(v.x);
+        b = lanes_sum<WAVES>(v.y);
     }
 }
 
@@ -105,26 +112,28 @@ __global__ __launch_bounds__(threads_of(LANES), fwd_waves(LANES, CH)) void k_nor
 }
 
 template <class T, class W, int LANES, int CH, bool PAST>
-__global__ __launch_bounds__(threads_of(LANES)) void k_norm_bwd(const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x,
+__global__ __launch_bounds__(bwd_threads(LANES), bwd_waves(CH)) void k_norm_bwd(const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x,
                                                                 int64_t rows, int width, int64_t stride, const W *__restrict__ w,
                                                                 const float *__restrict__ mean, const float *__restrict__ rstd,
                                                                 T *__restrict__ dx, float *__restrict__ parts) {
-    constexpr int VEC = vec_of<T>(), THREADS = threads_of(LANES), GROUPS = THREADS / LANES, COLS = LANES * CH * VEC;
+    constexpr int VEC = vec_of<T>(), THREADS = bwd_threads(LANES), GROUPS = THREADS / LANES, COLS = LANES * CH * VEC;
     __shared__ float2 scratch[2][16];
     __shared__ float sums[GROUPS > 1 ? GROUPS * COLS : 1];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int turn = 0;
-    int64_t row = (int64_t)blockIdx.x * GROUPS + group;
     Pack<W, VEC> wv[CH];
     read_weight<W, LANES, CH, VEC>(wv, w, lane, width, (W)1.f);
     float gw[CH][VEC] = {}, gb[CH][VEC] = {};
     const float inv = 1.f / (float)width;
-    for (; row < rows; row += step) {
-        const float mu = mean[row], r = rstd[row];
+    // all groups of a workgroup make the same number of rounds (the row sums hold barriers)
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += step) {
+        const int64_t row = first + group;
+        const bool have = row < rows;
+        const float mu = have ? mean[row] : 0.f, r = have ? rstd[row] : 0.f;
         Pack<T, VEC> a[CH], g[CH];
-        read_row<T, LANES, CH, VEC>(a, x + row * stride, lane, width, (T)0.f);
-        read_row<T, LANES, CH, VEC>(g, dy + row * dy_stride, lane, width, (T)0.f);
+        read_row<T, LANES, CH, VEC>(a, x + row * stride, lane, have ? width : 0, (T)0.f);
+        read_row<T, LANES, CH, VEC>(g, dy + row * dy_stride, lane, have ? width : 0, (T)0.f);
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
@@ -148,7 +157,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void k_norm_bwd(const T *__restr
                 const float h = ((float)a[c].v[i] - mu) * r;
                 o.v[i] = (T)(r * (__builtin_fmaf((float)g[c].v[i], (float)wv[c].v[i], -c1) - h * c2));
             }
-            put_part<PAST>(dx + row * width + col, width - col, o);
+            put_part<PAST>(dx + row * width + col, have ? width - col : 0, o);
         }
     }
     if (!parts) return;
@@ -241,14 +250,14 @@ inline int fwd_grid(int64_t rows, int lanes) {
     const int64_t need = groups_of_rows(rows, lanes), most = lanes == 1024 ? 1024 : lanes == 512 || lanes < 64 ? 4096 : 8192;
     return (int)(need < most ? need : most);
 }
-// Backward: each workgroup writes its columns' sums, which k_norm_reduce reads again, so only about as many
-// as fit at once (65,536 x 1,024 bf16: 118, 83 and 103 us at 1,024, 2,048 and 4,096 of 128 lanes; 16,384 x 8,192: 168,
-// 160 and 173 at 256, 512 and 1,024), and two rows each at least where there are more than 512
-// (8,192 x 256: 7.9 us at 512, 9.1 at 1,024).
-inline int bwd_grid(int64_t rows, int lanes) {
-    const int64_t need = groups_of_rows(rows, lanes), half = (need + 1) / 2, few = need < 512 ? need : half < 512 ? 512 : half;
-    const int threads = threads_of(lanes), most = 256 * (threads == 128 ? 8 : threads == 256 ? 5 : threads == 512 ? 3 : 2);
-    return (int)(few < most ? few : most);
+// Backward: each workgroup writes its columns' sums, which k_norm_reduce reads again, so no more than fit at once:
+// two or three of 512 threads a CU (65,536 x 1,024 bf16 81.4 us at 512, 78.0 at 768, 90.9 at 1,024), two where the
+// rows are few beside the sums (5,778 x 861 14.1, 14.9 and 17.3), two of 1,024 lanes (16,384 x 8,192 174, 160 and 178 at 256, 512
+// and 768), one where a lane holds several chunks (7,554 x 11,823 144 at 256, 156 at 512).
+inline int bwd_grid(int64_t rows, int lanes, int ch) {
+    const int groups = bwd_threads(lanes) / lanes;
+    const int64_t need = (rows + groups - 1) / groups, most = ch > 1 ? 256 : lanes <= 512 && rows >= 16384 ? 768 : 512;
+    return (int)(need < most ? need : most);
 }
 
 // Whether the result goes past the caches: large ones of rows of several chunks a lane (8,192 x 16,384 bf16 forward 129 us
@@ -284,7 +293,7 @@ void launch(const Fwd &a, int grid) {
 }
 template <class T, class W, int LANES, int CH, bool PAST>
 void launch(const Bwd &a, int grid) {
-    k_norm_bwd<T, W, LANES, CH, PAST><<<grid, threads_of(LANES), 0, a.stream>>>(
+    k_norm_bwd<T, W, LANES, CH, PAST><<<grid, bwd_threads(LANES), 0, a.stream>>>(
         (const T *)a.dy, a.dy_stride, (const T *)a.x, a.rows, a.width, a.stride, (const W *)a.w, a.mean, a.rstd, (T *)a.dx,
         a.parts);
 }
@@ -315,7 +324,7 @@ int run(const Fwd &a) {
 template <class T, class W>
 int run(const Bwd &a) {
     int lanes = 0;
-    const int ch = shape_of(a.width, a.type, lanes), grid = bwd_grid(a.rows, lanes);
+    const int ch = shape_of(a.width, a.type, lanes), grid = bwd_grid(a.rows, lanes, ch);
     if (a.rows > 0) {
         const int e = dispatch<T, W>(a, lanes, ch, grid);
         if (e) return e;
@@ -351,8 +360,8 @@ extern "C" int d1_norm_fwd(const void *x, int type, int64_t rows, int width, int
 extern "C" int64_t d1_norm_work_bytes(int64_t rows, int width, int type) {
     if (!norm_args(type, type, rows, width, 0)) return D1_E_ARG;
     int lanes = 0;
-    shape_of(width, type, lanes);
-    return (int64_t)bwd_grid(rows, lanes) * 2 * width * sizeof(float);
+    const int ch = shape_of(width, type, lanes);
+    return (int64_t)bwd_grid(rows, lanes, ch) * 2 * width * sizeof(float);
 }
 
 extern "C" int d1_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int type, int64_t rows, int width, int64_t stride,
