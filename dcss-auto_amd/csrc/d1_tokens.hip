@@ -7,7 +7,7 @@
 // Each entry is read once: m, S and E run along, rescaled when m grows. The backward pass reads m
 // and S again and no sums.
 //
-// Rows of up to 1,024 entries stay in the registers of 4 to 64 lanes (k_tokens_small). A longer row
+// Rows of up to 512 entries stay in the registers of 4 to 32 lanes (k_tokens_small). A longer row
 // is cut into segments of one workgroup each, as many as fill the card when rows are few
 // (k_tokens_part), and where there are several k_tokens_join adds their m, S, E and merges their best entries.
 //
@@ -19,7 +19,7 @@ namespace d1o {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float FAR = -1e4f;          // below any difference whose exponential is not 0
-constexpr int SMALL_VOCAB = 1024;
+constexpr int SMALL_VOCAB = 512, SMALL_BWD_VOCAB = 1024;
 
 __device__ __forceinline__ float exp_nat(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 // e (x-m) for e = exp(x-m): 0 also for x = -inf, NaN where e is
@@ -520,9 +520,9 @@ __global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
     }
 }
 
-template <class T, bool MASK, bool PAST>
-__global__ __launch_bounds__(256) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
-    constexpr int VEC = 16 / (int)sizeof(T), STEP = 256 * VEC;
+template <class T, int PART, bool MASK, bool PAST>
+__global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int splits, int seg) {
+    constexpr int VEC = 16 / (int)sizeof(T), STEP = PART * VEC;
     const int64_t units = a.rows * splits;
     for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int64_t row = unit / splits;
@@ -573,7 +573,11 @@ inline int splits_of(int64_t rows, int vocab, int type, int &seg) {
 }
 inline unsigned blocks_of(int64_t units) { return (unsigned)(units < (1 << 20) ? units : (1 << 20)); }
 
-#define D1O_SMALL_SHAPES(X) X(4, 1) X(8, 1) X(16, 1) X(64, 1) X(64, 4)
+// Lanes a row and chunks of four a lane for short rows: several rows a wave and several chunks a lane, since reductions over
+// lanes cost as much as the entries (83,378 x 189 bf16: 12.4 us on 16 lanes x 4 chunks, 21.3 on 64 x 1; 62,655 x 89 with 20
+// alternatives 32 on 8 x 4, 111 on 64 x 1; 30,000 x 500 fp32 with 5 24.5 on 32 x 4, 41 on 64 x 4; 65,536 x 25 with 3 and a
+// mask 6.4 on 8 x 1, 9.7 on 16 x 1).
+#define D1O_SMALL_SHAPES(X) X(4, 1) X(8, 1) X(8, 2) X(8, 4) X(16, 4) X(32, 4)
 
 template <class T, bool MASK>
 int small_fwd(const Args &a, hipStream_t s) {
@@ -593,7 +597,7 @@ int small_bwd(const BackArgs &a, hipStream_t s) {
         k_tokens_small_bwd<T, L, C, MASK><<<blocks_of((a.rows + 256 / L - 1) / (256 / L)), 256, 0, s>>>(a);       \
         return (int)hipGetLastError();                                                                            \
     }
-    D1O_SMALL_SHAPES(X)
+    D1O_SMALL_SHAPES(X) X(64, 4)       // no sums over lanes here: wider rows too
 #undef X
     return D1_E_ARG;
 }
@@ -615,15 +619,22 @@ int fwd(const Args &a, const Parts &p, hipStream_t s) {
 }
 template <class T, bool MASK>
 int bwd(const BackArgs &a, hipStream_t s) {
-    if (a.vocab <= SMALL_VOCAB) return small_bwd<T, MASK>(a, s);
-    // Large outputs go past the caches, and a workgroup takes two rounds of them (4,096 x 131,072 bf16: 359 us, 391 with one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2)
-    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > PAST_BYTES;
-    const int seg = (past ? 2 : 1) * AT_ONCE * 256 * (16 / (int)sizeof(T)), splits = (a.vocab + seg - 1) / seg;
+    if (a.vocab <= SMALL_BWD_VOCAB) return small_bwd<T, MASK>(a, s);
+    // Large outputs go past the caches, and a workgroup takes two rounds of them (4,096 x 131,072 bf16: 359 us, 391 with
+    // one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2). Rows up to 4,096 entries leave most of 256
+    // threads idle in their last round: a wave with twice the rounds takes them (20,000 x 1,100 bf16 23.8 us, 39.2 on 256;
+    // 8,192 x 1,500 12.9 and 18.4; 10,000 x 2,500 22.9 and 28.5; 16,000 x 6,377 94 and 83).
+    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > PAST_BYTES, wave = a.vocab <= 4096;
+    const int seg = (past ? 2 : 1) * AT_ONCE * (wave ? 128 : 256) * (16 / (int)sizeof(T)), splits = (a.vocab + seg - 1) / seg;
     const unsigned grid = blocks_of(a.rows * splits);
-    if (past)
-        k_tokens_bwd<T, MASK, true><<<grid, 256, 0, s>>>(a, splits, seg);
+    if (wave && past)
+        k_tokens_bwd<T, 64, MASK, true><<<grid, 64, 0, s>>>(a, splits, seg);
+    else if (wave)
+        k_tokens_bwd<T, 64, MASK, false><<<grid, 64, 0, s>>>(a, splits, seg);
+    else if (past)
+        k_tokens_bwd<T, 256, MASK, true><<<grid, 256, 0, s>>>(a, splits, seg);
     else
-        k_tokens_bwd<T, MASK, false><<<grid, 256, 0, s>>>(a, splits, seg);
+        k_tokens_bwd<T, 256, MASK, false><<<grid, 256, 0, s>>>(a, splits, seg);
     return (int)hipGetLastError();
 }
 
@@ -645,7 +656,7 @@ extern "C" int64_t d1_tokens_work_bytes(int64_t rows, int vocab, int top) {
     if (vocab <= SMALL_VOCAB || rows == 0) return 0;
     int seg;
     const int splits = splits_of(rows, vocab, D1_FP32, seg);     // fp32's segments are the shortest
-    return rows * splits * (16 + 8 * (int64_t)top);
+    return splits == 1 ? 0 : rows * splits * (16 + 8 * (int64_t)top);
 }
 
 extern "C" int d1_tokens_fwd(const void *logits, int type, int64_t rows, int vocab, int64_t stride, const int64_t *tokens,
@@ -658,10 +669,12 @@ extern "C" int d1_tokens_fwd(const void *logits, int type, int64_t rows, int voc
     const int64_t need = d1_tokens_work_bytes(rows, vocab, top);
     if (need && (!work || work_bytes < need || ((uintptr_t)work & 7))) return D1_E_ARG;
     Parts p{};
-    if (need) {
+    if (vocab > SMALL_VOCAB) {
         p.splits = splits_of(rows, vocab, type, p.seg);
-        p.keys = (uint64_t *)work;
-        p.sums = (float *)(p.keys + rows * p.splits * top);
+        if (p.splits > 1) {
+            p.keys = (uint64_t *)work;
+            p.sums = (float *)(p.keys + rows * p.splits * top);
+        }
     }
     const Args a{logits, rows, stride, vocab, top, tokens, mask, mask_stride, logp, entropy, stats, top_ids, top_logp};
     D1O_TOKEN_TYPES(fwd, a, p, (hipStream_t)stream)

@@ -14,7 +14,7 @@ from . import _lib
 from .rows import as_rows, call, like, type_of
 
 MAX_TOP, MAX_VOCAB = 64, 1 << 24
-REGISTER_VOCAB = 1024      # rows up to this need no scratch memory
+UNSPLIT_VOCAB = 1024       # rows up to this are never cut into segments: no scratch memory
 
 
 class TokenLogprobs(NamedTuple):
@@ -64,7 +64,7 @@ def _forward(logits, tokens, mask, top):
         ids, top_logp = tok.new_empty((*logp.shape, top)), logp.new_empty((*logp.shape, top))
         ids_ptr, top_ptr = ids.data_ptr(), top_logp.data_ptr()
     L = _lib.load_ops()
-    need = L.d1_tokens_work_bytes(n, vocab, top) if vocab > REGISTER_VOCAB else 0
+    need = L.d1_tokens_work_bytes(n, vocab, top) if vocab > UNSPLIT_VOCAB else 0
     if need:
         work = torch.empty(need, dtype=torch.uint8, device=logits.device)
     call(L.d1_tokens_fwd, index, rows.data_ptr(), code, n, vocab, rows.stride(0), tok.data_ptr(), mask_ptr, mask_stride, top,
