@@ -204,7 +204,7 @@ constexpr int AT_ONCE = 2, KEEP = 512, ROUND = 4;
 struct Parts {
     float *sums;              // [rows][splits][4]: m, s, e
     uint64_t *keys;           // [rows][splits][top]
-    int splits, seg;          // segments a row, entries of one (a multiple of a workgroup's vectors)
+    int splits, seg;          // segments a row, entries of one (a multiple of a vector)
 };
 
 // VEC allowed entries of a segment at offset i (n entries in all); what is outside reads -inf
@@ -236,14 +236,52 @@ __device__ __forceinline__ void block_sync() {
         __syncthreads();
 }
 
+// a bound on the k-th largest of the lanes' words (N a lane) from below, exact in its first 18 bits: bit by bit from the top,
+// as long as k words stay at or above it
+template <int N>
+__device__ __forceinline__ uint32_t kth_word(const uint32_t (&word)[N], int k) {
+    uint32_t floor = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 14; bit--) {
+        const uint32_t at = floor | (1u << bit);
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) above += __popcll(__ballot(word[i] >= at));
+        if (above >= k) floor = at;
+    }
+    return floor;
+}
+
 // A wave's list of keys in LDS: takes keys in any order, keeps at least the `top` largest seen.
 struct TopList {
     uint64_t *list, *sorted;     // KEEP and D1_TOKENS_MAX_TOP keys
     int top, count;
     uint64_t below;              // keys up to this one are not among the largest
 
+    // leaves out keys whose word is below the top-th largest word's first bits: where few are equal, little
+    // more than `top` stay (a list of 242 keys was sorted in 10 us without)
+    __device__ __forceinline__ void prune(int lane) {
+        uint64_t key[KEEP / 64];
+        uint32_t word[KEEP / 64];
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < KEEP / 64; i++) {
+            key[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
+            word[i] = (uint32_t)(key[i] >> 32);
+        }
+        const uint32_t floor = kth_word<KEEP / 64>(word, top);
+        wave_sync();
+        count = 0;
+#pragma unroll
+        for (int i = 0; i < KEEP / 64; i++) {
+            const uint64_t stay = __ballot(word[i] && word[i] >= floor);
+            if (word[i] && word[i] >= floor) list[count + __popcll(stay & ((1ull << lane) - 1))] = key[i];
+            count += __popcll(stay);
+        }
+    }
     // the `top` largest to `sorted`, falling; places without a key are 0. A key's place is the number of larger ones.
     __device__ __forceinline__ void sort(int lane) {
+        if (count > 64) prune(lane);
         wave_sync();
         if (lane < top) sorted[lane] = 0;
         wave_sync();
@@ -279,22 +317,6 @@ struct TopList {
         if (count > KEEP - 64 * ROUND) shrink(lane);
     }
 };
-
-// a bound on the k-th largest of the lanes' words (N a lane) from below, exact in its first 18 bits: bit by bit from the top,
-// as long as k words stay at or above it
-template <int N>
-__device__ __forceinline__ uint32_t kth_word(const uint32_t (&word)[N], int k) {
-    uint32_t floor = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 14; bit--) {
-        const uint32_t at = floor | (1u << bit);
-        int above = 0;
-#pragma unroll
-        for (int i = 0; i < N; i++) above += __popcll(__ballot(word[i] >= at));
-        if (above >= k) floor = at;
-    }
-    return floor;
-}
 
 template <class T, int PART, bool MASK, bool TOP>
 __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts parts) {
@@ -428,11 +450,16 @@ __global__ __launch_bounds__(64) void k_tokens_join(const Args a, const Parts pa
             const float *p = parts.sums + (row * parts.splits + lane) * 4;
             t = {p[0], p[1], p[2]};
         }
-        const uint64_t *keys = parts.keys + (row * parts.splits + lane) * a.top;
+        const uint64_t *all = parts.keys + row * parts.splits * a.top, *keys = all + lane * a.top;
+        const int total = parts.splits * a.top;
+        const bool flat = total <= ROUND * 64;
         constexpr int FIRST = 2 * ROUND;
-        uint64_t key[FIRST];             // the first of the lane's list
+        uint64_t key[FIRST];             // few keys: all of them, whoever's; many: the first of the lane's list
 #pragma unroll
-        for (int j = 0; j < FIRST; j++) key[j] = mine && j < a.top ? keys[j] : 0;
+        for (int j = 0; j < FIRST; j++) {
+            const int at = j * 64 + lane;
+            key[j] = flat ? at < total ? all[at] : 0 : mine && j < a.top ? keys[j] : 0;
+        }
         const Given given = given_of<T>(a, row);
         t = lanes_joined<64>(t);
         if (lane == 0) finish(a, row, t, given);
@@ -451,7 +478,7 @@ __global__ __launch_bounds__(64) void k_tokens_join(const Args a, const Parts pa
                     if ((uint32_t)(four[j] >> 32) < floor) four[j] = 0;
                 }
                 best.add(four, lane);
-                if (!__ballot(four[ROUND - 1] > best.below)) break;     // the lists fall: nothing larger follows
+                if (flat || !__ballot(four[ROUND - 1] > best.below)) break;     // the lists fall: nothing larger follows
             }
             best.sort(lane);
             if (lane < a.top) put_top(a, row, lane, sorted[lane], finite_base(t.m), logf(t.s), t.s);
@@ -561,14 +588,14 @@ __global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int split
 // (8,192 x 1,500 bf16 with 5 alternatives 14.7 us on 64 threads, 33.7 on 256; none 10.0 and 16.5; 16,384 x 9,000 with
 // 5 80 and 107). Elsewhere 256 (16,384 x 20,000 185 us on 64 and 175 on 256; 1,024 x 9,000 17.0 and 10.4).
 inline int part_of(int64_t rows, int vocab) { return rows >= 2048 && vocab <= 12288 ? 64 : 256; }
-// Segments of a row: as many as make about six workgroups for each of the 256 CUs where rows are fewer than that, none
-// shorter than one vector a thread, at most 64 (the join's lanes). 512 x 50,001 fp16 with 5 alternatives: 28.0 us at
+// Segments of a row, equally long: as many as make about six workgroups for each of the 256 CUs where rows are fewer than
+// that, of one vector a thread at least where the row has it, at most 64 (the join's lanes). 512 x 50,001 fp16 with 5 alternatives: 28.0 us at
 // 512 workgroups, 25.6 at 1,536, 28.9 at 4,096; 300 x 131,072 bf16 with 20: 82 at 300, 39 at 1,200, 41 at 4,800.
 inline int splits_of(int64_t rows, int vocab, int type, int &seg) {
     const int step = part_of(rows, vocab) * (type == D1_FP32 ? 4 : 8);
     const int64_t want = (1536 + rows - 1) / rows, most = (vocab + step - 1) / step, few = want < 64 ? want : 64;
     const int splits = (int)(few < most ? few : most);
-    seg = ((vocab + splits - 1) / splits + step - 1) / step * step;
+    seg = ((vocab + splits - 1) / splits + 7) / 8 * 8;
     return (vocab + seg - 1) / seg;
 }
 inline unsigned blocks_of(int64_t units) { return (unsigned)(units < (1 << 20) ? units : (1 << 20)); }
