@@ -4,6 +4,7 @@ and the learning task's libraries.
 
 There is no fallback: without the built library every entry point raises."""
 import ctypes as C
+import importlib
 import pathlib
 
 HERE = pathlib.Path(__file__).resolve().parent
@@ -22,7 +23,7 @@ LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', '
 OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
                'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read')
 _LEARN = {}
-_OPS = None
+_OPS = _OPS_TORCH = None
 
 
 class D1PPOStep(C.Structure):
@@ -120,6 +121,18 @@ def load_ops():
             getattr(L, name).restype = C.c_int64
         _OPS = L
     return _OPS
+
+
+def load_ops_torch():
+    """_d1ops.so: libd1ops.so's calls on torch tensors (csrc/d1_ops_torch.cpp)."""
+    global _OPS_TORCH
+    if _OPS_TORCH is None:
+        path = HERE / '_d1ops.so'
+        if not path.exists():
+            raise RuntimeError(f'{path} is missing: build it with __graft_entry__.build() '
+                               '(the operators have no CPU fallback)')
+        _OPS_TORCH = importlib.import_module('._d1ops', __package__)
+    return _OPS_TORCH
 
 
 def load_learn(clump=0):

@@ -8,64 +8,18 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .rows import TYPES, as_rows, call, like, type_of
-
-MAX_WIDTH = 16384
-
-
-def _check(x, weight, bias):
-    """-> (x's type code, the weights' type code, x as rows, weight, bias)."""
-    code = type_of(x, 'x')
-    width, index, dtype = x.shape[-1], x.get_device(), x.dtype
-    if width > MAX_WIDTH:
-        raise ValueError(f'x: rows of at most {MAX_WIDTH} elements')
-    first = bias if weight is None else weight
-    if first is not None:
-        dtype = first.dtype
-        if dtype != x.dtype and dtype != torch.float32:
-            raise ValueError(f"weight and bias must be fp32 or of x's type, not {dtype}")
-        if weight is not None:
-            weight = like(weight, (width,), index, 'weight', dtype)
-        if bias is not None:
-            bias = like(bias, (width,), index, 'bias', dtype)
-    return code, TYPES[dtype], as_rows(x), weight, bias
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+from .ops import call
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     """-> (y like x, mean fp32 [...], rstd fp32 [...]): y = (x - mean) * rstd * weight + bias."""
-    code, wcode, rows, weight, bias = _check(x, weight, bias)
-    n, width = rows.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    call(_lib.load_ops().d1_norm_fwd, x.get_device(), rows.data_ptr(), code, n, width, rows.stride(0), _ptr(weight), _ptr(bias),
-         wcode, eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
-    return y, mean, rstd
+    return call('norm_fwd', x, x, weight, bias, eps)
 
 
 def layer_norm_bwd(dy, x, weight, bias, mean, rstd):
     """-> (dx, dweight, dbias) from layer_norm_fwd's arguments and its mean and rstd; dweight and
     dbias are None where the weight or the bias is."""
-    code, wcode, rows, weight, bias = _check(x, weight, bias)
-    index, shape, (n, width) = x.get_device(), x.shape[:-1], rows.shape
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.get_device() != index:
-        raise ValueError(f'dy must be {x.dtype} of shape {tuple(x.shape)} on {x.device}')
-    drows = as_rows(dy)
-    mean, rstd = like(mean, shape, index, 'mean'), like(rstd, shape, index, 'rstd')
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = None if weight is None else torch.empty_like(weight)
-    db = None if bias is None else torch.empty_like(bias)
-    L = _lib.load_ops()
-    need = 0 if dw is None and db is None else L.d1_norm_work_bytes(n, width, code)
-    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    call(L.d1_norm_bwd, index, drows.data_ptr(), drows.stride(0), rows.data_ptr(), code, n, width, rows.stride(0),
-         _ptr(weight), wcode, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), need)
-    return dx, dw, db
+    return call('norm_bwd', x, dy, x, weight, bias, mean, rstd)
 
 
 class _LayerNorm(torch.autograd.Function):

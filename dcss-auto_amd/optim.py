@@ -4,17 +4,11 @@
 an 8-bit moment stands for. The step count, the global norm of a clip and the skip of a step whose
 norm is not finite stay on the device, so a step can be captured in a HIP graph.
 """
-import ctypes as C
-import struct
-
 import torch
 
-from . import _lib
-from .rows import call
+from .ops import call
 
 BLOCK = 256                         # elements of an 8-bit moment that share an exponent
-_TYPES = {torch.float32: 0, torch.bfloat16: 1}
-_ENTRY = '7Q2q2di2B2x'              # D1AdamWTensor
 
 
 def moment_blocks(numel):
@@ -22,12 +16,8 @@ def moment_blocks(numel):
     return -(-numel // BLOCK)
 
 
-def _each(value, count, name):
-    if isinstance(value, (int, float)):
-        return [value] * count
-    if len(value) != count:
-        raise ValueError(f'{name}: {len(value)} values for {count} parameters')
-    return value
+def _each(value, count):
+    return [value] * count if isinstance(value, (int, float)) else value
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
@@ -46,76 +36,14 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     With max_grad_norm > 0 the gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with
     the norm over all of them, and a step whose norm is not finite changes nothing and is counted."""
     count = len(params)
-    eight = exps is not None
-    lists = dict(grads=grads, exp_avg=exp_avg, exp_avg_sq=exp_avg_sq)
-    for name, given in (('copies', copies), ('counters', counters), ('lags', lags)):
-        if given is not None:
-            lists[name] = given
-    if eight:
-        lists['exps[0]'], lists['exps[1]'] = exps
-    for name, given in lists.items():
-        if len(given) != count:
-            raise ValueError(f'{name}: {len(given)} for {count} parameters')
-    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and max_grad_norm >= 0):
-        raise ValueError('betas must be in [0, 1), eps and max_grad_norm not negative')
-    if step.dtype != torch.int32 or step.shape != (8,) or not step.is_cuda or not step.is_contiguous():
-        raise ValueError('step must be a contiguous int32 CUDA tensor of 8 elements')
-    index, moment = step.get_device(), torch.uint8 if eight else torch.float32
-    words, held = [], []
-    lr, weight_decay = _each(lr, count, 'lr'), _each(weight_decay, count, 'weight_decay')
-    for i in range(count):
-        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
-        n = p.numel()
-        if not g.is_contiguous():
-            g = g.contiguous()
-            held.append(g)
-        ptype, gtype = _TYPES.get(p.dtype), _TYPES.get(g.dtype)
-        if ptype is None or gtype is None:
-            raise ValueError(f'tensor {i}: parameter and gradient must be fp32 or bf16, not {p.dtype} and {g.dtype}')
-        if m.dtype != moment or v.dtype != moment or not g.numel() == m.numel() == v.numel() == n:
-            raise ValueError(f'tensor {i}: the gradient must have the size of the parameter, the moments too, in {moment}')
-        if not p.get_device() == g.get_device() == m.get_device() == v.get_device() == index:
-            raise ValueError(f'tensor {i}: parameter, gradient and moments must be on {step.device}')
-        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            raise ValueError(f'tensor {i}: parameter and moments must be contiguous')
-        if not (lr[i] >= 0 and weight_decay[i] >= 0):
-            raise ValueError(f'tensor {i}: lr and weight_decay must not be negative')
-        me = ve = copy = 0
-        if copies is not None and (c := copies[i]) is not None:
-            if c.dtype != torch.bfloat16 or c.numel() != n or not c.is_contiguous() or c.get_device() != index or ptype:
-                raise ValueError(f'tensor {i}: a copy is contiguous bf16 of the size of an fp32 parameter')
-            copy = c.data_ptr()
-        if eight:
-            me, ve = exps[0][i], exps[1][i]
-            for e in (me, ve):
-                if e.dtype != torch.uint8 or e.numel() != moment_blocks(n) or not e.is_contiguous() or e.get_device() != index:
-                    raise ValueError(f'tensor {i}: exponents are contiguous uint8, one for each {BLOCK} elements')
-            me, ve = me.data_ptr(), ve.data_ptr()
-        words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), me, ve, copy,
-                  n, 0 if counters is None else counters[i], lr[i], weight_decay[i], 0 if lags is None else lags[i],
-                  ptype, gtype)
-    table = struct.pack('=' + _ENTRY * count, *words)
-    h = _lib.D1AdamW(betas[0], betas[1], eps, max_grad_norm, seed & 0xFFFFFFFFFFFFFFFF, 8 if eight else 32)
-    L = _lib.load_ops()
-    need = L.d1_adamw_work_bytes(table, count, C.byref(h)) if max_grad_norm > 0 else 0
-    _lib.check(min(need, 0), 'd1_adamw_work_bytes')
-    work = torch.empty(need, dtype=torch.uint8, device=step.device) if need else None
-    call(L.d1_adamw_step, index, table, count, C.byref(h), step.data_ptr(), work.data_ptr() if need else None, need)
+    m_exps, v_exps = exps if exps is not None else (None, None)
+    call('adamw_step', step, params, grads, exp_avg, exp_avg_sq, step, _each(lr, count), _each(weight_decay, count), betas[0],
+         betas[1], eps, max_grad_norm, copies, m_exps, v_exps, counters, lags, seed & 0xFFFFFFFFFFFFFFFF)
 
 
 def read_moment(code, exp, signed, out=None):
     """fp32 values of an 8-bit moment: uint8 codes and their exponents (signed: exp_avg's)."""
-    n = code.numel()
-    if code.dtype != torch.uint8 or exp.dtype != torch.uint8 or not code.is_cuda or exp.device != code.device \
-            or not code.is_contiguous() or not exp.is_contiguous() or exp.numel() != moment_blocks(n):
-        raise ValueError(f'code and exp must be contiguous uint8 CUDA tensors, one exponent for each {BLOCK} codes')
-    if out is None:
-        out = torch.empty(code.shape, dtype=torch.float32, device=code.device)
-    elif out.dtype != torch.float32 or out.numel() != n or not out.is_contiguous() or out.device != code.device:
-        raise ValueError('out must be contiguous fp32 of the size of the codes, on their device')
-    call(_lib.load_ops().d1_adamw_read, code.get_device(), code.data_ptr(), exp.data_ptr(), n, 1 if signed else 0,
-         out.data_ptr())
-    return out
+    return call('adamw_read', code, code, exp, bool(signed), out)
 
 
 class AdamW(torch.optim.Optimizer):
