@@ -204,7 +204,7 @@ constexpr int AT_ONCE = 2, KEEP = 512, ROUND = 4;
 struct Parts {
     float *sums;              // [rows][splits][4]: m, s, e
     uint64_t *keys;           // [rows][splits][top]
-    int splits, seg;          // segments a row, entries of one (a multiple of a vector)
+    int part, splits, seg;    // threads of a workgroup, segments a row, entries of one (a multiple of a vector)
 };
 
 // VEC allowed entries of a segment at offset i (n entries in all); what is outside reads -inf
@@ -400,16 +400,22 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
             wave_sync();
             const int total = __popcll(open) * each;
             for (int q0 = 0; q0 < total; q0 += ROUND * 64) {
-                uint64_t key[ROUND];
+                T entry[ROUND];
+                bool in[ROUND];
+                int at[ROUND];
 #pragma unroll
                 for (int u = 0; u < ROUND; u++) {                // all loads in flight
                     const int q = q0 + u * 64 + lane, k = q / each, r = q - k * each;
-                    key[u] = 0;
-                    if (q < total) {
-                        const int at = (r / VEC * PART + wave * 64 + who[k]) * VEC + r % VEC;
-                        if (at < n && (!MASK || mask[at])) key[u] = key_of((float)x[at], begin + at);
-                        if ((uint32_t)(key[u] >> 32) < floor) key[u] = 0;
-                    }
+                    at[u] = q < total ? (r / VEC * PART + wave * 64 + who[k]) * VEC + r % VEC : n;
+                    in[u] = at[u] < n;
+                    entry[u] = in[u] ? x[at[u]] : (T)0.f;
+                    if (MASK) in[u] = in[u] && mask[at[u]];
+                }
+                uint64_t key[ROUND];
+#pragma unroll
+                for (int u = 0; u < ROUND; u++) {
+                    key[u] = in[u] ? key_of((float)entry[u], begin + at[u]) : 0;
+                    if ((uint32_t)(key[u] >> 32) < floor) key[u] = 0;
                 }
                 best.add(key, lane);
             }
@@ -583,20 +589,28 @@ __global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int split
     }
 }
 
-// Threads of a workgroup for long rows: a wave each where there are rows enough for all CUs and a lane's share of
-// a row is short, since with alternatives a workgroup's search costs as much for few entries as for many
-// (8,192 x 1,500 bf16 with 5 alternatives 14.7 us on 64 threads, 33.7 on 256; none 10.0 and 16.5; 16,384 x 9,000 with
-// 5 80 and 107). Elsewhere 256 (16,384 x 20,000 185 us on 64 and 175 on 256; 1,024 x 9,000 17.0 and 10.4).
-inline int part_of(int64_t rows, int vocab) { return rows >= 2048 && vocab <= 12288 ? 64 : 256; }
-// Segments of a row, equally long: as many as make about six workgroups for each of the 256 CUs where rows are fewer than
-// that, of one vector a thread at least where the row has it, at most 64 (the join's lanes). 512 x 50,001 fp16 with 5 alternatives: 28.0 us at
-// 512 workgroups, 25.6 at 1,536, 28.9 at 4,096; 300 x 131,072 bf16 with 20: 82 at 300, 39 at 1,200, 41 at 4,800.
-inline int splits_of(int64_t rows, int vocab, int type, int &seg) {
-    const int step = part_of(rows, vocab) * (type == D1_FP32 ? 4 : 8);
-    const int64_t want = (1536 + rows - 1) / rows, most = (vocab + step - 1) / step, few = want < 64 ? want : 64;
-    const int splits = (int)(few < most ? few : most);
-    seg = ((vocab + splits - 1) / splits + 7) / 8 * 8;
-    return (vocab + seg - 1) / seg;
+// How long rows are cut. A workgroup takes a whole row, which saves k_tokens_join and its launch, where that still fills the card or
+// the row is short; us for bf16 without and with 20 alternatives:
+//   64 threads, many short rows: 8,192 x 1,500 10.0 and (5 alternatives) 14.7 against 16.5 and 33.7 on 256; 16,384 x 20,000 with 5
+//     185 against 175 on 256
+//   256, rows up to 12 KB, or 48 KB from 512 rows on: 1 x 5,000 4.1 and 6.4 against 6.6 and 11.1 in segments; 1,024 x 20,000
+//     11.6 and 20.0 against 15.9 and 28.8
+//   512, up to 104 KB for fewer rows than fill the card on 256: 1 x 20,000 4.4 and 8.9 against 6.7 and 11.8 in segments; 512 x 50,001
+//     15.7 and 24.6 against 19.0 and 30.4; 128 x 100,000 15.2 and 26.9 against 11.8 and 22.0
+//   else segments of 256 threads, equally long, about six workgroups a CU, of one vector a thread at least, at most 64 (the
+//     join's lanes): 300 x 131,072 with 20 82 us at 300 workgroups, 39 at 1,200, 41 at 4,800
+struct Cut {
+    int part, splits, seg;        // threads, segments a row, entries of one
+};
+inline Cut cut_of(int64_t rows, int vocab, int type) {
+    const int64_t size = type == D1_FP32 ? 4 : 2, bytes = vocab * size;
+    if (rows >= 2048 && vocab <= 12288) return {64, 1, vocab};
+    if (bytes <= 12 << 10 || (rows >= 512 && bytes <= 48 << 10) || rows >= 1536) return {256, 1, vocab};
+    if (bytes <= 104 << 10) return {512, 1, vocab};
+    const int64_t step = 256 * (16 / size), want = (1536 + rows - 1) / rows, most = (vocab + step - 1) / step;
+    const int64_t few = want < 64 ? want : 64, splits = few < most ? few : most;
+    const int seg = (int)(((vocab + splits - 1) / splits + 7) / 8 * 8);
+    return {256, (vocab + seg - 1) / seg, seg};
 }
 inline unsigned blocks_of(int64_t units) { return (unsigned)(units < (1 << 20) ? units : (1 << 20)); }
 
@@ -633,11 +647,12 @@ template <class T, bool MASK>
 int fwd(const Args &a, const Parts &p, hipStream_t s) {
     if (a.vocab <= SMALL_VOCAB) return small_fwd<T, MASK>(a, s);
     const unsigned grid = blocks_of(a.rows * p.splits);
-    const int part = part_of(a.rows, a.vocab);
-#define X(P) \
-    if (part == P && a.top) k_tokens_part<T, P, MASK, true><<<grid, P, 0, s>>>(a, p); \
-    if (part == P && !a.top) k_tokens_part<T, P, MASK, false><<<grid, P, 0, s>>>(a, p);
-    X(64) X(256)
+#define X(P)                                                              \
+    if (p.part == P && a.top)                                             \
+        k_tokens_part<T, P, MASK, true><<<grid, P, 0, s>>>(a, p);         \
+    else if (p.part == P)                                                 \
+        k_tokens_part<T, P, MASK, false><<<grid, P, 0, s>>>(a, p);
+    X(64) X(256) X(512)
 #undef X
     const int e = (int)hipGetLastError();
     if (e || p.splits == 1) return e;
@@ -681,8 +696,7 @@ static bool token_args(int type, int64_t rows, int vocab, int64_t stride, int64_
 extern "C" int64_t d1_tokens_work_bytes(int64_t rows, int vocab, int top) {
     if (!token_args(D1_FP32, rows, vocab, 0, 0) || top < 0 || top > D1_TOKENS_MAX_TOP || top > vocab) return D1_E_ARG;
     if (vocab <= SMALL_VOCAB || rows == 0) return 0;
-    int seg;
-    const int splits = splits_of(rows, vocab, D1_FP32, seg);     // fp32's segments are the shortest
+    const int splits = cut_of(rows, vocab, D1_FP32).splits;      // no type has more
     return splits == 1 ? 0 : rows * splits * (16 + 8 * (int64_t)top);
 }
 
@@ -697,7 +711,10 @@ extern "C" int d1_tokens_fwd(const void *logits, int type, int64_t rows, int voc
     if (need && (!work || work_bytes < need || ((uintptr_t)work & 7))) return D1_E_ARG;
     Parts p{};
     if (vocab > SMALL_VOCAB) {
-        p.splits = splits_of(rows, vocab, type, p.seg);
+        const Cut c = cut_of(rows, vocab, type);
+        p.part = c.part;
+        p.splits = c.splits;
+        p.seg = c.seg;
         if (p.splits > 1) {
             p.keys = (uint64_t *)work;
             p.sums = (float *)(p.keys + rows * p.splits * top);

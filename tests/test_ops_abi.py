@@ -41,10 +41,10 @@ def test_struct_layout(lib, tmp_path, name):
 
 def test_tokens_arguments(lib):
     L = lib.load_ops()
-    assert L.d1_tokens_work_bytes(8, 1000, 5) == 0 and L.d1_tokens_work_bytes(8, 5000, 5) > 0
+    assert L.d1_tokens_work_bytes(8, 1000, 5) == 0 and L.d1_tokens_work_bytes(8, 5000, 5) == 0 and L.d1_tokens_work_bytes(8, 100000, 5) > 0
     for rows, vocab, top in ((-1, 5, 0), (1, 0, 0), (1, 5, 6), (1, 100, 65), (1, 5, -1), (1, (1 << 24) + 1, 0)):
         assert L.d1_tokens_work_bytes(rows, vocab, top) == -1
-    good = [F, 0, 4, 5000, 5000, F, None, 0, 3, F, F, F, F, F, F, 1 << 20, None]
+    good = [F, 0, 4, 100000, 100000, F, None, 0, 3, F, F, F, F, F, F, 1 << 20, None]     # long enough to be cut into segments
     assert L.d1_tokens_fwd(*good[:2], 0, *good[3:]) == 0
     for at, bad in ((0, None), (1, 3), (1, -1), (2, -1), (3, 0), (4, -1), (5, None), (7, -1), (8, 65), (9, None), (10, None),
                     (11, None), (12, None), (13, None), (14, None), (14, F + 4), (15, 7)):

@@ -345,3 +345,30 @@ def test_refusals(T):
     for dl, de in ((g.double(), h), (g[:3], h), (g, h.cpu())):
         with pytest.raises(ValueError):
             T.token_logprobs_bwd(x, tokens, out, dl, de)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('rows,vocab', [(1, 120001), (5, 60008), (37, 53251), (200, 57344), (1030, 70001)])
+def test_rows_in_segments(T, rows, vocab, dtype):
+    """Rows long enough to be cut: masks that empty whole segments, ties over the cuts, NaN, infinities."""
+    print(f'[tokens] segments {rows} x {vocab} {dtype}', flush=True)
+    logits, tokens, g, h = inputs(rows, vocab, dtype, 2 * rows + vocab, pad=1)
+    gen = torch.Generator(device='cuda').manual_seed(rows)
+    mask = torch.rand(rows, vocab, generator=gen, device='cuda') < 0.6
+    check(T, logits, tokens, top=20, g=g, h=h)
+    check(T, logits, tokens, mask=mask, top=64, g=g, h=h)
+    mask[:, vocab // 9:] = False                            # all later segments empty
+    mask[rows // 2] = False
+    mask[rows // 2, vocab - 2:] = True                      # the last two entries alone
+    tokens[0] = -1
+    check(T, logits, tokens, mask=mask, top=5, g=g, h=h)
+    ties = (torch.arange(vocab, device='cuda') % 50 == 49).to(dtype).expand(rows, vocab)
+    check(T, ties, tokens, top=33)
+    odd = logits.clone()
+    odd[:, 7::1001] = -math.inf
+    odd[rows - 1] = torch.finfo(dtype).min
+    check(T, odd, tokens, top=3, g=g, h=h)
+    odd[rows - 1, vocab - 1] = math.nan
+    out = T.token_logprobs(odd, tokens, top=1)
+    assert torch.isnan(out.entropy[rows - 1]) and out.top_ids[rows - 1, 0] == vocab - 1
+    assert not torch.isnan(out.entropy[:rows - 1]).any()
