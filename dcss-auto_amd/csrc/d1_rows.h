@@ -43,6 +43,18 @@ __device__ __forceinline__ void store_part(T *p, int n, const Pack<T, N> &a) {
         if (i < n) p[i] = a.v[i];
 }
 
+// A lane's pack of elements i to i + N - 1 of n, moved back where it would pass the end: one whole load without a
+// branch, of which the first `skip` elements are the lanes' before it (all N of them where i >= n). Both lanes store
+// the same values there. There have to be N elements before the end.
+struct Place {
+    int at, skip;
+};
+template <int N>
+__device__ __forceinline__ Place place_of(int i, int n) {
+    const int at = i < n - N ? i : n - N;
+    return {at, i - at};
+}
+
 // the same past the caches, for outputs that are larger than the L2s of all chiplets (8 x 4 MB) and so
 // would only push out what is read
 constexpr int64_t PAST_BYTES = 32 << 20;

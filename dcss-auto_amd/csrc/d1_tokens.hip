@@ -108,21 +108,39 @@ __device__ __forceinline__ void put_top(const Args &a, int64_t row, int k, uint6
 
 template <class T, int LANES, int CH, bool MASK>
 struct SmallRow {
-    float x[CH][4];
-    bool in[CH][4];       // an entry of the row that is allowed
-    __device__ __forceinline__ void read(const T *logits, const uint8_t *mask, int vocab, int lane) {
+    float x[CH][4];       // -inf where `in` is not set
+    bool in[CH][4];       // an allowed entry of the lane's
+    int at[CH];           // index of the chunk's first entry
+    // chunks of rows of 4 entries or more are whole loads; `shared`: what they hold of the lane before counts too
+    __device__ __forceinline__ void read(const T *logits, const uint8_t *mask, int vocab, int lane, bool shared) {
+        Pack<T, 4> p[CH];
+        Pack<uint8_t, 4> q[CH];
+        int skip[CH];
+        if (vocab >= 4) {
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int col = (c * LANES + lane) * 4, n = vocab - col;
-            const Pack<T, 4> p = load_part<T, 4>(logits + col, n, (T)0.f);
-            Pack<uint8_t, 4> q;
-            if (MASK) q = load_part<uint8_t, 4>(mask + col, n, 0);
+            for (int c = 0; c < CH; c++) {
+                const Place w = place_of<4>((c * LANES + lane) * 4, vocab);
+                at[c] = w.at;
+                skip[c] = w.skip;
+                p[c] = load<T, 4>(logits + w.at);
+                if (MASK) q[c] = load<uint8_t, 4>(mask + w.at);
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                in[c][i] = MASK ? q.v[i] != 0 : i < n;
-                x[c][i] = in[c][i] ? (float)p.v[i] : -INFINITY;
+            for (int c = 0; c < CH; c++) {
+                at[c] = (c * LANES + lane) * 4;
+                skip[c] = at[c] ? 4 : 0;
+                p[c] = load_part<T, 4>(logits, at[c] ? 0 : vocab, (T)0.f);
+                if (MASK) q[c] = load_part<uint8_t, 4>(mask, at[c] ? 0 : vocab, 0);
             }
         }
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                in[c][i] = (shared ? skip[c] < 4 : i >= skip[c]) && at[c] + i < vocab && (!MASK || q[c].v[i]);
+                x[c][i] = in[c][i] ? (float)p[c].v[i] : -INFINITY;
+            }
     }
 };
 
@@ -132,7 +150,7 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows; row += (int64_t)gridDim.x * GROUPS) {
         SmallRow<T, LANES, CH, MASK> r;
-        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane);
+        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane, false);
         const int64_t tok = a.tokens[row];
         float m = -INFINITY;
 #pragma unroll
@@ -161,8 +179,9 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
         }
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int64_t at = tok - (c * LANES + lane) * 4;
-            if (at >= 0 && at < 4 && tok < a.vocab) {
+            const int64_t col = (c * LANES + lane) * 4;
+            if (tok >= col && tok < col + 4 && tok < a.vocab) {
+                const int at = (int)tok - r.at[c];
                 const float x = at < 2 ? (at ? r.x[c][1] : r.x[c][0]) : (at == 2 ? r.x[c][2] : r.x[c][3]);
                 a.logp[row] = logp_of(x, t, base, ls);
             }
@@ -183,12 +202,12 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
 #pragma unroll
                 for (int c = CH - 1; c >= 0; c--)
 #pragma unroll
-                    for (int i = 3; i >= 0; i--) first = word[c][i] == best ? (c * LANES + lane) * 4 + i : first;
+                    for (int i = 3; i >= 0; i--) first = word[c][i] == best ? r.at[c] + i : first;
                 first = lanes_u<LANES>(first, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
 #pragma unroll
                 for (int c = 0; c < CH; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) word[c][i] = (uint32_t)((c * LANES + lane) * 4 + i) == first ? 0 : word[c][i];
+                    for (int i = 0; i < 4; i++) word[c][i] = (uint32_t)(r.at[c] + i) == first ? 0 : word[c][i];
                 if (lane == 0) put_top(a, row, k, ((uint64_t)best << 32) | (uint32_t)~first, base, ls, s);
             }
         }
@@ -207,18 +226,16 @@ struct Parts {
     int part, splits, seg;    // threads of a workgroup, segments a row, entries of one (a multiple of a vector)
 };
 
-// VEC allowed entries of a segment at offset i (n entries in all); what is outside reads -inf
+// VEC allowed entries of a segment from `at` on; the first `skip` and what the mask leaves out read -inf
 template <class T, int VEC, bool MASK>
-__device__ __forceinline__ void read_vec(const T *x, const uint8_t *mask, int i, int n, float (&v)[VEC]) {
-    const Pack<T, VEC> p = load_part<T, VEC>(x + i, n - i, (T)-INFINITY);
-    if (MASK) {
-        const Pack<uint8_t, VEC> q = load_part<uint8_t, VEC>(mask + i, n - i, 0);
+__device__ __forceinline__ void read_vec(const T *x, const uint8_t *mask, Place w, Pack<T, VEC> &p, Pack<uint8_t, VEC> &q) {
+    p = load<T, VEC>(x + w.at);
+    if (MASK) q = load<uint8_t, VEC>(mask + w.at);
+}
+template <class T, int VEC, bool MASK>
+__device__ __forceinline__ void widen_vec(const Pack<T, VEC> &p, const Pack<uint8_t, VEC> &q, int skip, float (&v)[VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = q.v[j] ? (float)p.v[j] : -INFINITY;
-    } else {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = (float)p.v[j];
-    }
+    for (int j = 0; j < VEC; j++) v[j] = j >= skip && (!MASK || q.v[j]) ? (float)p.v[j] : -INFINITY;
 }
 
 // what the lanes of a wave wrote to LDS is there for the others after this
@@ -337,10 +354,27 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
         Sums t = {-INFINITY, 0.f, 0.f};
         Given given = {-1, 0.f};
         if (parts.splits == 1 && threadIdx.x == 0) given = given_of<T>(a, row);
-        for (int i = threadIdx.x * VEC; i < n; i += STEP * AT_ONCE) {
+        uint64_t allowed = 0;            // of TOP and MASK: not 0 where the lane saw an allowed entry (or one of its neighbour's)
+        auto take = [&](int i, bool whole) {       // AT_ONCE vectors from entry i on, every lane of a whole round inside the row
+            Pack<T, VEC> p[AT_ONCE];
+            Pack<uint8_t, VEC> q[AT_ONCE];
+            Place w[AT_ONCE];
             float v[AT_ONCE][VEC];
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) read_vec<T, VEC, MASK>(x, mask, i + u * STEP, n, v[u]);
+            for (int u = 0; u < AT_ONCE; u++) {
+                w[u] = whole ? Place{i + u * STEP, 0} : place_of<VEC>(i + u * STEP, n);
+                read_vec<T, VEC, MASK>(x, mask, w[u], p[u], q[u]);
+            }
+            if (TOP && MASK) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) {
+                    uint64_t bits = 0;
+                    __builtin_memcpy(&bits, &q[u], sizeof q[u]);
+                    allowed |= bits;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) widen_vec<T, VEC, MASK>(p[u], q[u], w[u].skip, v[u]);
             float m = t.m;
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++)
@@ -354,18 +388,22 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
             for (int u = 0; u < AT_ONCE; u++)
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float d = v[u][j] - base, w = exp_nat(d);
-                    t.s += w;
-                    t.e += weighted(w, d);
+                    const float d = v[u][j] - base, e = exp_nat(d);
+                    t.s += e;
+                    t.e += weighted(e, d);
                 }
-        }
+        };
+        int i0 = 0;
+        for (; i0 + STEP * AT_ONCE <= n; i0 += STEP * AT_ONCE) take(i0 + threadIdx.x * VEC, true);
+        if (i0 < n) take(i0 + threadIdx.x * VEC, false);
         const Sums wave_sum = lanes_joined<64>(t);
         uint32_t most = 0;               // of TOP: a word that no entry of the lane passes
         if (TOP) {
             // The maximum leaves NaN out, which is the largest of all; the sum knows of it (or of +inf).
-            // A lane without an entry above -inf may still hold allowed ones there: it counts as one.
+            // A lane without an entry above -inf may still hold allowed ones there: it counts as one, unless its mask
+            // allows none (a row that is masked out was looked through whole: 8 x 27,868 25 us, one of them empty).
             const bool odd = t.s != t.s;
-            const uint32_t word = (int)threadIdx.x * VEC >= n ? 0 : odd && t.m != INFINITY ? 0xFFFFFFFEu : ordered(t.m);
+            const uint32_t word = (int)threadIdx.x * VEC >= n || (MASK && !allowed) ? 0 : odd && t.m != INFINITY ? 0xFFFFFFFEu : ordered(t.m);
             words[threadIdx.x] = word;
             most = odd ? 0xFFFFFFFEu : word;
         }
@@ -537,7 +575,7 @@ __global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < a.rows; row += (int64_t)gridDim.x * GROUPS) {
         SmallRow<T, LANES, CH, MASK> r;
-        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane);
+        r.read((const T *)a.logits + row * a.stride, MASK ? a.mask + row * a.mask_stride : nullptr, a.vocab, lane, true);
         const RowGrad q = row_grad(a, row);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
@@ -545,10 +583,10 @@ __global__ __launch_bounds__(256) void k_tokens_small_bwd(const BackArgs a) {
             Pack<T, 4> o;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float d = grad_of(q, r.x[c][i]) + (col + i == q.tok ? q.g : 0.f);
+                const float d = grad_of(q, r.x[c][i]) + (r.at[c] + i == q.tok ? q.g : 0.f);
                 o.v[i] = (T)(r.in[c][i] ? d : 0.f);
             }
-            store_part<T, 4>((T *)a.dlogits + row * a.vocab + col, a.vocab - col, o);
+            store_part<T, 4>((T *)a.dlogits + row * a.vocab + r.at[c], col >= a.vocab ? 0 : a.vocab < 4 ? a.vocab : 4, o);
         }
     }
 }
@@ -565,27 +603,29 @@ __global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int split
         const uint8_t *mask = MASK ? a.mask + row * a.mask_stride + begin : nullptr;
         T *out = (T *)a.dlogits + row * a.vocab + begin;
         const RowGrad q = row_grad(a, row);
-        for (int i0 = threadIdx.x * VEC; i0 < n; i0 += STEP * AT_ONCE) {
+        auto take = [&](int i, bool whole) {
             Pack<T, VEC> p[AT_ONCE];
-            Pack<uint8_t, VEC> w[AT_ONCE];
+            Pack<uint8_t, VEC> in[AT_ONCE];
+            Place w[AT_ONCE];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
-                const int i = i0 + u * STEP;
-                p[u] = load_part<T, VEC>(x + i, n - i, (T)0.f);
-                if (MASK) w[u] = load_part<uint8_t, VEC>(mask + i, n - i, 0);
+                w[u] = whole ? Place{i + u * STEP, 0} : place_of<VEC>(i + u * STEP, n);
+                read_vec<T, VEC, MASK>(x, mask, w[u], p[u], in[u]);
             }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
-                const int i = i0 + u * STEP;
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
-                    const float d = grad_of(q, (float)p[u].v[j]) + (begin + i + j == q.tok ? q.g : 0.f);
-                    o.v[j] = (T)(!MASK || w[u].v[j] ? d : 0.f);
+                    const float d = grad_of(q, (float)p[u].v[j]) + (begin + w[u].at + j == q.tok ? q.g : 0.f);
+                    o.v[j] = (T)(!MASK || in[u].v[j] ? d : 0.f);
                 }
-                put_part<PAST>(out + i, n - i, o);
+                if (whole || w[u].skip < VEC) put_part<PAST>(out + w[u].at, VEC, o);
             }
-        }
+        };
+        int i0 = 0;
+        for (; i0 + STEP * AT_ONCE <= n; i0 += STEP * AT_ONCE) take(i0 + threadIdx.x * VEC, true);
+        if (i0 < n) take(i0 + threadIdx.x * VEC, false);
     }
 }
 
