@@ -54,9 +54,10 @@ __device__ __forceinline__ void read_row(Pack<T, VEC> (&a)[CH], const T *row, in
 }
 
 // Where a lane's chunks lie in the forward pass: whole packs, moved back at the row's end so that none passes it and no
-// branch keeps a load waiting (16,384 x 4,095 bf16: 61 us, 66 with branches; 7,554 x 11,823 fp16 85 and 97; 32,768 x 2,048 50 either way). The first
-// elements of a moved pack are another lane's, left out of the sums and stored twice alike. The first half of several
-// chunks always lies inside, since shorter rows take a smaller shape; only the smallest shape has rows below a pack.
+// branch keeps a load waiting (16,384 x 4,095 bf16: 61 us, 66 with branches; 7,554 x 11,823 fp16 85 and 97; 32,768 x
+// 2,048 50 either way). The first elements of a moved pack are another lane's, left out of the sums and stored twice
+// alike. The first half of several chunks always lies inside, since shorter rows take a smaller shape; only the smallest
+// shape has rows below a pack.
 template <int LANES, int CH, int VEC>
 struct Columns {
     int lane, width, back[CH];   // elements by which chunk c is moved back, VEC where it holds none of its own

@@ -6,7 +6,9 @@
 // a workgroup of 256 takes CHUNK adjacent elements of one of them, four at a time a lane, so each
 // operand is one 16-byte access. k_adamw_begin, one workgroup before the step, advances the step
 // count on the device, forms the two bias corrections in fp64 and, for a clip, adds the partial
-// sums of squares of k_adamw_norm (fp64, a fixed order: the same bits each time).
+// sums of squares of k_adamw_norm (fp64, a fixed order: the same bits each time). Up to JOIN_PARTS
+// partial sums are added by each of the step's workgroups instead, one launch less: the policy's
+// 0.53 M elements 10.9 -> 9.7 us, 1 M 12.5 and 12.2, but 4.2 M (2,048 sums) 29.1 and 31.2.
 //
 // 8-bit moments. 256 adjacent elements (a wave's four a lane) share one power of two, the exponent
 // e of their largest magnitude. An element is scaled by 2^(top-e) so that its fp32 exponent field
@@ -19,9 +21,9 @@
 
 namespace d1o {
 
-constexpr int CHUNK = 4096, SMALL_CHUNK = 1024, MAX_TENSORS = 40, NORM_GRID = 2048;
+constexpr int CHUNK = 4096, SMALL_CHUNK = 1024, MAX_TENSORS = 40, NORM_GRID = 2048, JOIN_PARTS = 1024;
 // of ctl
-constexpr int STEP = 0, SKIPPED = 1, COEF = 2, INV_BC1 = 3, INV_BC2 = 4, NORM = 5, GO = 6;
+constexpr int STEP = 0, SKIPPED = 1, COEF = 2, INV_BC1 = 3, INV_BC2 = 4, NORM = 5, GO = 6, BEFORE = 7;
 
 struct Tensors {
     void *p[MAX_TENSORS];
@@ -40,6 +42,24 @@ struct Rates {
     double log_b1, log_b2;
     uint64_t seed;
 };
+// The gradients' partial sums of squares where the step's workgroups add them themselves (nullptr: k_adamw_begin has).
+// `first`: workgroup 0 of this launch writes the new step count, the skips and the norm.
+struct Join {
+    const double *parts;
+    int32_t count, first;
+    double max_norm;
+};
+
+__device__ __forceinline__ void corrections(double log_b1, double log_b2, int step, float &inv1, float &inv2) {
+    inv1 = (float)(1.0 / -expm1((double)step * log_b1));
+    inv2 = (float)(1.0 / sqrt(-expm1((double)step * log_b2)));
+}
+// the factor of a clip; false for a norm that is not finite
+__device__ __forceinline__ bool clip_of(double norm, double max_norm, double &coef) {
+    coef = max_norm / (norm + 1e-6);
+    if (!(coef < 1.0)) coef = 1.0;
+    return isfinite(norm);
+}
 
 // the tensor of a chunk, and the chunk's number within it
 __device__ __forceinline__ int tensor_of(const Tensors &t, int chunk, int &within) {
@@ -81,9 +101,20 @@ __device__ __forceinline__ void add_squares(double &sum, const T *g, int64_t beg
 }
 
 // partial sums of squares of the gradients: each workgroup walks `per` chunks in a row
-__global__ __launch_bounds__(256) void k_adamw_norm(const Tensors t, int per, double *__restrict__ parts) {
+// For a step that joins them itself (`ctl`), workgroup 0 keeps the count before it and forms the bias corrections, since
+// the step's workgroups read these while one of them writes the new count.
+__global__ __launch_bounds__(256) void k_adamw_norm(const Tensors t, int per, double *__restrict__ parts, int32_t *__restrict__ ctl,
+                                                    double log_b1, double log_b2) {
     __shared__ double s[256];
     double sum = 0.0;
+    if (ctl && blockIdx.x == 0 && threadIdx.x == 255) {
+        const int before = ctl[STEP];
+        float inv1, inv2;
+        corrections(log_b1, log_b2, before + 1, inv1, inv2);
+        ctl[BEFORE] = before;
+        ctl[INV_BC1] = __float_as_int(inv1);
+        ctl[INV_BC2] = __float_as_int(inv2);
+    }
     int chunk = blockIdx.x * per, within;
     const int end = chunk + per < t.chunks ? chunk + per : t.chunks;
     int k = tensor_of(t, chunk, within);
@@ -107,11 +138,6 @@ __global__ __launch_bounds__(256) void k_adamw_norm(const Tensors t, int per, do
     if (threadIdx.x == 0) parts[blockIdx.x] = s[0];
 }
 
-__device__ __forceinline__ void corrections(double log_b1, double log_b2, int step, float &inv1, float &inv2) {
-    inv1 = (float)(1.0 / -expm1((double)step * log_b1));
-    inv2 = (float)(1.0 / sqrt(-expm1((double)step * log_b2)));
-}
-
 __global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl, const double *__restrict__ parts, int nparts,
                                                       double max_norm, double log_b1, double log_b2) {
     __shared__ double s[1024];
@@ -127,9 +153,7 @@ __global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl,
             __syncthreads();
         }
         const double norm = sqrt(s[0]);
-        go = isfinite(norm);
-        coef = max_norm / (norm + 1e-6);
-        if (!(coef < 1.0)) coef = 1.0;
+        go = clip_of(norm, max_norm, coef);
         if (threadIdx.x == 0) ctl[NORM] = __float_as_int((float)norm);
     }
     if (threadIdx.x) return;
@@ -268,12 +292,35 @@ __device__ __forceinline__ void step_chunk(const Tensors &t, int k, int within, 
 }
 
 template <int BITS, bool PAST>
-__global__ __launch_bounds__(256) void k_adamw_step(const Tensors t, const Rates r, const int32_t *__restrict__ ctl) {
-    if (!ctl[GO]) return;
+__global__ __launch_bounds__(256) void k_adamw_step(const Tensors t, const Rates r, const Join join, int32_t *ctl) {
+    __shared__ double s[4];
+    float coef;
+    int step;
+    if (join.parts) {
+        double sum = 0.0, c;
+        for (int i = threadIdx.x; i < join.count; i += 256) sum += join.parts[i];
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        const double norm = sqrt((s[0] + s[1]) + (s[2] + s[3]));
+        const bool go = clip_of(norm, join.max_norm, c);
+        step = ctl[BEFORE] + 1;
+        if (join.first && blockIdx.x == 0 && threadIdx.x == 0) {
+            ctl[NORM] = __float_as_int((float)norm);
+            if (go)
+                ctl[STEP] = step;
+            else
+                ctl[SKIPPED]++;
+        }
+        if (!go) return;
+        coef = (float)c;
+    } else {
+        if (!ctl[GO]) return;
+        coef = __int_as_float(ctl[COEF]);
+        step = ctl[STEP];
+    }
     int within;
     const int k = tensor_of(t, blockIdx.x, within);
-    const float coef = __int_as_float(ctl[COEF]);
-    const int step = ctl[STEP];
     float inv1 = __int_as_float(ctl[INV_BC1]), inv2 = __int_as_float(ctl[INV_BC2]);
     if (t.lag[k]) corrections(r.log_b1, r.log_b2, step > t.lag[k] ? step - t.lag[k] : 1, inv1, inv2);
     switch (t.types[k]) {
@@ -400,16 +447,20 @@ extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h
     Tensors l;
     double *parts = h->max_norm > 0 ? (double *)work : nullptr;
     int nparts = 0, e;
+    const bool join = parts && need <= JOIN_PARTS * (int64_t)sizeof(double) && need;
     if (parts)
         for (int at = 0; at < count;) {
             at = take(t, count, chunk, at, l);
             if (!l.count) break;
-            k_adamw_norm<<<norm_blocks(l), 256, 0, s>>>(l, norm_per(l), parts + nparts);
+            k_adamw_norm<<<norm_blocks(l), 256, 0, s>>>(l, norm_per(l), parts + nparts, join && !nparts ? ctl : nullptr, log_b1, log_b2);
             if ((e = (int)hipGetLastError())) return e;
             nparts += norm_blocks(l);
         }
-    k_adamw_begin<<<1, parts ? 1024 : 64, 0, s>>>(ctl, nparts ? parts : nullptr, nparts, h->max_norm, log_b1, log_b2);
-    if ((e = (int)hipGetLastError())) return e;
+    if (!join) {
+        k_adamw_begin<<<1, parts ? 1024 : 64, 0, s>>>(ctl, nparts ? parts : nullptr, nparts, h->max_norm, log_b1, log_b2);
+        if ((e = (int)hipGetLastError())) return e;
+    }
+    Join j{join ? parts : nullptr, nparts, 1, h->max_norm};
     const bool past = past_of(t, count, h->bits);
     const Rates r{(float)h->beta1, (float)(1.0 - h->beta1), (float)h->beta2, (float)(1.0 - h->beta2), (float)h->eps,
                   log_b1, log_b2, h->seed};
@@ -417,14 +468,15 @@ extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h
         at = take(t, count, chunk, at, l);
         if (!l.count) break;
         if (h->bits == 8 && past)
-            k_adamw_step<8, true><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+            k_adamw_step<8, true><<<l.chunks, 256, 0, s>>>(l, r, j, ctl);
         else if (h->bits == 8)
-            k_adamw_step<8, false><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+            k_adamw_step<8, false><<<l.chunks, 256, 0, s>>>(l, r, j, ctl);
         else if (past)
-            k_adamw_step<32, true><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+            k_adamw_step<32, true><<<l.chunks, 256, 0, s>>>(l, r, j, ctl);
         else
-            k_adamw_step<32, false><<<l.chunks, 256, 0, s>>>(l, r, ctl);
+            k_adamw_step<32, false><<<l.chunks, 256, 0, s>>>(l, r, j, ctl);
         if ((e = (int)hipGetLastError())) return e;
+        j.first = 0;
     }
     return 0;
 }

@@ -83,6 +83,27 @@ def test_32_bit(A, sizes, pdtype, gdtype, clip):
             assert all(torch.equal(c, x.to(torch.bfloat16)) for c, x in zip(copies, p))
 
 
+# partial sums of the norm up to where the step's workgroups add them (1,024 of 1,024 elements) and past it, one and
+# several launches of up to 40 tensors, and the long chunks from 4 M elements on
+@pytest.mark.parametrize('sizes', [[1 << 20], [(1 << 20) + 1], [26000] * 40, [26000] * 41, [4194303], [4194304, 9]],
+                         ids=lambda s: f'{len(s)}x{max(s)}')
+def test_clip_over_many_elements(A, sizes):
+    print(f'[adamw] clip {len(sizes)} tensors up to {max(sizes)}', flush=True)
+    p, g, m, v = tensors(sizes, len(sizes))
+    step = torch.zeros(8, dtype=torch.int32, device='cuda')
+    call = lambda: A.adamw_step(p, g, m, v, step, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, max_grad_norm=0.5)  # noqa: E731
+    for t in (1, 2):
+        before = [tuple(x.clone() for x in z) for z in zip(p, g, m, v)]
+        call()
+        coef, norm = clip_of(g, 0.5)
+        compare(list(zip(p, m, v)), before, t, coef)
+        assert step[:2].tolist() == [t, 0] and abs(float(step[5:6].view(torch.float32)) - norm) <= 2 * U * norm
+    kept = [x.clone() for x in (*p, *m, *v)]
+    g[-1][-1] = math.inf
+    call()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (*p, *m, *v))) and step[:2].tolist() == [2, 1]
+
+
 def eight(A, sizes):
     zeros = lambda n: torch.zeros(n, dtype=torch.uint8, device='cuda')  # noqa: E731
     return ([zeros(n) for n in sizes], [zeros(n) for n in sizes],
