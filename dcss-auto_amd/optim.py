@@ -27,7 +27,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     params: fp32 or bf16, contiguous. grads: fp32 or bf16 of the same sizes. exp_avg, exp_avg_sq:
     fp32 (32-bit moments), or uint8 codes with exps = (list of exp_avg's, list of exp_avg_sq's)
     exponents, uint8 of moment_blocks(numel) each, and counters: the first counter of each tensor's
-    rounding draws (a multiple of nothing; ranges that do not overlap draw independently). Zero codes
+    rounding draws, one an element (tensors whose ranges overlap round alike there). Zero codes
     and exponents are zero moments. step: int32 [8] on the device, zeros before the first step; [0]
     counts the steps made, [1] those skipped. copies: bf16 tensors that get the new fp32 parameters
     (None in the list: no copy). lr and weight_decay: one value or one for each tensor. lags: steps
@@ -52,8 +52,10 @@ class AdamW(torch.optim.Optimizer):
     lr and weight_decay may differ between groups; betas, eps, state_bits (32 or 8) and
     max_grad_norm (the clip by the global norm of all groups' gradients, 0 for none) are the
     optimizer's. copies: {parameter: bf16 tensor} that a step writes beside fp32 parameters. A
-    parameter without a gradient is left as it is and keeps its own step count. With max_grad_norm a
-    step whose norm is not finite changes nothing; skipped_steps() counts those."""
+    parameter without a gradient is left as it is and keeps its own step count; the step in which it
+    first takes part after others have, or does so again, waits for the device's count. With
+    max_grad_norm a step whose norm is not finite changes nothing; skipped_steps() counts those. The
+    state dict holds moments and counts; betas, eps and the clip are those of the new optimizer."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  max_grad_norm=0.0, copies=None, seed=0):
@@ -67,12 +69,20 @@ class AdamW(torch.optim.Optimizer):
         self.betas, self.eps, self.state_bits, self.max_grad_norm, self.seed = betas, eps, state_bits, max_grad_norm, seed
         self.copies = copies or {}
         self.ctl = None                 # the device's step count, skips and norm (adamw_step's `step`)
-        self._calls = self._counter = 0
+        self._counter = 0
+
+    def __getstate__(self):             # copies and pickles: the base class's holds no more than its own
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in (
+            'betas', 'eps', 'state_bits', 'max_grad_norm', 'seed', 'copies', 'ctl', '_counter')}}
 
     def _state(self, p):
         s = self.state[p]
-        if not s:
-            s['calls'], s['counter'] = 0, self._counter
+        if s:
+            if s['left'] is not None:   # steps made since it last took part
+                s['lag'] += int(self.ctl[0]) - int(s['left'])
+                s['left'] = None
+        else:
+            s['lag'], s['left'], s['counter'] = 0 if self.ctl is None else int(self.ctl[0]), None, self._counter
             self._counter += moment_blocks(p.numel()) * BLOCK
             dtype = torch.uint8 if self.state_bits == 8 else torch.float32
             for name in ('exp_avg', 'exp_avg_sq'):
@@ -95,6 +105,8 @@ class AdamW(torch.optim.Optimizer):
                     states.append(self._state(p))
                     lr.append(group['lr'])
                     decay.append(group['weight_decay'])
+                elif p in self.state and self.state[p]['left'] is None:
+                    self.state[p]['left'] = self.ctl[:1].clone()
         if not params:
             return loss
         if self.ctl is None:
@@ -106,10 +118,7 @@ class AdamW(torch.optim.Optimizer):
                    copies=[self.copies.get(p) for p in params] if self.copies else None,
                    exps=(column('exp_avg_exp'), column('exp_avg_sq_exp')) if eight else None,
                    counters=column('counter') if eight else None, seed=self.seed,
-                   lags=[self._calls - s['calls'] for s in states])
-        self._calls += 1
-        for s in states:
-            s['calls'] += 1
+                   lags=column('lag'))
         return loss
 
     def skipped_steps(self):
@@ -132,7 +141,7 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self):
         d = super().state_dict()
-        d['d1'] = dict(state_bits=self.state_bits, ctl=None if self.ctl is None else self.ctl.clone(), calls=self._calls,
+        d['d1'] = dict(state_bits=self.state_bits, ctl=None if self.ctl is None else self.ctl.clone(),
                        counter=self._counter, seed=self.seed)
         return d
 
@@ -150,4 +159,4 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][name] = value.to(p.device, copy=True).contiguous()
         device = self.param_groups[0]['params'][0].device
         self.ctl = None if own['ctl'] is None else own['ctl'].to(device, copy=True)
-        self._calls, self._counter, self.seed = own['calls'], own['counter'], own['seed']
+        self._counter, self.seed = own['counter'], own['seed']

@@ -22,7 +22,7 @@ class TokenLogprobs(NamedTuple):
 
     @property
     def lse(self):
-        """log sum exp of each row's allowed logits."""
+        """log sum exp of each row's allowed logits (without a gradient)."""
         return self.stats[..., 0] + self.stats[..., 1].log()
 
 

@@ -2,6 +2,7 @@
 64 bits (u = 2^-24: a moment is two products and a sum, 3 u of its terms; the step lr m/den adds about
 12 u of itself, the parameter 2 u), 8-bit moments bit for bit against a numpy restatement, the clip,
 the skip of a step that is not finite, many tensors, steps that tensors miss, graphs, checkpoints."""
+import copy
 import importlib
 import math
 
@@ -270,7 +271,7 @@ def test_optimizer(A, bits):
             saved = (opt.state_dict(), [p.detach().clone() for p in ps])
             saved[0]['state'] = {k: {n: x.clone() if torch.is_tensor(x) else x for n, x in s.items()} for k, s in saved[0]['state'].items()}
     assert torch.equal(ps[3], start) and torch.equal(copies[ps[0]], ps[0].to(torch.bfloat16))
-    assert opt.skipped_steps() == 0 and opt.state[ps[1]]['calls'] == 6
+    assert opt.skipped_steps() == 0 and opt.state[ps[1]]['lag'] == 2
     qs, again, _ = make(2)
     with torch.no_grad():
         for q, p in zip(qs, saved[1]):
@@ -284,6 +285,53 @@ def test_optimizer(A, bits):
         assert all(torch.equal(x, y) for x, y in zip(opt.moments(a), again.moments(b)))
     with pytest.raises(ValueError):
         A.AdamW(qs, state_bits=40 - bits).load_state_dict(saved[0])
+
+
+def test_own_step_counts(A):
+    """A parameter's count holds the steps that were made with it alone: not those it missed, nor
+    those skipped while it was there or away, and it follows steps replayed from a graph."""
+    print('[adamw] own step counts', flush=True)
+    gen = torch.Generator(device='cuda').manual_seed(8)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=gen, device='cuda')) for n in (50, 70, 90)]
+    ref = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt = A.AdamW(ps, lr=LR, weight_decay=WD, betas=(B1, B2), eps=EPS, max_grad_norm=1e9)
+    plain = torch.optim.AdamW(ref, lr=LR, weight_decay=WD, betas=(B1, B2), eps=EPS)
+    # parameters with a gradient, and whether the step's gradients are finite
+    plan = [('a', True), ('ab', False), ('ab', True), ('a', False), ('a', True), ('a', False), ('abc', True), ('bc', False), ('abc', True)]
+
+    def step(who, finite):
+        for k, (p, q) in enumerate(zip(ps, ref)):
+            here = 'abc'[k] in who
+            p.grad = torch.randn(p.shape, generator=gen, device='cuda') if here else None
+            q.grad = p.grad.clone() if here else None
+        if not finite:
+            ps['abc'.index(who[0])].grad[3] = math.inf
+        opt.step()
+        if finite:
+            plain.step()
+
+    for t, (who, finite) in enumerate(plan):
+        step(who, finite)
+        for a, b in zip(ps, ref):
+            torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+        if t == 5:
+            opt = copy.deepcopy(opt)             # a copy has parameters of its own: go on with those
+            ps = opt.param_groups[0]['params']
+    assert opt.ctl[:2].tolist() == [5, 4] and [opt.state[p]['lag'] for p in ps] == [0, 2, 3]
+    ps[1].grad = ps[2].grad = ref[1].grad = ref[2].grad = None
+    opt.step()
+    plain.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        plain.step()
+    step('abc', True)
+    for a, b in zip(ps, ref):
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+    assert int(opt.ctl[0]) == 10 and [opt.state[p]['lag'] for p in ps] == [0, 6, 7]
 
 
 @pytest.mark.parametrize('bits', [32, 8])
