@@ -216,8 +216,8 @@ __global__ __launch_bounds__(256) void k_tokens_small(const Args a) {
 
 // ---- longer rows: segments
 
-// Vectors of 16 bytes that a thread takes at once: two; four (512 x 50,001 fp16 31 us against 28, 4,096 x
-// 131,072 bf16 210 against 192) and eight (222) cost more waves than they hide.
+// Vectors of 16 bytes that a thread takes at once, a round of its loop: two; four (512 x 50,001 fp16 31 us against 28, 4,096
+// x 131,072 bf16 210 against 192) and eight (222) cost more waves than they hide.
 constexpr int AT_ONCE = 2, KEEP = 512, ROUND = 4;
 
 struct Parts {
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(PART) void k_tokens_part(const Args a, const Parts 
         if (TOP) {
             // The maximum leaves NaN out, which is the largest of all; the sum knows of it (or of +inf).
             // A lane without an entry above -inf may still hold allowed ones there: it counts as one, unless its mask
-            // allows none (a row that is masked out was looked through whole: 8 x 27,868 25 us, one of them empty).
+            // allows none (8 x 27,868, one of them masked out: 12 us, 25 where that one is looked through whole).
             const bool odd = t.s != t.s;
             const uint32_t word = (int)threadIdx.x * VEC >= n || (MASK && !allowed) ? 0 : odd && t.m != INFINITY ? 0xFFFFFFFEu : ordered(t.m);
             words[threadIdx.x] = word;
@@ -629,26 +629,31 @@ __global__ __launch_bounds__(PART) void k_tokens_bwd(const BackArgs a, int split
     }
 }
 
-// How long rows are cut. A workgroup takes a whole row, which saves k_tokens_join and its launch, where that still fills the card or
-// the row is short; us for bf16 without and with 20 alternatives:
-//   64 threads, many short rows: 8,192 x 1,500 10.0 and (5 alternatives) 14.7 against 16.5 and 33.7 on 256; 16,384 x 20,000 with 5
-//     185 against 175 on 256
-//   256, rows up to 12 KB, or 48 KB from 512 rows on: 1 x 5,000 4.1 and 6.4 against 6.6 and 11.1 in segments; 1,024 x 20,000
-//     11.6 and 20.0 against 15.9 and 28.8
-//   512, up to 104 KB for fewer rows than fill the card on 256: 1 x 20,000 4.4 and 8.9 against 6.7 and 11.8 in segments; 512 x 50,001
-//     15.7 and 24.6 against 19.0 and 30.4; 128 x 100,000 15.2 and 26.9 against 11.8 and 22.0
-//   else segments of 256 threads, equally long, about six workgroups a CU, of one vector a thread at least, at most 64 (the
-//     join's lanes): 300 x 131,072 with 20 82 us at 300 workgroups, 39 at 1,200, 41 at 4,800
+// How long rows are cut. A workgroup takes a whole row, which saves k_tokens_join and its launch, where that still fills the
+// card or the row is short; us for bf16 without and with 20 alternatives:
+//   64 threads, many short rows (4 KB; 12 KB from 2,048 rows, 20 KB from 4,096): 8,192 x 1,500 9.6 and 18.5, on 256 threads
+//     18.3 and 39.4; 4,096 x 8,000 15.9 and 33.1, 16.7 and 31.9; 2,048 x 12,000 14.9 and 33.6, 12.4 and 22.9
+//   256, up to 40 KB: 1 x 5,000 3.0 and 5.8, in segments 4.5 and 10.6; 1,024 x 20,000 10.3 and 17.8, in four 17.7 and 33.2
+//   512, up to 64 KB, 128 KB from 96 rows, any from 384: 256 x 60,000 8.9 and 15.9, in four segments 11.8 and 21.5; 512 x
+//     131,072 28.3 and 38.7, in three 31.1 and 53.6; but 300 x 131,072 25.9 and 34.8, in four 21.8 and 33.9
+//   256 again from 768 rows up to 160 KB: 1,200 x 60,000 31.6 and 47.6, on 512 36.0 and 51.8; 2,000 x 131,072 101 and 151,
+//     95 and 131
+//   else segments of 256 threads, equally long, at most 64 (the join's lanes): up to two workgroups a CU of a vector a thread
+//     at least, up to four of a round at least: 128 x 250,000 18.9 and 30.4 at 1,024 workgroups, 21.8 and 37.7 at 512, 20.1 and
+//     34.7 at 1,536; 70 x 131,072 10.4 and 18.5 at 980, 11.3 and 19.7 at 1,050; 16 x 60,000 5.4 and 11.5 at 16 segments, 5.8 and
+//     11.7 at 32; 3 x 131,072 4.9 and 10.8 at 42, 5.3 and 11.8 at 21
 struct Cut {
     int part, splits, seg;        // threads, segments a row, entries of one
 };
 inline Cut cut_of(int64_t rows, int vocab, int type) {
     const int64_t size = type == D1_FP32 ? 4 : 2, bytes = vocab * size;
-    if (rows >= 2048 && vocab <= 12288) return {64, 1, vocab};
-    if (bytes <= 12 << 10 || (rows >= 512 && bytes <= 48 << 10) || rows >= 1536) return {256, 1, vocab};
-    if (bytes <= 104 << 10) return {512, 1, vocab};
-    const int64_t step = 256 * (16 / size), want = (1536 + rows - 1) / rows, most = (vocab + step - 1) / step;
-    const int64_t few = want < 64 ? want : 64, splits = few < most ? few : most;
+    if (bytes <= (rows >= 4096 ? 20 : rows >= 2048 ? 12 : 4) << 10) return {64, 1, vocab};
+    if (bytes <= 40 << 10) return {256, 1, vocab};
+    if (bytes <= 64 << 10 || (rows >= 96 && bytes <= 128 << 10) || rows >= 384)
+        return {rows >= 768 && bytes <= 160 << 10 ? 256 : 512, 1, vocab};
+    const auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+    const int64_t step = 256 * (16 / size), few = least(512 / rows, (vocab + step - 1) / step);
+    const int64_t many = least(1024 / rows, vocab / (step * AT_ONCE)), splits = least(few > many ? few : many, 64);
     const int seg = (int)(((vocab + splits - 1) / splits + 7) / 8 * 8);
     return {256, (vocab + seg - 1) / seg, seg};
 }
@@ -702,19 +707,23 @@ int fwd(const Args &a, const Parts &p, hipStream_t s) {
 template <class T, bool MASK>
 int bwd(const BackArgs &a, hipStream_t s) {
     if (a.vocab <= SMALL_BWD_VOCAB) return small_bwd<T, MASK>(a, s);
-    // Large outputs go past the caches, and a workgroup takes two rounds of them (4,096 x 131,072 bf16: 359 us, 391 with
-    // one round, 449 through the caches; 512 x 50,001 fp16: 22.3, 23.0 and 28.2). Rows up to 4,096 entries leave most of 256
-    // threads idle in their last round: a wave with twice the rounds takes them (20,000 x 1,100 bf16 23.8 us, 39.2 on 256;
-    // 8,192 x 1,500 12.9 and 18.4; 10,000 x 2,500 22.9 and 28.5; 16,000 x 6,377 94 and 83).
-    const bool past = a.rows * (int64_t)a.vocab * (int64_t)sizeof(T) > PAST_BYTES, wave = a.vocab <= 4096;
-    const int seg = (past ? 2 : 1) * AT_ONCE * (wave ? 128 : 256) * (16 / (int)sizeof(T)), splits = (a.vocab + seg - 1) / seg;
+    // Results that the last cache (256 MB) does not hold go past the caches, a wave a round of one (4,096 x 131,072 bf16 343 us,
+    // 348 on 256 threads, 367 there with two rounds; 4,096 x 131,071 377, 412 and 436) or of a row up to two (100,000 x 1,100
+    // 83 whole, 108 in rounds). Others stay where the next kernel reads them (16,000 x 4,000 42 us, 51 past the caches; 1,024 x
+    // 50,000 fp32 71 and 67).
+    // Of those, many rows go whole to 64 threads up to 8 KB (20,000 x 1,100 20.5, on 256 34; 16,000 x 4,001 46.5 and 56) or 256
+    // up to 32 KB (8,000 x 9,000 47, in two-round segments 62); longer rows take two rounds a workgroup (1,024 x 50,000 33.8, one
+    // round 35.9, four 39.9), where there are few one (300 x 60,001 13.4, two 14.8; 300 x 131,072 27.8 and 26.4).
+    const int64_t size = sizeof(T), bytes = a.vocab * size;
+    const bool past = a.rows * bytes > 8 * PAST_BYTES, whole = past ? bytes <= 4 << 10 : a.rows >= 1024 && bytes <= 32 << 10;
+    const int round = AT_ONCE * (past ? 64 : 256) * (16 / (int)size);
+    const int seg = whole ? a.vocab : past || a.rows < 512 ? round : 2 * round;
+    const int splits = (a.vocab + seg - 1) / seg;
     const unsigned grid = blocks_of(a.rows * splits);
-    if (wave && past)
+    if (past)
         k_tokens_bwd<T, 64, MASK, true><<<grid, 64, 0, s>>>(a, splits, seg);
-    else if (wave)
+    else if (whole && bytes <= 8 << 10)
         k_tokens_bwd<T, 64, MASK, false><<<grid, 64, 0, s>>>(a, splits, seg);
-    else if (past)
-        k_tokens_bwd<T, 256, MASK, true><<<grid, 256, 0, s>>>(a, splits, seg);
     else
         k_tokens_bwd<T, 256, MASK, false><<<grid, 256, 0, s>>>(a, splits, seg);
     return (int)hipGetLastError();

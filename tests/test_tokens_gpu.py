@@ -372,3 +372,16 @@ def test_rows_in_segments(T, rows, vocab, dtype):
     out = T.token_logprobs(odd, tokens, top=1)
     assert torch.isnan(out.entropy[rows - 1]) and out.top_ids[rows - 1, 0] == vocab - 1
     assert not torch.isnan(out.entropy[:rows - 1]).any()
+
+
+@pytest.mark.parametrize('rows,vocab,dtype', [(rows, vocab, dtype) for rows, vocab in ((2050, 3001), (4100, 5000), (1100, 9001), (800, 33001))
+                                              for dtype in (torch.float32, torch.bfloat16, torch.float16)]
+                         + [(127000, 1100, torch.bfloat16), (64100, 2111, torch.bfloat16)],
+                         ids=lambda x: str(x).replace('torch.', ''))
+def test_many_rows(T, rows, vocab, dtype):
+    """Whole rows on a wave and on workgroups; results past what the caches hold."""
+    print(f'[tokens] many rows {rows} x {vocab} {dtype}', flush=True)
+    logits, tokens, g, h = inputs(rows, vocab, dtype, rows + vocab, pad=3)
+    check(T, logits, tokens, top=4, g=g, h=h)
+    mask = torch.rand(vocab, device='cuda', generator=torch.Generator(device='cuda').manual_seed(vocab)) < 0.4
+    check(T, logits, tokens, mask=mask, g=g, h=h)
