@@ -206,6 +206,42 @@ def test_not_finite(A, bits):
         assert not math.isfinite(float(p[1][4321])) and int((~torch.isfinite(p[1])).sum()) == 1 and torch.isfinite(p[0]).all()
 
 
+def test_offsets_past_32_bits(A):
+    """A tensor of more than 2^32 elements: its last ones, in both kinds of moments."""
+    print('[adamw] offsets', flush=True)
+    n, tail = 2 ** 32 + 1031, 2000
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device='cuda'), torch.zeros(n, dtype=torch.bfloat16, device='cuda')
+    last, lastg, m0, v0 = (x[0] for x in tensors([tail], 12, torch.bfloat16, torch.bfloat16))
+    zero = torch.zeros_like(m0)
+    for bits in (32, 8):
+        p[-tail:], g[-tail:] = last, lastg
+        dtype = torch.uint8 if bits == 8 else torch.float32
+        m, v = torch.zeros(n, dtype=dtype, device='cuda'), torch.zeros(n, dtype=dtype, device='cuda')
+        exps = tuple([torch.zeros(A.moment_blocks(n), dtype=torch.uint8, device='cuda')] for _ in range(2)) if bits == 8 else None
+        step = torch.zeros(8, dtype=torch.int32, device='cuda')
+        A.adamw_step([p], [g], [m], [v], step, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, max_grad_norm=0.05, exps=exps)
+        coef, norm = clip_of([lastg], 0.05)
+        assert abs(float(step[5:6].view(torch.float32)) - norm) <= 2 * U * norm
+        if bits == 32:
+            compare([(p[-tail:], m[-tail:], v[-tail:])], [(last, lastg, zero, zero)], 1, coef)
+        else:
+            q = [x.clone() for x in (last, lastg)]
+            one = A.adamw_step
+            state = eight(A, [tail])
+            twin = torch.zeros(8, dtype=torch.int32, device='cuda')
+            one([q[0]], [q[1]], state[0], state[1], twin, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, max_grad_norm=0.05, exps=state[2])
+            assert torch.equal(p[-tail:], q[0])          # the step is made before moments are rounded
+            read = A.read_moment(m, exps[0][0], signed=True)
+            wide = formula(last, lastg, zero, zero, 1, coef)[1]
+            block = wide.abs().max()
+            assert float(((read[-tail:].double() - wide).abs() - wide.abs() / 8 - block * 2.0 ** -16).max()) <= 0
+            del read
+        assert not bool(p[:tail].any()) and not bool(m[:tail].any())
+        del m, v, exps
+    del p, g
+    torch.cuda.empty_cache()
+
+
 def test_strides_and_streams(A):
     print('[adamw] strides', flush=True)
     flat = torch.randn(5000, device='cuda')

@@ -229,3 +229,29 @@ def test_refusals(N):
                  (dy, x, w, b, mean.double(), rstd)):
         with pytest.raises(ValueError):
             N.layer_norm_bwd(*args)
+
+
+def test_offsets_past_32_bits(N):
+    """Rows 2^31 elements apart, and results of more than 2^32 elements."""
+    print('[norm] offsets', flush=True)
+    rows, width, apart = 3, 1031, 2 ** 31 + 8
+    x, dy, w, b = inputs(rows, width, torch.bfloat16, torch.float32, 5)
+    far, fardy = (torch.empty((rows - 1) * apart + width, dtype=torch.bfloat16, device='cuda').as_strided((rows, width), (apart, 1))
+                  for _ in range(2))
+    far.copy_(x)
+    fardy.copy_(dy)
+    check(N, far, fardy, w, b)
+    del far, fardy
+    rows, width = 262400, 16384
+    x, dy, w, b = inputs(1, width, torch.bfloat16, torch.float32, 6)
+    y, mean, rstd = N.layer_norm_fwd(x.expand(rows, width), w, b)
+    one = N.layer_norm_fwd(x, w, b)
+    assert torch.equal(y[rows - 1:], one[0]) and torch.equal(y[rows - 2:rows - 1], one[0]) and bool((mean == one[1]).all())
+    del y
+    dx, dw, db = N.layer_norm_bwd(dy.expand(rows, width), x.expand(rows, width), w, b, mean, rstd)
+    one = N.layer_norm_bwd(dy, x, w, b, *one[1:])
+    assert torch.equal(dx[rows - 1:], one[0]) and torch.equal(dx[rows - 2:rows - 1], one[0])
+    # rows equal terms of a column: partial sums of a workgroup's rows one after the other, then of the workgroups
+    assert float(((db.double() - rows * one[2].double()).abs() - U * (rows / 256 + 64) * rows * dy[0].double().abs()).max()) <= 0
+    del dx
+    torch.cuda.empty_cache()

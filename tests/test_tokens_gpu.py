@@ -385,3 +385,29 @@ def test_many_rows(T, rows, vocab, dtype):
     check(T, logits, tokens, top=4, g=g, h=h)
     mask = torch.rand(vocab, device='cuda', generator=torch.Generator(device='cuda').manual_seed(vocab)) < 0.4
     check(T, logits, tokens, mask=mask, g=g, h=h)
+
+
+def test_offsets_past_32_bits(T):
+    """Rows 2^31 elements apart, masks too, and a gradient of more than 2^32 elements."""
+    print('[tokens] offsets', flush=True)
+    rows, vocab, apart = 3, 1031, 2 ** 31 + 8
+    logits, tokens, g, h = inputs(rows, vocab, torch.float16, 77)
+    mask = torch.rand(rows, vocab, device='cuda', generator=torch.Generator(device='cuda').manual_seed(3)) < 0.5
+    far = torch.empty((rows - 1) * apart + vocab, dtype=torch.float16, device='cuda').as_strided((rows, vocab), (apart, 1))
+    far_mask = torch.empty((rows - 1) * apart + vocab, dtype=torch.bool, device='cuda').as_strided((rows, vocab), (apart, 1))
+    far.copy_(logits)
+    far_mask.copy_(mask)
+    check(T, far, tokens, mask=far_mask, top=5, g=g, h=h)
+    check(T, far[:, :200], tokens.clamp(max=199), mask=far_mask[:, :200], top=5, g=g, h=h)
+    del far, far_mask
+    rows, vocab = 260, 1 << 24
+    one = torch.randn(1, vocab, device='cuda', generator=torch.Generator(device='cuda').manual_seed(4)).to(torch.bfloat16)
+    logits, tokens = one.expand(rows, vocab), torch.full((rows,), vocab - 5, device='cuda')
+    g, h = torch.ones(rows, device='cuda'), torch.ones(rows, device='cuda')
+    out = T.token_logprobs(logits, tokens)
+    first = T.token_logprobs(one, tokens[:1])
+    close(out.logp, first.logp.double().expand(rows), 1e-5, 'logp')
+    d = T.token_logprobs_bwd(logits, tokens, out, g, h)
+    assert torch.equal(d[rows - 1], d[0]) and torch.equal(d[rows - 2], d[0]) and float(d[rows - 1, vocab - 5]) > 0.9
+    del d
+    torch.cuda.empty_cache()
