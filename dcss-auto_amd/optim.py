@@ -53,7 +53,8 @@ class AdamW(torch.optim.Optimizer):
     max_grad_norm (the clip by the global norm of all groups' gradients, 0 for none) are the
     optimizer's. copies: {parameter: bf16 tensor} that a step writes beside fp32 parameters. A
     parameter without a gradient is left as it is and keeps its own step count; the step in which it
-    first takes part after others have, or does so again, waits for the device's count. With
+    first takes part after others have, or does so again, waits for the device's count. A step can be
+    captured in a graph after one with the same parameters taking part. With
     max_grad_norm a step whose norm is not finite changes nothing; skipped_steps() counts those. The
     state dict holds moments and counts; betas, eps and the clip are those of the new optimizer."""
 
@@ -75,13 +76,20 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), **{k: getattr(self, k) for k in (
             'betas', 'eps', 'state_bits', 'max_grad_norm', 'seed', 'copies', 'ctl', '_counter')}}
 
+    @staticmethod
+    def _not_captured():                # what a replay would do again, or not at all
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('before a step is captured, make one with the same parameters taking part')
+
     def _state(self, p):
         s = self.state[p]
         if s:
             if s['left'] is not None:   # steps made since it last took part
+                self._not_captured()
                 s['lag'] += int(self.ctl[0]) - int(s['left'])
                 s['left'] = None
         else:
+            self._not_captured()
             s['lag'], s['left'], s['counter'] = 0 if self.ctl is None else int(self.ctl[0]), None, self._counter
             self._counter += moment_blocks(p.numel()) * BLOCK
             dtype = torch.uint8 if self.state_bits == 8 else torch.float32
@@ -105,7 +113,8 @@ class AdamW(torch.optim.Optimizer):
                     states.append(self._state(p))
                     lr.append(group['lr'])
                     decay.append(group['weight_decay'])
-                elif p in self.state and self.state[p]['left'] is None:
+                elif self.state.get(p) and self.state[p]['left'] is None:
+                    self._not_captured()
                     self.state[p]['left'] = self.ctl[:1].clone()
         if not params:
             return loss
@@ -133,7 +142,9 @@ class AdamW(torch.optim.Optimizer):
 
     def moments(self, p):
         """fp32 (exp_avg, exp_avg_sq) of a parameter."""
-        s = self.state[p]
+        s = self.state.get(p)
+        if not s:
+            raise ValueError('no step was made with this parameter')
         if self.state_bits == 32:
             return s['exp_avg'], s['exp_avg_sq']
         return (read_moment(s['exp_avg'], s['exp_avg_exp'], signed=True),

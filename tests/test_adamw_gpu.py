@@ -370,6 +370,36 @@ def test_own_step_counts(A):
     assert int(opt.ctl[0]) == 10 and [opt.state[p]['lag'] for p in ps] == [0, 6, 7]
 
 
+def test_capture_needs_a_step_before(A, monkeypatch):
+    """Moments made, or a count taken, inside a capture would be made again at each replay."""
+    print('[adamw] before a capture', flush=True)
+    ps = [torch.nn.Parameter(torch.ones(5, device='cuda')) for _ in range(2)]
+    opt = A.AdamW(ps, lr=LR)
+    with pytest.raises(ValueError):
+        opt.moments(ps[0])
+
+    def step(first, second, captured):
+        for p, here in zip(ps, (first, second)):
+            p.grad = torch.ones(5, device='cuda') if here else None
+        with monkeypatch.context() as patch:
+            patch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: captured)
+            opt.step()
+
+    with pytest.raises(RuntimeError):
+        step(True, False, True)
+    opt = A.AdamW(ps, lr=LR)
+    step(True, True, False)
+    step(True, True, True)
+    with pytest.raises(RuntimeError):
+        step(True, False, True)
+    step(True, False, False)
+    step(True, False, True)
+    with pytest.raises(RuntimeError):
+        step(True, True, True)
+    step(True, True, False)
+    assert int(opt.ctl[0]) == 5 and [opt.state[p]['lag'] for p in ps] == [0, 2]
+
+
 @pytest.mark.parametrize('bits', [32, 8])
 def test_graph_replays(A, bits):
     """The step count advances on the device: each replay is the next step."""
