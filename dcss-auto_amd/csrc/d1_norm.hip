@@ -286,8 +286,8 @@ inline int64_t groups_of_rows(int64_t rows, int lanes) {
     return (rows + groups - 1) / groups;
 }
 // Forward: workgroups walk the rows with a stride of the grid; more of them than fit at once even out
-// their ends, up to where reading the weights again costs (65,536 x 256 bf16: 14.2 us at 4,096, 15.0 at 1,024, 15.9
-// at 8,192; 65,536 x 1,024: 88, 52.2 and 52.6 at 1,024, 4,096 and 8,192; 16,384 x 8,192: 103 at 1,024, 109 at 4,096).
+// their ends, up to where reading the weights again costs (65,536 x 256 bf16: 14.8 us at 1,024, 14.3 at 4,096, 14.4
+// at 8,192; 65,536 x 1,024: 87, 52.3 and 52.9; 16,384 x 8,192: 102, 105 and 111).
 inline int fwd_grid(int64_t rows, int lanes) {
     const int64_t need = groups_of_rows(rows, lanes), most = lanes == 1024 ? 1024 : lanes == 512 || lanes < 64 ? 4096 : 8192;
     return (int)(need < most ? need : most);
@@ -302,8 +302,8 @@ inline int bwd_grid(int64_t rows, int lanes, int ch) {
     return (int)(need < most ? need : most);
 }
 
-// Whether the result goes past the caches: large ones of rows of several chunks a lane (8,192 x 16,384 bf16 forward 129 us
-// through the caches, 97 past them, backward 208 and 187). At one chunk a lane it is as fast or slower
+// Whether the result goes past the caches: large ones of rows of several chunks a lane (8,192 x 16,384 bf16 forward 100 us
+// through the caches, 97 past them, backward 195 and 169; 6,000 x 16,384 fp32 234 and 234). At one chunk a lane it is as fast or slower
 // (65,536 x 512 forward 25.7 and 28.3, backward 42.2 and 41.7).
 inline bool past_of(int64_t rows, int width, int ch, size_t size) { return ch > 1 && rows * width * (int64_t)size > PAST_BYTES; }
 

@@ -671,7 +671,7 @@ inline unsigned blocks_of(int64_t units) { return (unsigned)(units < (1 << 20) ?
 
 // Lanes a row and chunks of four a lane for short rows: several rows a wave and several chunks a lane, since reductions over
 // lanes cost as much as the entries (83,378 x 189 bf16: 12.4 us on 16 lanes x 4 chunks, 21.3 on 64 x 1; 62,655 x 89 with 20
-// alternatives 32 on 8 x 4, 111 on 64 x 1; 30,000 x 500 fp32 with 5 24.5 on 32 x 4, 41 on 64 x 4; 65,536 x 25 with 3 and a
+// alternatives 34 on 8 x 4, 111 on 64 x 1; 30,000 x 500 fp32 with 5 24.5 on 32 x 4, 41 on 64 x 4; 65,536 x 25 with 3 and a
 // mask 6.4 on 8 x 1, 9.7 on 16 x 1).
 #define D1O_SMALL_SHAPES(X) X(4, 1) X(8, 1) X(8, 2) X(8, 4) X(16, 4) X(32, 4)
 
