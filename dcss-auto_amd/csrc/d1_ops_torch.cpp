@@ -58,6 +58,12 @@ Tensor like(const Tensor &t, at::IntArrayRef shape, at::ScalarType type, const T
 void *ptr(const Tensor &t) { return t.data_ptr(); }
 void *ptr(const Maybe &t) { return t ? t->data_ptr() : nullptr; }
 Tensor scratch(int64_t bytes, const Tensor &x) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
+// The kernels write through raw pointers, which torch does not see: a caller's tensor that a call has changed gets a new
+// version, as from any operation in place, for autograd's check of saved tensors and for what is kept by version
+// (Policy.packed). Tensors made under inference mode have none.
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // ---- tokens
 
@@ -288,6 +294,15 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
     Maybe work;
     if (need) work = scratch(need, step);
     check(d1_adamw_step(table.data(), (int)count, &h, (int32_t *)ptr(step), ptr(work), need, (void *)stream), "d1_adamw_step");
+    for (size_t i = 0; i < count; i++) {
+        for (const Tensor *t : {&params[i], &exp_avg[i], &exp_avg_sq[i]}) written(*t);
+        if (copies && (*copies)[i]) written(*(*copies)[i]);
+        if (eight) {
+            written((*m_exps)[i]);
+            written((*v_exps)[i]);
+        }
+    }
+    written(step);
 }
 
 Tensor adamw_read(const Tensor &code, const Tensor &exp, bool is_signed, const Maybe &out_, int64_t stream) {
@@ -300,6 +315,7 @@ Tensor adamw_read(const Tensor &code, const Tensor &exp, bool is_signed, const M
     const Tensor out = out_ ? *out_ : at::empty(code.sizes(), code.options().dtype(at::kFloat));
     check(d1_adamw_read((const uint8_t *)ptr(code), (const uint8_t *)ptr(exp), n, is_signed, (float *)ptr(out), (void *)stream),
           "d1_adamw_read");
+    written(out);
     return out;
 }
 

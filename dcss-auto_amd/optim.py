@@ -30,7 +30,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     rounding draws, one an element (tensors whose ranges overlap round alike there). Zero codes
     and exponents are zero moments. step: int32 [8] on the device, zeros before the first step; [0]
     counts the steps made, [1] those skipped. copies: bf16 tensors that get the new fp32 parameters
-    (None in the list: no copy). lr and weight_decay: one value or one for each tensor. lags: steps
+    (None in the list: no copy). What the call changes gets a new version, as from torch's operations in
+    place; the replay of a captured call cannot give it one. lr and weight_decay: one value or one for each tensor. lags: steps
     that each tensor has missed.
 
     With max_grad_norm > 0 the gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with

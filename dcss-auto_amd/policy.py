@@ -55,7 +55,7 @@ class Policy(nn.Module):
     def packed(self, dtype=torch.bfloat16, refresh=False):
         """(packed bf16 weights, b1, b2, b3) for d1_policy_fwd, rebuilt when a parameter's
         storage or version counter changes (optimizer steps and copy_ bump it; writes through
-        .data do not: pass refresh=True after those)."""
+        .data and steps that a graph replays do not: pass refresh=True after those)."""
         params = (self.l1.weight, self.l2.weight, self.head.weight, self.l1.bias, self.l2.bias, self.head.bias)
         key = (dtype,) + tuple((q.data_ptr(), q._version) for q in params)
         if refresh or getattr(self, '_packed_key', None) != key:
