@@ -32,7 +32,16 @@ int type_of(at::ScalarType t) {
     return t == at::kFloat ? D1_FP32 : t == at::kBFloat16 ? D1_BF16 : t == at::kHalf ? D1_FP16 : -1;
 }
 
+// Forward-mode tangents are lost in a kernel call, so they are refused here. Inside an autograd function's forward torch
+// hides them and refuses by itself.
+void no_tangent(const Tensor &t, const char *name) {
+    if (!t._fw_grad(0).defined()) return;
+    PyErr_SetString(PyExc_NotImplementedError, (std::string(name) + " has a forward-mode tangent: the operators have none").c_str());
+    throw py::error_already_set();
+}
+
 int rows_type(const Tensor &x, const char *name) {
+    no_tangent(x, name);
     if (!x.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor (there is no CPU fallback)");
     const int code = type_of(x.scalar_type());
     if (code < 0) refuse(std::string(name) + " must be fp32, bf16 or fp16, not " + c10::toString(x.scalar_type()));
@@ -49,6 +58,7 @@ Tensor as_rows(const Tensor &x) {
 
 // t as a contiguous tensor of that type and shape on x's device
 Tensor like(const Tensor &t, at::IntArrayRef shape, at::ScalarType type, const Tensor &x, const char *name) {
+    no_tangent(t, name);
     if (t.scalar_type() != type || t.sizes() != shape || t.device() != x.device())
         refuse(std::string(name) + " must be " + c10::toString(type) + " of " + c10::str(shape) + " on " + x.device().str() +
                ", not " + describe(t));
@@ -183,6 +193,7 @@ py::tuple norm_fwd(const Tensor &x, const Maybe &weight, const Maybe &bias, doub
 py::tuple norm_bwd(const Tensor &dy, const Tensor &x, const Maybe &weight, const Maybe &bias, const Tensor &mean_, const Tensor &rstd_,
                    int64_t stream) {
     const NormArgs a = norm_args(x, weight, bias);
+    no_tangent(dy, "dy");
     if (dy.sizes() != x.sizes() || dy.scalar_type() != x.scalar_type() || dy.device() != x.device())
         refuse("dy must be like x, " + describe(x) + ", not " + describe(dy));
     const Tensor drows = as_rows(dy);
@@ -238,6 +249,8 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
         Tensor g = grads[i];
         const int64_t n = p.numel();
         auto fail = [&](const std::string &why) { refuse("tensor " + std::to_string(i) + ": " + why); };
+        no_tangent(p, "parameter");
+        no_tangent(g, "gradient");
         const int ptype = type_of(p.scalar_type()), gtype = type_of(g.scalar_type());
         if (!(ptype == D1_FP32 || ptype == D1_BF16) || !(gtype == D1_FP32 || gtype == D1_BF16))
             fail("parameter and gradient must be fp32 or bf16, not " + describe(p) + " and " + describe(g));
