@@ -8,7 +8,7 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from .ops import call
+from .ops import call, call_recorded
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
@@ -25,7 +25,7 @@ def layer_norm_bwd(dy, x, weight, bias, mean, rstd):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_fwd(x, weight, bias, eps)
+        y, mean, rstd = call_recorded('norm_fwd', x, x, weight, bias, eps)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
 
@@ -38,9 +38,9 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm of x [..., width] (fp32, bf16 or fp16; rows of any stride, up to 16,384 elements)
     with an optional weight and bias [width] in fp32 or x's type; statistics in fp32."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_fwd(x, weight, bias, eps)[0]
+    return call_recorded('norm_fwd', x, x, weight, bias, eps)[0]
 
 
 class LayerNorm(nn.Module):

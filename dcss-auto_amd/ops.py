@@ -13,7 +13,15 @@ _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or \
 
 
 def call(name, x, *args):
-    """An operator's C++ call with x's GPU as the current device and its current stream."""
+    """call_recorded, refused in torch.jit.trace: that would record the outputs being made, but not what fills them."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f'{name} cannot be part of a trace (token_logprobs and layer_norm can)')
+    return call_recorded(name, x, *args)
+
+
+def call_recorded(name, x, *args):
+    """An operator's C++ call with x's GPU as the current device and its current stream; for an autograd function's
+    forward, which a trace records whole."""
     function = getattr(_lib.load_ops_torch(), name)
     index = x.get_device()
     if index < 0:
