@@ -4,6 +4,7 @@
 // three allocations take in Python (11 us a call there, 6 here, 3 of them the launch itself). Checks, outputs
 // and scratch memory are therefore made here; the kernels and their C ABI know nothing of torch. Argument errors
 // are ValueError before any launch. The caller has made the tensors' device the current one and gives its stream.
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -38,6 +39,13 @@ void no_tangent(const Tensor &t, const char *name) {
     if (!t._fw_grad(0).defined()) return;
     PyErr_SetString(PyExc_NotImplementedError, (std::string(name) + " has a forward-mode tangent: the operators have none").c_str());
     throw py::error_already_set();
+}
+
+// torch.jit.trace would record that outputs are made, but not what fills them. Only the forward of an autograd function
+// may run in one, which records the function as a whole.
+void no_trace(const char *name) {
+    if (torch::jit::tracer::isTracing())
+        throw std::runtime_error(std::string(name) + " cannot be part of a trace (token_logprobs and layer_norm can)");
 }
 
 int rows_type(const Tensor &x, const char *name) {
@@ -134,6 +142,7 @@ py::tuple tokens_fwd(const Tensor &logits, const Tensor &tokens, const Maybe &ma
 
 Tensor tokens_bwd(const Tensor &logits, const Tensor &tokens, const Tensor &stats_, const Tensor &entropy_, const Maybe &dlogp_,
                   const Maybe &dentropy_, const Maybe &mask, int64_t stream) {
+    no_trace("token_logprobs_bwd");
     const TokenArgs a = token_args(logits, tokens, mask);
     const auto shape = a.tokens.sizes();
     std::vector<int64_t> two(shape.begin(), shape.end());
@@ -190,8 +199,14 @@ py::tuple norm_fwd(const Tensor &x, const Maybe &weight, const Maybe &bias, doub
     return py::make_tuple(y, mean, rstd);
 }
 
+py::tuple norm_fwd_alone(const Tensor &x, const Maybe &weight, const Maybe &bias, double eps, int64_t stream) {
+    no_trace("layer_norm_fwd");
+    return norm_fwd(x, weight, bias, eps, stream);
+}
+
 py::tuple norm_bwd(const Tensor &dy, const Tensor &x, const Maybe &weight, const Maybe &bias, const Tensor &mean_, const Tensor &rstd_,
                    int64_t stream) {
+    no_trace("layer_norm_bwd");
     const NormArgs a = norm_args(x, weight, bias);
     no_tangent(dy, "dy");
     if (dy.sizes() != x.sizes() || dy.scalar_type() != x.scalar_type() || dy.device() != x.device())
@@ -220,6 +235,7 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
                 double max_norm, const std::optional<std::vector<Maybe>> &copies, const std::optional<Tensors> &m_exps,
                 const std::optional<Tensors> &v_exps, const std::optional<std::vector<int64_t>> &counters,
                 const std::optional<std::vector<int64_t>> &lags, uint64_t seed, int64_t stream) {
+    no_trace("adamw_step");
     const size_t count = params.size();
     const bool eight = m_exps.has_value();
     auto same = [&](size_t n, const char *name) {
@@ -319,6 +335,7 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
 }
 
 Tensor adamw_read(const Tensor &code, const Tensor &exp, bool is_signed, const Maybe &out_, int64_t stream) {
+    no_trace("read_moment");
     const int64_t n = code.numel();
     if (code.scalar_type() != at::kByte || exp.scalar_type() != at::kByte || !code.is_cuda() || exp.device() != code.device() ||
         !code.is_contiguous() || !exp.is_contiguous() || exp.numel() != (n + D1_ADAMW_BLOCK - 1) / D1_ADAMW_BLOCK)
@@ -338,6 +355,7 @@ PYBIND11_MODULE(_d1ops, m) {
     m.def("tokens_fwd", &tokens_fwd);
     m.def("tokens_bwd", &tokens_bwd);
     m.def("norm_fwd", &norm_fwd);
+    m.def("norm_fwd_alone", &norm_fwd_alone);
     m.def("norm_bwd", &norm_bwd);
     m.def("adamw_step", &adamw_step);
     m.def("adamw_read", &adamw_read);

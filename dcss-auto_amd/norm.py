@@ -8,12 +8,12 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from .ops import call, call_recorded
+from .ops import call, is_tracing
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5):
     """-> (y like x, mean fp32 [...], rstd fp32 [...]): y = (x - mean) * rstd * weight + bias."""
-    return call('norm_fwd', x, x, weight, bias, eps)
+    return call('norm_fwd_alone', x, x, weight, bias, eps)
 
 
 def layer_norm_bwd(dy, x, weight, bias, mean, rstd):
@@ -25,7 +25,7 @@ def layer_norm_bwd(dy, x, weight, bias, mean, rstd):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = call_recorded('norm_fwd', x, x, weight, bias, eps)
+        y, mean, rstd = call('norm_fwd', x, x, weight, bias, eps)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         return y
 
@@ -38,9 +38,9 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm of x [..., width] (fp32, bf16 or fp16; rows of any stride, up to 16,384 elements)
     with an optional weight and bias [width] in fp32 or x's type; statistics in fp32."""
-    if torch.jit.is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return call_recorded('norm_fwd', x, x, weight, bias, eps)[0]
+    return call('norm_fwd', x, x, weight, bias, eps)[0]
 
 
 class LayerNorm(nn.Module):

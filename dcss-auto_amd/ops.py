@@ -10,18 +10,12 @@ from . import _lib
 # the stream's handle without a Stream object around it (0.1 us against 2.5)
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
+# whether torch.jit.trace is recording (0.09 us against 0.19)
+is_tracing = getattr(torch._C, '_is_tracing', None) or torch.jit.is_tracing
 
 
 def call(name, x, *args):
-    """call_recorded, refused in torch.jit.trace: that would record the outputs being made, but not what fills them."""
-    if torch.jit.is_tracing():
-        raise RuntimeError(f'{name} cannot be part of a trace (token_logprobs and layer_norm can)')
-    return call_recorded(name, x, *args)
-
-
-def call_recorded(name, x, *args):
-    """An operator's C++ call with x's GPU as the current device and its current stream; for an autograd function's
-    forward, which a trace records whole."""
+    """An operator's C++ call with x's GPU as the current device and its current stream."""
     function = getattr(_lib.load_ops_torch(), name)
     index = x.get_device()
     if index < 0:

@@ -10,7 +10,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from .ops import call, call_recorded
+from .ops import call, is_tracing
 
 
 class TokenLogprobs(NamedTuple):
@@ -29,7 +29,7 @@ class TokenLogprobs(NamedTuple):
 def _forward(logits, tokens, mask, top):
     if type(top) is not int:
         raise ValueError(f'top must be an int, not {top!r}')
-    return TokenLogprobs(*call_recorded('tokens_fwd', logits, logits, tokens, mask, top))
+    return TokenLogprobs(*call('tokens_fwd', logits, logits, tokens, mask, top))
 
 
 def token_logprobs_bwd(logits, tokens, result, dlogp, dentropy, mask=None):
@@ -65,6 +65,6 @@ def token_logprobs(logits, tokens, mask=None, top=0):
     mask: bool or uint8, [..., V] or [V]; only entries that are true take part. A negative token is
     padding (logp 0, no gradient through it), a token of V or more gives NaN, a masked one -inf. A
     row that allows nothing gives logp -inf, entropy 0, no alternatives and a gradient of 0."""
-    if torch.jit.is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
+    if is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, mask, top))
     return _forward(logits, tokens, mask, top)
