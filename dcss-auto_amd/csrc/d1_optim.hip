@@ -17,6 +17,10 @@
 // adds a 16-bit draw below the code's last bit and cuts. Its expectation is the value: a moment that
 // moves by less than a step an update (v moves by a thousandth, a step is an eighth) still follows
 // its mean, where rounding to the nearest would leave it where it is.
+// An element whose m or v is infinite (without a clip nothing keeps such a gradient out, nor one whose square overflows)
+// does not count for the block's largest, which would put the 255 others below their codes' range; it starts anew
+// from m = 0 and the largest v that its block's codes hold. A NaN, which no maximum takes in, becomes a block's largest code
+// too; the parameter is NaN by then.
 #include "d1_rows.h"
 
 namespace d1o {
@@ -257,6 +261,16 @@ __device__ __forceinline__ void step_chunk(const Tensors &t, int k, int within, 
         put_part<PAST>(p + i, have, out);
         if (copy) put_part<PAST>(copy + i, have, half);
         if (BITS == 8) {
+            // the wave's 256 counters share their upper word but where they pass 2^32
+            const uint64_t c0 = (uint64_t)t.counter[k] + (uint64_t)first;
+            const uint32_t low = (uint32_t)c0, key = draw_key(r.seed, step, (uint32_t)(c0 >> 32));
+            const uint32_t next = low > 0xFFFFFF00u ? draw_key(r.seed, step, (uint32_t)(c0 >> 32) + 1) : key;
+            uint32_t word[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t c = low + (threadIdx.x & 63) * 4 + j;
+                word[j] = mix(c ^ (c < low ? next : key));
+            }
             float ma = 0.f, va = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -267,16 +281,24 @@ __device__ __forceinline__ void step_chunk(const Tensors &t, int k, int within, 
             }
             me = block_exp(lanes_max<64>(ma));
             ve = block_exp(lanes_max<64>(va));
-            // the wave's 256 counters share their upper word but where they pass 2^32
-            const uint64_t c0 = (uint64_t)t.counter[k] + (uint64_t)first;
-            const uint32_t low = (uint32_t)c0, key = draw_key(r.seed, step, (uint32_t)(c0 >> 32));
-            const uint32_t next = low > 0xFFFFFF00u ? draw_key(r.seed, step, (uint32_t)(c0 >> 32) + 1) : key;
+            if ((me > ve ? me : ve) == 255) {      // an infinity (or close to it): the maxima again without
+                ma = va = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool lost = !(fabsf(m.v[j]) < INFINITY && v.v[j] < INFINITY);
+                    m.v[j] = lost ? 0.f : m.v[j];
+                    ma = fmaxf(ma, fabsf(m.v[j]));
+                    va = fmaxf(va, lost ? 0.f : v.v[j]);
+                    v.v[j] = lost ? INFINITY : v.v[j];
+                }
+                me = block_exp(lanes_max<64>(ma));
+                ve = block_exp(lanes_max<64>(va));
+            }
             Pack<uint8_t, 4> mc, vc;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t c = low + (threadIdx.x & 63) * 4 + j, word = mix(c ^ (c < low ? next : key));
-                mc.v[j] = (uint8_t)(encode<15>(fabsf(m.v[j]), me, word >> 16) | (m.v[j] < 0.f ? 128u : 0u));
-                const uint32_t code = encode<31>(v.v[j], ve, word & 0xFFFF);
+                mc.v[j] = (uint8_t)(encode<15>(fabsf(m.v[j]), me, word[j] >> 16) | (m.v[j] < 0.f ? 128u : 0u));
+                const uint32_t code = encode<31>(v.v[j], ve, word[j] & 0xFFFF);
                 vc.v[j] = (uint8_t)(code == 0 && v.v[j] > 0.f ? 1 : code);
             }
             put_part<PAST>((uint8_t *)t.m[k] + i, have, mc);

@@ -35,7 +35,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     that each tensor has missed.
 
     With max_grad_norm > 0 the gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with
-    the norm over all of them, and a step whose norm is not finite changes nothing and is counted."""
+    the norm over all of them, and a step whose norm is not finite changes nothing and is counted.
+    Without, an element whose gradient (or its square) is not finite is lost alone; its 8-bit moments
+    start anew, 32-bit ones stay not finite."""
     count = len(params)
     m_exps, v_exps = exps if exps is not None else (None, None)
     call('adamw_step', step, params, grads, exp_avg, exp_avg_sq, step, _each(lr, count), _each(weight_decay, count), betas[0],

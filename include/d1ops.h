@@ -105,7 +105,11 @@ typedef struct D1AdamW {
  * 8-bit moments: x = +-(code) 2^exp with 3 bits of mantissa, 4 bits of exponent and a sign for m, 5
  * bits of exponent for v; the parameter's step is made from the moments before they are rounded;
  * rounding goes up or down by chance, a hash of (seed, step, counter + element) against the part
- * that is dropped, so that its expectation is the value; a v that is not 0 never becomes 0. */
+ * that is dropped, so that its expectation is the value; a v that is not 0 never becomes 0. An element
+ * whose m or v is not finite after the step (a gradient that is not, or whose square overflows, with
+ * max_norm 0) leaves the others of its block as they are and gets finite moments: m 0 and its block's
+ * largest v where they were infinite, codes of its block's largest where they were NaN; with 32-bit moments it keeps what is not finite. The parameter is what the formula gives either way (v
+ * past 2^104 counts as infinite for the 8-bit step: the parameter only decays). */
 int64_t d1_adamw_work_bytes(const D1AdamWTensor *t, int count, const D1AdamW *h);
 int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, void *work, int64_t work_bytes,
                   void *stream);
