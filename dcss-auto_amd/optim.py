@@ -11,6 +11,17 @@ from .ops import call
 BLOCK = 256                         # elements of an 8-bit moment that share an exponent
 
 
+# options of the whole optimizer, which a group of parameters cannot have of its own
+WHOLE = frozenset(('betas', 'eps', 'max_grad_norm', 'state_bits', 'seed', 'copies', 'amsgrad', 'maximize'))
+
+
+def _check_group(group):
+    if not WHOLE.isdisjoint(group):
+        names = sorted(k for k in WHOLE.intersection(group) if group[k] or k not in ('amsgrad', 'maximize'))
+        if names:
+            raise ValueError(f'a group has lr and weight_decay of its own, not {", ".join(names)}')
+
+
 def moment_blocks(numel):
     """Exponent bytes of an 8-bit moment of `numel` elements."""
     return -(-numel // BLOCK)
@@ -54,12 +65,14 @@ class AdamW(torch.optim.Optimizer):
 
     lr and weight_decay may differ between groups; betas, eps, state_bits (32 or 8) and
     max_grad_norm (the clip by the global norm of all groups' gradients, 0 for none) are the
-    optimizer's. copies: {parameter: bf16 tensor} that a step writes beside fp32 parameters. A
-    parameter without a gradient is left as it is and keeps its own step count; the step in which it
-    first takes part after others have, or does so again, waits for the device's count. A step can be
-    captured in a graph after one with the same parameters taking part. With
-    max_grad_norm a step whose norm is not finite changes nothing; skipped_steps() counts those. The
-    state dict holds moments and counts; betas, eps and the clip are those of the new optimizer."""
+    optimizer's, and a group that names them is refused. copies: {parameter: bf16 tensor} that a step
+    writes beside fp32 parameters. A parameter without a gradient is left as it is and keeps its own
+    step count; the step in which it first takes part after others have, or does so again, waits for
+    the device's count. A step can be captured in a graph after one with the same parameters taking
+    part; replays use the lr, weight_decay, clip and seed of the capture, so a change of lr needs a
+    new one. With max_grad_norm a step whose norm is not finite changes nothing; skipped_steps()
+    counts those. The state dict holds moments and counts; betas, eps and the clip are those of the
+    new optimizer."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  max_grad_norm=0.0, copies=None, seed=0):
@@ -74,6 +87,10 @@ class AdamW(torch.optim.Optimizer):
         self.copies = copies or {}
         self.ctl = None                 # the device's step count, skips and norm (adamw_step's `step`)
         self._counter = 0
+
+    def add_param_group(self, param_group):
+        _check_group(param_group)
+        super().add_param_group(param_group)
 
     def __getstate__(self):             # copies and pickles: the base class's holds no more than its own
         return {**super().__getstate__(), **{k: getattr(self, k) for k in (
@@ -104,6 +121,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        for group in self.param_groups:
+            _check_group(group)
         loss = None
         if closure is not None:
             with torch.enable_grad():
