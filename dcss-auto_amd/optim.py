@@ -179,7 +179,9 @@ class AdamW(torch.optim.Optimizer):
         return d
 
     def load_state_dict(self, state_dict):
-        own = state_dict['d1']
+        own = state_dict.get('d1')
+        if own is None:
+            raise ValueError("not a state of this AdamW: another optimizer's moments and counts are kept otherwise")
         if own['state_bits'] != self.state_bits:
             raise ValueError(f"the state was saved with {own['state_bits']}-bit moments, this optimizer has {self.state_bits}")
         super().load_state_dict({k: v for k, v in state_dict.items() if k != 'd1'})

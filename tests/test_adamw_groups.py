@@ -37,3 +37,10 @@ def test_options_that_a_group_may_have(A):
     a, b = two()
     opt = A.AdamW([dict(params=[a], lr=0.5, weight_decay=0.25, name='trunk', amsgrad=False), dict(params=[b])], lr=0.125)
     assert [g['lr'] for g in opt.param_groups] == [0.5, 0.125] and opt.param_groups[0]['name'] == 'trunk'
+
+
+def test_another_optimizers_state_is_refused(A):
+    a, _ = two()
+    plain = torch.optim.AdamW([a])
+    with pytest.raises(ValueError, match='AdamW'):
+        A.AdamW([a]).load_state_dict(plain.state_dict())
