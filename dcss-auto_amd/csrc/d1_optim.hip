@@ -162,6 +162,7 @@ __global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl,
         if (threadIdx.x == 0) ctl[NORM] = __float_as_int((float)norm);
     }
     if (threadIdx.x) return;
+    if (!parts && max_norm > 0.0) ctl[NORM] = 0;       // a clip of no elements
     ctl[GO] = go;
     if (!go) {
         ctl[SKIPPED]++;
