@@ -788,7 +788,7 @@ extern "C" int d1_tokens_bwd(const void *logits, int type, int64_t rows, int voc
                              const float *dlogp, const float *dentropy, void *dlogits, void *stream) {
     if (!token_args(type, rows, vocab, stride, mask_stride)) return D1_E_ARG;
     if (rows == 0) return 0;
-    if (!logits || !tokens || !stats || !dlogits || (dentropy && !entropy)) return D1_E_ARG;
+    if (!logits || !tokens || !stats || !dlogits || dlogits == logits || (dentropy && !entropy)) return D1_E_ARG;
     const BackArgs a{logits, rows, stride, vocab, tokens, mask, mask_stride, stats, entropy, dlogp, dentropy, dlogits};
     D1O_TOKEN_TYPES(bwd, a, (hipStream_t)stream)
 }

@@ -52,7 +52,8 @@ int d1_tokens_fwd(const void *logits, int type, int64_t rows, int vocab, int64_t
 /* dlogits [rows, vocab] (contiguous, the logits' type) from the gradients of logp and entropy
  * (either may be null: zero): dlogp (1[j = t] - p[j]) - dentropy p[j] (log p[j] + entropy). Masked
  * entries and rows without an allowed entry get 0, padding no dlogp part; a token of vocab or more
- * makes its row's allowed entries NaN when dlogp is given. */
+ * makes its row's allowed entries NaN when dlogp is given. dlogits must not overlap the logits: an
+ * entry may be read again after its gradient was written (dlogits == logits is rejected). */
 int d1_tokens_bwd(const void *logits, int type, int64_t rows, int vocab, int64_t stride, const int64_t *tokens,
                   const uint8_t *mask, int64_t mask_stride, const float *stats, const float *entropy,
                   const float *dlogp, const float *dentropy, void *dlogits, void *stream);
