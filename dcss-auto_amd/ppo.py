@@ -45,9 +45,12 @@ class PPO:
     def __init__(self, model, lr=3e-4, eps=1e-5, clip=0.2, vcoef=0.5, ecoef=0.01, max_grad_norm=0.5,
                  epochs=4, minibatch=8192, gamma=0.99, lam=0.95, autocast=True):
         self.model = model
-        self.opt = torch.optim.Adam(model.parameters(), lr=lr, eps=eps, fused=True)
+        self.opt = self._optimizer(lr, eps)
         self.clip, self.vcoef, self.ecoef, self.max_grad_norm = clip, vcoef, ecoef, max_grad_norm
         self.epochs, self.minibatch, self.gamma, self.lam, self.autocast = epochs, minibatch, gamma, lam, autocast
+
+    def _optimizer(self, lr, eps):
+        return torch.optim.Adam(self.model.parameters(), lr=lr, eps=eps, fused=True)
 
     def advantages(self, buf):
         adv, ret = P.gae(buf.rewards, buf.dones, buf.values, buf.bootstrap, self.gamma, self.lam)
@@ -92,10 +95,12 @@ class ModulePPO(PPO):
                  minibatch=8192, gamma=0.99, lam=0.95, autocast=True, weight_decay=0.0, state_bits=32, seed=0):
         if not max_grad_norm > 0:
             raise ValueError('ModulePPO needs a gradient clip: its norm is what tells a non-finite loss')
+        self._adamw = dict(weight_decay=weight_decay, state_bits=state_bits, max_grad_norm=max_grad_norm, seed=seed)
         super().__init__(model, lr=lr, eps=eps, clip=clip, vcoef=vcoef, ecoef=ecoef, max_grad_norm=max_grad_norm,
                          epochs=epochs, minibatch=minibatch, gamma=gamma, lam=lam, autocast=autocast)
-        self.opt = AdamW(model.parameters(), lr=lr, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                         max_grad_norm=max_grad_norm, seed=seed)
+
+    def _optimizer(self, lr, eps):
+        return AdamW(self.model.parameters(), lr=lr, eps=eps, **self._adamw)
 
     def minibatch_step(self, obs, actions, old_logp, adv, ret):
         with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
