@@ -66,8 +66,9 @@ class Policy(nn.Module):
 
 
 class NormPolicy(nn.Module):
-    """Policy with a layer norm behind each trunk layer, of any width and number of actions; it trains
-    with ModulePPO (ppo.py), through the layer norm and log-probability kernels."""
+    """Policy with a layer norm behind each trunk layer, of any width (up to 16,384) and number of actions
+    (act samples up to 64); it trains with ModulePPO (ppo.py), through the layer norm and
+    log-probability kernels."""
 
     def __init__(self, width=256, n_actions=N_ACTIONS, obs=OBS, seed=0):
         super().__init__()
