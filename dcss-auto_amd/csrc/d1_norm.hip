@@ -6,7 +6,10 @@
 // wave, or a workgroup of 128 to 1,024), CH chunks of 16 bytes a lane, so the variance is
 // taken about the mean itself and not from a difference of sums. The backward pass keeps the
 // columns' dw and db sums in registers over all rows that a workgroup walks, writes them once, and
-// k_norm_reduce adds the workgroups' sums in a fixed order (no atomics: the same bits each time).
+// k_norm_reduce adds the workgroups' sums in a fixed order (no atomics: the same bits each time). These sums are fp32: a
+// lane adds its rows alone (16,384 rows of 8,192 over 512 workgroups: 32) and the reduction some 50 parts, so a column's
+// error is that of rows/512 + 50 additions; fp64 would take twice the registers of the widest rows, which have none left.
+// Backward times are of k_norm_bwd alone where it says so, else of a whole call with the reduction (7 us at 8,192 columns).
 #include "d1_rows.h"
 
 namespace d1o {
@@ -43,7 +46,7 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float2 (*scratch)[1
 }
 
 // The CH chunks of a lane from a row of `width` elements, `fill` past its end: the backward pass, which has no registers
-// left for the places below (16,384 x 8,192 bf16: 161 us, 172 with them)
+// left for the places below (16,384 x 8,192 bf16: a call 161 us, 172 with them)
 template <class T, int LANES, int CH, int VEC>
 __device__ __forceinline__ void read_row(Pack<T, VEC> (&a)[CH], const T *row, int lane, int width, T fill) {
 #pragma unroll
@@ -96,7 +99,7 @@ __device__ __forceinline__ void fill_row(Pack<T, VEC> (&a)[CH], T value) {
 }
 
 // One reading, one writing, two sums a row; weight and bias stay in registers over the rows. Bound by memory: 16,384 x 8,192 bf16
-// 103 us, 5.2 TB/s; 65,536 x 256 12 us, 5.5 TB/s; below about 4 us by the launch.
+// 103 us at best, 5.2 TB/s (115 in a loop of it alone); 65,536 x 256 12 us, 5.5 TB/s; below about 4 us by the launch.
 template <class T, class W, int LANES, int CH, bool PAST>
 __global__ __launch_bounds__(threads_of(LANES), fwd_waves(LANES, CH)) void k_norm_fwd(const T *__restrict__ x, int64_t rows, int width, int64_t stride,
                                                                 const W *__restrict__ w, const W *__restrict__ b, float eps,
@@ -151,7 +154,8 @@ __global__ __launch_bounds__(threads_of(LANES), fwd_waves(LANES, CH)) void k_nor
 }
 
 // One reading of x and dy, one writing of dx, two sums a row and two a column. Bound by memory and, where a lane holds
-// little, by the number of rows in flight: 16,384 x 8,192 bf16 150 us, 5.4 TB/s; 65,536 x 1,024 78 us, 5.2 TB/s.
+// little, by the number of rows in flight: 16,384 x 8,192 bf16 150 us alone, 5.4 TB/s; 65,536 x 1,024 78 us with the reduction, 5.2 TB/s;
+// 1,000,000 x 32 bf16 35 with it, 5.4 TB/s (on 4 lanes, where bwd_waves' bound spills two or three registers to the stack).
 template <class T, class W, int LANES, int CH, bool PAST>
 __global__ __launch_bounds__(bwd_threads(LANES), bwd_waves(CH)) void k_norm_bwd(const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ x,
                                                                 int64_t rows, int width, int64_t stride, const W *__restrict__ w,
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float *__restrict__ 
 // Lanes a row and chunks a lane for a width: the fewest lanes that hold it at one chunk each. Few
 // registers a lane and many waves do more for the bandwidth than many chunks a lane: 16,384 rows of
 // 8,192 bf16 forward 103 us on 1,024 lanes x 1 chunk, 122 on 512 x 2, 136 at best on 256 x 4 (one
-// row ahead in registers); backward 160, 179 and 251. Reading a row ahead costs more
+// row ahead in registers); backward 161, 179 and 251. Reading a row ahead costs more
 // waves than it hides (112 and 198 us on 1,024 x 1), so no shape does.
 #define D1O_NORM_SHAPES(X)                                                                                          \
     X(4, 1) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2) X(1024, 4)
@@ -294,7 +298,7 @@ inline int fwd_grid(int64_t rows, int lanes) {
 }
 // Backward: each workgroup writes its columns' sums, which k_norm_reduce reads again, so no more than fit at once:
 // two or three of 512 threads a CU (65,536 x 1,024 bf16 81.4 us at 512, 78.0 at 768, 90.9 at 1,024), two where the
-// rows are few beside the sums (5,778 x 861 14.1, 14.9 and 17.3), two of 1,024 lanes (16,384 x 8,192 174, 160 and 178 at 256, 512
+// rows are few beside the sums (5,778 x 861 14.1, 14.9 and 17.3), two of 1,024 lanes (16,384 x 8,192 174, 161 and 178 at 256, 512
 // and 768), one where a lane holds several chunks (7,554 x 11,823 144 at 256, 156 at 512).
 inline int bwd_grid(int64_t rows, int lanes, int ch) {
     const int groups = bwd_threads(lanes) / lanes;
