@@ -269,8 +269,7 @@ def _own_loss(s):
     names = ('ref_logp', 'entropy', 'values', 'returns', 'old_values', 'mask')
     more = dict({name: s[name] for name in names}, clip=CLIP, value_clip=VALUE_CLIP, kl_coef=KL, value_coef=VALUE,
                 entropy_coef=ENTROPY, level=s['level'])
-    r = L.policy_loss_fwd(s['logp'], s['old_logp'], s['advantages'], **more)
-    dlogp, dentropy, dvalues = L.policy_loss_bwd(r, None, s['logp'], s['old_logp'], s['advantages'], **more)
+    r, dlogp, dentropy, dvalues = L.policy_loss_grads(s['logp'], s['old_logp'], s['advantages'], **more)
     out = dict(policy=r.policy, clipped=r.clipped, drift=r.drift)
     if s['ref_logp'] is not None:
         out['kl'] = r.kl
