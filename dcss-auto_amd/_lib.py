@@ -21,7 +21,8 @@ LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', '
                  'learn_action_size', 'learn_out_size', 'learn_config_bytes', 'learn_init', 'learn_step',
                  'learn_step_active', 'learn_heuristic')
 OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
-               'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read')
+               'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read', 'd1_policy_loss_work_bytes',
+               'd1_policy_loss', 'd1_scale', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd')
 _LEARN = {}
 _OPS = _OPS_TORCH = None
 
@@ -98,6 +99,27 @@ class D1AdamW(C.Structure):
                 ('seed', C.c_uint64), ('bits', C.c_int32), ('pad', C.c_int32)]
 
 
+class D1LossInput(C.Structure):
+    """The D1LossInput struct of include/d1ops.h."""
+    _fields_ = [('data', C.c_void_p), ('row', C.c_int64), ('step', C.c_int64), ('type', C.c_int32), ('pad', C.c_int32)]
+
+
+class D1PolicyLoss(C.Structure):
+    """The D1PolicyLoss struct of include/d1ops.h."""
+    _fields_ = [*((name, D1LossInput) for name in ('logp', 'old_logp', 'advantages', 'ref_logp', 'entropy', 'values', 'returns',
+                                                   'old_values', 'mask')),
+                ('rows', C.c_int64), ('length', C.c_int64), ('clip_low', C.c_double), ('clip_high', C.c_double),
+                ('value_clip', C.c_double), ('kl_coef', C.c_double), ('value_coef', C.c_double), ('entropy_coef', C.c_double),
+                ('sequence', C.c_int32), ('pad', C.c_int32)]
+
+
+class D1Scan(C.Structure):
+    """The D1Scan struct of include/d1ops.h."""
+    _fields_ = [('x', C.c_void_p), ('gate', C.c_void_p), ('reset', C.c_void_p), ('state', C.c_void_p), ('marks', C.c_void_p),
+                *((name, C.c_int64) for name in ('x_t', 'x_n', 'gate_t', 'gate_n', 'reset_t', 'reset_n', 'steps', 'rows')),
+                ('width', C.c_int32), ('type', C.c_int32)]
+
+
 def load_ops():
     """libd1ops.so: the operators of a policy update beside the fused step (include/d1ops.h)."""
     global _OPS
@@ -117,7 +139,15 @@ def load_ops():
         L.d1_adamw_work_bytes.argtypes = [p, i, p]
         L.d1_adamw_step.argtypes = [p, i, p, p, p, n, p]
         L.d1_adamw_read.argtypes = [p, p, n, i, p, p]
-        for name in ('d1_tokens_work_bytes', 'd1_norm_work_bytes', 'd1_adamw_work_bytes'):
+        L.d1_policy_loss_work_bytes.argtypes = [p]
+        L.d1_policy_loss.argtypes = [p, p, p, p, p, p, n, p]
+        L.d1_scale.argtypes = [p, i, n, p, p]
+        L.d1_scan_marks.argtypes = [n]
+        L.d1_scan_work_bytes.argtypes = [p]
+        L.d1_scan_fwd.argtypes = [p, p, n, n, p, p, n, p]
+        L.d1_scan_bwd.argtypes = [p, p, n, n, p, p, n, n, p, n, n, p, p, n, p]
+        for name in ('d1_tokens_work_bytes', 'd1_norm_work_bytes', 'd1_adamw_work_bytes', 'd1_policy_loss_work_bytes',
+                     'd1_scan_marks', 'd1_scan_work_bytes'):
             getattr(L, name).restype = C.c_int64
         _OPS = L
     return _OPS

@@ -349,9 +349,221 @@ Tensor adamw_read(const Tensor &code, const Tensor &exp, bool is_signed, const M
     return out;
 }
 
+// ---- the policy loss
+
+// t as an input of [rows, length] tokens, a view where its strides allow it; what it refers to is put into `held`
+D1LossInput loss_input(const Tensor &t, const Tensor &logp, int64_t rows, int64_t length, const char *name, Tensors &held) {
+    no_tangent(t, name);
+    const int code = type_of(t.scalar_type());
+    if (code < 0 || t.sizes() != logp.sizes() || t.device() != logp.device())
+        refuse(std::string(name) + " must be fp32, bf16 or fp16 of " + c10::str(logp.sizes()) + " on " + logp.device().str() + ", not " +
+               describe(t));
+    D1LossInput in{};
+    in.type = code;
+    if (t.dim() <= 2) {
+        in.row = t.dim() == 2 ? t.stride(0) : length;
+        in.step = t.stride(-1);
+        in.data = t.data_ptr();
+        held.push_back(t);
+    } else {
+        const Tensor r = t.reshape({rows, length});
+        in.row = r.stride(0);
+        in.step = r.stride(1);
+        in.data = r.data_ptr();
+        held.push_back(r);
+    }
+    return in;
+}
+
+// -> (loss, terms [8], dlogp, dentropy, dvalues); a gradient that is not asked for is None
+py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &advantages, const Maybe &ref_logp, const Maybe &entropy,
+                      const Maybe &values, const Maybe &returns, const Maybe &old_values, const Maybe &mask, double clip_low,
+                      double clip_high, double kl_coef, double value_coef, double value_clip, double entropy_coef, bool sequence, int64_t grads,
+                      int64_t stream) {
+    no_trace("policy_loss");
+    if (!logp.is_cuda()) refuse("logp must be a CUDA tensor (there is no CPU fallback)");
+    if (logp.dim() == 0) refuse("logp must have at least one dimension");
+    if (values.has_value() != returns.has_value()) refuse("values and returns come together");
+    if (!(clip_low >= 0 && clip_low <= 1 && clip_high >= 0)) refuse("clip must be (0 to 1, 0 or more)");
+    if (!(value_clip >= 0)) refuse("value_clip must not be negative");
+    if (value_clip > 0 && values && !old_values) refuse("value_clip needs old_values");
+    for (double c : {kl_coef, value_coef, entropy_coef})
+        if (!std::isfinite(c)) refuse("coefficients must be finite");
+    Tensors held;
+    D1PolicyLoss h{};
+    h.length = logp.size(-1);
+    h.rows = h.length ? logp.numel() / h.length : 0;
+    auto given = [&](const Tensor &t, const char *name) { return loss_input(t, logp, h.rows, h.length, name, held); };
+    h.logp = given(logp, "logp");
+    h.old_logp = given(old_logp, "old_logp");
+    if (advantages.sizes() == logp.sizes()) {
+        h.advantages = given(advantages, "advantages");
+    } else {                 // one a sequence
+        no_tangent(advantages, "advantages");
+        const int code = type_of(advantages.scalar_type());
+        if (code < 0 || advantages.sizes() != logp.sizes().slice(0, logp.dim() - 1) || advantages.device() != logp.device())
+            refuse("advantages must be fp32, bf16 or fp16 of " + c10::str(logp.sizes()) + " or without its last dimension on " +
+                   logp.device().str() + ", not " + describe(advantages));
+        held.push_back(advantages.dim() == 1 ? advantages : advantages.reshape({h.rows}));
+        h.advantages = {held.back().data_ptr(), held.back().stride(0), 0, code, 0};
+    }
+    if (ref_logp) h.ref_logp = given(*ref_logp, "ref_logp");
+    if (entropy) h.entropy = given(*entropy, "entropy");
+    if (values) {
+        h.values = given(*values, "values");
+        h.returns = given(*returns, "returns");
+        if (old_values) h.old_values = given(*old_values, "old_values");
+    }
+    if (mask) {
+        if ((mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) || mask->sizes() != logp.sizes() ||
+            mask->device() != logp.device())
+            refuse("mask must be bool or uint8 of " + c10::str(logp.sizes()) + " on " + logp.device().str() + ", not " + describe(*mask));
+        held.push_back(mask->dim() == 2 ? *mask : mask->reshape({h.rows, h.length}));
+        h.mask = {held.back().data_ptr(), held.back().stride(0), held.back().stride(1), 0, 0};
+    }
+    h.clip_low = clip_low;
+    h.clip_high = clip_high;
+    h.value_clip = value_clip;
+    h.kl_coef = kl_coef;
+    h.value_coef = value_coef;
+    h.entropy_coef = entropy_coef;
+    h.sequence = sequence;
+    const Tensor terms = at::empty({8}, logp.options().dtype(at::kFloat));
+    Maybe dlogp, dentropy, dvalues, work;
+    if (grads & 1) dlogp = at::empty(logp.sizes(), logp.options());
+    if ((grads & 2) && entropy) dentropy = at::empty(logp.sizes(), entropy->options());
+    if ((grads & 4) && values) dvalues = at::empty(logp.sizes(), values->options());
+    const int64_t need = d1_policy_loss_work_bytes(&h);
+    check(need < 0 ? (int)need : 0, "d1_policy_loss_work_bytes");
+    if (need) work = scratch(need, logp);
+    check(d1_policy_loss(&h, (float *)ptr(terms), ptr(dlogp), ptr(dentropy), ptr(dvalues), ptr(work), need, (void *)stream),
+          "d1_policy_loss");
+    return py::make_tuple(terms, dlogp, dentropy, dvalues);
+}
+
+// gradients that no one else holds, times a number on the device
+void scale_grads(const Tensor &by, const std::vector<Maybe> &grads, int64_t stream) {
+    if (by.scalar_type() != at::kFloat || by.numel() != 1 || !by.is_cuda()) refuse("the loss's gradient must be one fp32 number");
+    for (const Maybe &g : grads)
+        if (g) check(d1_scale(ptr(g), type_of(g->scalar_type()), g->numel(), (const float *)ptr(by), (void *)stream), "d1_scale");
+}
+
+// ---- the gated recurrence
+
+struct ScanArgs {
+    D1Scan h{};
+    Tensor x, gate;
+    Maybe state, reset;
+    std::vector<int64_t> cells;          // the state's shape
+};
+
+// [steps, rows, width] or [steps, width], adjacent channels
+Tensor scan_sequence(const Tensor &t, const Tensor &x, const char *name) {
+    no_tangent(t, name);
+    if (t.sizes() != x.sizes() || t.scalar_type() != x.scalar_type() || t.device() != x.device())
+        refuse(std::string(name) + " must be like x, " + describe(x) + ", not " + describe(t));
+    return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t;
+}
+int64_t row_stride(const Tensor &t) { return t.dim() == 3 ? t.stride(1) : 0; }
+
+ScanArgs scan_args(const Tensor &x, const Tensor &gate, const Maybe &state, const Maybe &reset) {
+    ScanArgs a;
+    if (!x.is_cuda()) refuse("x must be a CUDA tensor (there is no CPU fallback)");
+    a.h.type = type_of(x.scalar_type());
+    if (a.h.type < 0) refuse(std::string("x must be fp32, bf16 or fp16, not ") + c10::toString(x.scalar_type()));
+    if (x.dim() != 2 && x.dim() != 3) refuse("x must be [steps, rows, width] or [steps, width], not " + c10::str(x.sizes()));
+    if (x.size(-1) > D1_SCAN_MAX_WIDTH || x.size(0) > D1_SCAN_MAX_STEPS) refuse("x: too many steps or channels");
+    a.x = scan_sequence(x, x, "x");
+    a.gate = scan_sequence(gate, x, "gate");
+    a.cells.assign(x.sizes().begin() + 1, x.sizes().end());
+    a.h.steps = x.size(0);
+    a.h.rows = x.dim() == 3 ? x.size(1) : 1;
+    a.h.width = (int32_t)x.size(-1);
+    if (state) {
+        a.state = like(*state, a.cells, at::kFloat, x, "state");
+        a.h.state = (const float *)ptr(a.state);
+    }
+    if (reset) {
+        if ((reset->scalar_type() != at::kBool && reset->scalar_type() != at::kByte) || reset->device() != x.device() ||
+            reset->sizes() != x.sizes().slice(0, x.dim() - 1))
+            refuse("reset must be bool or uint8 of " + c10::str(x.sizes().slice(0, x.dim() - 1)) + " on " + x.device().str() + ", not " +
+                   describe(*reset));
+        a.reset = reset;
+        a.h.reset = (const uint8_t *)ptr(a.reset);
+        a.h.reset_t = reset->stride(0);
+        a.h.reset_n = reset->dim() == 2 ? reset->stride(1) : 0;
+    }
+    a.h.x = ptr(a.x);
+    a.h.x_t = a.x.stride(0);
+    a.h.x_n = row_stride(a.x);
+    a.h.gate = ptr(a.gate);
+    a.h.gate_t = a.gate.stride(0);
+    a.h.gate_n = row_stride(a.gate);
+    return a;
+}
+
+// an output like a sequence: its strides where they leave channels adjacent and no two elements on one place
+Tensor scan_like(const Tensor &t) {
+    const Tensor out = at::empty_like(t);
+    return t.size(-1) > 1 && out.stride(-1) != 1 ? at::empty(t.sizes(), t.options()) : out;
+}
+
+// -> (h, last, marks); marks only where `keep` asks for them and a backward pass needs them
+py::tuple scan_fwd(const Tensor &x, const Tensor &gate, const Maybe &state, const Maybe &reset, bool keep, int64_t stream) {
+    no_trace("gated_scan");
+    ScanArgs a = scan_args(x, gate, state, reset);
+    const auto fp32 = x.options().dtype(at::kFloat);
+    const Tensor h = scan_like(a.x);
+    if (a.h.steps == 0) return py::make_tuple(h, a.state ? a.state->clone() : at::zeros(a.cells, fp32), Maybe());
+    const Tensor last = at::empty(a.cells, fp32);
+    Maybe marks, work;
+    if (keep && d1_scan_marks(a.h.steps)) {
+        marks = at::empty({d1_scan_marks(a.h.steps), a.h.rows * a.h.width}, fp32);
+        a.h.marks = (float *)ptr(marks);
+    }
+    const int64_t need = d1_scan_work_bytes(&a.h);
+    check(need < 0 ? (int)need : 0, "d1_scan_work_bytes");
+    if (need) work = scratch(need, x);
+    check(d1_scan_fwd(&a.h, ptr(h), h.stride(0), row_stride(h), (float *)ptr(last), ptr(work), need, (void *)stream), "d1_scan_fwd");
+    return py::make_tuple(h, last, marks);
+}
+
+py::tuple scan_bwd(const Maybe &dh_, const Maybe &dlast_, const Tensor &x, const Tensor &gate, const Maybe &state, const Maybe &reset,
+                   const Maybe &marks, int64_t stream) {
+    no_trace("gated_scan_bwd");
+    ScanArgs a = scan_args(x, gate, state, reset);
+    const Tensor dh = dh_ ? scan_sequence(*dh_, x, "dh") : at::zeros(x.sizes(), x.options());
+    Maybe dlast, dstate, work;
+    if (dlast_) dlast = like(*dlast_, a.cells, at::kFloat, x, "dlast");
+    const Tensor dx = scan_like(a.x), dgate = scan_like(a.gate);
+    if (a.h.steps == 0) {
+        if (state) dstate = dlast ? dlast->clone() : at::zeros(a.cells, x.options().dtype(at::kFloat));
+        return py::make_tuple(dx, dgate, dstate);
+    }
+    if (state) dstate = at::empty(a.cells, x.options().dtype(at::kFloat));
+    const int64_t count = d1_scan_marks(a.h.steps);
+    if (count) {
+        if (!marks || marks->scalar_type() != at::kFloat || !marks->is_contiguous() || marks->device() != x.device() ||
+            marks->numel() != count * a.h.rows * a.h.width)
+            refuse("marks must be those of gated_scan_fwd with the same arguments");
+        a.h.marks = (float *)ptr(*marks);
+    }
+    const int64_t need = d1_scan_work_bytes(&a.h);
+    check(need < 0 ? (int)need : 0, "d1_scan_work_bytes");
+    if (need) work = scratch(need, x);
+    check(d1_scan_bwd(&a.h, ptr(dh), dh.stride(0), row_stride(dh), (const float *)ptr(dlast), ptr(dx), dx.stride(0), row_stride(dx),
+                      ptr(dgate), dgate.stride(0), row_stride(dgate), (float *)ptr(dstate), ptr(work), need, (void *)stream),
+          "d1_scan_bwd");
+    return py::make_tuple(dx, dgate, dstate);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_d1ops, m) {
+    m.def("scan_fwd", &scan_fwd);
+    m.def("scan_bwd", &scan_bwd);
+    m.def("policy_loss", &policy_loss);
+    m.def("scale_grads", &scale_grads);
     m.def("tokens_fwd", &tokens_fwd);
     m.def("tokens_bwd", &tokens_bwd);
     m.def("norm_fwd", &norm_fwd);

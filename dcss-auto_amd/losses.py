@@ -1,0 +1,115 @@
+"""The clipped policy loss with value, entropy and reference-KL terms, and its gradients (csrc/d1_loss.hip).
+
+`policy_loss` is the differentiable function; `policy_loss_grads` gives the loss and its gradients in one pass for
+code that runs without autograd. `ppo.ModulePPO` trains on it.
+"""
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .ops import call
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                   # fp32, the sum with the coefficients; differentiable
+    terms: torch.Tensor                  # fp32 [8]: the loss and what is named below, without a gradient
+
+    @property
+    def policy(self):
+        return self.terms[1]
+
+    @property
+    def value(self):
+        """Half the (clipped) squared error."""
+        return self.terms[2]
+
+    @property
+    def entropy(self):
+        return self.terms[3]
+
+    @property
+    def kl(self):
+        """Estimate of KL(policy || reference)."""
+        return self.terms[4]
+
+    @property
+    def clipped(self):
+        """The share of the weight whose clip is active."""
+        return self.terms[5]
+
+    @property
+    def drift(self):
+        """Estimate of KL(old policy || policy) that is never negative."""
+        return self.terms[6]
+
+    @property
+    def count(self):
+        """Tokens that count, or sequences with one (level 'sequence')."""
+        return self.terms[7]
+
+
+def _pair(clip):
+    return (clip, clip) if isinstance(clip, (int, float)) else clip
+
+
+def _call(grads, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef, value_coef,
+          value_clip, entropy_coef, level):
+    if level not in ('token', 'sequence'):
+        raise ValueError(f"level is 'token' or 'sequence', not {level!r}")
+    low, high = _pair(clip)
+    return call('policy_loss', logp, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, low, high,
+                kl_coef, value_coef, value_clip or 0.0, entropy_coef, level == 'sequence', grads)
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings):
+        want = [ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]]
+        ctx.bits, ctx.settings = sum(w << k for k, w in enumerate(want)), settings
+        terms, *ctx.grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
+        ctx.save_for_backward(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask)
+        ctx.mark_non_differentiable(terms)
+        return terms[0].clone(), terms
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _):
+        grads, ctx.grads = ctx.grads, None
+        logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask = ctx.saved_tensors
+        if grads is None:                # the graph was kept: the first backward pass took them
+            grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask,
+                          *ctx.settings)[1:]
+        call('scale_grads', logp, dloss, grads)
+        return (*grads, *[None] * 7)
+
+
+def policy_loss(logp, old_logp, advantages, ref_logp=None, entropy=None, values=None, returns=None, old_values=None, mask=None,
+                clip=0.2, kl_coef=0.0, value_coef=0.5, value_clip=None, entropy_coef=0.01, level='token'):
+    """The clipped policy loss of tokens (actions) logp [..., length] -> PolicyLoss, differentiable in logp, entropy and
+    values:
+
+        policy + value_coef * value - entropy_coef * entropy + kl_coef * kl
+
+    old_logp: under the policy that took the tokens. advantages: [..., length], or [...]: one a sequence. clip: the ratio
+    exp(logp - old_logp) is held in [1 - clip, 1 + clip], or (low, high) for [1 - low, 1 + high]. ref_logp: under a reference
+    policy, for the kl term exp(x) - x - 1 with x = ref_logp - logp. entropy: of each distribution. values and returns:
+    half the squared error, with value_clip the larger of it and that of the value held within value_clip of old_values.
+    mask (bool or uint8): only tokens that are true count, whatever the others hold. level: 'token' weighs all tokens
+    alike, 'sequence' the sequences that have one, over their own tokens. All are fp32, bf16 or fp16, each of its own
+    type, with any strides; everything is computed in fp32 and summed in fp64. Without a token that counts all terms
+    and gradients are 0."""
+    settings = (clip, kl_coef, value_coef, value_clip, entropy_coef, level)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logp, entropy, values)):
+        return PolicyLoss(*_PolicyLoss.apply(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings))
+    terms = _call(0, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)[0]
+    return PolicyLoss(terms[0], terms)
+
+
+def policy_loss_grads(logp, old_logp, advantages, ref_logp=None, entropy=None, values=None, returns=None, old_values=None, mask=None,
+                      clip=0.2, kl_coef=0.0, value_coef=0.5, value_clip=None, entropy_coef=0.01, level='token'):
+    """-> (PolicyLoss, dlogp, dentropy, dvalues): policy_loss with the gradients of its loss, each like its input, in one
+    pass; None where the input is."""
+    terms, *grads = _call(7, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef,
+                          value_coef, value_clip, entropy_coef, level)
+    return (PolicyLoss(terms[0], terms), *grads)

@@ -4,6 +4,8 @@
  *                 probable alternatives, and the gradient of the logits
  *   d1_norm_*     layer norm, its backward pass and the reduction of the weight's and the bias's gradient
  *   d1_adamw_*    one AdamW step over many tensors, moments in 32 or 8 bits, clip by the global norm
+ *   d1_policy_loss*   the clipped policy loss with value, entropy and reference-KL terms, and its gradients
+ *   d1_scan_*     a gated linear recurrence over long sequences, forward and backward
  *
  * Conventions as in d1hip.h: device pointers unless said otherwise, asynchronous on `stream`
  * (0 = the null stream), 0 on success, a hipError_t code for launch failures or a negative D1_E_*
@@ -30,6 +32,8 @@ extern "C" {
 #define D1_TOKENS_MAX_TOP 64
 #define D1_TOKENS_MAX_VOCAB (1 << 24)
 #define D1_NORM_MAX_WIDTH 16384
+#define D1_SCAN_MAX_WIDTH (1 << 24)
+#define D1_SCAN_MAX_STEPS (1 << 30)
 #define D1_ADAMW_BLOCK 256            /* elements of an 8-bit moment that share an exponent */
 
 /* For row i of logits [rows, vocab] over its allowed entries (mask[i * mask_stride + j] != 0; all
@@ -116,6 +120,68 @@ int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *
                   void *stream);
 /* out[i] (fp32) = the value that an 8-bit moment's code stands for; is_signed 1 for m, 0 for v. */
 int d1_adamw_read(const uint8_t *code, const uint8_t *exp, int64_t n, int is_signed, float *out, void *stream);
+
+/* An input of the policy loss: element t of sequence r is at data[r * row + t * step], strides in elements, none
+ * negative; data null: not given. */
+typedef struct D1LossInput {
+    const void *data;
+    int64_t row, step;
+    int32_t type;             /* D1_FP32, D1_BF16 or D1_FP16; not read for the mask, whose elements are bytes */
+    int32_t pad;
+} D1LossInput;
+
+typedef struct D1PolicyLoss {
+    D1LossInput logp, old_logp, advantages;
+    D1LossInput ref_logp, entropy, values, returns, old_values, mask;      /* each may be null; values need returns */
+    int64_t rows, length;     /* `rows` sequences of `length` tokens */
+    double clip_low, clip_high;          /* 0 <= clip_low <= 1, clip_high >= 0 */
+    double value_clip;        /* 0: none, else it needs old_values */
+    double kl_coef, value_coef, entropy_coef;
+    int32_t sequence;         /* 0: every token counts alike; 1: every sequence with a token does, its tokens sharing its weight */
+    int32_t pad;
+} D1PolicyLoss;
+
+/* With d = logp - old_logp, r = e^d, x = ref_logp - logp and w a token's weight (0 where mask is 0, whatever the other
+ * inputs hold there; 1/tokens, or 1/(tokens of its sequence * sequences with a token)):
+ *   terms[0] loss = policy + value_coef * value - entropy_coef * entropy + kl_coef * kl
+ *   terms[1] policy = -sum w min(r A, min(max(r, 1 - clip_low), 1 + clip_high) A)
+ *   terms[2] value = sum w max((v - R)^2, (v' - R)^2) / 2, v' = v held within value_clip of old_values
+ *   terms[3] entropy = sum w entropy;  terms[4] kl = sum w (e^x - x - 1)
+ *   terms[5] clipped = sum of the weights of tokens whose clip is active;  terms[6] drift = sum w (e^d - d - 1)
+ *   terms[7] the tokens, or the sequences with one
+ * A term whose input is not given is 0, all are where no token is left. dlogp, dentropy and dvalues (each may be null,
+ * then it is not made; contiguous [rows, length], the type of their input) are the gradients of the loss. They must not
+ * overlap the inputs. The same inputs give the same bits. */
+int64_t d1_policy_loss_work_bytes(const D1PolicyLoss *h);
+int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentropy, void *dvalues, void *work,
+                   int64_t work_bytes, void *stream);
+/* data[0..n) (D1_FP32, D1_BF16 or D1_FP16) *= *by; nothing is written where *by is 1. */
+int d1_scale(void *data, int type, int64_t n, const float *by, void *stream);
+
+/* h[t] = (1 - z[t]) m[t] h[t-1] + z[t] x[t] with z = sigmoid(gate), for `rows` sequences of `steps` steps of `width`
+ * channels; m[t] is 0 where reset[t * reset_t + row * reset_n] is not (what was before is dropped, whatever it holds),
+ * else 1. Element (t, row, c) of x is x[t * x_t + row * x_n + c], likewise the others; strides in elements. All of a
+ * call's sequences are of one type; states are fp32 [rows, width], contiguous, and everything is computed in fp32. */
+typedef struct D1Scan {
+    const void *x, *gate;
+    const uint8_t *reset;     /* or null: none */
+    const float *state;       /* before the first step, or null: zeros */
+    float *marks;             /* fp32 [d1_scan_marks(steps), rows, width]: written by d1_scan_fwd where it is not null, read by
+                                 d1_scan_bwd, which needs it where d1_scan_marks is not 0 */
+    int64_t x_t, x_n, gate_t, gate_n, reset_t, reset_n;
+    int64_t steps, rows;
+    int32_t width, type;
+} D1Scan;
+
+int64_t d1_scan_marks(int64_t steps);
+int64_t d1_scan_work_bytes(const D1Scan *h);       /* of either call */
+/* out (x's type) and, where it is not null, last [rows, width] = the state after the last step. With no steps nothing
+ * is written. Outputs must not overlap inputs. */
+int d1_scan_fwd(const D1Scan *h, void *out, int64_t out_t, int64_t out_n, float *last, void *work, int64_t work_bytes, void *stream);
+/* The gradients of x, gate and (where dstate is not null) the state from those of the outputs; dlast may be null (zero). */
+int d1_scan_bwd(const D1Scan *h, const void *dh, int64_t dh_t, int64_t dh_n, const float *dlast, void *dx, int64_t dx_t,
+                int64_t dx_n, void *dgate, int64_t dgate_t, int64_t dgate_n, float *dstate, void *work, int64_t work_bytes,
+                void *stream);
 
 #ifdef __cplusplus
 }
