@@ -22,7 +22,8 @@ LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', '
                  'learn_step_active', 'learn_heuristic')
 OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
                'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read', 'd1_policy_loss_work_bytes',
-               'd1_policy_loss', 'd1_scale', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd')
+               'd1_policy_loss', 'd1_scale', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd',
+               'd1_muon_check', 'd1_muon_work_bytes', 'd1_muon_step')
 _LEARN = {}
 _OPS = _OPS_TORCH = None
 
@@ -120,6 +121,19 @@ class D1Scan(C.Structure):
                 ('width', C.c_int32), ('type', C.c_int32)]
 
 
+class D1MuonTensor(C.Structure):
+    """The D1MuonTensor struct of include/d1ops.h."""
+    _fields_ = [('g', C.c_void_p), ('momentum', C.c_void_p), ('out', C.c_void_p), ('copy', C.c_void_p), ('rows', C.c_int64),
+                ('cols', C.c_int64), ('lr', C.c_double), ('scale', C.c_double), ('weight_decay', C.c_double), ('type', C.c_int32),
+                ('gtype', C.c_int32)]
+
+
+class D1Muon(C.Structure):
+    """The D1Muon struct of include/d1ops.h."""
+    _fields_ = [*((name, C.c_double) for name in ('a', 'b', 'c', 'eps', 'momentum')),
+                *((name, C.c_int32) for name in ('steps', 'nesterov', 'terms', 'pad'))]
+
+
 def load_ops():
     """libd1ops.so: the operators of a policy update beside the fused step (include/d1ops.h)."""
     global _OPS
@@ -146,8 +160,11 @@ def load_ops():
         L.d1_scan_work_bytes.argtypes = [p]
         L.d1_scan_fwd.argtypes = [p, p, n, n, p, p, n, p]
         L.d1_scan_bwd.argtypes = [p, p, n, n, p, p, n, n, p, n, n, p, p, n, p]
+        L.d1_muon_check.argtypes = [p]
+        L.d1_muon_work_bytes.argtypes = [p, i, p]
+        L.d1_muon_step.argtypes = [p, i, p, p, p, n, p]
         for name in ('d1_tokens_work_bytes', 'd1_norm_work_bytes', 'd1_adamw_work_bytes', 'd1_policy_loss_work_bytes',
-                     'd1_scan_marks', 'd1_scan_work_bytes'):
+                     'd1_scan_marks', 'd1_scan_work_bytes', 'd1_muon_work_bytes'):
             getattr(L, name).restype = C.c_int64
         _OPS = L
     return _OPS

@@ -2,7 +2,7 @@
 
 libd1hip.so          environment, wait workload, LOS compiler, MFMA trunk layer, sampling, GAE, PPO step
 libd1ops.so          token log probabilities, layer norm, the AdamW step over many tensors, the policy
-                     loss, the gated recurrence (include/d1ops.h)
+                     loss, the gated recurrence, orthogonalised updates (include/d1ops.h)
 _d1ops.so            the Python module that calls it on torch tensors
 libd1learn_clump0.so the d1-stairs-v2 learning task (learn_* ABI), CLUMP_MODE 0
 libd1learn_clump1.so the same task with clumped placement in a third of resets
@@ -19,7 +19,7 @@ TARGETS = {
     'libd1hip.so': ([CSRC / 'd1_env.hip', CSRC / 'd1_policy.hip', CSRC / 'd1_forward.hip', CSRC / 'd1_ppo.hip',
                      CSRC / 'd1_maps.hip'], []),
     'libd1ops.so': ([CSRC / 'd1_tokens.hip', CSRC / 'd1_norm.hip', CSRC / 'd1_optim.hip', CSRC / 'd1_loss.hip',
-                    CSRC / 'd1_scan.hip'], []),
+                    CSRC / 'd1_scan.hip', CSRC / 'd1_muon.hip'], []),
     'libd1learn_clump0.so': ([CSRC / 'd1_learn.hip'], ['-DD1_CLUMP_MODE=0']),
     'libd1learn_clump1.so': ([CSRC / 'd1_learn.hip'], ['-DD1_CLUMP_MODE=1']),
 }

@@ -557,9 +557,134 @@ py::tuple scan_bwd(const Maybe &dh_, const Maybe &dlast_, const Tensor &x, const
     return py::make_tuple(dx, dgate, dstate);
 }
 
+// ---- orthogonalised updates
+
+D1Muon muon_settings(double a, double b, double c, double eps, int64_t steps, int64_t terms, double momentum, bool nesterov) {
+    if (steps < 1 || steps > D1_MUON_MAX_STEPS) refuse("steps must be 1 to " + std::to_string(D1_MUON_MAX_STEPS));
+    if (!(eps >= 0)) refuse("eps must not be negative");
+    if (!(momentum >= 0 && momentum < 1)) refuse("momentum must be in [0, 1)");
+    if (terms != 0 && terms != 1 && terms != 3) refuse("product_bits is None, 16 or 32");
+    D1Muon h{};
+    h.a = a;
+    h.b = b;
+    h.c = c;
+    h.eps = eps;
+    h.momentum = momentum;
+    h.steps = (int32_t)steps;
+    h.nesterov = nesterov;
+    h.terms = (int32_t)terms;
+    if (d1_muon_check(&h)) refuse("coefficients: singular values in [0, 1] must stay under 3.8 through all steps");
+    return h;
+}
+
+void muon_launch(const std::vector<D1MuonTensor> &table, const D1Muon &h, int32_t *ctl, const Tensor &on, int64_t stream) {
+    const int64_t need = d1_muon_work_bytes(table.data(), (int)table.size(), &h);
+    check(need < 0 ? (int)need : 0, "d1_muon_work_bytes");
+    const Tensor work = scratch(need, on);
+    check(d1_muon_step(table.data(), (int)table.size(), &h, ctl, ptr(work), need, (void *)stream), "d1_muon_step");
+}
+
+// matrices [..., rows, cols] -> the same, orthogonalised, contiguous and of their types
+Tensors orthogonalize(const Tensors &updates, double a, double b, double c, double eps, int64_t steps, int64_t terms, int64_t stream) {
+    no_trace("orthogonalize");
+    const D1Muon h = muon_settings(a, b, c, eps, steps, terms, 0.0, false);
+    Tensors out, held;
+    std::vector<D1MuonTensor> table;
+    for (const Tensor &u : updates) {
+        no_tangent(u, "update");
+        const int code = type_of(u.scalar_type());
+        if (code < 0 || u.dim() < 2 || !u.is_cuda() || u.device() != updates[0].device())
+            refuse("an update must be an fp32, bf16 or fp16 CUDA tensor of two dimensions or more, all on one device, not " + describe(u));
+        if (u.size(-1) > D1_MUON_MAX_SIDE || u.size(-2) > D1_MUON_MAX_SIDE)
+            refuse("an update has sides of at most " + std::to_string(D1_MUON_MAX_SIDE));
+        held.push_back(u.contiguous());
+        out.push_back(at::empty(u.sizes(), u.options()));
+        const int64_t each = u.size(-1) * u.size(-2), bytes = each * u.element_size();
+        for (int64_t i = 0; each && i < u.numel() / each; i++) {
+            D1MuonTensor t{};
+            t.g = (const char *)ptr(held.back()) + i * bytes;
+            t.out = (char *)ptr(out.back()) + i * bytes;
+            t.rows = u.size(-2);
+            t.cols = u.size(-1);
+            t.type = t.gtype = code;
+            table.push_back(t);
+        }
+    }
+    if (!table.empty()) muon_launch(table, h, nullptr, updates[0], stream);
+    return out;
+}
+
+void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momenta, const Tensor &step, const std::vector<double> &lr,
+               const std::vector<double> &scale, const std::vector<double> &weight_decay, const std::optional<std::vector<Maybe>> &copies,
+               double momentum, bool nesterov, double a, double b, double c, double eps, int64_t steps, int64_t terms, int64_t stream) {
+    no_trace("muon_step");
+    const D1Muon h = muon_settings(a, b, c, eps, steps, terms, momentum, nesterov);
+    const size_t count = params.size();
+    auto same = [&](size_t n, const char *name) {
+        if (n != count) refuse(std::string(name) + ": " + std::to_string(n) + " for " + std::to_string(count) + " parameters");
+    };
+    same(grads.size(), "grads");
+    same(momenta.size(), "momenta");
+    same(lr.size(), "lr");
+    same(scale.size(), "scales");
+    same(weight_decay.size(), "weight_decay");
+    if (copies) same(copies->size(), "copies");
+    if (step.scalar_type() != at::kInt || step.dim() != 1 || step.size(0) != 8 || !step.is_cuda() || !step.is_contiguous())
+        refuse("step must be a contiguous int32 CUDA tensor of 8 elements");
+    std::vector<D1MuonTensor> table(count);
+    Tensors held;
+    for (size_t i = 0; i < count; i++) {
+        const Tensor &p = params[i], &m = momenta[i], &g = grads[i];
+        auto fail = [&](const std::string &why) { refuse("matrix " + std::to_string(i) + ": " + why); };
+        no_tangent(p, "parameter");
+        no_tangent(g, "gradient");
+        const int ptype = type_of(p.scalar_type()), gtype = type_of(g.scalar_type());
+        if (!(ptype == D1_FP32 || ptype == D1_BF16) || !(gtype == D1_FP32 || gtype == D1_BF16))
+            fail("parameter and gradient must be fp32 or bf16, not " + describe(p) + " and " + describe(g));
+        if (p.dim() < 2) fail("a parameter must have two dimensions or more, not " + c10::str(p.sizes()));
+        if (m.scalar_type() != at::kFloat || m.sizes() != p.sizes() || g.sizes() != p.sizes())
+            fail("gradient and momentum (fp32) must have the parameter's shape");
+        if (p.device() != step.device() || g.device() != step.device() || m.device() != step.device())
+            fail("parameter, gradient and momentum must be on " + step.device().str());
+        if (!p.is_contiguous() || !m.is_contiguous()) fail("parameter and momentum must be contiguous");
+        if (!(lr[i] >= 0 && weight_decay[i] >= 0 && scale[i] >= 0) || !std::isfinite(lr[i] * scale[i]) || !std::isfinite(lr[i] * weight_decay[i]))
+            fail("lr, scale and weight_decay must be finite and not negative");
+        held.push_back(g.contiguous());
+        D1MuonTensor &t = table[i];
+        t = D1MuonTensor{};
+        t.g = ptr(held.back());
+        t.momentum = (float *)ptr(m);
+        t.out = ptr(p);
+        t.rows = p.size(0);
+        t.cols = t.rows ? p.numel() / t.rows : 0;
+        if (t.rows > D1_MUON_MAX_SIDE || t.cols > D1_MUON_MAX_SIDE) fail("a matrix has sides of at most " + std::to_string(D1_MUON_MAX_SIDE));
+        t.lr = lr[i];
+        t.scale = scale[i];
+        t.weight_decay = weight_decay[i];
+        t.type = ptype;
+        t.gtype = gtype;
+        if (copies && (*copies)[i]) {
+            const Tensor &c_ = *(*copies)[i];
+            if (c_.scalar_type() != at::kBFloat16 || c_.numel() != p.numel() || !c_.is_contiguous() || c_.device() != step.device() ||
+                ptype != D1_FP32)
+                fail("a copy is contiguous bf16 of the size of an fp32 parameter");
+            t.copy = ptr(c_);
+        }
+    }
+    muon_launch(table, h, (int32_t *)ptr(step), step, stream);
+    for (size_t i = 0; i < count; i++) {
+        written(params[i]);
+        written(momenta[i]);
+        if (copies && (*copies)[i]) written(*(*copies)[i]);
+    }
+    written(step);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_d1ops, m) {
+    m.def("orthogonalize", &orthogonalize);
+    m.def("muon_step", &muon_step);
     m.def("scan_fwd", &scan_fwd);
     m.def("scan_bwd", &scan_bwd);
     m.def("policy_loss", &policy_loss);

@@ -1,9 +1,13 @@
-"""AdamW over many tensors in a few launches, with moments in 32 or 8 bits (csrc/d1_optim.hip).
+"""AdamW over many tensors in a few launches, with moments in 32 or 8 bits (csrc/d1_optim.hip), and steps along
+orthogonalised momenta for matrices (csrc/d1_muon.hip).
 
-`AdamW` is the torch optimizer, `adamw_step` the step itself on lists of tensors, `read_moment` what
+`Muon` is the torch optimizer of the latter, `muon_step` its step on lists of tensors, `orthogonalize` the
+Newton-Schulz products alone. `AdamW` is the torch optimizer, `adamw_step` the step itself on lists of tensors, `read_moment` what
 an 8-bit moment stands for. The step count, the global norm of a clip and the skip of a step whose
 norm is not finite stay on the device, so a step can be captured in a HIP graph.
 """
+import math
+
 import torch
 
 from .ops import call
@@ -195,3 +199,57 @@ class AdamW(torch.optim.Optimizer):
         device = self.param_groups[0]['params'][0].device
         self.ctl = None if own['ctl'] is None else own['ctl'].to(device, copy=True)
         self._counter, self.seed = own['counter'], own['seed']
+
+
+# the quintic a s + b s^3 + c s^5 that pulls singular values from (0, 1] to about 0.7 to 1.2 in five steps
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+_TERMS = {None: 0, 16: 1, 32: 3}
+
+
+def _terms(product_bits):
+    if product_bits not in _TERMS:
+        raise ValueError('product_bits is None, 16 or 32')
+    return _TERMS[product_bits]
+
+
+def orthogonalize(updates, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, product_bits=None):
+    """The matrices with their singular values moved towards 1 by `steps` Newton-Schulz steps:
+
+        X = U / (|U|_F + eps); then X = a X + (b A + c A A) X with A = X X^T (on the smaller side)
+
+    updates: a tensor [..., rows, cols] or a list of such (they share launches), fp32, bf16 or fp16; the results are of the
+    same types, contiguous. product_bits: operands of the products, 16 (fp16) or 32 (two fp16 halves, 22 bits); None: 32
+    for fp32 matrices, 16 for others. Accumulation is fp32. A matrix that is not finite gives NaN or what the formula
+    gives. coefficients: singular values from [0, 1] have to stay under 3.8 through all steps."""
+    a, b, c = coefficients
+    alone = torch.is_tensor(updates)
+    updates = [updates] if alone else list(updates)
+    if not updates:
+        return []
+    out = call('orthogonalize', updates[0], updates, a, b, c, eps, steps, _terms(product_bits))
+    return out[0] if alone else out
+
+
+def muon_scale(shape, rms=False):
+    """The factor of a matrix's step: sqrt(max(1, rows / cols)), or with `rms` 0.2 sqrt(max(rows, cols)), which
+    gives an update the size of AdamW's."""
+    rows, cols = shape[0], math.prod(shape[1:])
+    return 0.2 * math.sqrt(max(rows, cols)) if rms else math.sqrt(max(1.0, rows / cols)) if cols else 1.0
+
+
+def muon_step(params, grads, momenta, step, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+              coefficients=NEWTON_SCHULZ, eps=1e-7, scales=None, copies=None, product_bits=None):
+    """One step in place along the orthogonalised momenta of lists of matrices:
+
+        m = momentum * m + g;  u = g + momentum * m (nesterov) or m;  p = p (1 - lr wd) - lr scale orthogonalize(u)
+
+    params: fp32 or bf16, contiguous, of two dimensions or more (those behind the first count as one). grads: fp32 or bf16 of
+    the same shapes. momenta: fp32. step: int32 [8] on the device, zeros before the first step; [0] counts the steps made,
+    [1] those skipped: a step with a matrix whose u has no finite norm changes nothing else. scales: one for each matrix
+    (None: muon_scale of its shape). copies: bf16 tensors that get the new fp32 parameters (None in the list: no copy).
+    lr and weight_decay: one value or one for each matrix. product_bits: as in orthogonalize, None by the parameters' types."""
+    count = len(params)
+    a, b, c = coefficients
+    scales = [muon_scale(p.shape) for p in params] if scales is None else scales
+    call('muon_step', step, params, grads, momenta, step, _each(lr, count), scales, _each(weight_decay, count), copies,
+         momentum, nesterov, a, b, c, eps, steps, _terms(product_bits))

@@ -6,6 +6,7 @@
  *   d1_adamw_*    one AdamW step over many tensors, moments in 32 or 8 bits, clip by the global norm
  *   d1_policy_loss*   the clipped policy loss with value, entropy and reference-KL terms, and its gradients
  *   d1_scan_*     a gated linear recurrence over long sequences, forward and backward
+ *   d1_muon_*     updates orthogonalised by Newton-Schulz products, and the momentum step made of them
  *
  * Conventions as in d1hip.h: device pointers unless said otherwise, asynchronous on `stream`
  * (0 = the null stream), 0 on success, a hipError_t code for launch failures or a negative D1_E_*
@@ -34,6 +35,8 @@ extern "C" {
 #define D1_NORM_MAX_WIDTH 16384
 #define D1_SCAN_MAX_WIDTH (1 << 24)
 #define D1_SCAN_MAX_STEPS (1 << 30)
+#define D1_MUON_MAX_SIDE (1 << 17)
+#define D1_MUON_MAX_STEPS 32
 #define D1_ADAMW_BLOCK 256            /* elements of an 8-bit moment that share an exponent */
 
 /* For row i of logits [rows, vocab] over its allowed entries (mask[i * mask_stride + j] != 0; all
@@ -182,6 +185,36 @@ int d1_scan_fwd(const D1Scan *h, void *out, int64_t out_t, int64_t out_n, float 
 int d1_scan_bwd(const D1Scan *h, const void *dh, int64_t dh_t, int64_t dh_n, const float *dlast, void *dx, int64_t dx_t,
                 int64_t dx_n, void *dgate, int64_t dgate_t, int64_t dgate_n, float *dstate, void *work, int64_t work_bytes,
                 void *stream);
+
+/* One matrix [rows, cols], contiguous. With `momentum` (fp32) it is a parameter's step, else out = O(g). */
+typedef struct D1MuonTensor {
+    const void *g;            /* gradient, or the matrix that is orthogonalised */
+    float *momentum;
+    void *out;                /* the parameter (D1_FP32 or D1_BF16), or the result (any type) */
+    void *copy;               /* of a step: bf16 copy of the new parameter, or null */
+    int64_t rows, cols;
+    double lr, scale, weight_decay;
+    int32_t type, gtype;      /* of out and of g; of a step D1_FP32 or D1_BF16 */
+} D1MuonTensor;
+
+typedef struct D1Muon {
+    double a, b, c;           /* of the quintic a s + b s^3 + c s^5 */
+    double eps, momentum;
+    int32_t steps, nesterov;
+    int32_t terms;            /* operands of the products: 1: fp16, 3: two fp16 halves (22 bits), 0: 3 for fp32 results, 1 for others */
+    int32_t pad;
+} D1Muon;
+
+/* 0 where the coefficients can be used: `steps` times the quintic, from singular values in [0, 1], stays under 3.8 and its
+ * factor a + b s^2 + c s^4 under 15, the range of what the products hold; else D1_E_ARG. */
+int d1_muon_check(const D1Muon *h);
+/* O(U): X = U / (|U|_F + eps), then `steps` times X = a X + (b A + c A A) X with A = X X^T (on the smaller side).
+ * Of a step: m = momentum m + g;  U = nesterov ? g + momentum m : m;  p = p (1 - lr weight_decay) - lr scale O(U).
+ * ctl as in d1_adamw_step, [0] steps made, [1] steps skipped, or null: with it a step with a U whose norm is not finite
+ * changes nothing but ctl[1]. `t` and `h` are host arrays, read before the call returns. Matrices with no elements are left
+ * out. Results must not overlap each other or gradients. The same inputs give the same bits. */
+int64_t d1_muon_work_bytes(const D1MuonTensor *t, int count, const D1Muon *h);
+int d1_muon_step(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl, void *work, int64_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,245 @@
+"""orthogonalize and muon_step against their definition in 64 bits: sizes that end inside tiles, both ways round, types,
+lists and batches, steps that are skipped, graphs, refusals. How far the products may be off follows an emulation
+that rounds at the same places to the same bits."""
+import importlib
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda'
+TYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+
+
+@pytest.fixture(scope='module')
+def O():
+    return importlib.import_module('dcss-auto_amd.optim')
+
+
+def matrix(rows, cols, seed=0, dtype=torch.float32, rank=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    u = torch.randn(rows, cols, generator=g, device=DEV)
+    if rank:
+        u = 0.3 * u + torch.randn(rows, rank, generator=g, device=DEV) @ torch.randn(rank, cols, generator=g, device=DEV)
+    return (u * 1e-3).to(dtype)
+
+
+def newton_schulz(u, coefficients, steps=5, eps=1e-7, held=lambda x: x, product=lambda x, y: x @ y):
+    a, b, c = coefficients
+    x = u.double() / (u.double().norm() + eps)
+    flip = x.shape[0] > x.shape[1]
+    x = held(x.t() if flip else x)
+    for step in range(steps):
+        g = held(product(x, x.t()))
+        p = b * g + c * product(g, g)
+        p.diagonal().add_(a)
+        x = product(held(p), x)
+        if step < steps - 1:
+            x = held(x)
+    return x.t() if flip else x
+
+
+def emulation(u, coefficients, terms, **k):
+    """The roundings of the operands (fp16, or two halves), sums in fp32."""
+    def held(x):
+        x = x * 4096
+        hi = x.half().double()
+        return (hi + ((x - hi).half().double() if terms == 3 else 0)) / 4096
+    return newton_schulz(u, coefficients, held=held, product=lambda x, y: (x.float().contiguous() @ y.float().contiguous()).double(), **k)
+
+
+def check(O, got, u, terms, coefficients=None, dtype=None, **k):
+    coefficients = coefficients or O.NEWTON_SCHULZ
+    want = newton_schulz(u, coefficients, **k)
+    dtype = dtype or u.dtype
+    assert got.dtype == dtype and got.shape == u.shape
+    size = float(want.norm())
+    r = 2.0 ** (-22 if terms == 3 else -11)
+    emulated = float((emulation(u, coefficients, terms, **k) - want).norm())
+    # The errors' size over a matrix varies little from one order of sums to another, but for a few entries alone: then the
+    # first-order bound, 20 r sqrt(m) a step for the roundings of A, B and X, carried on by at most 3.9 (the quintic's slope) a step
+    few = min(u.shape) < 16
+    bound = 3 * emulated + (6200 if few else 16) * r * size + torch.finfo(dtype).eps / 2 * size + 1e-12
+    off = got.double() - want
+    assert float(off.norm()) <= bound, (tuple(u.shape), float(off.norm()) / size, bound / size)
+    # and no entry stands out: 8 times the mean's root is past what 10^7 normal errors reach, but for those of a last
+    # rounding, half a step of the entry
+    worst = 8 * bound / math.sqrt(u.numel()) if not few else bound
+    assert bool((off.abs() <= worst + torch.finfo(dtype).eps / 2 * want.abs()).all()), (tuple(u.shape), float(off.abs().max()), worst)
+
+
+@pytest.mark.parametrize('bits', [16, 32])
+@pytest.mark.parametrize('rows,cols', [(1, 1), (1, 9), (7, 1), (2, 2), (17, 256), (31, 33), (64, 64), (65, 63), (96, 400), (130, 129),
+                                       (256, 1800), (1800, 256), (500, 1111), (999, 1001), (1, 5000), (3000, 70)])
+def test_sizes(O, rows, cols, bits):
+    print(f'[muon] {rows} {cols} {bits}', flush=True)
+    for rank in (0, 3):
+        u = matrix(rows, cols, rows + cols, rank=rank)
+        check(O, O.orthogonalize(u, product_bits=bits), u, 3 if bits == 32 else 1)
+
+
+@pytest.mark.parametrize('bits', [16, 32])
+@pytest.mark.parametrize('count,rows,cols', [(1, 2100, 2070), (32, 780, 801), (9, 1500, 400), (1, 300, 9001), (3, 1030, 4100)])
+def test_tiles(O, count, rows, cols, bits):
+    """Every kind of tile, ends inside them."""
+    print(f'[muon] tiles {count} {rows} {cols} {bits}', flush=True)
+    u = [matrix(rows, cols, k) for k in range(count)]
+    out = O.orthogonalize(u, product_bits=bits)
+    for k in {0, count // 2, count - 1}:
+        check(O, out[k], u[k], 3 if bits == 32 else 1)
+
+
+@pytest.mark.parametrize('dtype', list(TYPES))
+def test_types(O, dtype):
+    for rows, cols in ((40, 300), (300, 40), (700, 650)):
+        u = matrix(rows, cols, 3, TYPES[dtype]) * (1000 if dtype == 'fp16' else 1)
+        check(O, O.orthogonalize(u), u, 3 if dtype == 'fp32' else 1)
+        check(O, O.orthogonalize(u, product_bits=32), u, 3)
+
+
+def test_lists_and_batches(O):
+    """A list of any sizes and types is its matrices one by one; leading dimensions are matrices; strides; nothing."""
+    print('[muon] lists', flush=True)
+    u = [matrix(r, c, i, TYPES[t]) for i, (r, c, t) in enumerate([(17, 256, 'fp32'), (256, 256, 'bf16'), (256, 1800, 'fp32'), (5, 3, 'bf16'),
+                                                                  (300, 200, 'fp32')] * 9)]
+    u.insert(3, torch.zeros(0, 5, device=DEV))
+    out = O.orthogonalize(u)
+    assert out[3].shape == (0, 5)
+    for a, b in zip(out, u):
+        if a.numel():
+            check(O, a, b, 3 if b.dtype == torch.float32 else 1)
+    batch = torch.stack([matrix(50, 70, k) for k in range(6)]).view(2, 3, 50, 70)
+    out = O.orthogonalize(batch)
+    assert out.shape == batch.shape
+    for i in range(2):
+        for j in range(3):
+            assert torch.equal(out[i, j], O.orthogonalize(batch[i, j]))
+    assert torch.equal(O.orthogonalize(batch[0, 0].t().contiguous().t()), out[0, 0])
+    assert O.orthogonalize([]) == [] and O.orthogonalize(torch.zeros(3, 0, 4, device=DEV)).shape == (3, 0, 4)
+
+
+def test_other_polynomials_and_scales(O):
+    """Cubic steps that converge, one step alone, matrices of any size of entries; a matrix of zeros stays one."""
+    u = matrix(120, 200, 5)
+    cubic = (1.5, -0.5, 0.0)
+    out = O.orthogonalize(u, steps=25, coefficients=cubic)
+    assert float((out.double() @ out.double().t() - torch.eye(120, dtype=torch.float64, device=DEV)).abs().max()) < 1e-4
+    check(O, O.orthogonalize(u, steps=1), u, 3, steps=1)
+    for factor in (1e-20, 1e20):
+        big = u * factor
+        check(O, O.orthogonalize(big, eps=0.0), big, 3, eps=0.0)
+    zero = torch.zeros(70, 90, device=DEV)
+    assert torch.equal(O.orthogonalize(zero), zero)
+    bad = u.clone()
+    bad[3, 4] = math.nan
+    both = O.orthogonalize([bad, u])
+    assert bool(both[0].isnan().any()) and torch.equal(both[1], O.orthogonalize(u))
+
+
+@pytest.mark.parametrize('ptype,gtype', [('fp32', 'fp32'), ('fp32', 'bf16'), ('bf16', 'bf16'), ('bf16', 'fp32')])
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_step(O, ptype, gtype, nesterov):
+    print(f'[muon] step {ptype} {gtype} {nesterov}', flush=True)
+    shapes = [(256, 90), (17, 256), (300, 300), (40, 3, 5)]
+    lr, wd, mu = [0.02, 0.01, 0.5, 0.02], [0.0, 0.1, 0.1, 0.0], 0.9
+    p = [torch.randn(s, device=DEV, generator=torch.Generator(DEV).manual_seed(i)).to(TYPES[ptype]) for i, s in enumerate(shapes)]
+    m = [torch.zeros(s, device=DEV) for s in shapes]
+    step = torch.zeros(8, dtype=torch.int32, device=DEV)
+    copies = [torch.zeros(s, device=DEV, dtype=torch.bfloat16) if i % 2 else None for i, s in enumerate(shapes)] if ptype == 'fp32' else None
+    terms = 3 if ptype == 'fp32' else 1
+    for n in range(3):
+        g = [matrix(s[0], math.prod(s[1:]), 10 * n + i, TYPES[gtype]).view(s) for i, s in enumerate(shapes)]
+        old, versions = [x.double() for x in p], [x._version for x in p]
+        momenta = [x.double() for x in m]
+        O.muon_step(p, g, m, step, lr=lr, momentum=mu, nesterov=nesterov, weight_decay=wd, copies=copies)
+        assert int(step[0]) == n + 1 and int(step[1]) == 0
+        for i, s in enumerate(shapes):
+            want_m = mu * momenta[i] + g[i].double()
+            # mu rounded, a product and a sum
+            assert bool(((m[i].double() - want_m).abs() <= 3 * 2.0 ** -24 * ((mu * momenta[i]).abs() + g[i].double().abs())).all())
+            u = (g[i].double() + mu * want_m if nesterov else want_m).view(s[0], -1)
+            scale = math.sqrt(max(1, s[0] / math.prod(s[1:])))
+            o = newton_schulz(u, O.NEWTON_SCHULZ).view(s)
+            e = emulation(u, O.NEWTON_SCHULZ, terms)
+            few = min(u.shape) < 16
+            r = 2.0 ** (-22 if terms == 3 else -11)
+            near = 3 * float((e.view(s) - o).norm()) + (6200 if few else 16) * r * float(o.norm())
+            want = old[i] * (1 - lr[i] * wd[i]) - lr[i] * scale * o
+            # an entry's share of what the products may be off, and the step's own roundings
+            bound = lr[i] * scale * 8 * near / math.sqrt(u.numel()) + 4 * 2.0 ** -24 * (old[i].abs() + lr[i] * scale * o.abs())
+            bound = bound + torch.finfo(p[i].dtype).eps / 2 * want.abs()
+            assert bool(((p[i].double() - want).abs() <= bound).all())
+            assert p[i]._version > versions[i]
+            if copies and copies[i] is not None:
+                assert torch.equal(copies[i], p[i].bfloat16())
+
+
+def test_not_finite_is_skipped(O):
+    """A step with any norm that is not finite changes nothing but the count, on the device; the next goes on."""
+    p, m = [torch.randn(50, 60, device=DEV) for _ in range(2)], [torch.randn(50, 60, device=DEV) for _ in range(2)]
+    step = torch.zeros(8, dtype=torch.int32, device=DEV)
+    for value in (math.nan, math.inf, -math.inf):
+        before = [x.clone() for x in p + m]
+        g = [torch.randn(50, 60, device=DEV) for _ in range(2)]
+        g[1][49, 59] = value
+        O.muon_step(p, g, m, step)
+        assert all(torch.equal(a, b) for a, b in zip(before, p + m))
+    assert step[:2].tolist() == [0, 3]
+    O.muon_step(p, [torch.randn(50, 60, device=DEV) for _ in range(2)], m, step)
+    assert step[:2].tolist() == [1, 3] and not torch.equal(p[0], before[0])
+    # a learning rate of 0 leaves parameters and moves momenta
+    before = [x.clone() for x in p + m]
+    O.muon_step(p, [torch.randn(50, 60, device=DEV) for _ in range(2)], m, step, lr=0.0)
+    assert torch.equal(p[0], before[0]) and not torch.equal(m[0], before[2])
+
+
+def test_stream_and_graph(O):
+    print('[muon] graph', flush=True)
+    shapes = [(70, 200), (300, 100)]
+    p, q = ([torch.randn(s, device=DEV, generator=torch.Generator(DEV).manual_seed(i)) for i, s in enumerate(shapes)] for _ in range(2))
+    g = [torch.zeros(s, device=DEV) for s in shapes]
+    m, n = ([torch.zeros(s, device=DEV) for s in shapes] for _ in range(2))
+    sp, sq = (torch.zeros(8, dtype=torch.int32, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        O.orthogonalize(torch.randn(70, 200, device=DEV))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        O.muon_step(p, g, m, sp)
+    for i in range(4):
+        for x in g:
+            x.normal_()
+        O.muon_step(q, g, n, sq)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(p + m + [sp], q + n + [sq])), i
+
+
+def test_repeats(O):
+    u = [matrix(700, 900, k) for k in range(3)]
+    a, b = O.orthogonalize(u), O.orthogonalize(u)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_refusals(O):
+    u = matrix(8, 9)
+    for bad in (u.cpu(), u.double(), u[0], [u, u.cpu()]):
+        with pytest.raises(ValueError):
+            O.orthogonalize(bad)
+    for k in (dict(steps=0), dict(steps=33), dict(eps=-1.0), dict(product_bits=8), dict(coefficients=(10.0, 0.0, 0.0)),
+              dict(coefficients=(math.nan, 0.0, 0.0)), dict(coefficients=(3.0, -3.0, 5.0))):
+        with pytest.raises(ValueError):
+            O.orthogonalize(u, **k)
+    p, g, m, step = [u.clone()], [u], [torch.zeros_like(u)], torch.zeros(8, dtype=torch.int32, device=DEV)
+    for args in (([p[0].half()], g, m, step), (p, [u.half()], m, step), (p, [u[:, :3]], m, step), (p, g, [m[0].bfloat16()], step),
+                 (p, g, m, step[:4]), (p, g, m, step.float()), (p, [], m, step), ([u.t()], [u.t()], [u.t()], step), ([u[0]], [u[0]], [u[0]], step)):
+        with pytest.raises(ValueError):
+            O.muon_step(*args)
+    for k in (dict(lr=-1.0), dict(lr=math.nan), dict(weight_decay=-1.0), dict(momentum=1.0), dict(scales=[1.0, 2.0]), dict(scales=[math.inf]),
+              dict(copies=[u])):
+        with pytest.raises(ValueError):
+            O.muon_step(p, g, m, step, **k)
