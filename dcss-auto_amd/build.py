@@ -13,7 +13,7 @@ import sysconfig
 
 HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / 'csrc'
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-ffp-contract=off',
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off',
          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 TARGETS = {
     'libd1hip.so': ([CSRC / 'd1_env.hip', CSRC / 'd1_policy.hip', CSRC / 'd1_forward.hip', CSRC / 'd1_ppo.hip',
@@ -44,37 +44,47 @@ def _binding_commands(obj, out):
 
 
 def build(verbose=False):
+    """Every source file is an object of its own (compiled side by side, the longest first to start), then the links."""
     start = lambda cmd: subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)  # noqa: E731
-    jobs, built, errors = [], [], []
-    obj, bound, bound_tmp = HERE / '_d1ops.o', HERE / BINDING, HERE / (BINDING + '.tmp')
-    compile_, link = _binding_commands(obj, bound_tmp)
-    for name, (sources, defs) in TARGETS.items():
-        out = HERE / name
-        tmp = out.with_suffix('.so.tmp')
-        cmd = ['hipcc', *FLAGS, *defs, '-I', str(HERE.parent / 'include'), '-o', str(tmp), *map(str, sources)]
-        jobs.append((out, tmp, cmd, start(cmd)))
-    jobs.append((obj, None, compile_, start(compile_)))
-    for out, tmp, cmd, proc in jobs:
+    built, errors = [], []
+
+    def finish(what, cmd, proc):
         _, err = proc.communicate()
         if proc.returncode:
-            errors.append(f'{out.name}: {cmd[0]} failed:\n{err}')
-            continue
-        if tmp is not None:
-            tmp.replace(out)
-            built.append(out)
-        if verbose:
+            errors.append(f'{what}: {cmd[0]} failed:\n{err}')
+        elif verbose:
             print(' '.join(cmd))
+
+    include = ['-I', str(HERE.parent / 'include')]
+    binding_obj, bound, bound_tmp = HERE / '_d1ops.o', HERE / BINDING, HERE / (BINDING + '.tmp')
+    compile_, link_binding = _binding_commands(binding_obj, bound_tmp)
+    objects, jobs = {}, [(BINDING, compile_, start(compile_))]
+    for name, (sources, defs) in TARGETS.items():
+        objects[name] = [HERE / f'{pathlib.Path(name).stem}.{src.stem}.o' for src in sources]
+        for src, obj in zip(sources, objects[name]):
+            cmd = ['hipcc', *FLAGS, *defs, *include, '-c', str(src), '-o', str(obj)]
+            jobs.append((name, cmd, start(cmd)))
+    for job in jobs:
+        finish(*job)
     if not errors:
-        proc = start(link)
-        _, err = proc.communicate()
-        if proc.returncode:
-            errors.append(f'{BINDING}: g++ failed:\n{err}')
-        else:
+        jobs = []
+        for name, objs in objects.items():
+            out, tmp = HERE / name, (HERE / name).with_suffix('.so.tmp')
+            cmd = ['hipcc', '--offload-arch=gfx950', '-fPIC', '-shared', '-o', str(tmp), *map(str, objs)]
+            jobs.append((out, tmp, cmd, start(cmd)))
+        for out, tmp, cmd, proc in jobs:
+            finish(out.name, cmd, proc)
+            if tmp.exists() and not proc.returncode:
+                tmp.replace(out)
+                built.append(out)
+    if not errors:
+        proc = start(link_binding)
+        finish(BINDING, link_binding, proc)
+        if not proc.returncode:
             bound_tmp.replace(bound)
-            obj.unlink()
             built.append(bound)
-            if verbose:
-                print(' '.join(link))
+    for obj in [binding_obj, *(o for objs in objects.values() for o in objs)]:
+        obj.unlink(missing_ok=True)
     if errors:
         raise RuntimeError('\n'.join(errors))
     return built

@@ -18,7 +18,7 @@ namespace d1o {
 enum { LOGP, OLD, ADV, REF, ENT, VAL, RET, OLDV, INPUTS };
 enum { ABSENT, FLAT, PER_ROW, STRIDED };
 enum { S_POLICY, S_VALUE, S_ENTROPY, S_KL, S_CLIPPED, S_DRIFT, SUMS };
-constexpr int LOSS_GRID = 1024, COUNT_GRID = 1024, SINGLE = 4096;
+constexpr int LOSS_GRID = 1024, COUNT_GRID = 1024, SINGLE = 8192;
 
 struct Input {
     const void *p;
@@ -29,44 +29,38 @@ struct Loss {
     Input in[INPUTS];
     Input mask;
     int64_t rows, length, total;
-    double log_low, log_high, vclip, inv_length;
+    int64_t jump_rows, jump_t;           // a thread's next tokens: so many rows and tokens on
+    double log_low, log_high, vclip;
     float low, high, kl, vcoef, ecoef;
-    int32_t sequence, value_clip;
+    int32_t sequence, value_clip, by_row;
     void *dlogp, *dentropy, *dvalues;
 };
 
-// i = row * length + t for i < 2^52
-__device__ __forceinline__ int64_t row_of(int64_t i, int64_t length, double inv_length, int64_t &t) {
-    int64_t row = (int64_t)((double)i * inv_length);
-    t = i - row * length;
-    if (t < 0) {
-        row--;
-        t += length;
-    } else if (t >= length) {
-        row++;
-        t -= length;
-    }
-    return row;
-}
-
-// four tokens' elements as they lie in memory; converted once all loads are under way
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// four tokens from i = row * length + t (row and t only where a.by_row is set); `have` of them are there
 struct Where {
     int64_t i, row, t, length;
-    int have;                 // of the four
+    int have;
 };
-template <class B>
-__device__ __forceinline__ void fetch_strided(const Input &in, const Where &w, B *out) {
+// their elements as they lie in memory; converted once all loads are under way
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool ANY, class B>
+__device__ __forceinline__ void fetch_each(const Input &in, const Where &w, B *out) {
+    if (!ANY && in.mode != PER_ROW) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[j] = ((const B *)in.p)[w.i + (j < w.have ? j : w.have - 1)];
+        return;
+    }
     int64_t row = w.row, t = w.t;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        out[j] = j < w.have ? ((const B *)in.p)[row * in.row + t * in.step] : (B)0;
+        out[j] = j < w.have ? ((const B *)in.p)[row * in.row + (ANY ? t * in.step : 0)] : (B)0;
         if (++t == w.length) {
             t = 0;
             row++;
         }
     }
 }
+template <bool ANY>
 __device__ __forceinline__ u32x4 fetch(const Input &in, const Where &w) {
     u32x4 r = {0, 0, 0, 0};
     if (in.mode == FLAT && w.have == 4) {
@@ -81,17 +75,18 @@ __device__ __forceinline__ u32x4 fetch(const Input &in, const Where &w) {
     } else if (in.mode != ABSENT) {
         if (in.type == D1_FP32) {
             uint32_t v[4];
-            fetch_strided<uint32_t>(in, w, v);
+            fetch_each<ANY>(in, w, v);
             r = u32x4{v[0], v[1], v[2], v[3]};
         } else {
             uint16_t v[4];
-            fetch_strided<uint16_t>(in, w, v);
+            fetch_each<ANY>(in, w, v);
             r[0] = v[0] | (uint32_t)v[1] << 16;
             r[1] = v[2] | (uint32_t)v[3] << 16;
         }
     }
     return r;
 }
+template <bool ANY>
 __device__ __forceinline__ uint32_t fetch_mask(const Input &in, const Where &w) {
     if (in.mode == ABSENT) return 0x01010101u;
     uint32_t r = 0;
@@ -99,15 +94,27 @@ __device__ __forceinline__ uint32_t fetch_mask(const Input &in, const Where &w) 
         __builtin_memcpy(&r, (const uint8_t *)in.p + w.i, 4);
     } else {
         uint8_t v[4];
-        fetch_strided<uint8_t>(in, w, v);
+        fetch_each<ANY>(in, w, v);
         r = v[0] | v[1] << 8 | v[2] << 16 | (uint32_t)v[3] << 24;
     }
     return r;
 }
-__device__ __forceinline__ float value_of(u32x4 r, int j, int type) {
-    if (type == D1_FP32) return __uint_as_float(r[j]);
-    const uint32_t h = r[j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
-    return type == D1_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+struct Four {
+    float v[4];
+};
+__device__ __forceinline__ Four values_of(u32x4 r, int type) {
+    Four f;
+    if (type == D1_FP32) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) f.v[j] = __uint_as_float(r[j]);
+    } else if (type == D1_BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) f.v[j] = __uint_as_float(j & 1 ? r[j >> 1] & 0xFFFF0000u : r[j >> 1] << 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) f.v[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[j >> 1] >> (16 * (j & 1))));
+    }
+    return f;
 }
 __device__ __forceinline__ void put(void *p, int type, const Where &w, const float *v) {
     if (type == D1_FP32) {
@@ -142,103 +149,139 @@ __device__ __forceinline__ float excess(float x, float e, float &rise) {
 template <int THREADS, class T>
 __device__ __forceinline__ T block_sum(T x, T *s) {
     for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    if (THREADS == 64) return x;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
     __syncthreads();
     T sum = 0;
+#pragma unroll 4
     for (int w = 0; w < THREADS / 64; w++) sum += s[w];
     return sum;
 }
-
-__device__ __forceinline__ int bytes_set(uint32_t m) {
-    return ((m & 0xFFu) != 0) + ((m & 0xFF00u) != 0) + ((m & 0xFF0000u) != 0) + ((m & 0xFF000000u) != 0);
+// All sums at once: 32 threads each, which add what the workgroup's threads left in LDS (one after another through lane
+// moves they took 10 us of a workgroup's end). The result is in thread 32 k's `sum` for k < SUMS.
+template <int THREADS>
+__device__ __forceinline__ double block_sums(const double *sums, double (*s)[THREADS + 1]) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SUMS; k++) s[k][threadIdx.x] = sums[k];
+    __syncthreads();
+    double x = 0.0;
+    if (threadIdx.x < 32 * SUMS)
+#pragma unroll 8
+        for (int i = threadIdx.x & 31; i < THREADS; i += 32) x += s[threadIdx.x >> 5][i];
+    for (int d = 16; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
 }
 
-// The mask's counts. Token level: parts[block] = tokens of the block's share. Sequence level: counts[row], and
-// parts[block] = rows with a token among the block's rows (a wave a row).
-__global__ __launch_bounds__(256) void k_loss_count(const Loss a, int64_t *__restrict__ parts, int64_t *__restrict__ counts) {
+__device__ __forceinline__ int bytes_set(uint32_t m) { return __popc((((m & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | m) & 0x80808080u); }
+
+// The mask's counts. Token level: parts[block] = tokens of the block's share. Sequence level: inverse[row] = 1 / tokens (0
+// where there is none), and parts[block] = rows with a token among the block's rows (LANES threads a row).
+template <int LANES>
+__global__ __launch_bounds__(256) void k_loss_count_rows(const Loss a, int64_t *__restrict__ parts, float *__restrict__ inverse) {
+    constexpr int ROWS = 256 / LANES;
+    __shared__ int64_t s[4];
+    const int lane = threadIdx.x % LANES;
+    int64_t some = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+        const uint8_t *m = (const uint8_t *)a.mask.p + row * a.mask.row;
+        int64_t n = 0;
+        if (a.mask.step == 1) {
+            int64_t t = (int64_t)lane * 16;
+#pragma unroll 4
+            for (; t + 16 <= a.length; t += LANES * 16) {
+                const Pack<uint32_t, 4> v = load<uint32_t, 4>((const uint32_t *)(m + t));
+                n += bytes_set(v.v[0]) + bytes_set(v.v[1]) + bytes_set(v.v[2]) + bytes_set(v.v[3]);
+            }
+            for (int j = 0; j < 16; j++) n += t + j < a.length && m[t + j];
+        } else {
+            for (int64_t t = lane; t < a.length; t += LANES) n += m[t * a.mask.step] != 0;
+        }
+        n = block_sum<LANES>(n, s);
+        if (lane == 0) {
+            inverse[row] = n ? 1.f / (float)n : 0.f;
+            some += n > 0;
+        }
+    }
+    some = block_sum<256>(some, s);
+    if (threadIdx.x == 0) parts[blockIdx.x] = some;
+}
+__global__ __launch_bounds__(256) void k_loss_count(const Loss a, int64_t *__restrict__ parts) {
     __shared__ int64_t s[4];
     int64_t sum = 0;
-    if (a.sequence) {
-        for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows; row += (int64_t)gridDim.x * 4) {
-            int64_t n = 0;
-            for (int64_t t = (threadIdx.x & 63) * 4; t < a.length; t += 256) {
-                const int have = a.length - t < 4 ? (int)(a.length - t) : 4;
-                n += bytes_set(fetch_mask(a.mask, {row * a.length + t, row, t, a.length, have}));
-            }
-            for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-            if ((threadIdx.x & 63) == 0) {
-                counts[row] = n;
-                sum += n > 0;
-            }
+    if (a.mask.mode == FLAT) {
+        const uint8_t *m = (const uint8_t *)a.mask.p;
+        int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+#pragma unroll 4
+        for (; i + 16 <= a.total; i += (int64_t)gridDim.x * 4096) {
+            const Pack<uint32_t, 4> v = load<uint32_t, 4>((const uint32_t *)(m + i));
+            sum += bytes_set(v.v[0]) + bytes_set(v.v[1]) + bytes_set(v.v[2]) + bytes_set(v.v[3]);
         }
+        for (int j = 0; j < 16; j++) sum += i + j < a.total && m[i + j];
     } else {
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < a.total; i += (int64_t)gridDim.x * 1024) {
-            Where w = {i, 0, 0, a.length, a.total - i < 4 ? (int)(a.total - i) : 4};
-            if (a.mask.mode != FLAT || w.have < 4) w.row = row_of(i, a.length, a.inv_length, w.t);
-            sum += bytes_set(fetch_mask(a.mask, w));
-        }
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.total; i += (int64_t)gridDim.x * 256)
+            sum += ((const uint8_t *)a.mask.p)[i / a.length * a.mask.row + i % a.length * a.mask.step] != 0;
     }
     sum = block_sum<256>(sum, s);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
-template <bool GRAD>
-__device__ __forceinline__ void four(const Loss &a, const Where &w, float unit, const int64_t *counts, double rows_some, double *sums) {
-    const uint32_t mask = fetch_mask(a.mask, w);
+template <bool VALUES, bool ANY>
+__device__ __forceinline__ void four(const Loss &a, const Where &w, float unit, const float *inverse, double *sums) {
+    const uint32_t mask = fetch_mask<ANY>(a.mask, w);
     u32x4 raw[INPUTS];
 #pragma unroll
-    for (int k = 0; k < INPUTS; k++) raw[k] = fetch(a.in[k], w);
+    for (int k = 0; k < (VALUES ? INPUTS : VAL); k++) raw[k] = fetch<ANY>(a.in[k], w);
     float weight[4];
-    if (counts) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) weight[j] = unit;
+    if (inverse) {
         int64_t row = w.row, t = w.t;
-        float one = 0.f;
+        float one = inverse[row] * unit;
+#pragma unroll
         for (int j = 0; j < 4; j++) {
-            if (j == 0 || t == 0) one = j < w.have ? (float)(1.0 / ((double)counts[row] * rows_some)) : 0.f;
             weight[j] = one;
-            if (++t == w.length) {
+            if (++t == w.length && j + 1 < w.have) {
                 t = 0;
-                row++;
+                one = inverse[++row] * unit;
             }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) weight[j] = unit;
     }
+    Four x[INPUTS];
+#pragma unroll
+    for (int k = 0; k < (VALUES ? INPUTS : VAL); k++) x[k] = values_of(raw[k], a.in[k].type);
     float dl[4], de[4], dv[4], sum[SUMS] = {};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const bool in = j < w.have && (mask >> (8 * j) & 0xFFu);
         const float wt = in ? weight[j] : 0.f;
-        const float logp = value_of(raw[LOGP], j, a.in[LOGP].type), adv = value_of(raw[ADV], j, a.in[ADV].type);
-        const double d = (double)logp - (double)value_of(raw[OLD], j, a.in[OLD].type);
+        const float logp = x[LOGP].v[j], adv = x[ADV].v[j];
+        const double d = (double)logp - (double)x[OLD].v[j];
         const bool past = adv > 0.f ? d > a.log_high : adv < 0.f && d < a.log_low;
         const float df = (float)d, r = expf(df);
-        float g = past ? 0.f : -adv * r;
-        if (in) {
-            sum[S_POLICY] -= (past ? (adv > 0.f ? 1.f + a.high : 1.f - a.low) : r) * adv * wt;
-            sum[S_CLIPPED] += past ? wt : 0.f;
-            float rise;
-            sum[S_DRIFT] += excess(df, r, rise) * wt;
-        }
+        float g = past ? 0.f : -adv * r, rise;
+        const float gain = (past ? (adv > 0.f ? 1.f + a.high : 1.f - a.low) : r) * adv, drift = excess(df, r, rise);
+        sum[S_POLICY] -= in ? gain * wt : 0.f;
+        sum[S_CLIPPED] += past ? wt : 0.f;
+        sum[S_DRIFT] += in ? drift * wt : 0.f;
         if (a.in[REF].mode) {
-            const float x = (float)((double)value_of(raw[REF], j, a.in[REF].type) - (double)logp);
-            float rise;
-            const float q = excess(x, expf(x), rise);
-            if (in) sum[S_KL] += q * wt;
+            const float gap = (float)((double)x[REF].v[j] - (double)logp);
+            const float q = excess(gap, expf(gap), rise);
+            sum[S_KL] += in ? q * wt : 0.f;
             g -= a.kl * rise;
         }
         dl[j] = in ? g * wt : 0.f;
         if (a.in[ENT].mode) {
-            if (in) sum[S_ENTROPY] += value_of(raw[ENT], j, a.in[ENT].type) * wt;
+            sum[S_ENTROPY] += in ? x[ENT].v[j] * wt : 0.f;
             de[j] = -a.ecoef * wt;
         }
-        if (a.in[VAL].mode) {
-            const double v = value_of(raw[VAL], j, a.in[VAL].type), ret = value_of(raw[RET], j, a.in[RET].type);
+        if (VALUES) {
+            const double v = x[VAL].v[j], ret = x[RET].v[j];
             double far = v - ret;
             bool free = true;
             if (a.value_clip) {
-                const double old = value_of(raw[OLDV], j, a.in[OLDV].type), gap = v - old;
+                const double old = x[OLDV].v[j], gap = v - old;
                 if (!(fabs(gap) <= a.vclip) && gap == gap) {
                     const double held = old + (gap > 0.0 ? a.vclip : -a.vclip) - ret;
                     free = !(held * held > far * far);
@@ -246,74 +289,96 @@ __device__ __forceinline__ void four(const Loss &a, const Where &w, float unit, 
                 }
             }
             const float f = (float)far;
-            if (in) sum[S_VALUE] += 0.5f * f * f * wt;
+            sum[S_VALUE] += in ? 0.5f * f * f * wt : 0.f;
             dv[j] = in && free ? f * wt * a.vcoef : 0.f;
         }
     }
 #pragma unroll
     for (int k = 0; k < SUMS; k++) sums[k] += (double)sum[k];
-    if (GRAD) {
-        if (a.dlogp) put(a.dlogp, a.in[LOGP].type, w, dl);
-        if (a.dentropy) put(a.dentropy, a.in[ENT].type, w, de);
-        if (a.dvalues) put(a.dvalues, a.in[VAL].type, w, dv);
-    }
+    if (a.dlogp) put(a.dlogp, a.in[LOGP].type, w, dl);
+    if (a.dentropy) put(a.dentropy, a.in[ENT].type, w, de);
+    if (VALUES && a.dvalues) put(a.dvalues, a.in[VAL].type, w, dv);
 }
 
-// loss, policy, value, entropy, kl, clipped, drift and the count (tokens, or sequences with a token)
-__device__ __forceinline__ void finish(const Loss &a, const double *sums, double count, float *terms) {
-    terms[0] = (float)(sums[S_POLICY] + (double)a.vcoef * sums[S_VALUE] - (double)a.ecoef * sums[S_ENTROPY] + (double)a.kl * sums[S_KL]);
-    for (int k = 0; k < SUMS; k++) terms[1 + k] = (float)sums[k];
+// loss, policy, value, entropy, kl, clipped, drift and the count (tokens, or sequences with a token): thread 32 k has sum k
+__device__ __forceinline__ void finish(const Loss &a, double sum, double count, float *terms, double *all) {
+    if ((threadIdx.x & 31) == 0 && threadIdx.x < 32 * SUMS) {
+        all[threadIdx.x >> 5] = sum;
+        terms[1 + (threadIdx.x >> 5)] = (float)sum;
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+    terms[0] = (float)(all[S_POLICY] + (double)a.vcoef * all[S_VALUE] - (double)a.ecoef * all[S_ENTROPY] + (double)a.kl * all[S_KL]);
     terms[7] = (float)count;
 }
 
-template <int THREADS, bool GRAD>
+// A single workgroup counts its mask by itself (THREADS 1,024).
+template <int THREADS, bool VALUES, bool ANY>
 __global__ __launch_bounds__(THREADS) void k_loss(const Loss a, const int64_t *__restrict__ count_parts, int nparts,
-                                                  const int64_t *__restrict__ counts, double *__restrict__ parts, float *__restrict__ terms) {
+                                                  const float *__restrict__ inverse, double *__restrict__ parts, float *__restrict__ terms) {
     __shared__ int64_t si[THREADS / 64];
-    __shared__ double sd[THREADS / 64];
+    __shared__ double sd[SUMS][THREADS + 1], all[SUMS];
+    Where w = {((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4, 0, 0, a.length, 4};
+    if (a.by_row) {
+        w.row = w.i / a.length;
+        w.t = w.i - w.row * a.length;
+    }
     int64_t count = a.sequence && a.length ? a.rows : a.total;
     if (nparts) {
         count = 0;
         for (int i = threadIdx.x; i < nparts; i += THREADS) count += count_parts[i];
         count = block_sum<THREADS>(count, si);
-    } else if (a.mask.mode && THREADS == 1024) {        // the only workgroup counts by itself
+    } else if (THREADS == 1024 && a.mask.mode) {
         count = 0;
-        for (int64_t i = (int64_t)threadIdx.x * 4; i < a.total; i += THREADS * 4) {
-            Where w = {i, 0, 0, a.length, a.total - i < 4 ? (int)(a.total - i) : 4};
-            w.row = row_of(i, a.length, a.inv_length, w.t);
-            count += bytes_set(fetch_mask(a.mask, w));
+        for (Where v = w; v.i < a.total; v.i += THREADS * 4) {
+            v.have = a.total - v.i < 4 ? (int)(a.total - v.i) : 4;
+            uint32_t m = fetch_mask<ANY>(a.mask, v);
+            if (v.have < 4) m &= (1u << (8 * v.have)) - 1;
+            count += bytes_set(m);
+            v.row += a.jump_rows;
+            v.t += a.jump_t;
+            if (v.t >= a.length) {
+                v.t -= a.length;
+                v.row++;
+            }
         }
         count = block_sum<THREADS>(count, si);
     }
     // every sequence alike without a mask: 1 / (length x rows)
-    const float unit = (float)(1.0 / (a.sequence && !counts ? (double)a.total : count > 0 ? (double)count : 1.0));
+    const float unit = (float)(1.0 / (a.sequence && !inverse && !a.mask.mode ? (double)a.total : count > 0 ? (double)count : 1.0));
     double sums[SUMS] = {};
-    for (int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4; i < a.total; i += (int64_t)gridDim.x * THREADS * 4) {
-        Where w = {i, 0, 0, a.length, a.total - i < 4 ? (int)(a.total - i) : 4};
-        w.row = row_of(i, a.length, a.inv_length, w.t);
-        four<GRAD>(a, w, unit, counts, (double)count, sums);
+    for (; w.i < a.total; w.i += (int64_t)gridDim.x * THREADS * 4) {
+        w.have = a.total - w.i < 4 ? (int)(a.total - w.i) : 4;
+        four<VALUES, ANY>(a, w, unit, inverse, sums);
+        w.row += a.jump_rows;
+        w.t += a.jump_t;
+        if (w.t >= a.length) {
+            w.t -= a.length;
+            w.row++;
+        }
     }
-#pragma unroll
-    for (int k = 0; k < SUMS; k++) sums[k] = block_sum<THREADS>(sums[k], sd);
-    if (threadIdx.x) return;
-    if (gridDim.x == 1)
-        return finish(a, sums, (double)count, terms);
-    for (int k = 0; k < SUMS; k++) parts[(int64_t)k * gridDim.x + blockIdx.x] = sums[k];
-    if (blockIdx.x == 0) parts[(int64_t)SUMS * gridDim.x] = (double)count;
+    const double sum = block_sums<THREADS>(sums, sd);
+    if (a.sequence && a.rows == 1) count = count > 0;
+    if (gridDim.x == 1) return finish(a, sum, (double)count, terms, all);
+    if ((threadIdx.x & 31) == 0 && threadIdx.x < 32 * SUMS) parts[(int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x] = sum;
+    if (blockIdx.x == 0 && threadIdx.x == 0) parts[(int64_t)SUMS * gridDim.x] = (double)count;
 }
 
-__global__ __launch_bounds__(1024) void k_loss_finish(const Loss a, const double *__restrict__ parts, int n, float *__restrict__ terms) {
-    __shared__ double sd[16];
+__global__ __launch_bounds__(256) void k_loss_finish(const Loss a, const double *__restrict__ parts, int n, float *__restrict__ terms) {
+    __shared__ double sd[SUMS][257], all[SUMS];
     double sums[SUMS];
 #pragma unroll
     for (int k = 0; k < SUMS; k++) {
-        double x = 0.0;
-        for (int i = threadIdx.x; i < n; i += 1024) x += parts[(int64_t)k * n + i];
-        sums[k] = x;
-    }
+        double x[LOSS_GRID / 256];
 #pragma unroll
-    for (int k = 0; k < SUMS; k++) sums[k] = block_sum<1024>(sums[k], sd);
-    if (threadIdx.x == 0) finish(a, sums, parts[(int64_t)SUMS * n], terms);
+        for (int u = 0; u < LOSS_GRID / 256; u++) {
+            const int i = u * 256 + threadIdx.x;
+            x[u] = i < n ? parts[(int64_t)k * n + i] : 0.0;
+        }
+        sums[k] = (x[0] + x[1]) + (x[2] + x[3]);
+    }
+    const double sum = block_sums<256>(sums, sd);
+    finish(a, sum, parts[(int64_t)SUMS * n], terms, all);
 }
 
 // Gradients made for a loss gradient of 1, scaled by the real one; nothing is read or written where that is 1.
@@ -321,12 +386,12 @@ __global__ __launch_bounds__(256) void k_loss_scale(void *p, int type, int64_t n
     const float f = *by;
     if (f == 1.f) return;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-        const Where w = {i, 0, i, n, n - i < 4 ? (int)(n - i) : 4};
-        const u32x4 r = fetch({p, 0, 1, FLAT, type}, w);
-        float v[4];
+        const Where w = {i, 0, 0, n, n - i < 4 ? (int)(n - i) : 4};
+        const u32x4 r = fetch<false>({p, 0, 1, FLAT, type}, w);
+        Four x = values_of(r, type);
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = value_of(r, j, type) * f;
-        put(p, type, w, v);
+        for (int j = 0; j < 4; j++) x.v[j] *= f;
+        put(p, type, w, x.v);
     }
 }
 
@@ -334,14 +399,17 @@ inline int loss_grid(int64_t total) {
     const int64_t n = (total + 1023) / 1024;
     return (int)(n < LOSS_GRID ? n : LOSS_GRID);
 }
+// A sequence alone is its tokens. Rows are counted by a wave each, long ones by a workgroup.
+inline bool rows_counted(const D1PolicyLoss *h) { return h->sequence && h->rows > 1 && h->mask.data; }
+inline bool rows_long(const D1PolicyLoss *h) { return h->length > 8192; }
 inline int count_grid(const D1PolicyLoss *h) {
-    const int64_t n = h->sequence ? (h->rows + 3) / 4 : (h->rows * h->length + 4095) / 4096;
+    const int64_t n = !rows_counted(h) ? (h->rows * h->length + 16383) / 16384 : rows_long(h) ? h->rows : (h->rows + 3) / 4;
     return (int)(n < 1 ? 1 : n < COUNT_GRID ? n : COUNT_GRID);
 }
-// One workgroup of 1,024 threads does all in one launch. A mask by sequences has counts a row to keep.
+// One workgroup of 1,024 threads does all in one launch, but for the counts of several sequences.
 inline bool is_single(const D1PolicyLoss *h) {
     const int64_t total = h->rows * h->length;
-    return total == 0 || (total <= SINGLE && !(h->sequence && h->mask.data));
+    return total == 0 || (total <= SINGLE && !rows_counted(h));
 }
 
 static bool loss_args(const D1PolicyLoss *h) {
@@ -361,8 +429,22 @@ static bool loss_args(const D1PolicyLoss *h) {
 static Input input(const D1LossInput &t, const D1PolicyLoss *h) {
     Input in{t.data, t.row, t.step, ABSENT, t.type};
     if (t.data)
-        in.mode = (t.step == 1 || h->length <= 1) && (t.row == h->length || h->rows <= 1) ? FLAT : STRIDED;
+        in.mode = (t.step == 1 || h->length <= 1) && (t.row == h->length || h->rows <= 1) ? FLAT : t.step == 0 ? PER_ROW : STRIDED;
     return in;
+}
+
+template <int THREADS>
+static void loss_launch(const Loss &a, bool any, int grid, const int64_t *count_parts, int nparts, const float *inverse, double *parts,
+                        float *terms, hipStream_t stream) {
+    const dim3 g(grid), b(THREADS);
+    if (a.in[VAL].mode && any)
+        hipLaunchKernelGGL((k_loss<THREADS, true, true>), g, b, 0, stream, a, count_parts, nparts, inverse, parts, terms);
+    else if (a.in[VAL].mode)
+        hipLaunchKernelGGL((k_loss<THREADS, true, false>), g, b, 0, stream, a, count_parts, nparts, inverse, parts, terms);
+    else if (any)
+        hipLaunchKernelGGL((k_loss<THREADS, false, true>), g, b, 0, stream, a, count_parts, nparts, inverse, parts, terms);
+    else
+        hipLaunchKernelGGL((k_loss<THREADS, false, false>), g, b, 0, stream, a, count_parts, nparts, inverse, parts, terms);
 }
 
 }  // namespace d1o
@@ -375,7 +457,7 @@ int64_t d1_policy_loss_work_bytes(const D1PolicyLoss *h) {
     const int64_t total = h->rows * h->length;
     if (is_single(h)) return 0;
     return (int64_t)sizeof(double) * (SUMS * loss_grid(total) + 1) +
-           (h->mask.data ? (int64_t)sizeof(int64_t) * (count_grid(h) + (h->sequence ? h->rows : 0)) : 0);
+           (h->mask.data ? (int64_t)sizeof(int64_t) * count_grid(h) + (rows_counted(h) ? (int64_t)sizeof(float) * h->rows : 0) : 0);
 }
 
 int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentropy, void *dvalues, void *work, int64_t work_bytes,
@@ -394,7 +476,6 @@ int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentr
     a.rows = h->rows;
     a.length = h->length;
     a.total = h->rows * h->length;
-    a.inv_length = h->length ? 1.0 / (double)h->length : 0.0;
     a.log_low = log1p(-h->clip_low);
     a.log_high = log1p(h->clip_high);
     a.low = (float)h->clip_low;
@@ -408,24 +489,33 @@ int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentr
     a.dlogp = dlogp;
     a.dentropy = dentropy;
     a.dvalues = dvalues;
-    const bool grad = dlogp || dentropy || dvalues;
-    if (is_single(h)) {
-        if (grad)
-            hipLaunchKernelGGL((k_loss<1024, true>), dim3(1), dim3(1024), 0, stream, a, nullptr, 0, nullptr, nullptr, terms);
-        else
-            hipLaunchKernelGGL((k_loss<1024, false>), dim3(1), dim3(1024), 0, stream, a, nullptr, 0, nullptr, nullptr, terms);
-        return (int)hipGetLastError();
+    bool any = a.mask.mode == STRIDED || a.mask.mode == PER_ROW, rows = any;
+    for (const Input &in : a.in) {
+        any |= in.mode == STRIDED;
+        rows |= in.mode == STRIDED || in.mode == PER_ROW;
     }
-    const int grid = loss_grid(a.total), nparts = a.mask.mode ? count_grid(h) : 0;
+    const bool single = is_single(h);
+    const int grid = single ? 1 : loss_grid(a.total), nparts = !single && a.mask.mode ? count_grid(h) : 0;
     double *parts = (double *)work;
     int64_t *count_parts = (int64_t *)(parts + SUMS * grid + 1);
-    int64_t *counts = a.mask.mode && a.sequence ? count_parts + nparts : nullptr;
-    if (nparts) hipLaunchKernelGGL(k_loss_count, dim3(nparts), dim3(256), 0, stream, a, count_parts, counts);
-    if (grad)
-        hipLaunchKernelGGL((k_loss<256, true>), dim3(grid), dim3(256), 0, stream, a, count_parts, nparts, counts, parts, terms);
+    float *inverse = nparts && rows_counted(h) ? (float *)(count_parts + nparts) : nullptr;
+    a.by_row = rows || inverse;
+    if (a.by_row) {
+        const int64_t jump = (int64_t)grid * (single ? 1024 : 256) * 4;
+        a.jump_rows = a.length ? jump / a.length : 0;
+        a.jump_t = a.length ? jump % a.length : 0;
+    }
+    if (inverse && rows_long(h))
+        hipLaunchKernelGGL(k_loss_count_rows<256>, dim3(nparts), dim3(256), 0, stream, a, count_parts, inverse);
+    else if (inverse)
+        hipLaunchKernelGGL(k_loss_count_rows<64>, dim3(nparts), dim3(256), 0, stream, a, count_parts, inverse);
+    else if (nparts)
+        hipLaunchKernelGGL(k_loss_count, dim3(nparts), dim3(256), 0, stream, a, count_parts);
+    if (single)
+        loss_launch<1024>(a, any, 1, nullptr, 0, nullptr, nullptr, terms, stream);
     else
-        hipLaunchKernelGGL((k_loss<256, false>), dim3(grid), dim3(256), 0, stream, a, count_parts, nparts, counts, parts, terms);
-    if (grid > 1) hipLaunchKernelGGL(k_loss_finish, dim3(1), dim3(1024), 0, stream, a, parts, grid, terms);
+        loss_launch<256>(a, any, grid, count_parts, nparts, inverse, parts, terms, stream);
+    if (grid > 1) hipLaunchKernelGGL(k_loss_finish, dim3(1), dim3(256), 0, stream, a, parts, grid, terms);
     return (int)hipGetLastError();
 }
 

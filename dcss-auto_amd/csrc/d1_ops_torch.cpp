@@ -517,8 +517,10 @@ py::tuple scan_fwd(const Tensor &x, const Tensor &gate, const Maybe &state, cons
     if (a.h.steps == 0) return py::make_tuple(h, a.state ? a.state->clone() : at::zeros(a.cells, fp32), Maybe());
     const Tensor last = at::empty(a.cells, fp32);
     Maybe marks, work;
-    if (keep && d1_scan_marks(a.h.steps)) {
-        marks = at::empty({d1_scan_marks(a.h.steps), a.h.rows * a.h.width}, fp32);
+    const int64_t count = keep ? d1_scan_marks(&a.h) : 0;
+    check(count < 0 ? (int)count : 0, "d1_scan_marks");
+    if (count) {
+        marks = at::empty({count, a.h.rows * a.h.width}, fp32);
         a.h.marks = (float *)ptr(marks);
     }
     const int64_t need = d1_scan_work_bytes(&a.h);
@@ -541,7 +543,8 @@ py::tuple scan_bwd(const Maybe &dh_, const Maybe &dlast_, const Tensor &x, const
         return py::make_tuple(dx, dgate, dstate);
     }
     if (state) dstate = at::empty(a.cells, x.options().dtype(at::kFloat));
-    const int64_t count = d1_scan_marks(a.h.steps);
+    const int64_t count = d1_scan_marks(&a.h);
+    check(count < 0 ? (int)count : 0, "d1_scan_marks");
     if (count) {
         if (!marks || marks->scalar_type() != at::kFloat || !marks->is_contiguous() || marks->device() != x.device() ||
             marks->numel() != count * a.h.rows * a.h.width)

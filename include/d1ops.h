@@ -169,14 +169,14 @@ typedef struct D1Scan {
     const void *x, *gate;
     const uint8_t *reset;     /* or null: none */
     const float *state;       /* before the first step, or null: zeros */
-    float *marks;             /* fp32 [d1_scan_marks(steps), rows, width]: written by d1_scan_fwd where it is not null, read by
+    float *marks;             /* fp32 [d1_scan_marks(h), rows, width]: written by d1_scan_fwd where it is not null, read by
                                  d1_scan_bwd, which needs it where d1_scan_marks is not 0 */
     int64_t x_t, x_n, gate_t, gate_n, reset_t, reset_n;
     int64_t steps, rows;
     int32_t width, type;
 } D1Scan;
 
-int64_t d1_scan_marks(int64_t steps);
+int64_t d1_scan_marks(const D1Scan *h);             /* by steps, rows and width */
 int64_t d1_scan_work_bytes(const D1Scan *h);       /* of either call */
 /* out (x's type) and, where it is not null, last [rows, width] = the state after the last step. With no steps nothing
  * is written. Outputs must not overlap inputs. */
