@@ -16,6 +16,7 @@
 // only tiles on and under the diagonal are computed, and written in both places.
 #include <math.h>
 
+#include <algorithm>
 #include <new>
 
 #include "d1_rows.h"
@@ -28,7 +29,7 @@ typedef d1f::floatx16 acc_t;
 typedef d1f::u32x4 u32x4;
 
 constexpr int GROUP = 32;                  // matrices of a launch
-constexpr int NORM_PARTS = 256;            // workgroups that sum a matrix's squares
+constexpr int NORM_PARTS = 1024;           // workgroups that sum a matrix's squares
 constexpr float SCALE = 4096.f;            // of X, A and B as they are held
 enum { GRAM, POLY, APPLY, LAST };
 enum { C_STEP, C_SKIPPED, C_GO = 6 };
@@ -39,12 +40,14 @@ struct Mat {
     void *out, *copy;                      // rows x cols as the caller has them
     float size, keep;                      // of a step: out = out * keep - size * O, else out = O
     int32_t rows, cols, m64, n64;
-    int32_t last_tile;                     // tiles of this and all matrices before, for the launch
+    int32_t last_tile;                     // workgroups of this and all matrices before, for the launch
+    int32_t splits, first_part;            // workgroups that share a tile's contraction; the first one's partial result
     uint8_t flip, type, step, pad;
 };
 struct Mats {
     Mat t[GROUP];
     const int32_t *ctl;
+    float *parts;                          // partial results: per workgroup its 32 x 32 blocks as the lanes hold them
     float ca, cb, cc;
     int32_t count, turn, mode;             // turn: which xt is current
 };
@@ -66,6 +69,8 @@ struct Sources {
     int32_t count, nesterov;
 };
 
+static_assert(sizeof(Mats) <= 4096 && sizeof(Sources) <= 4096, "kernel arguments");
+
 template <class T>
 __device__ __forceinline__ int find(const T *t, int count, int i, int &within) {
     int lo = 0, hi = count - 1;
@@ -80,29 +85,70 @@ __device__ __forceinline__ int find(const T *t, int count, int i, int &within) {
     return lo;
 }
 
+struct Quad {
+    float v[4];
+};
+// four adjacent elements from any address, of which `have` (1 to 4) are there
+__device__ __forceinline__ Quad quad(const void *p, int type, int64_t i, int have) {
+    Quad q;
+    if (type == D1_FP32) {
+        const Pack<float, 4> a = load_part<float, 4>((const float *)p + i, have, 0.f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) q.v[j] = a.v[j];
+    } else if (type == D1_BF16) {
+        const Pack<__bf16, 4> a = load_part<__bf16, 4>((const __bf16 *)p + i, have, (__bf16)0.f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) q.v[j] = (float)a.v[j];
+    } else {
+        const Pack<_Float16, 4> a = load_part<_Float16, 4>((const _Float16 *)p + i, have, (_Float16)0.f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) q.v[j] = (float)a.v[j];
+    }
+    return q;
+}
 __device__ __forceinline__ float element(const void *p, int type, int64_t i) {
     return type == D1_FP32 ? ((const float *)p)[i] : type == D1_BF16 ? (float)((const __bf16 *)p)[i] : (float)((const _Float16 *)p)[i];
 }
-// what is orthogonalised, and the new momentum
-__device__ __forceinline__ float update_of(const Source &t, const Sources &s, int64_t i, float &m) {
-    const float g = element(t.g, t.type, i);
+// what is orthogonalised, and the new momentum, from the gradient and the momentum before
+__device__ __forceinline__ Quad update_of(const Source &t, const Sources &s, Quad g, Quad &m) {
     if (!t.mom) return g;
-    m = s.mu * t.mom[i] + g;
-    return s.nesterov ? __builtin_fmaf(s.mu, m, g) : m;
+    Quad u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        m.v[j] = s.mu * m.v[j] + g.v[j];
+        u.v[j] = s.nesterov ? __builtin_fmaf(s.mu, m.v[j], g.v[j]) : m.v[j];
+    }
+    return u;
 }
 
-// sums of squares, a share of the matrix a workgroup
+// sums of squares, a share of the matrix a workgroup; four packs a thread on their way at a time
 __global__ __launch_bounds__(256) void k_muon_norm(const Sources s) {
     __shared__ double sh[4];
     int part;
     const int k = find(s.t, s.count, blockIdx.x, part);
     const Source &t = s.t[k];
-    const int64_t n = (int64_t)t.rows * t.cols;
+    const int64_t n = (int64_t)t.rows * t.cols, stride = (int64_t)t.parts * 1024;
     double sum = 0.0;
-    for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n; i += (int64_t)t.parts * 256) {
-        float m;
-        const double u = update_of(t, s, i, m);
-        sum = __builtin_fma(u, u, sum);
+    for (int64_t i = (int64_t)part * 1024 + threadIdx.x * 4; i < n; i += 4 * stride) {
+        Quad g[4], m[4];
+        int have[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t at = i + u * stride;
+            have[u] = n - at >= 4 ? 4 : n - at > 0 ? (int)(n - at) : 0;
+            const int64_t from = have[u] ? at : 0;
+            g[u] = quad(t.g, t.type, from, have[u]);
+            m[u] = t.mom ? quad(t.mom, D1_FP32, from, have[u]) : Quad{};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const Quad x = update_of(t, s, g[u], m[u]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double d = j < have[u] ? (double)x.v[j] : 0.0;
+                sum = __builtin_fma(d, d, sum);
+            }
+        }
     }
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
@@ -140,7 +186,7 @@ __device__ __forceinline__ int64_t plane_of(int rows64, int k64) { return (int64
 // X and X^T in fragment order from 64 x 64 tiles of the update, zeros past its end; the new momentum
 template <int TERMS>
 __global__ __launch_bounds__(256) void k_muon_prepare(const Sources s) {
-    __shared__ float tile[64][65];
+    __shared__ __attribute__((aligned(16))) float tile[64][68];
     if (s.ctl && !s.ctl[C_GO]) return;
     int within;
     const int k = find(s.t, s.count, blockIdx.x, within);
@@ -148,17 +194,27 @@ __global__ __launch_bounds__(256) void k_muon_prepare(const Sources s) {
     const double scale = s.scales[k];
     const int cols64 = t.flip ? t.m64 : t.n64;
     const int r0 = within / cols64 * 64, c0 = within % cols64 * 64;
-    for (int e = threadIdx.x; e < 4096; e += 256) {
-        const int r = r0 + (e >> 6), c = c0 + (e & 63);
-        float v = 0.f;
-        if (r < t.rows && c < t.cols) {
-            const int64_t i = (int64_t)r * t.cols + c;
-            float m;
-            const float u = update_of(t, s, i, m);
-            if (t.mom) t.mom[i] = m;
-            v = (float)((double)u * scale);
+    const int c = c0 + (threadIdx.x & 15) * 4, have = t.cols - c >= 4 ? 4 : t.cols - c > 0 ? t.cols - c : 0;
+    Quad g[4], m[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int r = r0 + u * 16 + (threadIdx.x >> 4);
+        const int n = r < t.rows ? have : 0;
+        const int64_t i = n ? (int64_t)r * t.cols + c : 0;
+        g[u] = quad(t.g, t.type, i, n);
+        m[u] = t.mom ? quad(t.mom, D1_FP32, i, n) : Quad{};
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int r = r0 + u * 16 + (threadIdx.x >> 4);
+        Quad x = update_of(t, s, g[u], m[u]);
+        if (t.mom && r < t.rows) {
+            Pack<float, 4> out = {{m[u].v[0], m[u].v[1], m[u].v[2], m[u].v[3]}};
+            store_part<float, 4>(t.mom + (int64_t)r * t.cols + c, have, out);
         }
-        tile[e >> 6][e & 63] = v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x.v[j] = r < t.rows && j < have ? (float)((double)x.v[j] * scale) : 0.f;
+        *(Quad *)&tile[u * 16 + (threadIdx.x >> 4)][(threadIdx.x & 15) * 4] = x;
     }
     __syncthreads();
     // the tile's rows as rows of X (of X^T where the matrix is turned), then its columns as rows of the other
@@ -194,6 +250,8 @@ struct Operand {
 struct Job {
     Operand p, q;             // out = p q^T
     int bi, bj;               // tile
+    int k_lo, k_hi;           // steps of 16, multiples of 4
+    int part;                 // of the launch's partial results
     bool both;                // off the diagonal of a symmetric result: written in both places
 };
 
@@ -203,6 +261,9 @@ __device__ __forceinline__ int job_of(const Mats &s, int i, Job &job) {
     int within;
     const int k = find(s.t, s.count, i, within);
     const Mat &t = s.t[k];
+    job.part = t.first_part + within;
+    const int split = within % t.splits;
+    within /= t.splits;
     const int64_t pm = plane_of(t.m64, t.m64), px = plane_of(t.m64, t.n64);
     job.both = false;
     if (s.mode == GRAM || s.mode == POLY) {
@@ -226,6 +287,9 @@ __device__ __forceinline__ int job_of(const Mats &s, int i, Job &job) {
         job.bi = within % down;
         job.bj = within / down;
     }
+    const int chunks = job.p.k16 / 4, per = (chunks + t.splits - 1) / t.splits;
+    job.k_lo = split * per * 4;
+    job.k_hi = (split * per + per < chunks ? split * per + per : chunks) * 4;
     return k;
 }
 
@@ -308,13 +372,55 @@ __device__ __forceinline__ void put_tile(const Mats &s, const Mat &t, const Job 
     }
 }
 
+// A share of a tile's contraction: the wave's 32 x 32 block `at` of `blocks`, as the lanes hold it
+__device__ __forceinline__ void put_part(const Mats &s, const Mat &, const Job &job, acc_t d, int blocks, int at) {
+    float *p = s.parts + ((int64_t)job.part * blocks + at) * 1024 + (threadIdx.x & 63) * 4;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const Pack<float, 4> v = {{d[4 * g], d[4 * g + 1], d[4 * g + 2], d[4 * g + 3]}};
+        store<float, 4>(p + g * 256, v);
+    }
+}
+// and the shares joined, in their order: a wave a block
+template <int TERMS, int TILE>
+__global__ __launch_bounds__(256) void k_muon_join(const Mats s) {
+    constexpr int RB = TILE / 32, BLOCKS = RB * RB;
+    __shared__ __attribute__((aligned(16))) _Float16 scratch[4][32 * 40];
+    if (s.ctl && !s.ctl[C_GO]) return;
+    const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = (int)(id / BLOCKS), at = (int)(id % BLOCKS);
+    // tiles of the matrices whose contraction is shared; the others were finished where they were made
+    int k = 0, left = tile;
+    for (; k < s.count; k++) {
+        const int tiles = s.t[k].splits > 1 ? (s.t[k].last_tile - (k ? s.t[k - 1].last_tile : 0)) / s.t[k].splits : 0;
+        if (left < tiles) break;
+        left -= tiles;
+    }
+    if (k == s.count) return;
+    const Mat &t = s.t[k];
+    Job job;
+    job_of<TILE>(s, (k ? s.t[k - 1].last_tile : 0) + left * t.splits, job);
+    acc_t d;
+#pragma unroll
+    for (int r = 0; r < 16; r++) d[r] = 0.f;
+    for (int w = 0; w < t.splits; w++) {
+        const float *p = s.parts + ((int64_t)(job.part + w) * BLOCKS + at) * 1024 + (threadIdx.x & 63) * 4;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const Pack<float, 4> v = load<float, 4>(p + g * 256);
+#pragma unroll
+            for (int j = 0; j < 4; j++) d[4 * g + j] += v.v[j];
+        }
+    }
+    put_tile<TERMS>(s, t, job, d, job.bi * RB + at / RB, job.bj * RB + at % RB, scratch[threadIdx.x >> 6]);
+}
+
 // Small results: a workgroup a tile of 32 SIDE, its waves share the contraction and join in LDS; operands straight from
-// the caches into registers.
+// the caches into registers, the next ones on their way while some are multiplied.
 template <int TERMS, int SIDE>
 __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
-    constexpr int W = 4, PL = TERMS == 3 ? 2 : 1;
+    constexpr int W = 4, PL = TERMS == 3 ? 2 : 1, AT_ONCE = TERMS == 3 && SIDE == 2 ? 2 : 4;
     __shared__ float sums[W][SIDE * SIDE][16][64];
-    __shared__ __attribute__((aligned(16))) _Float16 scratch[W][32 * 40];
     if (s.ctl && !s.ctl[C_GO]) return;
     Job job;
     const Mat &t = s.t[job_of<32 * SIDE>(s, blockIdx.x, job)];
@@ -333,31 +439,44 @@ __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
         p[i] = job.p.p + (int64_t)(I < job.p.rb ? I : job.p.rb - 1) * job.p.k16 * 512 + lane * 8;
         q[i] = job.q.p + (int64_t)(J < job.q.rb ? J : job.q.rb - 1) * job.q.k16 * 512 + lane * 8;
     }
-    const int chunks = job.p.k16 / 4, per = (chunks + W - 1) / W;
-    const int lo = wave * per, hi = lo + per < chunks ? lo + per : chunks;
-    for (int c = lo; c < hi; c++) {
-        half8 a[4][PL][SIDE], b[4][PL][SIDE];
+    const int first = job.k_lo / AT_ONCE, batches = job.k_hi / AT_ONCE, per = (batches - first + W - 1) / W;      // multiples of 4
+    const int lo = first + wave * per, hi = lo + per < batches ? lo + per : batches;
+    half8 a[2][AT_ONCE][PL][SIDE], b[2][AT_ONCE][PL][SIDE];
+    auto operands = [&](int batch, int to) {
+        const int at = batch * AT_ONCE * 512;
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < AT_ONCE; k++)
 #pragma unroll
             for (int pl = 0; pl < PL; pl++)
 #pragma unroll
                 for (int i = 0; i < SIDE; i++) {
-                    a[k][pl][i] = *(const half8 *)(p[i] + pl * job.p.plane + (c * 4 + k) * 512);
-                    b[k][pl][i] = *(const half8 *)(q[i] + pl * job.q.plane + (c * 4 + k) * 512);
+                    a[to][k][pl][i] = *(const half8 *)(p[i] + pl * job.p.plane + at + k * 512);
+                    b[to][k][pl][i] = *(const half8 *)(q[i] + pl * job.q.plane + at + k * 512);
                 }
+    };
+    auto multiply = [&](int of) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < AT_ONCE; k++)
 #pragma unroll
             for (int i = 0; i < SIDE; i++)
 #pragma unroll
                 for (int j = 0; j < SIDE; j++) {
-                    acc[i][j] = mma(a[k][0][i], b[k][0][j], acc[i][j]);
+                    acc[i][j] = mma(a[of][k][0][i], b[of][k][0][j], acc[i][j]);
                     if (TERMS == 3) {
-                        acc[i][j] = mma(a[k][0][i], b[k][PL - 1][j], acc[i][j]);
-                        acc[i][j] = mma(a[k][PL - 1][i], b[k][0][j], acc[i][j]);
+                        acc[i][j] = mma(a[of][k][0][i], b[of][k][PL - 1][j], acc[i][j]);
+                        acc[i][j] = mma(a[of][k][PL - 1][i], b[of][k][0][j], acc[i][j]);
                     }
                 }
+    };
+    if (lo < hi) {
+        operands(lo, 0);
+        for (int c = lo; c < hi; c += 2) {
+            if (c + 1 < hi) operands(c + 1, 1);
+            multiply(0);
+            if (c + 1 >= hi) break;
+            if (c + 2 < hi) operands(c + 2, 0);
+            multiply(1);
+        }
     }
 #pragma unroll
     for (int i = 0; i < SIDE; i++)
@@ -366,16 +485,26 @@ __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
 #pragma unroll
             for (int r = 0; r < 16; r++) sums[wave][i * SIDE + j][r][lane] = acc[i][j][r];
     __syncthreads();
-    for (int e = wave; e < SIDE * SIDE; e += W) {
-        acc_t d;
+    acc_t d;
+    if (wave < SIDE * SIDE)
 #pragma unroll
-        for (int r = 0; r < 16; r++) d[r] = (sums[0][e][r][lane] + sums[1][e][r][lane]) + (sums[2][e][r][lane] + sums[3][e][r][lane]);
-        put_tile<TERMS>(s, t, job, d, job.bi * SIDE + e / SIDE, job.bj * SIDE + e % SIDE, scratch[wave]);
-    }
+        for (int r = 0; r < 16; r++) {
+            float x[W];
+#pragma unroll
+            for (int w = 0; w < W; w++) x[w] = sums[w][wave][r][lane];
+            d[r] = (x[0] + x[1]) + (x[2] + x[3]);
+        }
+    __syncthreads();
+    if (wave >= SIDE * SIDE) return;
+    if (t.splits > 1)
+        put_part(s, t, job, d, SIDE * SIDE, wave);
+    else
+        put_tile<TERMS>(s, t, job, d, job.bi * SIDE + wave / SIDE, job.bj * SIDE + wave % SIDE, (_Float16 *)sums[wave]);
 }
 
-// Large results: a workgroup a tile of TILE x TILE, operands through two LDS buffers: while one is multiplied the next
-// stage lands in the other, straight from memory.
+// Large results: a workgroup a tile of TILE x TILE, operands through a ring of LDS buffers that memory fills directly:
+// while one is multiplied, three more are on their way (with one ahead the matrix units idled nearly half the time: a
+// stage's products are over before the next stage's loads from the last cache).
 constexpr int waves_of(int tile) { return tile == 256 ? 8 : 4; }
 template <int TERMS, int TILE>
 struct Large {
@@ -383,17 +512,25 @@ struct Large {
     static constexpr int DOWN = 2, ACROSS = WAVES / 2;                    // waves
     static constexpr int NI = TILE / 32 / DOWN, NJ = TILE / 32 / ACROSS;  // results a wave
     static constexpr int PL = TERMS == 3 ? 2 : 1, RB = TILE / 32;
-    static constexpr int QS = TERMS == 3 ? 2 : 4;                         // steps of 16 a stage
+    static constexpr int QS = TERMS == 3 ? 1 : 2;                         // steps of 16 a stage
     static constexpr int PIECES = 2 * PL * RB * QS;                       // kilobytes a stage
+    static constexpr int MINE = PIECES / WAVES;                           // a wave's
     static constexpr int STAGE = PIECES * 512;                            // halves
+    static constexpr int RING = 4;
 };
 typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
 
+// All but the last LEFT of this wave's loads have landed and its LDS reads are done; then the workgroup's.
+template <int LEFT>
+__device__ __forceinline__ void wait_stage() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// (apart from the kernel, whose host side does not know buffer descriptors)
 template <int TERMS, int TILE>
-__global__ __launch_bounds__(64 * waves_of(TILE)) void k_muon_large(const Mats s) {
+__device__ __forceinline__ void large_tile(const Mats &s) {
     typedef Large<TERMS, TILE> L;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2][L::STAGE];
+    __shared__ __attribute__((aligned(16))) _Float16 lds[L::RING][L::STAGE];
     if (s.ctl && !s.ctl[C_GO]) return;
     Job job;
     const Mat &t = s.t[job_of<TILE>(s, blockIdx.x, job)];
@@ -406,60 +543,102 @@ __global__ __launch_bounds__(64 * waves_of(TILE)) void k_muon_large(const Mats s
         for (int j = 0; j < L::NJ; j++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
-    // kilobyte e of a stage: operand, plane, row block, step
-    constexpr int MINE = L::PIECES / L::WAVES;
-    const _Float16 *from[MINE];
+    // kilobyte e of a stage: operand, plane, row block, step. (Buffer loads: behind global loads to LDS the compiler
+    // waits for all LDS reads where it needs the earlier ones alone.)
+    __amdgpu_buffer_rsrc_t from[L::MINE];
 #pragma unroll
-    for (int e = 0; e < MINE; e++) {
+    for (int e = 0; e < L::MINE; e++) {
         const int piece = e * L::WAVES + wave, k = piece % L::QS, rb = piece / L::QS % L::RB, pl = piece / (L::QS * L::RB) % L::PL,
                   side = piece / (L::QS * L::RB * L::PL);
         const Operand &o = side ? job.q : job.p;
         int R = (side ? job.bj : job.bi) * L::RB + rb;
         if (R >= o.rb) R = o.rb - 1;
-        from[e] = o.p + pl * o.plane + ((int64_t)R * o.k16 + k) * 512 + lane * 8;
+        from[e] = __builtin_amdgcn_make_buffer_rsrc((void *)(o.p + pl * o.plane + ((int64_t)R * o.k16 + job.k_lo + k) * 512), 0,
+                                                    (o.k16 - job.k_lo - k) * 1024, 0x00020000);
     }
-    auto fetch = [&](int stage, int buf) {
+    auto fetch = [&](int stage) {
 #pragma unroll
-        for (int e = 0; e < MINE; e++)
-            __builtin_amdgcn_global_load_lds((global_void *)(from[e] + (int64_t)stage * L::QS * 512),
-                                             (lds_void *)(lds[buf] + (e * L::WAVES + wave) * 512), 16, 0, 0);
+        for (int e = 0; e < L::MINE; e++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from[e], (lds_void *)(lds[stage % L::RING] + (e * L::WAVES + wave) * 512), 16,
+                                                     lane * 16, stage * L::QS * 1024, 0, 0);
     };
-    const int stages = job.p.k16 / L::QS;
-    fetch(0, 0);
-    for (int st = 0; st < stages; st++) {
-        __syncthreads();                   // this stage has landed, and no wave still reads the other buffer
-        if (st + 1 < stages) fetch(st + 1, (st + 1) & 1);
-        const _Float16 *a0 = lds[st & 1] + (wi * L::NI * L::QS) * 512 + lane * 8;
-        const _Float16 *b0 = lds[st & 1] + (L::PL * L::RB * L::QS + wj * L::NJ * L::QS) * 512 + lane * 8;
+    // A step's operands are read while the step before is multiplied, also into the next stage: by its barrier every wave has
+    // read all of the stage before, whose buffer is then filled again.
+    half8 a[2][L::PL][L::NI], b[2][L::PL][L::NJ];
+    auto operands = [&](int step, int to) {
+        const _Float16 *at = lds[step / L::QS % L::RING] + step % L::QS * 512 + lane * 8;
+        const _Float16 *a0 = at + wi * L::NI * L::QS * 512, *b0 = at + (L::PL * L::RB + wj * L::NJ) * L::QS * 512;
 #pragma unroll
-        for (int k = 0; k < L::QS; k++) {
-            half8 a[L::PL][L::NI], b[L::PL][L::NJ];
+        for (int pl = 0; pl < L::PL; pl++) {
 #pragma unroll
-            for (int pl = 0; pl < L::PL; pl++) {
+            for (int i = 0; i < L::NI; i++) a[to][pl][i] = *(const half8 *)(a0 + (pl * L::RB + i) * L::QS * 512);
 #pragma unroll
-                for (int i = 0; i < L::NI; i++) a[pl][i] = *(const half8 *)(a0 + ((pl * L::RB + i) * L::QS + k) * 512);
+            for (int j = 0; j < L::NJ; j++) b[to][pl][j] = *(const half8 *)(b0 + (pl * L::RB + j) * L::QS * 512);
+        }
+    };
+    const int steps = job.k_hi - job.k_lo, stages = steps / L::QS;       // steps: a multiple of 4
+    for (int st = 0; st < L::RING && st < stages; st++) fetch(st);
+    if (L::RING - 1 < stages)
+        wait_stage<(L::RING - 1) * L::MINE>();
+    else
+        wait_stage<0>();
+    operands(0, 0);
+    auto multiply = [&](int of) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < L::NJ; j++) b[pl][j] = *(const half8 *)(b0 + ((pl * L::RB + j) * L::QS + k) * 512);
-            }
+        for (int i = 0; i < L::NI; i++)
 #pragma unroll
-            for (int i = 0; i < L::NI; i++)
-#pragma unroll
-                for (int j = 0; j < L::NJ; j++) {
-                    acc[i][j] = mma(a[0][i], b[0][j], acc[i][j]);
-                    if (TERMS == 3) {
-                        acc[i][j] = mma(a[0][i], b[L::PL - 1][j], acc[i][j]);
-                        acc[i][j] = mma(a[L::PL - 1][i], b[0][j], acc[i][j]);
-                    }
+            for (int j = 0; j < L::NJ; j++) {
+                acc[i][j] = mma(a[of][0][i], b[of][0][j], acc[i][j]);
+                if (TERMS == 3) {
+                    acc[i][j] = mma(a[of][0][i], b[of][L::PL - 1][j], acc[i][j]);
+                    acc[i][j] = mma(a[of][L::PL - 1][i], b[of][0][j], acc[i][j]);
                 }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // without conditions as long as there is a stage to fetch, so that the waits are those of one path
+    int g = 0;
+    for (; (g + 4) / L::QS + L::RING - 1 < stages; g += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int next = g + u + 1;
+            if ((u + 1) % L::QS == 0) {
+                wait_stage<(L::RING - 2) * L::MINE>();
+                fetch(next / L::QS + L::RING - 1);
+            }
+            operands(next, (u + 1) & 1);
+            multiply(u & 1);
         }
     }
-    __syncthreads();                       // the buffers become the waves' scratch
+    for (; g < steps; g += 4) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int next = g + u + 1;
+            if ((u + 1) % L::QS == 0 && next < steps) {
+                wait_stage<0>();
+                if (next / L::QS + L::RING - 1 < stages) fetch(next / L::QS + L::RING - 1);
+            }
+            operands(next, (u + 1) & 1);       // behind the last step something that is not used
+            multiply(u & 1);
+        }
+    }
+    wait_stage<0>();                       // the ring becomes the waves' scratch
     _Float16 *scratch = lds[0] + wave * 32 * 40;
 #pragma unroll
     for (int i = 0; i < L::NI; i++)
 #pragma unroll
-        for (int j = 0; j < L::NJ; j++)
-            put_tile<TERMS>(s, t, job, acc[i][j], job.bi * L::RB + wi * L::NI + i, job.bj * L::RB + wj * L::NJ + j, scratch);
+        for (int j = 0; j < L::NJ; j++) {
+            const int I = wi * L::NI + i, J = wj * L::NJ + j;
+            if (t.splits > 1)
+                put_part(s, t, job, acc[i][j], L::RB * L::RB, I * L::RB + J);
+            else
+                put_tile<TERMS>(s, t, job, acc[i][j], job.bi * L::RB + I, job.bj * L::RB + J, scratch);
+        }
+}
+template <int TERMS, int TILE>
+__global__ __launch_bounds__(64 * waves_of(TILE)) void k_muon_large(const Mats s) {
+    large_tile<TERMS, TILE>(s);
 }
 
 // ---- the host's side
@@ -503,8 +682,57 @@ inline int parts_of(const D1MuonTensor &t) {
     const int64_t n = (t.rows * t.cols + 4095) / 4096;
     return (int)(n < 1 ? 1 : n < NORM_PARTS ? n : NORM_PARTS);
 }
-inline int kind_of(int64_t tiles256, int64_t tiles128, int64_t tiles64) {
-    return tiles256 >= 192 ? 3 : tiles128 >= 192 ? 2 : tiles64 >= 192 ? 1 : 0;
+// How a launch shares its products: the kind of tile and how many steps of 64 of the contraction a workgroup takes at most.
+// The estimate, in us: workgroups in rounds over the 256 CUs, a kind's time for 64 of a tile's contraction where it has the CU
+// full (WORK) and alone (ALONE), and for shared tiles the join's launch and bytes at 4 TB/s.
+struct Plan {
+    int kind;
+    int64_t most;             // steps of 64
+};
+constexpr int ON_CU[4] = {4, 2, 2, 1};
+inline int64_t chunks_of(int mode, const Shape &h) { return mode == GRAM ? h.n64 : h.m64; }
+inline int64_t splits_of(int64_t chunks, int64_t most) { return (chunks + most - 1) / most; }
+static double plan_time(const D1MuonTensor *t, const int *at, int count, int mode, int terms, int kind, int64_t most) {
+    static const double WORK[2][4] = {{0.117, 0.38, 0.55, 1.75}, {0.26, 0.87, 1.87, 5.3}}, ALONE[2][4] = {{0.2, 0.35, 0.9, 1.75}, {0.42, 0.8, 2.2, 5.3}};
+    const double c = WORK[terms == 3][kind], l = ALONE[terms == 3][kind];
+    double work = 0, groups = 0, longest = 0, joined = 0;
+    for (int k = 0; k < count; k++) {
+        const Shape h = shape_of(t[at[k]]);
+        const int64_t chunks = chunks_of(mode, h), splits = splits_of(chunks, most), each = (chunks + splits - 1) / splits;
+        const double n = (double)tiles_of(mode, h, side_of(kind)) * splits;
+        work += n * each;
+        groups += n;
+        if (each > longest) longest = (double)each;
+        if (splits > 1) joined += n * side_of(kind) * side_of(kind) * 8;
+    }
+    const double on = ON_CU[kind], rounds = std::ceil(groups / (256 * on));
+    double time = work / groups * c * on * rounds;          // of equal workgroups
+    if (work * c / 256 > time) time = work * c / 256;
+    if (longest * l > time) time = longest * l;
+    return time + (joined ? 7.0 + joined / 4e6 : 0.0);
+}
+static Plan plan_of(const D1MuonTensor *t, const int *at, int count, int mode, int terms) {
+    Plan best{0, 1 << 20};
+    double least = 1e30;
+    for (int kind = 0; kind < 4; kind++)
+        for (int64_t most : {(int64_t)1 << 20, (int64_t)64, (int64_t)32, (int64_t)16, (int64_t)8, (int64_t)4}) {
+            const double time = plan_time(t, at, count, mode, terms, kind, most);
+            if (time < least) {
+                least = time;
+                best = {kind, most};
+            }
+        }
+    return best;
+}
+// bytes of a launch's partial results
+static int64_t plan_bytes(const D1MuonTensor *t, const int *at, int count, int mode, const Plan &p) {
+    int64_t bytes = 0;
+    for (int k = 0; k < count; k++) {
+        const Shape h = shape_of(t[at[k]]);
+        const int64_t splits = splits_of(chunks_of(mode, h), p.most);
+        if (splits > 1) bytes += tiles_of(mode, h, side_of(p.kind)) * splits * side_of(p.kind) * side_of(p.kind) * 4;
+    }
+    return bytes;
 }
 
 // The singular values of X lie in [0, 1] after the norm; the largest that the steps make of them, from a fine grid and the
@@ -538,23 +766,40 @@ static bool muon_args(const D1MuonTensor *t, int count, const D1Muon *h) {
     return true;
 }
 
+// the matrices with elements, in the order of the launches: alike in terms, the longest products first, so that none
+// starts when the others are over
+static int muon_order(const D1MuonTensor *t, int count, const D1Muon *h, int *at) {
+    int live = 0;
+    for (int i = 0; i < count; i++)
+        if (t[i].rows && t[i].cols) at[live++] = i;
+    auto longest = [&](int i) { return terms_of(t[i], h) * (int64_t)1000000 + (t[i].rows > t[i].cols ? t[i].rows : t[i].cols); };
+    std::stable_sort(at, at + live, [&](int x, int y) { return longest(x) > longest(y); });
+    return live;
+}
 struct MuonWork {
-    int64_t parts, sums, scales, mats;    // offsets; the rest is one group's operands
+    int64_t parts, sums, scales, mats, shares, total;    // offsets: sums' counts, sums, factors, a group's operands, partial results
 };
-static int64_t muon_work(const D1MuonTensor *t, int count, const D1Muon *h, MuonWork &w) {
+static MuonWork muon_work(const D1MuonTensor *t, int count, const D1Muon *h, const int *at, int live) {
+    MuonWork w;
     w.parts = 0;
     w.sums = ((int64_t)count * 4 + 255) & ~(int64_t)255;
     w.scales = w.sums + (int64_t)count * NORM_PARTS * 8;
     w.mats = (w.scales + (int64_t)count * 8 + 255) & ~(int64_t)255;
-    int64_t most = 0, bytes = 0;
-    for (int i = 0; i < count; i++) {
-        const int64_t b = t[i].rows && t[i].cols ? mat_bytes(t[i], terms_of(t[i], h)) : 0;
-        most = b > most ? b : most;
-        bytes += b;
+    int64_t most = 0, shares = 0;
+    for (int from = 0, to; from < live; from = to) {
+        to = group_end(t, at, live, from, h);
+        const int terms = terms_of(t[at[from]], h);
+        int64_t bytes = 0;
+        for (int k = from; k < to; k++) bytes += mat_bytes(t[at[k]], terms);
+        most = bytes > most ? bytes : most;
+        for (int mode : {(int)GRAM, (int)POLY, (int)APPLY}) {
+            const int64_t b = plan_bytes(t, at + from, to - from, mode, plan_of(t, at + from, to - from, mode, terms));
+            shares = b > shares ? b : shares;
+        }
     }
-    // a group is at most GROUP_BYTES or one matrix
-    const int64_t room = bytes < GROUP_BYTES ? bytes : GROUP_BYTES > most ? GROUP_BYTES : most;
-    return w.mats + room;
+    w.shares = w.mats + most;
+    w.total = w.shares + shares;
+    return w;
 }
 
 template <int TERMS>
@@ -569,14 +814,22 @@ static void muon_products(const Mats &s, int64_t tiles, int kind, hipStream_t st
     else
         hipLaunchKernelGGL((k_muon_small<TERMS, 1>), grid, dim3(256), 0, stream, s);
 }
+// `blocks`: 32 x 32 blocks of the shared tiles
+template <int TERMS>
+static void muon_join(const Mats &s, int64_t blocks, int kind, hipStream_t stream) {
+    const dim3 grid((unsigned)((blocks + 3) / 4)), block(256);
+    if (kind == 3)
+        hipLaunchKernelGGL((k_muon_join<TERMS, 256>), grid, block, 0, stream, s);
+    else if (kind == 2)
+        hipLaunchKernelGGL((k_muon_join<TERMS, 128>), grid, block, 0, stream, s);
+    else if (kind == 1)
+        hipLaunchKernelGGL((k_muon_join<TERMS, 64>), grid, block, 0, stream, s);
+    else
+        hipLaunchKernelGGL((k_muon_join<TERMS, 32>), grid, block, 0, stream, s);
+}
 
-static int muon_run(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl, char *work, const MuonWork &w, hipStream_t stream) {
-    int *at = new (std::nothrow) int[count + 1];
-    if (!at) return (int)hipErrorOutOfMemory;
-    int live = 0;
-    for (int terms : {3, 1})
-        for (int i = 0; i < count; i++)
-            if (t[i].rows && t[i].cols && terms_of(t[i], h) == terms) at[live++] = i;
+static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *work, const MuonWork &w, const int *at, int live,
+                    hipStream_t stream) {
     double *sums = (double *)(work + w.sums), *scales = (double *)(work + w.scales);
     int32_t *parts = (int32_t *)(work + w.parts);
     auto sources = [&](int from, int to, bool prepare, Sources &s) {
@@ -655,28 +908,41 @@ static int muon_run(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *
             hipLaunchKernelGGL(k_muon_prepare<3>, dim3((unsigned)tiles), dim3(256), 0, stream, s);
         else
             hipLaunchKernelGGL(k_muon_prepare<1>, dim3((unsigned)tiles), dim3(256), 0, stream, s);
+        p.parts = (float *)(work + w.shares);
+        Plan plans[3];
+        for (int mode : {(int)GRAM, (int)POLY, (int)APPLY}) plans[mode] = plan_of(t, at + from, p.count, mode, terms);
         for (int step = 0; step < h->steps; step++) {
             p.turn = step & 1;
             for (int mode : {(int)GRAM, (int)POLY, step + 1 < h->steps ? (int)APPLY : (int)LAST}) {
                 p.mode = mode;
-                int64_t n[4] = {};
-                for (int k = 0; k < p.count; k++)
-                    for (int kind = 0; kind < 4; kind++) n[kind] += tiles_of(mode, shape_of(t[at[from + k]]), side_of(kind));
-                const int kind = kind_of(n[3], n[2], n[1]);
-                int64_t sum = 0;
+                const Plan &plan = plans[mode == LAST ? (int)APPLY : mode];
+                const int side = side_of(plan.kind);
+                int64_t groups = 0, parts = 0, blocks = 0;
                 for (int k = 0; k < p.count; k++) {
-                    sum += tiles_of(mode, shape_of(t[at[from + k]]), side_of(kind));
-                    p.t[k].last_tile = (int32_t)sum;
+                    const Shape sh = shape_of(t[at[from + k]]);
+                    const int64_t chunks = chunks_of(mode, sh), tiles = tiles_of(mode, sh, side);
+                    int64_t splits = splits_of(chunks, plan.most);
+                    splits = splits_of(chunks, (chunks + splits - 1) / splits);       // none without a step
+                    p.t[k].splits = (int32_t)splits;
+                    p.t[k].first_part = (int32_t)parts;
+                    groups += tiles * splits;
+                    if (splits > 1) {
+                        parts += tiles * splits;
+                        blocks += tiles * (side / 32) * (side / 32);
+                    }
+                    p.t[k].last_tile = (int32_t)groups;
                 }
-                if (terms == 3)
-                    muon_products<3>(p, sum, kind, stream);
-                else
-                    muon_products<1>(p, sum, kind, stream);
+                if (terms == 3) {
+                    muon_products<3>(p, groups, plan.kind, stream);
+                    if (blocks) muon_join<3>(p, blocks, plan.kind, stream);
+                } else {
+                    muon_products<1>(p, groups, plan.kind, stream);
+                    if (blocks) muon_join<1>(p, blocks, plan.kind, stream);
+                }
             }
         }
         from = to;
     }
-    delete[] at;
     return (int)hipGetLastError();
 }
 
@@ -687,8 +953,11 @@ using namespace d1o;
 extern "C" {
 int64_t d1_muon_work_bytes(const D1MuonTensor *t, int count, const D1Muon *h) {
     if (!muon_args(t, count, h)) return D1_E_ARG;
-    MuonWork w;
-    return muon_work(t, count, h, w);
+    int *at = new (std::nothrow) int[count + 1];
+    if (!at) return D1_E_ARG;
+    const MuonWork w = muon_work(t, count, h, at, muon_order(t, count, h, at));
+    delete[] at;
+    return w.total;
 }
 
 int d1_muon_check(const D1Muon *h) { return muon_args(nullptr, 0, h) && reach_of(h) < 3.8 ? 0 : D1_E_ARG; }
@@ -696,9 +965,13 @@ int d1_muon_check(const D1Muon *h) { return muon_args(nullptr, 0, h) && reach_of
 int d1_muon_step(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl, void *work, int64_t work_bytes, void *stream) {
     if (!muon_args(t, count, h) || ((uintptr_t)ctl & 3)) return D1_E_ARG;
     if (d1_muon_check(h)) return D1_E_ARG;
-    MuonWork w;
-    const int64_t need = muon_work(t, count, h, w);
-    if (!work || work_bytes < need || ((uintptr_t)work & 255)) return D1_E_ARG;
-    return muon_run(t, count, h, ctl, (char *)work, w, (hipStream_t)stream);
+    int *at = new (std::nothrow) int[count + 1];
+    if (!at) return (int)hipErrorOutOfMemory;
+    const int live = muon_order(t, count, h, at);
+    const MuonWork w = muon_work(t, count, h, at, live);
+    int code = D1_E_ARG;
+    if (work && work_bytes >= w.total && !((uintptr_t)work & 255)) code = muon_run(t, h, ctl, (char *)work, w, at, live, (hipStream_t)stream);
+    delete[] at;
+    return code;
 }
 }
