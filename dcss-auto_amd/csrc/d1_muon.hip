@@ -40,26 +40,27 @@ struct Mat {
     void *out, *copy;                      // rows x cols as the caller has them
     float size, keep;                      // of a step: out = out * keep - size * O, else out = O
     int32_t rows, cols, m64, n64;
-    int32_t last_tile;                     // workgroups of this and all matrices before, for the launch
     int32_t splits, first_part;            // workgroups that share a tile's contraction; the first one's partial result
     uint8_t flip, type, step, pad;
 };
 struct Mats {
+    int32_t last[GROUP];                   // workgroups of this and all matrices before, for the launch; past them the largest number
     Mat t[GROUP];
     const int32_t *ctl;
     float *parts;                          // partial results: per workgroup its 32 x 32 blocks as the lanes hold them
     float ca, cb, cc;
-    int32_t count, turn, mode;             // turn: which xt is current
+    int32_t count, turn;                   // turn: which xt is current
 };
 // and as its elements come and go
 struct Source {
     const void *g;                         // the gradient, or the matrix itself
     float *mom;                            // null: the matrix itself
     _Float16 *x, *xt;
-    int32_t rows, cols, m64, n64, last_tile, parts;
+    int32_t rows, cols, m64, n64, parts;
     uint8_t flip, type, pad[2];
 };
 struct Sources {
+    int32_t last[GROUP];
     Source t[GROUP];
     double *sums;                          // [matrix][NORM_PARTS], of the group's first
     double *scales;
@@ -71,18 +72,18 @@ struct Sources {
 
 static_assert(sizeof(Mats) <= 4096 && sizeof(Sources) <= 4096, "kernel arguments");
 
-template <class T>
-__device__ __forceinline__ int find(const T *t, int count, int i, int &within) {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (i < t[mid].last_tile)
-            hi = mid;
-        else
-            lo = mid + 1;
+// The matrix of workgroup i: all numbers in one load of kernel arguments, which come from memory (0.7 us each time that one
+// load's address waits for another).
+__device__ __forceinline__ int find(const int32_t *last, int i, int &within) {
+    int k = 0, before = 0;
+#pragma unroll
+    for (int j = 0; j < GROUP; j++) {
+        const int n = last[j];
+        k += i >= n;
+        before = i >= n ? n : before;
     }
-    within = i - (lo ? t[lo - 1].last_tile : 0);
-    return lo;
+    within = i - before;
+    return k;
 }
 
 struct Quad {
@@ -106,9 +107,6 @@ __device__ __forceinline__ Quad quad(const void *p, int type, int64_t i, int hav
     }
     return q;
 }
-__device__ __forceinline__ float element(const void *p, int type, int64_t i) {
-    return type == D1_FP32 ? ((const float *)p)[i] : type == D1_BF16 ? (float)((const __bf16 *)p)[i] : (float)((const _Float16 *)p)[i];
-}
 // what is orthogonalised, and the new momentum, from the gradient and the momentum before
 __device__ __forceinline__ Quad update_of(const Source &t, const Sources &s, Quad g, Quad &m) {
     if (!t.mom) return g;
@@ -125,7 +123,7 @@ __device__ __forceinline__ Quad update_of(const Source &t, const Sources &s, Qua
 __global__ __launch_bounds__(256) void k_muon_norm(const Sources s) {
     __shared__ double sh[4];
     int part;
-    const int k = find(s.t, s.count, blockIdx.x, part);
+    const int k = find(s.last, blockIdx.x, part);
     const Source &t = s.t[k];
     const int64_t n = (int64_t)t.rows * t.cols, stride = (int64_t)t.parts * 1024;
     double sum = 0.0;
@@ -189,7 +187,7 @@ __global__ __launch_bounds__(256) void k_muon_prepare(const Sources s) {
     __shared__ __attribute__((aligned(16))) float tile[64][68];
     if (s.ctl && !s.ctl[C_GO]) return;
     int within;
-    const int k = find(s.t, s.count, blockIdx.x, within);
+    const int k = find(s.last, blockIdx.x, within);
     const Source &t = s.t[k];
     const double scale = s.scales[k];
     const int cols64 = t.flip ? t.m64 : t.n64;
@@ -256,18 +254,18 @@ struct Job {
 };
 
 // the launch's tile `i` of TILE x TILE
-template <int TILE>
+template <int MODE, int TILE>
 __device__ __forceinline__ int job_of(const Mats &s, int i, Job &job) {
     int within;
-    const int k = find(s.t, s.count, i, within);
+    const int k = find(s.last, i, within);
     const Mat &t = s.t[k];
     job.part = t.first_part + within;
     const int split = within % t.splits;
     within /= t.splits;
     const int64_t pm = plane_of(t.m64, t.m64), px = plane_of(t.m64, t.n64);
     job.both = false;
-    if (s.mode == GRAM || s.mode == POLY) {
-        job.p = s.mode == GRAM ? Operand{t.x, px, t.m64 * 2, t.n64 * 4} : Operand{t.a, pm, t.m64 * 2, t.m64 * 4};
+    if (MODE == GRAM || MODE == POLY) {
+        job.p = MODE == GRAM ? Operand{t.x, px, t.m64 * 2, t.n64 * 4} : Operand{t.a, pm, t.m64 * 2, t.m64 * 4};
         job.q = job.p;
         int bi = (int)((sqrtf(8.f * within + 1.f) - 1.f) * 0.5f);
         while ((bi + 1) * (bi + 2) / 2 <= within) bi++;
@@ -278,7 +276,7 @@ __device__ __forceinline__ int job_of(const Mats &s, int i, Job &job) {
     } else {
         job.p = {t.b, pm, t.m64 * 2, t.m64 * 4};
         job.q = {t.xt[s.turn], px, t.n64 * 2, t.m64 * 4};
-        if (s.mode == LAST && t.flip) {
+        if (MODE == LAST && t.flip) {
             const Operand o = job.p;
             job.p = job.q;
             job.q = o;
@@ -295,47 +293,83 @@ __device__ __forceinline__ int job_of(const Mats &s, int i, Job &job) {
 
 __device__ __forceinline__ acc_t mma(half8 a, half8 b, acc_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// A 32 x 32 result: lane l of register r holds row 8 (r / 4) + 4 (l / 32) + r % 4 of block I, column l % 32 of block J.
-// `scratch`: the wave's 32 x 40 halves of LDS.
-template <int TERMS>
-__device__ __forceinline__ void put_tile(const Mats &s, const Mat &t, const Job &job, acc_t d, int I, int J, _Float16 *scratch) {
-    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-    if (I >= job.p.rb || J >= job.q.rb) return;              // the whole wave
-    if (s.mode == LAST) {
-        const int c = J * 32 + col;
-        const float scale = 1.f / (SCALE * SCALE);
-        if (c >= t.cols) return;
+// The block of A that POLY's result needs, as the lanes hold the result
+struct Held {
+    half4 hi[4], lo[4];
+};
+__device__ __forceinline__ int64_t natural(int nch, int I, int J) {
+    const int lane = threadIdx.x & 63;
+    return ((((int64_t)J * nch + (I >> 1)) * 4) * 64 + (lane & 31) + 32 * (I & 1)) * 8 + 4 * (lane >> 5);
+}
+template <int MODE, int TERMS>
+__device__ __forceinline__ Held held_of(const Mats &s, const Mat &t, const Job &job, int I, int J) {
+    Held h = {};
+    if (MODE != POLY || I >= job.p.rb || J >= job.q.rb) return h;
+    const int64_t at = natural(t.m64, I, J), plane = plane_of(t.m64, t.m64);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        h.hi[g] = *(const half4 *)(t.a + at + g * 512);
+        if (TERMS == 3) h.lo[g] = *(const half4 *)(t.a + plane + at + g * 512);
+    }
+    return h;
+}
+
+// A result's last form: O itself, or the parameter's step; all of the parameter's loads before the first store
+template <class T>
+__device__ __forceinline__ void put_last(T *out, const Mat &t, acc_t d, int64_t at, int rows) {
+    constexpr float DOWN = 1.f / (SCALE * SCALE);
+    T p[16];
+    if (t.step)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            const int row = I * 32 + d1f::drow(r, h);
-            if (row >= t.rows) continue;
-            const int64_t i = (int64_t)row * t.cols + c;
-            float v = d[r] * scale;
-            if (t.step) v = element(t.out, t.type, i) * t.keep - t.size * v;
-            if (t.type == D1_FP32) ((float *)t.out)[i] = v;
-            else if (t.type == D1_BF16) ((__bf16 *)t.out)[i] = (__bf16)v;
-            else ((_Float16 *)t.out)[i] = (_Float16)v;
-            if (t.copy) ((__bf16 *)t.copy)[i] = (__bf16)v;
+            const int row = d1f::drow(r, 0);
+            p[r] = row < rows ? out[at + (int64_t)row * t.cols] : (T)0.f;
         }
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const int row = d1f::drow(r, 0);
+        const float o = d[r] * DOWN, v = t.step ? (float)p[r] * t.keep - t.size * o : o;
+        if (row < rows) {
+            out[at + (int64_t)row * t.cols] = (T)v;
+            if (t.copy) ((__bf16 *)t.copy)[at + (int64_t)row * t.cols] = (__bf16)v;
+        }
+    }
+}
+
+// A 32 x 32 result: lane l of register r holds row 8 (r / 4) + 4 (l / 32) + r % 4 of block I, column l % 32 of block J.
+// `scratch`: the wave's 32 x 40 halves of LDS.
+template <int MODE, int TERMS>
+__device__ __forceinline__ void put_tile(const Mats &s, const Mat &t, const Job &job, acc_t d, const Held &held, int I, int J,
+                                         _Float16 *scratch) {
+    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+    if (I >= job.p.rb || J >= job.q.rb) return;              // the whole wave
+    if (MODE == LAST) {
+        const int c = J * 32 + col;
+        if (c >= t.cols) return;
+        const int64_t at = (int64_t)(I * 32 + 4 * h) * t.cols + c;
+        const int rows = t.rows - I * 32 - 4 * h;            // of this lane's first row's on
+        if (t.type == D1_FP32)
+            put_last((float *)t.out, t, d, at, rows);
+        else if (t.type == D1_BF16)
+            put_last((__bf16 *)t.out, t, d, at, rows);
+        else
+            put_last((_Float16 *)t.out, t, d, at, rows);
         return;
     }
-    _Float16 *to = s.mode == GRAM ? t.a : s.mode == POLY ? t.b : t.xt[s.turn ^ 1];      // rows J, contraction I
+    _Float16 *to = MODE == GRAM ? t.a : MODE == POLY ? t.b : t.xt[s.turn ^ 1];      // rows J, contraction I
     const int nch = t.m64;
-    const int64_t plane = s.mode == APPLY ? plane_of(t.m64, t.n64) : plane_of(t.m64, t.m64);
-    const int64_t at = ((((int64_t)J * nch + (I >> 1)) * 4) * 64 + col + 32 * (I & 1)) * 8 + 4 * h;
+    const int64_t plane = MODE == APPLY ? plane_of(t.m64, t.n64) : plane_of(t.m64, t.m64);
+    const int64_t at = natural(nch, I, J);
     half4 hi[4], lo[4];
 #pragma unroll
     for (int g = 0; g < 4; g++) {
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = d[4 * g + j] * (1.f / SCALE);
-        if (s.mode == POLY) {
-            const half4 ah = *(const half4 *)(t.a + at + g * 512);
-            half4 al = {0, 0, 0, 0};
-            if (TERMS == 3) al = *(const half4 *)(t.a + plane + at + g * 512);
+        if (MODE == POLY) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float a = TERMS == 3 ? (float)ah[j] + (float)al[j] : (float)ah[j];
+                const float a = TERMS == 3 ? (float)held.hi[g][j] + (float)held.lo[g][j] : (float)held.hi[g][j];
                 v[j] = __builtin_fmaf(s.cc, v[j], s.cb * a);
                 if (I == J && 8 * g + 4 * h + j == col) v[j] += s.ca * SCALE;
             }
@@ -348,10 +382,10 @@ __device__ __forceinline__ void put_tile(const Mats &s, const Mat &t, const Job 
         *(half4 *)(to + at + g * 512) = hi[g];
         if (TERMS == 3) *(half4 *)(to + plane + at + g * 512) = lo[g];
     }
-    if (s.mode != APPLY && !job.both) return;
+    if (MODE != APPLY && !job.both) return;
     // the other order: rows I, contraction J
-    if (s.mode == APPLY) to = t.x;
-    const int nch2 = s.mode == APPLY ? t.n64 : t.m64;
+    if (MODE == APPLY) to = t.x;
+    const int nch2 = MODE == APPLY ? t.n64 : t.m64;
 #pragma unroll
     for (int p = 0; p < (TERMS == 3 ? 2 : 1); p++) {
         __builtin_amdgcn_wave_barrier();
@@ -382,7 +416,7 @@ __device__ __forceinline__ void put_part(const Mats &s, const Mat &, const Job &
     }
 }
 // and the shares joined, in their order: a wave a block
-template <int TERMS, int TILE>
+template <int MODE, int TERMS, int TILE>
 __global__ __launch_bounds__(256) void k_muon_join(const Mats s) {
     constexpr int RB = TILE / 32, BLOCKS = RB * RB;
     __shared__ __attribute__((aligned(16))) _Float16 scratch[4][32 * 40];
@@ -392,14 +426,15 @@ __global__ __launch_bounds__(256) void k_muon_join(const Mats s) {
     // tiles of the matrices whose contraction is shared; the others were finished where they were made
     int k = 0, left = tile;
     for (; k < s.count; k++) {
-        const int tiles = s.t[k].splits > 1 ? (s.t[k].last_tile - (k ? s.t[k - 1].last_tile : 0)) / s.t[k].splits : 0;
+        const int tiles = s.t[k].splits > 1 ? (s.last[k] - (k ? s.last[k - 1] : 0)) / s.t[k].splits : 0;
         if (left < tiles) break;
         left -= tiles;
     }
     if (k == s.count) return;
     const Mat &t = s.t[k];
     Job job;
-    job_of<TILE>(s, (k ? s.t[k - 1].last_tile : 0) + left * t.splits, job);
+    job_of<MODE, TILE>(s, (k ? s.last[k - 1] : 0) + left * t.splits, job);
+    const Held held = held_of<MODE, TERMS>(s, t, job, job.bi * RB + at / RB, job.bj * RB + at % RB);
     acc_t d;
 #pragma unroll
     for (int r = 0; r < 16; r++) d[r] = 0.f;
@@ -412,18 +447,19 @@ __global__ __launch_bounds__(256) void k_muon_join(const Mats s) {
             for (int j = 0; j < 4; j++) d[4 * g + j] += v.v[j];
         }
     }
-    put_tile<TERMS>(s, t, job, d, job.bi * RB + at / RB, job.bj * RB + at % RB, scratch[threadIdx.x >> 6]);
+    put_tile<MODE, TERMS>(s, t, job, d, held, job.bi * RB + at / RB, job.bj * RB + at % RB, scratch[threadIdx.x >> 6]);
 }
 
 // Small results: a workgroup a tile of 32 SIDE, its waves share the contraction and join in LDS; operands straight from
-// the caches into registers, the next ones on their way while some are multiplied.
-template <int TERMS, int SIDE>
+// the caches into registers; other workgroups of the CU multiply while one loads (with the next operands on their way there
+// were half as many: 544 tiles of 32 with a contraction of 256 in two halves 11.3 us, 7.8 without).
+template <int MODE, int TERMS, int SIDE>
 __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
     constexpr int W = 4, PL = TERMS == 3 ? 2 : 1, AT_ONCE = TERMS == 3 && SIDE == 2 ? 2 : 4;
     __shared__ float sums[W][SIDE * SIDE][16][64];
     if (s.ctl && !s.ctl[C_GO]) return;
     Job job;
-    const Mat &t = s.t[job_of<32 * SIDE>(s, blockIdx.x, job)];
+    const Mat &t = s.t[job_of<MODE, 32 * SIDE>(s, blockIdx.x, job)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     acc_t acc[SIDE][SIDE];
 #pragma unroll
@@ -441,42 +477,31 @@ __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
     }
     const int first = job.k_lo / AT_ONCE, batches = job.k_hi / AT_ONCE, per = (batches - first + W - 1) / W;      // multiples of 4
     const int lo = first + wave * per, hi = lo + per < batches ? lo + per : batches;
-    half8 a[2][AT_ONCE][PL][SIDE], b[2][AT_ONCE][PL][SIDE];
-    auto operands = [&](int batch, int to) {
-        const int at = batch * AT_ONCE * 512;
+    Held held = {};
+    if (wave < SIDE * SIDE) held = held_of<MODE, TERMS>(s, t, job, job.bi * SIDE + wave / SIDE, job.bj * SIDE + wave % SIDE);
+    for (int c = lo; c < hi; c++) {
+        half8 a[AT_ONCE][PL][SIDE], b[AT_ONCE][PL][SIDE];
 #pragma unroll
         for (int k = 0; k < AT_ONCE; k++)
 #pragma unroll
             for (int pl = 0; pl < PL; pl++)
 #pragma unroll
                 for (int i = 0; i < SIDE; i++) {
-                    a[to][k][pl][i] = *(const half8 *)(p[i] + pl * job.p.plane + at + k * 512);
-                    b[to][k][pl][i] = *(const half8 *)(q[i] + pl * job.q.plane + at + k * 512);
+                    a[k][pl][i] = *(const half8 *)(p[i] + pl * job.p.plane + (c * AT_ONCE + k) * 512);
+                    b[k][pl][i] = *(const half8 *)(q[i] + pl * job.q.plane + (c * AT_ONCE + k) * 512);
                 }
-    };
-    auto multiply = [&](int of) {
 #pragma unroll
         for (int k = 0; k < AT_ONCE; k++)
 #pragma unroll
             for (int i = 0; i < SIDE; i++)
 #pragma unroll
                 for (int j = 0; j < SIDE; j++) {
-                    acc[i][j] = mma(a[of][k][0][i], b[of][k][0][j], acc[i][j]);
+                    acc[i][j] = mma(a[k][0][i], b[k][0][j], acc[i][j]);
                     if (TERMS == 3) {
-                        acc[i][j] = mma(a[of][k][0][i], b[of][k][PL - 1][j], acc[i][j]);
-                        acc[i][j] = mma(a[of][k][PL - 1][i], b[of][k][0][j], acc[i][j]);
+                        acc[i][j] = mma(a[k][0][i], b[k][PL - 1][j], acc[i][j]);
+                        acc[i][j] = mma(a[k][PL - 1][i], b[k][0][j], acc[i][j]);
                     }
                 }
-    };
-    if (lo < hi) {
-        operands(lo, 0);
-        for (int c = lo; c < hi; c += 2) {
-            if (c + 1 < hi) operands(c + 1, 1);
-            multiply(0);
-            if (c + 1 >= hi) break;
-            if (c + 2 < hi) operands(c + 2, 0);
-            multiply(1);
-        }
     }
 #pragma unroll
     for (int i = 0; i < SIDE; i++)
@@ -499,7 +524,7 @@ __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
     if (t.splits > 1)
         put_part(s, t, job, d, SIDE * SIDE, wave);
     else
-        put_tile<TERMS>(s, t, job, d, job.bi * SIDE + wave / SIDE, job.bj * SIDE + wave % SIDE, (_Float16 *)sums[wave]);
+        put_tile<MODE, TERMS>(s, t, job, d, held, job.bi * SIDE + wave / SIDE, job.bj * SIDE + wave % SIDE, (_Float16 *)sums[wave]);
 }
 
 // Large results: a workgroup a tile of TILE x TILE, operands through a ring of LDS buffers that memory fills directly:
@@ -527,13 +552,13 @@ __device__ __forceinline__ void wait_stage() {
 }
 
 // (apart from the kernel, whose host side does not know buffer descriptors)
-template <int TERMS, int TILE>
+template <int MODE, int TERMS, int TILE>
 __device__ __forceinline__ void large_tile(const Mats &s) {
     typedef Large<TERMS, TILE> L;
     __shared__ __attribute__((aligned(16))) _Float16 lds[L::RING][L::STAGE];
     if (s.ctl && !s.ctl[C_GO]) return;
     Job job;
-    const Mat &t = s.t[job_of<TILE>(s, blockIdx.x, job)];
+    const Mat &t = s.t[job_of<MODE, TILE>(s, blockIdx.x, job)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wi = wave / L::ACROSS, wj = wave % L::ACROSS;
     acc_t acc[L::NI][L::NJ];
@@ -633,12 +658,13 @@ __device__ __forceinline__ void large_tile(const Mats &s) {
             if (t.splits > 1)
                 put_part(s, t, job, acc[i][j], L::RB * L::RB, I * L::RB + J);
             else
-                put_tile<TERMS>(s, t, job, acc[i][j], job.bi * L::RB + I, job.bj * L::RB + J, scratch);
+                put_tile<MODE, TERMS>(s, t, job, acc[i][j], held_of<MODE, TERMS>(s, t, job, job.bi * L::RB + I, job.bj * L::RB + J), job.bi * L::RB + I,
+                                job.bj * L::RB + J, scratch);
         }
 }
-template <int TERMS, int TILE>
+template <int MODE, int TERMS, int TILE>
 __global__ __launch_bounds__(64 * waves_of(TILE)) void k_muon_large(const Mats s) {
-    large_tile<TERMS, TILE>(s);
+    large_tile<MODE, TERMS, TILE>(s);
 }
 
 // ---- the host's side
@@ -683,40 +709,54 @@ inline int parts_of(const D1MuonTensor &t) {
     return (int)(n < 1 ? 1 : n < NORM_PARTS ? n : NORM_PARTS);
 }
 // How a launch shares its products: the kind of tile and how many steps of 64 of the contraction a workgroup takes at most.
-// The estimate, in us: workgroups in rounds over the 256 CUs, a kind's time for 64 of a tile's contraction where it has the CU
-// full (WORK) and alone (ALONE), and for shared tiles the join's launch and bytes at 4 TB/s.
+// The estimate, in us: a kind's time for 64 of a tile's contraction where it has its CU full (WORK; the largest tiles, one
+// to a CU, in rounds) and alone (ALONE), and for shared tiles the join's launch and bytes at 4 TB/s.
 struct Plan {
     int kind;
     int64_t most;             // steps of 64
 };
-constexpr int ON_CU[4] = {4, 2, 2, 1};
 inline int64_t chunks_of(int mode, const Shape &h) { return mode == GRAM ? h.n64 : h.m64; }
 inline int64_t splits_of(int64_t chunks, int64_t most) { return (chunks + most - 1) / most; }
-static double plan_time(const D1MuonTensor *t, const int *at, int count, int mode, int terms, int kind, int64_t most) {
-    static const double WORK[2][4] = {{0.117, 0.38, 0.55, 1.75}, {0.26, 0.87, 1.87, 5.3}}, ALONE[2][4] = {{0.2, 0.35, 0.9, 1.75}, {0.42, 0.8, 2.2, 5.3}};
+struct Alike {
+    Shape h;
+    int n;
+};
+static double plan_time(const Alike *shapes, int count, int mode, int terms, int kind, int64_t most) {
+    static const double WORK[2][4] = {{0.117, 0.38, 0.68, 1.75}, {0.26, 0.87, 1.95, 5.3}}, ALONE[2][4] = {{0.15, 0.3, 0.9, 1.75}, {0.32, 0.6, 2.2, 5.3}};
     const double c = WORK[terms == 3][kind], l = ALONE[terms == 3][kind];
     double work = 0, groups = 0, longest = 0, joined = 0;
     for (int k = 0; k < count; k++) {
-        const Shape h = shape_of(t[at[k]]);
+        const Shape &h = shapes[k].h;
         const int64_t chunks = chunks_of(mode, h), splits = splits_of(chunks, most), each = (chunks + splits - 1) / splits;
-        const double n = (double)tiles_of(mode, h, side_of(kind)) * splits;
+        const double n = (double)tiles_of(mode, h, side_of(kind)) * splits * shapes[k].n;
         work += n * each;
         groups += n;
         if (each > longest) longest = (double)each;
         if (splits > 1) joined += n * side_of(kind) * side_of(kind) * 8;
     }
-    const double on = ON_CU[kind], rounds = std::ceil(groups / (256 * on));
-    double time = work / groups * c * on * rounds;          // of equal workgroups
-    if (work * c / 256 > time) time = work * c / 256;
+    double time = work * c / 256;
+    if (kind == 3 && work / groups * c * std::ceil(groups / 256) > time) time = work / groups * c * std::ceil(groups / 256);
     if (longest * l > time) time = longest * l;
-    return time + (joined ? 7.0 + joined / 4e6 : 0.0);
+    return time + (joined ? 9.0 + joined / 4e6 : 0.0);
 }
 static Plan plan_of(const D1MuonTensor *t, const int *at, int count, int mode, int terms) {
+    Alike shapes[GROUP];
+    int alike = 0;
+    int64_t longest = 0;
+    for (int k = 0; k < count; k++) {
+        const Shape h = shape_of(t[at[k]]);
+        if (chunks_of(mode, h) > longest) longest = chunks_of(mode, h);
+        int i = 0;
+        while (i < alike && (shapes[i].h.m64 != h.m64 || shapes[i].h.n64 != h.n64)) i++;
+        if (i == alike) shapes[alike++] = {h, 0};
+        shapes[i].n++;
+    }
     Plan best{0, 1 << 20};
     double least = 1e30;
     for (int kind = 0; kind < 4; kind++)
         for (int64_t most : {(int64_t)1 << 20, (int64_t)64, (int64_t)32, (int64_t)16, (int64_t)8, (int64_t)4}) {
-            const double time = plan_time(t, at, count, mode, terms, kind, most);
+            if (most < (1 << 20) && (most >= longest || mode == APPLY)) continue;
+            const double time = plan_time(shapes, alike, mode, terms, kind, most);
             if (time < least) {
                 least = time;
                 best = {kind, most};
@@ -802,30 +842,40 @@ static MuonWork muon_work(const D1MuonTensor *t, int count, const D1Muon *h, con
     return w;
 }
 
-template <int TERMS>
-static void muon_products(const Mats &s, int64_t tiles, int kind, hipStream_t stream) {
-    const dim3 grid((unsigned)tiles);
+// `groups` workgroups; `blocks`: 32 x 32 blocks of tiles whose contraction is shared (of A and B alone)
+template <int MODE, int TERMS>
+static void muon_products(const Mats &s, int kind, int64_t groups, int64_t blocks, hipStream_t stream) {
+    const dim3 grid((unsigned)groups), block(256), joins((unsigned)((blocks + 3) / 4));
     if (kind == 3)
-        hipLaunchKernelGGL((k_muon_large<TERMS, 256>), grid, dim3(512), 0, stream, s);
+        hipLaunchKernelGGL((k_muon_large<MODE, TERMS, 256>), grid, dim3(512), 0, stream, s);
     else if (kind == 2)
-        hipLaunchKernelGGL((k_muon_large<TERMS, 128>), grid, dim3(256), 0, stream, s);
+        hipLaunchKernelGGL((k_muon_large<MODE, TERMS, 128>), grid, block, 0, stream, s);
     else if (kind == 1)
-        hipLaunchKernelGGL((k_muon_small<TERMS, 2>), grid, dim3(256), 0, stream, s);
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 2>), grid, block, 0, stream, s);
     else
-        hipLaunchKernelGGL((k_muon_small<TERMS, 1>), grid, dim3(256), 0, stream, s);
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 1>), grid, block, 0, stream, s);
+    if constexpr (MODE == GRAM || MODE == POLY) {
+        if (!blocks) return;
+        if (kind == 3)
+            hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 256>), joins, block, 0, stream, s);
+        else if (kind == 2)
+            hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 128>), joins, block, 0, stream, s);
+        else if (kind == 1)
+            hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 64>), joins, block, 0, stream, s);
+        else
+            hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 32>), joins, block, 0, stream, s);
+    }
 }
-// `blocks`: 32 x 32 blocks of the shared tiles
 template <int TERMS>
-static void muon_join(const Mats &s, int64_t blocks, int kind, hipStream_t stream) {
-    const dim3 grid((unsigned)((blocks + 3) / 4)), block(256);
-    if (kind == 3)
-        hipLaunchKernelGGL((k_muon_join<TERMS, 256>), grid, block, 0, stream, s);
-    else if (kind == 2)
-        hipLaunchKernelGGL((k_muon_join<TERMS, 128>), grid, block, 0, stream, s);
-    else if (kind == 1)
-        hipLaunchKernelGGL((k_muon_join<TERMS, 64>), grid, block, 0, stream, s);
+static void muon_products(int mode, const Mats &s, int kind, int64_t groups, int64_t blocks, hipStream_t stream) {
+    if (mode == GRAM)
+        muon_products<GRAM, TERMS>(s, kind, groups, blocks, stream);
+    else if (mode == POLY)
+        muon_products<POLY, TERMS>(s, kind, groups, blocks, stream);
+    else if (mode == APPLY)
+        muon_products<APPLY, TERMS>(s, kind, groups, blocks, stream);
     else
-        hipLaunchKernelGGL((k_muon_join<TERMS, 32>), grid, block, 0, stream, s);
+        muon_products<LAST, TERMS>(s, kind, groups, blocks, stream);
 }
 
 static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *work, const MuonWork &w, const int *at, int live,
@@ -834,6 +884,7 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
     int32_t *parts = (int32_t *)(work + w.parts);
     auto sources = [&](int from, int to, bool prepare, Sources &s) {
         s = Sources{};
+        for (int32_t &n : s.last) n = INT32_MAX;
         s.sums = sums + (int64_t)from * NORM_PARTS;
         s.scales = scales + from;
         s.parts = parts + from;
@@ -855,7 +906,7 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
             o.type = a.gtype;
             o.parts = parts_of(a);
             tiles += prepare ? (int64_t)sh.m64 * sh.n64 : o.parts;
-            o.last_tile = (int32_t)tiles;
+            s.last[s.count - 1] = (int32_t)tiles;
         }
         return tiles;
     };
@@ -872,6 +923,7 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
         Sources s;
         const int64_t tiles = sources(from, to, true, s);
         Mats p{};
+        for (int32_t &n : p.last) n = INT32_MAX;
         p.ctl = ctl;
         p.ca = (float)h->a;
         p.cb = (float)h->b;
@@ -914,7 +966,6 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
         for (int step = 0; step < h->steps; step++) {
             p.turn = step & 1;
             for (int mode : {(int)GRAM, (int)POLY, step + 1 < h->steps ? (int)APPLY : (int)LAST}) {
-                p.mode = mode;
                 const Plan &plan = plans[mode == LAST ? (int)APPLY : mode];
                 const int side = side_of(plan.kind);
                 int64_t groups = 0, parts = 0, blocks = 0;
@@ -930,15 +981,12 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
                         parts += tiles * splits;
                         blocks += tiles * (side / 32) * (side / 32);
                     }
-                    p.t[k].last_tile = (int32_t)groups;
+                    p.last[k] = (int32_t)groups;
                 }
-                if (terms == 3) {
-                    muon_products<3>(p, groups, plan.kind, stream);
-                    if (blocks) muon_join<3>(p, blocks, plan.kind, stream);
-                } else {
-                    muon_products<1>(p, groups, plan.kind, stream);
-                    if (blocks) muon_join<1>(p, blocks, plan.kind, stream);
-                }
+                if (terms == 3)
+                    muon_products<3>(mode, p, plan.kind, groups, blocks, stream);
+                else
+                    muon_products<1>(mode, p, plan.kind, groups, blocks, stream);
             }
         }
         from = to;
