@@ -253,3 +253,126 @@ def muon_step(params, grads, momenta, step, lr=0.02, momentum=0.95, nesterov=Tru
     scales = [muon_scale(p.shape) for p in params] if scales is None else scales
     call('muon_step', step, params, grads, momenta, step, _each(lr, count), scales, _each(weight_decay, count), copies,
          momentum, nesterov, a, b, c, eps, steps, _terms(product_bits))
+
+
+class Muon(torch.optim.Optimizer):
+    """Steps along orthogonalised momenta for matrices, in a few launches for all of them.
+
+    params: of two dimensions or more (those behind the first count as one), fp32 or bf16. lr and weight_decay may differ
+    between groups; the rest is the optimizer's, as in muon_step. rms: scale steps to the size of AdamW's (lr is then
+    one for AdamW). copies: {parameter: bf16 tensor} that a step writes beside fp32 parameters. A parameter without a
+    gradient is left as it is. A step with a matrix whose update has no finite norm changes nothing;
+    skipped_steps() counts those. A step can be captured in a graph after one with the same parameters taking part."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ,
+                 eps=1e-7, rms=False, product_bits=None, copies=None):
+        if not (lr >= 0 and weight_decay >= 0):
+            raise ValueError('lr and weight_decay must not be negative')
+        if not 0 <= momentum < 1:
+            raise ValueError('momentum must be in [0, 1)')
+        _terms(product_bits)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+        self.settings = dict(momentum=momentum, nesterov=nesterov, steps=steps, coefficients=tuple(coefficients), eps=eps,
+                             product_bits=product_bits)
+        self.rms, self.copies = rms, copies or {}
+        self.ctl = None                 # the device's counts (muon_step's `step`)
+
+    def add_param_group(self, param_group):
+        names = set(param_group) - {'params', 'lr', 'weight_decay', 'param_names'}
+        if names:
+            raise ValueError(f'a group has lr and weight_decay of its own, not {", ".join(sorted(names))}')
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]['params']:
+            if p.dim() < 2:
+                raise ValueError(f'a parameter must have two dimensions or more, not {list(p.shape)}')
+
+    def __getstate__(self):
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in ('settings', 'rms', 'copies', 'ctl')}}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, lr, decay = [], [], []
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                if not self.state[p]:
+                    AdamW._not_captured()
+                    self.state[p]['momentum'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                params.append(p)
+                lr.append(group['lr'])
+                decay.append(group['weight_decay'])
+        if not params:
+            return loss
+        if self.ctl is None:
+            self.ctl = torch.zeros(8, dtype=torch.int32, device=params[0].device)
+        muon_step(params, [p.grad for p in params], [self.state[p]['momentum'] for p in params], self.ctl, lr=lr, weight_decay=decay,
+                  scales=[muon_scale(p.shape, self.rms) for p in params],
+                  copies=[self.copies.get(p) for p in params] if self.copies else None, **self.settings)
+        return loss
+
+    def skipped_steps(self):
+        """Steps left out because an update's norm was not finite (waits for the device)."""
+        return 0 if self.ctl is None else int(self.ctl[1].item())
+
+    def state_dict(self):
+        d = super().state_dict()
+        d['d1'] = dict(muon=True, ctl=None if self.ctl is None else self.ctl.clone())
+        return d
+
+    def load_state_dict(self, state_dict):
+        own = state_dict.get('d1')
+        if own is None or not own.get('muon'):
+            raise ValueError("not a state of Muon: another optimizer's is kept otherwise")
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != 'd1'})
+        # the base class casts tensors to the parameters' type: momenta stay as they were saved
+        ids = [i for group in state_dict['param_groups'] for i in group['params']]
+        for i, p in zip(ids, (p for group in self.param_groups for p in group['params'])):
+            if i in state_dict['state']:
+                self.state[p]['momentum'] = state_dict['state'][i]['momentum'].to(p.device, copy=True).contiguous()
+        device = self.param_groups[0]['params'][0].device
+        self.ctl = None if own['ctl'] is None else own['ctl'].to(device, copy=True)
+
+
+class MuonAdamW:
+    """Muon for the matrices of a model's trunk and AdamW for the rest, stepped together. `named`: the model's
+    named_parameters(); those of two dimensions or more are Muon's, but for heads and embeddings (a name with 'head' or
+    'embed'). muon, adamw: further arguments of each. Each skips a step by the norms of its own gradients."""
+
+    def __init__(self, named, muon=None, adamw=None):
+        named = list(named)
+        trunk = [p for n, p in named if p.dim() >= 2 and 'head' not in n and 'embed' not in n]
+        ids = {id(p) for p in trunk}
+        rest = [p for _, p in named if id(p) not in ids]
+        self.muon = Muon(trunk, **(muon or {})) if trunk else None
+        self.adamw = AdamW(rest, **(adamw or {})) if rest else None
+        self.both = [o for o in (self.muon, self.adamw) if o is not None]
+
+    @property
+    def param_groups(self):
+        return [g for o in self.both for g in o.param_groups]
+
+    def zero_grad(self, set_to_none=True):
+        for o in self.both:
+            o.zero_grad(set_to_none=set_to_none)
+
+    def step(self):
+        for o in self.both:
+            o.step()
+
+    def skipped_steps(self):
+        return sum(o.skipped_steps() for o in self.both)
+
+    def state_dict(self):
+        return dict(muon=self.muon and self.muon.state_dict(), adamw=self.adamw and self.adamw.state_dict())
+
+    def load_state_dict(self, state_dict):
+        for o, d in ((self.muon, state_dict['muon']), (self.adamw, state_dict['adamw'])):
+            if (o is None) != (d is None):
+                raise ValueError('the state is of another split of parameters')
+            if o is not None:
+                o.load_state_dict(d)

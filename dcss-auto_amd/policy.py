@@ -13,6 +13,7 @@ from torch import nn
 
 from . import _lib
 from .norm import LayerNorm
+from .recurrence import gated_scan
 from .tokens import token_logprobs
 
 OBS = 1800
@@ -103,6 +104,55 @@ class NormPolicy(nn.Module):
         logits, value = self(obs_u8)
         action, logp = sample(logits, seed, t)
         return action, action, logp, value
+
+
+class MemoryPolicy(nn.Module):
+    """Policy with a memory across steps: a gated linear recurrence (recurrence.gated_scan) between its trunk and its head,
+    which keeps what the view no longer shows. It trains with SequencePPO (ppo.py) over whole rollouts. The state is
+    fp32 [worlds, width]; where `reset` is set an episode begins and what was before is dropped."""
+
+    def __init__(self, width=256, n_actions=N_ACTIONS, obs=OBS, seed=0):
+        super().__init__()
+        self.width, self.n_actions = width, n_actions
+        self.l1, self.n1 = nn.Linear(obs, width), LayerNorm(width)
+        self.cell = nn.Linear(width, 2 * width)       # what is taken in | its gate
+        self.n2 = LayerNorm(width)
+        self.head = nn.Linear(width, n_actions + 1)   # logits | value
+        g = torch.Generator().manual_seed(seed)
+        with torch.no_grad():
+            for layer in (self.l1, self.cell, self.head):
+                layer.weight.copy_(torch.randn(layer.weight.shape, generator=g) * 0.02)
+                layer.bias.zero_()
+            # channels that remember from a few steps to some hundred
+            self.cell.bias[width:].copy_(-torch.linspace(0.0, 5.0, width))
+
+    def initial_state(self, n):
+        return torch.zeros(n, self.width, dtype=torch.float32, device=self.l1.weight.device)
+
+    def forward(self, obs_u8, state=None, reset=None):
+        """obs uint8 [T, n, 15, 15, 8] (or [T, n, 1800]), reset bool or uint8 [T, n] -> (fp32 logits [T, n, A], fp32 value [T, n],
+        the state after the last step)."""
+        dtype = self.l1.weight.dtype
+        if obs_u8.is_cuda and torch.is_autocast_enabled('cuda'):
+            dtype = torch.get_autocast_dtype('cuda')
+        steps, n = obs_u8.shape[:2]
+        h = torch.relu(self.n1(self.l1(widen(obs_u8.reshape(steps * n, -1), dtype))))
+        x, gate = self.cell(h).view(steps, n, 2 * self.width).split(self.width, dim=-1)
+        m, last = gated_scan(x, gate, state, reset)
+        out = self.head(self.n2(m + h.view(steps, n, self.width))).float()
+        return out[..., :self.n_actions], out[..., self.n_actions], last
+
+    def evaluate_sequence(self, obs_u8, actions, state, resets, mask=None):
+        """(log probability, entropy, value), fp32 [T, n], of the actions [T, n] that were taken from `state` on."""
+        logits, value, _ = self(obs_u8, state, resets)
+        r = token_logprobs(logits, actions, mask=mask)
+        return r.logp, r.entropy, value
+
+    def act(self, obs_u8, seed, t, state, reset=None):
+        """Counter-RNG sample at step t -> (action number, env action, log probability, value, the next state)."""
+        logits, value, state = self(obs_u8[None], state, None if reset is None else reset[None])
+        action, logp = sample(logits[0], seed, t)
+        return action, action, logp, value[0], state
 
 
 def pack_weights(w1, w2, w3, out=None):

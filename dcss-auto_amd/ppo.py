@@ -11,7 +11,8 @@ autocast while the optimizer keeps fp32 master weights; GAE is the HIP kernel.
 import torch
 
 from . import policy as P
-from .optim import AdamW
+from .losses import policy_loss
+from .optim import AdamW, MuonAdamW
 
 OBS = P.OBS
 
@@ -85,40 +86,111 @@ class PPO:
 
 class ModulePPO(PPO):
     """PPO for any policy module with evaluate(obs, actions) -> (log probability, entropy, value), such as
-    NormPolicy and ARPolicy: the module's layers by autograd, its log probabilities, layer norms and the
+    NormPolicy and ARPolicy: the module's layers by autograd, its log probabilities, layer norms, the loss and the
     update itself by this package's kernels. Interface and loss are PPO's; the optimizer is AdamW over all
-    tensors at once (state_bits: 32 or 8) with the gradient clip in the same call. Nothing waits
+    tensors at once (state_bits: 32 or 8) with the gradient clip in the same call, or with optimizer='muon' Muon (lr muon_lr) for
+    the trunk's matrices and AdamW for the rest (MuonAdamW). clip may be a pair (low, high), value_clip holds the new value
+    within that much of the old one; with `reference`, a policy that is left as it is, kl_coef times the KL to
+    it is added to the loss. `terms`: the last minibatch's loss in its parts (losses.PolicyLoss). Nothing waits
     for the device between minibatches: a minibatch whose gradient norm is not finite changes nothing,
     and `update` raises at its end."""
 
     def __init__(self, model, lr=3e-4, eps=1e-5, clip=0.2, vcoef=0.5, ecoef=0.01, max_grad_norm=0.5, epochs=4,
-                 minibatch=8192, gamma=0.99, lam=0.95, autocast=True, weight_decay=0.0, state_bits=32, seed=0):
+                 minibatch=8192, gamma=0.99, lam=0.95, autocast=True, weight_decay=0.0, state_bits=32, seed=0, value_clip=None,
+                 kl_coef=0.0, reference=None, optimizer='adamw', muon_lr=0.02):
         if not max_grad_norm > 0:
             raise ValueError('ModulePPO needs a gradient clip: its norm is what tells a non-finite loss')
+        if optimizer not in ('adamw', 'muon'):
+            raise ValueError(f"optimizer is 'adamw' or 'muon', not {optimizer!r}")
+        if kl_coef and reference is None:
+            raise ValueError('kl_coef needs a reference')
         self._adamw = dict(weight_decay=weight_decay, state_bits=state_bits, max_grad_norm=max_grad_norm, seed=seed)
+        self._muon = dict(lr=muon_lr, weight_decay=weight_decay) if optimizer == 'muon' else None
+        self.value_clip, self.kl_coef, self.reference, self.terms = value_clip, kl_coef, reference, None
         super().__init__(model, lr=lr, eps=eps, clip=clip, vcoef=vcoef, ecoef=ecoef, max_grad_norm=max_grad_norm,
                          epochs=epochs, minibatch=minibatch, gamma=gamma, lam=lam, autocast=autocast)
 
     def _optimizer(self, lr, eps):
-        return AdamW(self.model.parameters(), lr=lr, eps=eps, **self._adamw)
+        adamw = dict(lr=lr, eps=eps, **self._adamw)
+        if self._muon is None:
+            return AdamW(self.model.parameters(), **adamw)
+        return MuonAdamW(self.model.named_parameters(), muon=self._muon, adamw=adamw)
 
-    def minibatch_step(self, obs, actions, old_logp, adv, ret):
+    def _evaluate(self, evaluate, *args):
         with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
-            logp, entropy, value = self.model.evaluate(obs, actions)
-        ratio = torch.exp(logp - old_logp)
-        pg = -torch.minimum(ratio * adv, ratio.clamp(1 - self.clip, 1 + self.clip) * adv).mean()
-        vloss = 0.5 * (value.float() - ret).square().mean()
-        loss = pg + self.vcoef * vloss - self.ecoef * entropy.mean()
+            return evaluate(*args)
+
+    def _learn(self, evaluated, ref_logp, old_logp, adv, ret, old_values):
+        logp, entropy, value = evaluated
+        r = policy_loss(logp, old_logp, adv, ref_logp=ref_logp, entropy=entropy, values=value, returns=ret, old_values=old_values,
+                        clip=self.clip, kl_coef=self.kl_coef, value_coef=self.vcoef, value_clip=self.value_clip, entropy_coef=self.ecoef)
         self.opt.zero_grad(set_to_none=True)
-        loss.backward()
+        r.loss.backward()
         self.opt.step()
-        return loss.detach()
+        self.terms = r._replace(loss=r.loss.detach())
+        return self.terms.loss
+
+    def minibatch_step(self, obs, actions, old_logp, adv, ret, old_values=None):
+        evaluated = self._evaluate(self.model.evaluate, obs, actions)
+        ref_logp = None
+        if self.kl_coef:
+            with torch.no_grad():
+                ref_logp = self._evaluate(self.reference.evaluate, obs, actions)[0]
+        return self._learn(evaluated, ref_logp, old_logp, adv, ret, old_values)
+
+    def _epochs(self, buf, generator):
+        if self.value_clip is None:
+            return super().update(buf, generator)
+        adv, ret = self.advantages(buf)
+        n = buf.T * buf.N
+        obs, last = buf.obs.view(n, -1), None
+        flat = buf.actions.flatten(), buf.logp.flatten(), adv, ret, buf.values.flatten()
+        for _ in range(self.epochs):
+            perm = torch.randperm(n, device=obs.device, generator=generator)
+            for inds in perm.split(self.minibatch):
+                last = self.minibatch_step(obs.index_select(0, inds), *(t[inds] for t in flat))
+        return last
 
     def update(self, buf, generator=None):
         before = self.opt.skipped_steps()
-        last = super().update(buf, generator)
+        last = self._epochs(buf, generator)
         if self.opt.skipped_steps() > before:
             raise RuntimeError('Non-finite PPO loss')
+        return last
+
+
+class SequenceBuffer(RolloutBuffer):
+    """A rollout of a policy with memory: also its state before the first step and where episodes began."""
+
+    def __init__(self, T, N, width, device='cuda', obs_bytes=OBS):
+        super().__init__(T, N, device, obs_bytes)
+        self.state = torch.zeros((N, width), dtype=torch.float32, device=device)
+        self.resets = torch.zeros((T, N), dtype=torch.uint8, device=device)
+
+
+class SequencePPO(ModulePPO):
+    """ModulePPO for a policy with memory (MemoryPolicy), over a SequenceBuffer: a minibatch is the whole rollout of some worlds,
+    minibatch // T of them (one at least), whose states are made again from the one before the rollout through
+    evaluate_sequence(obs, actions, state, resets). A reference's memory begins empty with each rollout."""
+
+    def sequence_step(self, obs, actions, old_logp, adv, ret, state, resets, old_values=None):
+        """One minibatch of sequences: obs [T, n, ...], the others [T, n], state [n, width]."""
+        evaluated = self._evaluate(self.model.evaluate_sequence, obs, actions, state, resets)
+        ref_logp = None
+        if self.kl_coef:
+            with torch.no_grad():
+                ref_logp = self._evaluate(self.reference.evaluate_sequence, obs, actions, torch.zeros_like(state), resets)[0]
+        return self._learn(evaluated, ref_logp, old_logp, adv, ret, old_values)
+
+    def _epochs(self, buf, generator):
+        adv, ret = (x.view(buf.T, buf.N) for x in self.advantages(buf))
+        per, last = max(1, self.minibatch // buf.T), None
+        for _ in range(self.epochs):
+            perm = torch.randperm(buf.N, device=buf.obs.device, generator=generator)
+            for w in perm.split(per):
+                pick = lambda x: x.index_select(1, w)  # noqa: E731
+                last = self.sequence_step(pick(buf.obs), pick(buf.actions), pick(buf.logp), pick(adv), pick(ret), buf.state[w],
+                                          pick(buf.resets), pick(buf.values) if self.value_clip is not None else None)
         return last
 
 

@@ -252,32 +252,54 @@ class Trainer:
 
 class ModuleTrainer:
     """Rollouts and updates of any policy module with act(obs, seed, t) and evaluate(obs, actions)
-    (NormPolicy, ARPolicy): the module's forward and the sampling kernels for each of T decisions,
-    then ModulePPO over the buffer. Further arguments are ModulePPO's."""
+    (NormPolicy, ARPolicy), or with a memory (initial_state, evaluate_sequence: MemoryPolicy): the module's forward and the
+    sampling kernels for each of T decisions, then ModulePPO (SequencePPO) over the buffer. Further arguments are ModulePPO's."""
 
     def __init__(self, env, model, horizon=128, minibatch=8192, sample_seed=7, **ppo):
         if env.batch * horizon < minibatch:
             raise ValueError('a rollout must hold at least one minibatch')
         self.env, self.model, self.T, self.N = env, model, horizon, env.batch
-        self.ppo = ppo_mod.ModulePPO(model, minibatch=minibatch, **ppo)
-        self.buf = ppo_mod.RolloutBuffer(horizon, self.N, device=env.device)
         self.seed, self.t = sample_seed, 0
         self.next_obs = env.obs.reshape(self.N, -1).clone()
         self.gen = torch.Generator(device=env.device).manual_seed(sample_seed)
+        self.state = None
+        if hasattr(model, 'initial_state'):
+            self.state = model.initial_state(self.N)
+            self.reset = torch.zeros(self.N, dtype=torch.uint8, device=env.device)   # worlds whose episode begins
+            self.ppo = ppo_mod.SequencePPO(model, minibatch=minibatch, **ppo)
+            self.buf = ppo_mod.SequenceBuffer(horizon, self.N, self.state.shape[1], device=env.device)
+        else:
+            self.ppo = ppo_mod.ModulePPO(model, minibatch=minibatch, **ppo)
+            self.buf = ppo_mod.RolloutBuffer(horizon, self.N, device=env.device)
+
+    def _act(self, obs, t):
+        """(action number, env action, log probability, value); a memory goes on by a step."""
+        if self.state is None:
+            return self.model.act(obs, self.seed, t)
+        *out, self.state = self.model.act(obs, self.seed, t, self.state, self.reset)
+        return out
 
     @torch.no_grad()
     def rollout(self):
         """Fill the buffer with T decisions per world."""
         buf = self.buf
+        if self.state is not None:
+            buf.state.copy_(self.state)
         with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.ppo.autocast):
             for k in range(self.T):
                 buf.obs[k].copy_(self.next_obs)
-                number, action, logp, value = self.model.act(buf.obs[k], self.seed, self.t + k)
+                if self.state is not None:
+                    buf.resets[k].copy_(self.reset)
+                number, action, logp, value = self._act(buf.obs[k], self.t + k)
                 buf.actions[k].copy_(number)
                 buf.logp[k].copy_(logp)
                 buf.values[k].copy_(value)
                 self.env.step_into(action, self.next_obs, buf.rewards[k], buf.dones[k])
-            buf.bootstrap.copy_(self.model.act(self.next_obs, self.seed, self.t + self.T)[3])
+                if self.state is not None:
+                    self.reset.copy_(buf.dones[k])
+            state = self.state
+            buf.bootstrap.copy_(self._act(self.next_obs, self.t + self.T)[3])
+            self.state = state                       # the next rollout takes this step
         self.t += self.T
         return buf
 
