@@ -18,7 +18,7 @@ namespace d1o {
 enum { LOGP, OLD, ADV, REF, ENT, VAL, RET, OLDV, INPUTS };
 enum { ABSENT, FLAT, PER_ROW, STRIDED };
 enum { S_POLICY, S_VALUE, S_ENTROPY, S_KL, S_CLIPPED, S_DRIFT, SUMS };
-constexpr int LOSS_GRID = 1024, COUNT_GRID = 1024, SINGLE = 8192;
+constexpr int LOSS_GRID = 1024, COUNT_GRID = 1024, SINGLE = 2048;
 
 struct Input {
     const void *p;
@@ -117,18 +117,20 @@ __device__ __forceinline__ Four values_of(u32x4 r, int type) {
     return f;
 }
 __device__ __forceinline__ void put(void *p, int type, const Where &w, const float *v) {
-    if (type == D1_FP32) {
-        Pack<float, 4> a = {{v[0], v[1], v[2], v[3]}};
-        store_part<float, 4>((float *)p + w.i, w.have, a);
-    } else if (type == D1_BF16) {
-        Pack<__bf16, 4> a = {{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}};
-        store_part<__bf16, 4>((__bf16 *)p + w.i, w.have, a);
-    } else {
-        Pack<_Float16, 4> a = {{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]}};
-        store_part<_Float16, 4>((_Float16 *)p + w.i, w.have, a);
-    }
+    if (type == D1_FP32)
+        store_part((float *)p + w.i, w.have, Pack<float, 4>{{v[0], v[1], v[2], v[3]}});
+    else if (type == D1_BF16)
+        store_part((__bf16 *)p + w.i, w.have, Pack<__bf16, 4>{{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}});
+    else
+        store_part((_Float16 *)p + w.i, w.have, Pack<_Float16, 4>{{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]}});
 }
 
+// e^x: 2^p of the rounded product p = x log2 e times what the rounding dropped, within 2 halves of a step. (Infinities and NaN
+// pass through p; the maximum is for an infinite x, whose rest is NaN.) The library's takes half as many instructions again.
+__device__ __forceinline__ float exp_of(float x) {
+    const float p = x * 1.44269504f, rest = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269504f, -p));
+    return __builtin_amdgcn_exp2f(p) * __builtin_fmaf(fmaxf(rest, -1.f), 0.693147181f, 1.f);
+}
 // e^x - x - 1 given e = e^x; `rise` becomes e^x - 1. Below 1/2 the Taylor series to x^9, whose next term is 1e-9 of the
 // sum there.
 __device__ __forceinline__ float excess(float x, float e, float &rise) {
@@ -259,15 +261,15 @@ __device__ __forceinline__ void four(const Loss &a, const Where &w, float unit, 
         const float logp = x[LOGP].v[j], adv = x[ADV].v[j];
         const double d = (double)logp - (double)x[OLD].v[j];
         const bool past = adv > 0.f ? d > a.log_high : adv < 0.f && d < a.log_low;
-        const float df = (float)d, r = expf(df);
+        const float df = logp - x[OLD].v[j], r = exp_of(df);
         float g = past ? 0.f : -adv * r, rise;
         const float gain = (past ? (adv > 0.f ? 1.f + a.high : 1.f - a.low) : r) * adv, drift = excess(df, r, rise);
         sum[S_POLICY] -= in ? gain * wt : 0.f;
         sum[S_CLIPPED] += past ? wt : 0.f;
         sum[S_DRIFT] += in ? drift * wt : 0.f;
         if (a.in[REF].mode) {
-            const float gap = (float)((double)x[REF].v[j] - (double)logp);
-            const float q = excess(gap, expf(gap), rise);
+            const float gap = x[REF].v[j] - logp;
+            const float q = excess(gap, exp_of(gap), rise);
             sum[S_KL] += in ? q * wt : 0.f;
             g -= a.kl * rise;
         }
@@ -375,7 +377,9 @@ __global__ __launch_bounds__(256) void k_loss_finish(const Loss a, const double 
             const int i = u * 256 + threadIdx.x;
             x[u] = i < n ? parts[(int64_t)k * n + i] : 0.0;
         }
-        sums[k] = (x[0] + x[1]) + (x[2] + x[3]);
+        sums[k] = 0.0;
+#pragma unroll
+        for (int u = 0; u < LOSS_GRID / 256; u++) sums[k] += x[u];
     }
     const double sum = block_sums<256>(sums, sd);
     finish(a, sum, parts[(int64_t)SUMS * n], terms, all);
@@ -406,7 +410,8 @@ inline int count_grid(const D1PolicyLoss *h) {
     const int64_t n = !rows_counted(h) ? (h->rows * h->length + 16383) / 16384 : rows_long(h) ? h->rows : (h->rows + 3) / 4;
     return (int)(n < 1 ? 1 : n < COUNT_GRID ? n : COUNT_GRID);
 }
-// One workgroup of 1,024 threads does all in one launch, but for the counts of several sequences.
+// One workgroup of 1,024 threads does all in one launch, but for the counts of several sequences (8,192 tokens with every term
+// would take it 17 us, 8 workgroups and the join 9).
 inline bool is_single(const D1PolicyLoss *h) {
     const int64_t total = h->rows * h->length;
     return total == 0 || (total <= SINGLE && !rows_counted(h));

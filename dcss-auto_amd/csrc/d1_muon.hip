@@ -7,7 +7,7 @@
 // mantissa where bf16 would leave 8), or as the sum of two fp16 halves (for results in 32 bits): hi = fp16(v),
 // lo = fp16(v - hi), 22 bits, and a product is hi hi + hi lo + lo hi in one fp32 accumulator, three instructions for one.
 // X, A and B are held 2^12 times as large, which keeps both halves of entries down to 2^-14 of the largest out of fp16's
-// subnormal range; entries stay under 2^3, checked on the host from the coefficients.
+// subnormal range; entries stay under 2^4, checked on the host from the coefficients.
 //
 // All operands lie in fragment order (d1_frag.h): a wave's operand of one instruction, 32 rows by 16 of the contraction, is
 // one contiguous kilobyte, so loads are whole and LDS tiles are plain copies without conflicts. Rows and columns
@@ -775,18 +775,32 @@ static int64_t plan_bytes(const D1MuonTensor *t, const int *at, int count, int m
     return bytes;
 }
 
-// The singular values of X lie in [0, 1] after the norm; the largest that the steps make of them, from a fine grid and the
-// slope's bound between its points. What is held has to stay under 2^3 times the scale, and below that in A = s^2.
+// The singular values of X lie in [0, 1] after the norm; the largest that the steps make of them, from the ends and the
+// turning points of a s + b s^3 + c s^5 and of its factor a + b s^2 + c s^4. What is held has to stay under 2^4 times the scale.
 static double reach_of(const D1Muon *h) {
     double top = 1.0;
     for (int k = 0; k < h->steps; k++) {
-        double most = 0.0;
-        for (int i = 0; i <= 4096; i++) {
-            const double x = top * i / 4096, x2 = x * x, b = h->a + h->b * x2 + h->c * x2 * x2;
-            if (!(fabs(b) < 15.0) || !(x2 < 15.0)) return INFINITY;
-            if (fabs(b * x) > most) most = fabs(b * x);
+        const double x1 = top * top;
+        double x[5] = {0.0, x1, x1, x1, x1};               // s^2
+        if (h->c != 0) {
+            x[2] = -h->b / (2 * h->c);
+            const double d = 9 * h->b * h->b - 20 * h->a * h->c;
+            if (d >= 0) {
+                x[3] = (-3 * h->b + sqrt(d)) / (10 * h->c);
+                x[4] = (-3 * h->b - sqrt(d)) / (10 * h->c);
+            }
+        } else if (h->b != 0) {
+            x[3] = -h->a / (3 * h->b);
         }
-        top = most * 1.001 + 1e-3;
+        double most = 0.0;
+        for (double at : x) {
+            if (!(at > 0)) at = 0;
+            if (at > x1) at = x1;
+            const double factor = fabs(h->a + h->b * at + h->c * at * at);
+            if (!(factor < 15.0)) return INFINITY;
+            if (factor * sqrt(at) > most) most = factor * sqrt(at);
+        }
+        top = most + 1e-3;
         if (!(top < 3.8)) return INFINITY;
     }
     return top;

@@ -375,7 +375,7 @@ D1LossInput loss_input(const Tensor &t, const Tensor &logp, int64_t rows, int64_
     return in;
 }
 
-// -> (loss, terms [8], dlogp, dentropy, dvalues); a gradient that is not asked for is None
+// -> (terms [8], each of them, dlogp, dentropy, dvalues); a gradient that is not asked for is None
 py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &advantages, const Maybe &ref_logp, const Maybe &entropy,
                       const Maybe &values, const Maybe &returns, const Maybe &old_values, const Maybe &mask, double clip_low,
                       double clip_high, double kl_coef, double value_coef, double value_clip, double entropy_coef, bool sequence, int64_t grads,
@@ -428,6 +428,7 @@ py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &
     h.value_coef = value_coef;
     h.entropy_coef = entropy_coef;
     h.sequence = sequence;
+    const at::AutoDispatchBelowADInplaceOrView below;        // ten small tensors and views that autograd need not see
     const Tensor terms = at::empty({8}, logp.options().dtype(at::kFloat));
     Maybe dlogp, dentropy, dvalues, work;
     if (grads & 1) dlogp = at::empty(logp.sizes(), logp.options());
@@ -438,7 +439,7 @@ py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &
     if (need) work = scratch(need, logp);
     check(d1_policy_loss(&h, (float *)ptr(terms), ptr(dlogp), ptr(dentropy), ptr(dvalues), ptr(work), need, (void *)stream),
           "d1_policy_loss");
-    return py::make_tuple(terms, dlogp, dentropy, dvalues);
+    return py::make_tuple(terms, terms.unbind(0), dlogp, dentropy, dvalues);
 }
 
 // gradients that no one else holds, times a number on the device

@@ -13,40 +13,14 @@ from .ops import call
 
 class PolicyLoss(NamedTuple):
     loss: torch.Tensor                   # fp32, the sum with the coefficients; differentiable
-    terms: torch.Tensor                  # fp32 [8]: the loss and what is named below, without a gradient
-
-    @property
-    def policy(self):
-        return self.terms[1]
-
-    @property
-    def value(self):
-        """Half the (clipped) squared error."""
-        return self.terms[2]
-
-    @property
-    def entropy(self):
-        return self.terms[3]
-
-    @property
-    def kl(self):
-        """Estimate of KL(policy || reference)."""
-        return self.terms[4]
-
-    @property
-    def clipped(self):
-        """The share of the weight whose clip is active."""
-        return self.terms[5]
-
-    @property
-    def drift(self):
-        """Estimate of KL(old policy || policy) that is never negative."""
-        return self.terms[6]
-
-    @property
-    def count(self):
-        """Tokens that count, or sequences with one (level 'sequence')."""
-        return self.terms[7]
+    policy: torch.Tensor                 # fp32 numbers without a gradient, from here on
+    value: torch.Tensor                  # half the (clipped) squared error
+    entropy: torch.Tensor
+    kl: torch.Tensor                     # estimate of KL(policy || reference)
+    clipped: torch.Tensor                # the share of the weight whose clip is active
+    drift: torch.Tensor                  # estimate of KL(old policy || policy) that is never negative
+    count: torch.Tensor                  # tokens that count, or sequences with one (level 'sequence')
+    terms: torch.Tensor                  # [8]: all of them
 
 
 def _pair(clip):
@@ -67,10 +41,10 @@ class _PolicyLoss(torch.autograd.Function):
     def forward(ctx, logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings):
         want = [ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]]
         ctx.bits, ctx.settings = sum(w << k for k, w in enumerate(want)), settings
-        terms, *ctx.grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
+        terms, each, *ctx.grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
         ctx.save_for_backward(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask)
         ctx.mark_non_differentiable(terms)
-        return terms[0].clone(), terms
+        return each[0], terms
 
     @staticmethod
     @once_differentiable
@@ -79,7 +53,7 @@ class _PolicyLoss(torch.autograd.Function):
         logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask = ctx.saved_tensors
         if grads is None:                # the graph was kept: the first backward pass took them
             grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask,
-                          *ctx.settings)[1:]
+                          *ctx.settings)[2:]
         call('scale_grads', logp, dloss, grads)
         return (*grads, *[None] * 7)
 
@@ -101,15 +75,16 @@ def policy_loss(logp, old_logp, advantages, ref_logp=None, entropy=None, values=
     and gradients are 0."""
     settings = (clip, kl_coef, value_coef, value_clip, entropy_coef, level)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logp, entropy, values)):
-        return PolicyLoss(*_PolicyLoss.apply(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings))
-    terms = _call(0, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)[0]
-    return PolicyLoss(terms[0], terms)
+        loss, terms = _PolicyLoss.apply(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings)
+        return PolicyLoss(loss, *terms.unbind()[1:], terms)
+    terms, each, *_ = _call(0, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
+    return PolicyLoss(*each, terms)
 
 
 def policy_loss_grads(logp, old_logp, advantages, ref_logp=None, entropy=None, values=None, returns=None, old_values=None, mask=None,
                       clip=0.2, kl_coef=0.0, value_coef=0.5, value_clip=None, entropy_coef=0.01, level='token'):
     """-> (PolicyLoss, dlogp, dentropy, dvalues): policy_loss with the gradients of its loss, each like its input, in one
     pass; None where the input is."""
-    terms, *grads = _call(7, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef,
+    terms, each, *grads = _call(7, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef,
                           value_coef, value_clip, entropy_coef, level)
-    return (PolicyLoss(terms[0], terms), *grads)
+    return (PolicyLoss(*each, terms), *grads)

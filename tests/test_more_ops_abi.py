@@ -34,11 +34,11 @@ def test_loss_arguments(lib):
     flat = lambda type=0: lib.D1LossInput(data=F, row=100, step=1, type=type)  # noqa: E731
 
     def loss(**k):
-        base = dict(logp=flat(), old_logp=flat(), advantages=flat(), rows=50, length=100, clip_low=0.2, clip_high=0.2)
+        base = dict(logp=flat(), old_logp=flat(), advantages=flat(), rows=20, length=100, clip_low=0.2, clip_high=0.2)
         return lib.D1PolicyLoss(**dict(base, **k))
     good = loss()
     need = L.d1_policy_loss_work_bytes(C.byref(good))
-    assert need == 0                           # 5,000 tokens are one workgroup's
+    assert need == 0                           # 2,000 tokens are one workgroup's
     many = loss(rows=1000)
     assert L.d1_policy_loss_work_bytes(C.byref(many)) > 0
     masked = loss(rows=1000, mask=flat(), sequence=1)
