@@ -453,9 +453,9 @@ __global__ __launch_bounds__(256) void k_muon_join(const Mats s) {
 // Small results: a workgroup a tile of 32 SIDE, its waves share the contraction and join in LDS; operands straight from
 // the caches into registers; other workgroups of the CU multiply while one loads (with the next operands on their way there
 // were half as many: 544 tiles of 32 with a contraction of 256 in two halves 11.3 us, 7.8 without).
-template <int MODE, int TERMS, int SIDE>
-__global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
-    constexpr int W = 4, PL = TERMS == 3 ? 2 : 1, AT_ONCE = TERMS == 3 && SIDE == 2 ? 2 : 4;
+template <int MODE, int TERMS, int SIDE, int W>
+__global__ __launch_bounds__(64 * W) void k_muon_small(const Mats s) {
+    constexpr int PL = TERMS == 3 ? 2 : 1, AT_ONCE = TERMS == 3 && SIDE == 2 ? 2 : 4;
     __shared__ float sums[W][SIDE * SIDE][16][64];
     if (s.ctl && !s.ctl[C_GO]) return;
     Job job;
@@ -518,6 +518,7 @@ __global__ __launch_bounds__(256) void k_muon_small(const Mats s) {
 #pragma unroll
             for (int w = 0; w < W; w++) x[w] = sums[w][wave][r][lane];
             d[r] = (x[0] + x[1]) + (x[2] + x[3]);
+            if constexpr (W == 8) d[r] += (x[4] + x[5]) + (x[6] + x[7]);
         }
     __syncthreads();
     if (wave >= SIDE * SIDE) return;
@@ -685,8 +686,9 @@ inline int64_t mat_bytes(const D1MuonTensor &t, int terms) {
     return planes * 8192 * (3 * (int64_t)h.m64 * h.n64 + 2 * (int64_t)h.m64 * h.m64);
 }
 constexpr int64_t GROUP_BYTES = (int64_t)4 << 30;
-// Kinds of kernels: 0 small tiles of 32, 1 of 64, 2 large tiles of 128, 3 of 256
-constexpr int side_of(int kind) { return kind == 0 ? 32 : kind == 1 ? 64 : kind == 2 ? 128 : 256; }
+// Kinds of kernels: small tiles of 32 and 64, large ones of 128 (two workgroups a CU) and of 256
+enum { SMALL32, SMALL64, LARGE128, LARGE256, KINDS };
+constexpr int side_of(int kind) { return kind == SMALL32 ? 32 : kind == SMALL64 ? 64 : kind == LARGE256 ? 256 : 128; }
 inline int64_t tiles_of(int mode, const Shape &h, int side) {
     const int64_t m = ((int64_t)h.m64 * 64 + side - 1) / side, n = ((int64_t)h.n64 * 64 + side - 1) / side;
     return mode == GRAM || mode == POLY ? m * (m + 1) / 2 : m * n;
@@ -711,6 +713,9 @@ inline int parts_of(const D1MuonTensor &t) {
 // How a launch shares its products: the kind of tile and how many steps of 64 of the contraction a workgroup takes at most.
 // The estimate, in us: a kind's time for 64 of a tile's contraction where it has its CU full (WORK; the largest tiles, one
 // to a CU, in rounds) and alone (ALONE), and for shared tiles the join's launch and bytes at 4 TB/s.
+// steps of 64 above which eight waves share a small tile's contraction, not four (a matrix's product with itself: 256 x 1,800 in
+// halves by tiles of 32 10.8 us, 13.4 by four waves; 1,000 x 4,001 by tiles of 64 18.2, 24.0)
+constexpr int WIDE = 12;
 struct Plan {
     int kind;
     int64_t most;             // steps of 64
@@ -722,8 +727,9 @@ struct Alike {
     int n;
 };
 static double plan_time(const Alike *shapes, int count, int mode, int terms, int kind, int64_t most) {
-    static const double WORK[2][4] = {{0.117, 0.38, 0.68, 1.75}, {0.26, 0.87, 1.95, 5.3}}, ALONE[2][4] = {{0.15, 0.3, 0.9, 1.75}, {0.32, 0.6, 2.2, 5.3}};
-    const double c = WORK[terms == 3][kind], l = ALONE[terms == 3][kind];
+    static const double WORK[2][KINDS] = {{0.117, 0.38, 0.68, 1.75}, {0.26, 0.87, 1.95, 5.3}},
+                        ALONE[2][KINDS] = {{0.15, 0.3, 0.9, 1.75}, {0.32, 0.6, 2.2, 5.3}};
+    double c = WORK[terms == 3][kind], l = ALONE[terms == 3][kind];
     double work = 0, groups = 0, longest = 0, joined = 0;
     for (int k = 0; k < count; k++) {
         const Shape &h = shapes[k].h;
@@ -734,8 +740,10 @@ static double plan_time(const Alike *shapes, int count, int mode, int terms, int
         if (each > longest) longest = (double)each;
         if (splits > 1) joined += n * side_of(kind) * side_of(kind) * 8;
     }
+    if (kind <= SMALL64 && longest > WIDE) c *= 1.4, l *= 0.7;
     double time = work * c / 256;
-    if (kind == 3 && work / groups * c * std::ceil(groups / 256) > time) time = work / groups * c * std::ceil(groups / 256);
+    const double rounds = std::ceil(groups / 256) * work / groups;
+    if (kind == LARGE256 && rounds * c > time) time = rounds * c;
     if (longest * l > time) time = longest * l;
     return time + (joined ? 9.0 + joined / 4e6 : 0.0);
 }
@@ -753,7 +761,7 @@ static Plan plan_of(const D1MuonTensor *t, const int *at, int count, int mode, i
     }
     Plan best{0, 1 << 20};
     double least = 1e30;
-    for (int kind = 0; kind < 4; kind++)
+    for (int kind = 0; kind < KINDS; kind++)
         for (int64_t most : {(int64_t)1 << 20, (int64_t)64, (int64_t)32, (int64_t)16, (int64_t)8, (int64_t)4}) {
             if (most < (1 << 20) && (most >= longest || mode == APPLY)) continue;
             const double time = plan_time(shapes, alike, mode, terms, kind, most);
@@ -858,38 +866,42 @@ static MuonWork muon_work(const D1MuonTensor *t, int count, const D1Muon *h, con
 
 // `groups` workgroups; `blocks`: 32 x 32 blocks of tiles whose contraction is shared (of A and B alone)
 template <int MODE, int TERMS>
-static void muon_products(const Mats &s, int kind, int64_t groups, int64_t blocks, hipStream_t stream) {
+static void muon_products(const Mats &s, int kind, bool wide, int64_t groups, int64_t blocks, hipStream_t stream) {
     const dim3 grid((unsigned)groups), block(256), joins((unsigned)((blocks + 3) / 4));
-    if (kind == 3)
+    if (kind == LARGE256)
         hipLaunchKernelGGL((k_muon_large<MODE, TERMS, 256>), grid, dim3(512), 0, stream, s);
-    else if (kind == 2)
+    else if (kind == LARGE128)
         hipLaunchKernelGGL((k_muon_large<MODE, TERMS, 128>), grid, block, 0, stream, s);
-    else if (kind == 1)
-        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 2>), grid, block, 0, stream, s);
+    else if (kind == SMALL64 && wide)
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 2, 8>), grid, dim3(512), 0, stream, s);
+    else if (kind == SMALL64)
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 2, 4>), grid, block, 0, stream, s);
+    else if (wide)
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 1, 8>), grid, dim3(512), 0, stream, s);
     else
-        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 1>), grid, block, 0, stream, s);
+        hipLaunchKernelGGL((k_muon_small<MODE, TERMS, 1, 4>), grid, block, 0, stream, s);
     if constexpr (MODE == GRAM || MODE == POLY) {
         if (!blocks) return;
-        if (kind == 3)
+        if (kind == LARGE256)
             hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 256>), joins, block, 0, stream, s);
-        else if (kind == 2)
+        else if (kind == LARGE128)
             hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 128>), joins, block, 0, stream, s);
-        else if (kind == 1)
+        else if (kind == SMALL64)
             hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 64>), joins, block, 0, stream, s);
         else
             hipLaunchKernelGGL((k_muon_join<MODE, TERMS, 32>), joins, block, 0, stream, s);
     }
 }
 template <int TERMS>
-static void muon_products(int mode, const Mats &s, int kind, int64_t groups, int64_t blocks, hipStream_t stream) {
+static void muon_products(int mode, const Mats &s, int kind, bool wide, int64_t groups, int64_t blocks, hipStream_t stream) {
     if (mode == GRAM)
-        muon_products<GRAM, TERMS>(s, kind, groups, blocks, stream);
+        muon_products<GRAM, TERMS>(s, kind, wide, groups, blocks, stream);
     else if (mode == POLY)
-        muon_products<POLY, TERMS>(s, kind, groups, blocks, stream);
+        muon_products<POLY, TERMS>(s, kind, wide, groups, blocks, stream);
     else if (mode == APPLY)
-        muon_products<APPLY, TERMS>(s, kind, groups, blocks, stream);
+        muon_products<APPLY, TERMS>(s, kind, wide, groups, blocks, stream);
     else
-        muon_products<LAST, TERMS>(s, kind, groups, blocks, stream);
+        muon_products<LAST, TERMS>(s, kind, wide, groups, blocks, stream);
 }
 
 static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *work, const MuonWork &w, const int *at, int live,
@@ -982,13 +994,14 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
             for (int mode : {(int)GRAM, (int)POLY, step + 1 < h->steps ? (int)APPLY : (int)LAST}) {
                 const Plan &plan = plans[mode == LAST ? (int)APPLY : mode];
                 const int side = side_of(plan.kind);
-                int64_t groups = 0, parts = 0, blocks = 0;
+                int64_t groups = 0, parts = 0, blocks = 0, longest = 0;
                 for (int k = 0; k < p.count; k++) {
                     const Shape sh = shape_of(t[at[from + k]]);
                     const int64_t chunks = chunks_of(mode, sh), tiles = tiles_of(mode, sh, side);
                     int64_t splits = splits_of(chunks, plan.most);
                     splits = splits_of(chunks, (chunks + splits - 1) / splits);       // none without a step
                     p.t[k].splits = (int32_t)splits;
+                    longest = std::max(longest, (chunks + splits - 1) / splits);
                     p.t[k].first_part = (int32_t)parts;
                     groups += tiles * splits;
                     if (splits > 1) {
@@ -998,9 +1011,9 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
                     p.last[k] = (int32_t)groups;
                 }
                 if (terms == 3)
-                    muon_products<3>(mode, p, plan.kind, groups, blocks, stream);
+                    muon_products<3>(mode, p, plan.kind, longest > WIDE, groups, blocks, stream);
                 else
-                    muon_products<1>(mode, p, plan.kind, groups, blocks, stream);
+                    muon_products<1>(mode, p, plan.kind, longest > WIDE, groups, blocks, stream);
             }
         }
         from = to;
