@@ -155,7 +155,7 @@ def load_ops():
         L.d1_adamw_read.argtypes = [p, p, n, i, p, p]
         L.d1_policy_loss_work_bytes.argtypes = [p]
         L.d1_policy_loss.argtypes = [p, p, p, p, p, p, n, p]
-        L.d1_scale.argtypes = [p, i, n, p, p]
+        L.d1_scale.argtypes = [p, p, i, n, p, p]
         L.d1_scan_marks.argtypes = [p]
         L.d1_scan_work_bytes.argtypes = [p]
         L.d1_scan_fwd.argtypes = [p, p, n, n, p, p, n, p]

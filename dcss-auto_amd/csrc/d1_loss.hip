@@ -386,16 +386,15 @@ __global__ __launch_bounds__(256) void k_loss_finish(const Loss a, const double 
 }
 
 // Gradients made for a loss gradient of 1, scaled by the real one; nothing is read or written where that is 1.
-__global__ __launch_bounds__(256) void k_loss_scale(void *p, int type, int64_t n, const float *__restrict__ by) {
+__global__ __launch_bounds__(256) void k_loss_scale(const void *p, void *out, int type, int64_t n, const float *__restrict__ by) {
     const float f = *by;
-    if (f == 1.f) return;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
         const Where w = {i, 0, 0, n, n - i < 4 ? (int)(n - i) : 4};
         const u32x4 r = fetch<false>({p, 0, 1, FLAT, type}, w);
         Four x = values_of(r, type);
 #pragma unroll
         for (int j = 0; j < 4; j++) x.v[j] *= f;
-        put(p, type, w, x.v);
+        put(out, type, w, x.v);
     }
 }
 
@@ -524,11 +523,11 @@ int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentr
     return (int)hipGetLastError();
 }
 
-int d1_scale(void *data, int type, int64_t n, const float *by, void *stream) {
-    if (n < 0 || !is_type(type) || (n && (!data || !by))) return D1_E_ARG;
+int d1_scale(const void *data, void *out, int type, int64_t n, const float *by, void *stream) {
+    if (n < 0 || !is_type(type) || (n && (!data || !out || !by))) return D1_E_ARG;
     if (n == 0) return 0;
     const int64_t groups = (n + 1023) / 1024;
-    hipLaunchKernelGGL(k_loss_scale, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, (hipStream_t)stream, data, type, n, by);
+    hipLaunchKernelGGL(k_loss_scale, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, (hipStream_t)stream, data, out, type, n, by);
     return (int)hipGetLastError();
 }
 }

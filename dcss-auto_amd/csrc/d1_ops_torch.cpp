@@ -7,9 +7,11 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/d1ops.h"
@@ -442,11 +444,19 @@ py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &
     return py::make_tuple(terms, terms.unbind(0), dlogp, dentropy, dvalues);
 }
 
-// gradients that no one else holds, times a number on the device
-void scale_grads(const Tensor &by, const std::vector<Maybe> &grads, int64_t stream) {
+// policy_loss's gradients times a number on the device, in tensors of their own: a graph that is kept, or a pass that is
+// captured and replayed, finds them as they were
+std::vector<Maybe> scale_grads(const Tensor &by, const std::vector<Maybe> &grads, int64_t stream) {
+    no_tangent(by, "the loss's gradient");
     if (by.scalar_type() != at::kFloat || by.numel() != 1 || !by.is_cuda()) refuse("the loss's gradient must be one fp32 number");
-    for (const Maybe &g : grads)
-        if (g) check(d1_scale(ptr(g), type_of(g->scalar_type()), g->numel(), (const float *)ptr(by), (void *)stream), "d1_scale");
+    std::vector<Maybe> out(grads.size());
+    for (size_t i = 0; i < grads.size(); i++)
+        if (grads[i]) {
+            out[i] = at::empty(grads[i]->sizes(), grads[i]->options());
+            check(d1_scale(ptr(grads[i]), ptr(out[i]), type_of(grads[i]->scalar_type()), grads[i]->numel(), (const float *)ptr(by),
+                           (void *)stream), "d1_scale");
+        }
+    return out;
 }
 
 // ---- the gated recurrence
@@ -675,6 +685,19 @@ void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momen
             t.copy = ptr(c_);
         }
     }
+    // two of them on one place would step it twice, in any order
+    std::vector<std::pair<const char *, const char *>> places;
+    auto place = [&](const Tensor &t) {
+        if (t.numel()) places.emplace_back((const char *)ptr(t), (const char *)ptr(t) + t.nbytes());
+    };
+    for (size_t i = 0; i < count; i++) {
+        place(params[i]);
+        place(momenta[i]);
+        if (copies && (*copies)[i]) place(*(*copies)[i]);
+    }
+    std::sort(places.begin(), places.end());
+    for (size_t i = 1; i < places.size(); i++)
+        if (places[i].first < places[i - 1].second) refuse("parameters, momenta and copies must not overlap");
     muon_launch(table, h, (int32_t *)ptr(step), step, stream);
     for (size_t i = 0; i < count; i++) {
         written(params[i]);

@@ -16,6 +16,8 @@
 // A product A is -1 (sign bit) once a reset lies in it: what comes before is dropped, even where it is not finite.
 // Everything is computed in fp32. Bound by memory, in 16 bits nearly as much by the instructions (some 35 an element
 // forward, two thirds of them the sigmoid's).
+#include <type_traits>
+
 #include "d1_rows.h"
 
 namespace d1o {
@@ -32,7 +34,7 @@ struct Scan {
     float *parts;                         // composites of the segments: A then B, [segments][rows * width] each
     int64_t x_t, x_n, gate_t, gate_n, dh_t, dh_n, h_t, h_n, dx_t, dx_n, dgate_t, dgate_n, reset_t, reset_n;
     int64_t steps, cells;                 // cells = rows * width
-    uint32_t units;                       // rows * columns
+    uint32_t units;                       // the launch's rows * columns
     int32_t width, columns;               // columns: workgroups (waves, where each is on its own) beside each other on one row's channels
     int32_t past;                         // results past the caches
     int32_t segments, seg;                // seg: steps of a segment, a multiple of MARK
@@ -565,8 +567,7 @@ static bool scan_args(const D1Scan *h) {
     if (!h || !is_type(h->type) || h->steps < 0 || h->rows < 0 || h->width < 0 || h->width > D1_SCAN_MAX_WIDTH ||
         h->steps > D1_SCAN_MAX_STEPS)
         return false;
-    const int64_t columns = (h->width + 63) / 64;
-    return h->rows <= (int64_t)0x7FFFFFFF / (columns > 0 ? columns : 1);
+    return h->rows <= ((int64_t)1 << 48) / (h->width > 0 ? h->width : 1);
 }
 static bool scan_fill(const D1Scan *h, Scan &s, ScanCut &c, bool bwd) {
     c = scan_cut(h->steps, h->rows, h->width, h->type, bwd);
@@ -576,8 +577,7 @@ static bool scan_fill(const D1Scan *h, Scan &s, ScanCut &c, bool bwd) {
     s.columns = c.columns;
     s.segments = c.segments;
     s.seg = c.seg;
-    s.units = (uint32_t)(h->rows * c.columns);
-    s.past = h->steps * s.cells * (h->type == D1_FP32 ? 4 : 2) > PAST_BYTES;
+    s.past = (double)h->steps * s.cells * (h->type == D1_FP32 ? 4 : 2) > PAST_BYTES;
     s.x = h->x;
     s.x_t = h->x_t;
     s.x_n = h->x_n;
@@ -625,10 +625,40 @@ template <bool BWD, class T>
 static int scan_vec(const Scan &s, const ScanCut &c, hipStream_t stream) {
     return c.vec == 4 ? scan_kind<BWD, T, 4>(s, c, stream) : c.vec == 2 ? scan_kind<BWD, T, 2>(s, c, stream) : scan_kind<BWD, T, 1>(s, c, stream);
 }
+// A launch takes 2^22 units at most (a grid has under 2^32 threads); what is the rows' own is moved on for the next.
+constexpr int64_t LAUNCH_UNITS = (int64_t)1 << 22;
+static Scan scan_from(const Scan &s, int64_t row, int64_t rows, int type) {
+    Scan p = s;
+    const int64_t size = type == D1_FP32 ? 4 : 2, cell = row * s.width;
+    auto on = [&](auto *&at, int64_t bytes) {
+        if (at) at = (std::remove_reference_t<decltype(at)>)((uintptr_t)at + bytes);
+    };
+    on(p.x, row * s.x_n * size);
+    on(p.gate, row * s.gate_n * size);
+    on(p.h, row * s.h_n * size);
+    on(p.dh, row * s.dh_n * size);
+    on(p.dx, row * s.dx_n * size);
+    on(p.dgate, row * s.dgate_n * size);
+    on(p.reset, row * s.reset_n);
+    on(p.state, cell * 4);
+    on(p.last, cell * 4);
+    on(p.dlast, cell * 4);
+    on(p.dstate, cell * 4);
+    on(p.marks, cell * 4);
+    on(p.parts, cell * 4);
+    p.units = (uint32_t)(rows * s.columns);
+    return p;
+}
 template <bool BWD>
 static int scan_type(const Scan &s, const ScanCut &c, const D1Scan *h, hipStream_t stream) {
-    return h->type == D1_FP32 ? scan_vec<BWD, float>(s, c, stream)
-           : h->type == D1_BF16 ? scan_vec<BWD, __bf16>(s, c, stream) : scan_vec<BWD, _Float16>(s, c, stream);
+    const int64_t most = LAUNCH_UNITS / c.columns;            // columns: 2^18 at most
+    for (int64_t row = 0; row < h->rows; row += most) {
+        const Scan p = scan_from(s, row, h->rows - row < most ? h->rows - row : most, h->type);
+        const int code = h->type == D1_FP32 ? scan_vec<BWD, float>(p, c, stream)
+                         : h->type == D1_BF16 ? scan_vec<BWD, __bf16>(p, c, stream) : scan_vec<BWD, _Float16>(p, c, stream);
+        if (code) return code;
+    }
+    return 0;
 }
 
 }  // namespace d1o

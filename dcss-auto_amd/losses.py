@@ -20,7 +20,7 @@ class PolicyLoss(NamedTuple):
     clipped: torch.Tensor                # the share of the weight whose clip is active
     drift: torch.Tensor                  # estimate of KL(old policy || policy) that is never negative
     count: torch.Tensor                  # tokens that count, or sequences with one (level 'sequence')
-    terms: torch.Tensor                  # [8]: all of them
+    terms: torch.Tensor                  # [8]: all of them; the ones above are its elements, not copies
 
 
 def _pair(clip):
@@ -39,23 +39,16 @@ def _call(grads, logp, old_logp, advantages, ref_logp, entropy, values, returns,
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings):
-        want = [ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]]
-        ctx.bits, ctx.settings = sum(w << k for k, w in enumerate(want)), settings
-        terms, each, *ctx.grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
-        ctx.save_for_backward(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask)
+        want = sum(w << k for k, w in enumerate(ctx.needs_input_grad[:3]))
+        # the gradients of the loss come with it, so nothing of the inputs is kept
+        terms, each, *ctx.grads = _call(want, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, *settings)
         ctx.mark_non_differentiable(terms)
         return each[0], terms
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _):
-        grads, ctx.grads = ctx.grads, None
-        logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask = ctx.saved_tensors
-        if grads is None:                # the graph was kept: the first backward pass took them
-            grads = _call(ctx.bits, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask,
-                          *ctx.settings)[2:]
-        call('scale_grads', logp, dloss, grads)
-        return (*grads, *[None] * 7)
+        return (*call('scale_grads', dloss, dloss, ctx.grads), *[None] * 7)
 
 
 def policy_loss(logp, old_logp, advantages, ref_logp=None, entropy=None, values=None, returns=None, old_values=None, mask=None,

@@ -158,8 +158,8 @@ typedef struct D1PolicyLoss {
 int64_t d1_policy_loss_work_bytes(const D1PolicyLoss *h);
 int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentropy, void *dvalues, void *work,
                    int64_t work_bytes, void *stream);
-/* data[0..n) (D1_FP32, D1_BF16 or D1_FP16) *= *by; nothing is written where *by is 1. */
-int d1_scale(void *data, int type, int64_t n, const float *by, void *stream);
+/* out[0..n) = data[0..n) * *by (D1_FP32, D1_BF16 or D1_FP16); out may be data. */
+int d1_scale(const void *data, void *out, int type, int64_t n, const float *by, void *stream);
 
 /* h[t] = (1 - z[t]) m[t] h[t-1] + z[t] x[t] with z = sigmoid(gate), for `rows` sequences of `steps` steps of `width`
  * channels; m[t] is 0 where reset[t * reset_t + row * reset_n] is not (what was before is dropped, whatever it holds),

@@ -57,8 +57,8 @@ def test_loss_arguments(lib):
     assert L.d1_policy_loss(C.byref(many), F, None, None, None, None, 0, None) == -1
     assert L.d1_policy_loss(C.byref(many), F, None, None, None, F, 8, None) == -1
     assert L.d1_policy_loss(None, F, None, None, None, None, 0, None) == -1
-    assert L.d1_scale(F, 9, 4, F, None) == -1 and L.d1_scale(None, 0, 4, F, None) == -1 and L.d1_scale(F, 0, -1, F, None) == -1
-    assert L.d1_scale(None, 0, 0, None, None) == 0
+    assert L.d1_scale(F, F, 9, 4, F, None) == -1 and L.d1_scale(None, F, 0, 4, F, None) == -1 and L.d1_scale(F, F, 0, -1, F, None) == -1
+    assert L.d1_scale(F, None, 0, 4, F, None) == -1 and L.d1_scale(None, None, 0, 0, None, None) == 0
 
 
 def test_scan_arguments(lib):
@@ -71,7 +71,7 @@ def test_scan_arguments(lib):
     need = L.d1_scan_work_bytes(C.byref(good))
     assert need > 0 and L.d1_scan_work_bytes(C.byref(scan(steps=8))) == 0
     for k in (dict(steps=-1), dict(rows=-1), dict(width=-1), dict(type=3), dict(width=(1 << 24) + 1), dict(steps=(1 << 30) + 1),
-              dict(rows=1 << 31)):
+              dict(rows=1 << 43)):
         h = scan(**k)
         assert L.d1_scan_marks(C.byref(h)) == -1 and L.d1_scan_work_bytes(C.byref(h)) == -1, k
         assert L.d1_scan_fwd(C.byref(h), F, 64, 0, F, F, 1 << 30, None) == -1, k

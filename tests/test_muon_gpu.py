@@ -243,3 +243,11 @@ def test_refusals(O):
               dict(copies=[u])):
         with pytest.raises(ValueError):
             O.muon_step(p, g, m, step, **k)
+    # one place twice, whole or in part
+    flat = torch.zeros(3 * u.numel(), device=DEV)
+    first, part = flat[:u.numel()].view_as(u), flat[4:4 + u.numel()].view_as(u)
+    other = torch.zeros_like(u)
+    for pp, mm in ((p * 2, [m[0], other]), ([p[0], other], m * 2), ([first, part], [m[0], other]), ([first, other], [part, m[0]])):
+        with pytest.raises(ValueError, match='overlap'):
+            O.muon_step(pp, g * 2, mm, step)
+    assert int(step.abs().sum()) == 0
