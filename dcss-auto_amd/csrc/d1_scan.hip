@@ -674,6 +674,7 @@ int64_t d1_scan_marks(const D1Scan *h) {
 
 int64_t d1_scan_work_bytes(const D1Scan *h) {
     if (!scan_args(h)) return D1_E_ARG;
+    if (h->steps == 0 || h->rows == 0 || h->width == 0) return 0;         // nothing to cut
     const int f = scan_cut(h->steps, h->rows, h->width, h->type, false).segments, b = scan_cut(h->steps, h->rows, h->width, h->type, true).segments;
     const int most = f > b ? f : b;
     return most > 1 ? (int64_t)2 * sizeof(float) * most * h->rows * h->width : 0;
