@@ -60,8 +60,9 @@ __device__ __forceinline__ Cells<VEC> cells_of(const Scan &s, uint32_t unit) {
 
 // z = sigmoid(g) and a = sigmoid(-g), each exact to a few ulp where it is small too: 1 / (1 + e) and e / (1 + e) with
 // e = e^-|g|, which is 2^p of the rounded product p = -|g| log2 e times what the rounding dropped. A bf16 gate's product with
-// 16 bits of log2 e is exact, which leaves the constant's own rest. (A NaN passes through p; the maximum is for -inf,
-// whose rest is NaN.) The reciprocal is refined: one that is off to one side adds up over thousands of steps.
+// 16 bits of log2 e is exact, which leaves the constant's own rest. (A NaN passes through p. The bounds on the rest are for
+// gates whose product passes fp32's range, where e is 0: it is NaN for -inf, infinite below -2.36e38.) The reciprocal is
+// refined: one that is off to one side adds up over thousands of steps.
 template <class T>
 __device__ __forceinline__ void gate_of(float g, float &z, float &a) {
     const float y = -fabsf(g);
@@ -74,7 +75,7 @@ __device__ __forceinline__ void gate_of(float g, float &z, float &a) {
         rest = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, 1.44269504f, -p)) * 0.693147181f;
     }
     float e = __builtin_amdgcn_exp2f(p);
-    e = __builtin_fmaf(e, fmaxf(rest, -1.f), e);
+    e = __builtin_fmaf(e, fminf(fmaxf(rest, -1.f), 1.f), e);
     float big = __builtin_amdgcn_rcpf(1.f + e);
     big = __builtin_fmaf(__builtin_fmaf(-(1.f + e), big, 1.f), big, big);
     const float small = e * big;
