@@ -128,10 +128,11 @@ __device__ __forceinline__ void put(void *p, int type, const Where &w, const flo
 }
 
 // e^x: 2^p of the rounded product p = x log2 e times what the rounding dropped, within 2 halves of a step. (Infinities and NaN
-// pass through p; the maximum is for an infinite x, whose rest is NaN.) The library's takes half as many instructions again.
+// pass through p. The bounds on the rest are for an x whose product passes fp32's range: it is NaN for an infinite one, infinite past
+// 2.36e38 either way.) The library's takes half as many instructions again.
 __device__ __forceinline__ float exp_of(float x) {
     const float p = x * 1.44269504f, rest = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269504f, -p));
-    return __builtin_amdgcn_exp2f(p) * __builtin_fmaf(fmaxf(rest, -1.f), 0.693147181f, 1.f);
+    return __builtin_amdgcn_exp2f(p) * __builtin_fmaf(fminf(fmaxf(rest, -1.f), 1.f), 0.693147181f, 1.f);
 }
 // e^x - x - 1 given e = e^x; `rise` becomes e^x - 1. Below 1/2 the Taylor series to x^9, whose next term is 1e-9 of the
 // sum there.
