@@ -22,7 +22,7 @@ LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', '
                  'learn_step_active', 'learn_heuristic')
 OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
                'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read', 'd1_policy_loss_work_bytes',
-               'd1_policy_loss', 'd1_scale', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd',
+               'd1_policy_loss', 'd1_scale', 'd1_scale_to', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd',
                'd1_muon_check', 'd1_muon_work_bytes', 'd1_muon_step')
 _LEARN = {}
 _OPS = _OPS_TORCH = None
@@ -111,7 +111,7 @@ class D1PolicyLoss(C.Structure):
                                                    'old_values', 'mask')),
                 ('rows', C.c_int64), ('length', C.c_int64), ('clip_low', C.c_double), ('clip_high', C.c_double),
                 ('value_clip', C.c_double), ('kl_coef', C.c_double), ('value_coef', C.c_double), ('entropy_coef', C.c_double),
-                ('sequence', C.c_int32), ('pad', C.c_int32)]
+                ('sequence', C.c_int32), ('fp32_grads', C.c_int32)]
 
 
 class D1Scan(C.Structure):
@@ -155,7 +155,7 @@ def load_ops():
         L.d1_adamw_read.argtypes = [p, p, n, i, p, p]
         L.d1_policy_loss_work_bytes.argtypes = [p]
         L.d1_policy_loss.argtypes = [p, p, p, p, p, p, n, p]
-        L.d1_scale.argtypes = [p, p, i, n, p, p]
+        L.d1_scale.argtypes = L.d1_scale_to.argtypes = [p, p, i, n, p, p]
         L.d1_scan_marks.argtypes = [p]
         L.d1_scan_work_bytes.argtypes = [p]
         L.d1_scan_fwd.argtypes = [p, p, n, n, p, p, n, p]

@@ -377,7 +377,8 @@ D1LossInput loss_input(const Tensor &t, const Tensor &logp, int64_t rows, int64_
     return in;
 }
 
-// -> (terms [8], each of them, dlogp, dentropy, dvalues); a gradient that is not asked for is None
+// -> (terms [8], each of them, dlogp, dentropy, dvalues); a gradient that is not asked for is None. grads: a bit for each of them, and 8
+// for all in fp32
 py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &advantages, const Maybe &ref_logp, const Maybe &entropy,
                       const Maybe &values, const Maybe &returns, const Maybe &old_values, const Maybe &mask, double clip_low,
                       double clip_high, double kl_coef, double value_coef, double value_clip, double entropy_coef, bool sequence, int64_t grads,
@@ -430,12 +431,14 @@ py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &
     h.value_coef = value_coef;
     h.entropy_coef = entropy_coef;
     h.sequence = sequence;
+    h.fp32_grads = grads >> 3 & 1;
     const at::AutoDispatchBelowADInplaceOrView below;        // ten small tensors and views that autograd need not see
     const Tensor terms = at::empty({8}, logp.options().dtype(at::kFloat));
     Maybe dlogp, dentropy, dvalues, work;
-    if (grads & 1) dlogp = at::empty(logp.sizes(), logp.options());
-    if ((grads & 2) && entropy) dentropy = at::empty(logp.sizes(), entropy->options());
-    if ((grads & 4) && values) dvalues = at::empty(logp.sizes(), values->options());
+    auto gradient = [&](const Tensor &of) { return at::empty(logp.sizes(), h.fp32_grads ? of.options().dtype(at::kFloat) : of.options()); };
+    if (grads & 1) dlogp = gradient(logp);
+    if ((grads & 2) && entropy) dentropy = gradient(*entropy);
+    if ((grads & 4) && values) dvalues = gradient(*values);
     const int64_t need = d1_policy_loss_work_bytes(&h);
     check(need < 0 ? (int)need : 0, "d1_policy_loss_work_bytes");
     if (need) work = scratch(need, logp);
@@ -444,17 +447,17 @@ py::tuple policy_loss(const Tensor &logp, const Tensor &old_logp, const Tensor &
     return py::make_tuple(terms, terms.unbind(0), dlogp, dentropy, dvalues);
 }
 
-// policy_loss's gradients times a number on the device, in tensors of their own: a graph that is kept, or a pass that is
-// captured and replayed, finds them as they were
-std::vector<Maybe> scale_grads(const Tensor &by, const std::vector<Maybe> &grads, int64_t stream) {
+// policy_loss's gradients, kept in fp32, times a number on the device, rounded to `types`, in tensors of their own: a graph that
+// is kept, or a pass that is captured and replayed, finds them as they were
+std::vector<Maybe> scale_grads(const Tensor &by, const std::vector<Maybe> &grads, const std::vector<at::ScalarType> &types, int64_t stream) {
     no_tangent(by, "the loss's gradient");
     if (by.scalar_type() != at::kFloat || by.numel() != 1 || !by.is_cuda()) refuse("the loss's gradient must be one fp32 number");
     std::vector<Maybe> out(grads.size());
     for (size_t i = 0; i < grads.size(); i++)
         if (grads[i]) {
-            out[i] = at::empty(grads[i]->sizes(), grads[i]->options());
-            check(d1_scale(ptr(grads[i]), ptr(out[i]), type_of(grads[i]->scalar_type()), grads[i]->numel(), (const float *)ptr(by),
-                           (void *)stream), "d1_scale");
+            out[i] = at::empty(grads[i]->sizes(), grads[i]->options().dtype(types[i]));
+            check(d1_scale_to((const float *)ptr(grads[i]), ptr(out[i]), type_of(types[i]), grads[i]->numel(), (const float *)ptr(by),
+                              (void *)stream), "d1_scale_to");
         }
     return out;
 }

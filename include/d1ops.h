@@ -141,7 +141,7 @@ typedef struct D1PolicyLoss {
     double value_clip;        /* 0: none, else it needs old_values */
     double kl_coef, value_coef, entropy_coef;
     int32_t sequence;         /* 0: every token counts alike; 1: every sequence with a token does, its tokens sharing its weight */
-    int32_t pad;
+    int32_t fp32_grads;       /* 0: gradients in the type of their input, 1: all in fp32 */
 } D1PolicyLoss;
 
 /* With d = logp - old_logp, r = e^d, x = ref_logp - logp and w a token's weight (0 where mask is 0, whatever the other
@@ -153,13 +153,15 @@ typedef struct D1PolicyLoss {
  *   terms[5] clipped = sum of the weights of tokens whose clip is active;  terms[6] drift = sum w (e^d - d - 1)
  *   terms[7] the tokens, or the sequences with one
  * A term whose input is not given is 0, all are where no token is left. dlogp, dentropy and dvalues (each may be null,
- * then it is not made; contiguous [rows, length], the type of their input) are the gradients of the loss. They must not
- * overlap the inputs. The same inputs give the same bits. */
+ * then it is not made; contiguous [rows, length], the type of their input, or fp32 with fp32_grads) are the gradients of
+ * the loss. They must not overlap the inputs. The same inputs give the same bits. */
 int64_t d1_policy_loss_work_bytes(const D1PolicyLoss *h);
 int d1_policy_loss(const D1PolicyLoss *h, float *terms, void *dlogp, void *dentropy, void *dvalues, void *work,
                    int64_t work_bytes, void *stream);
 /* out[0..n) = data[0..n) * *by (D1_FP32, D1_BF16 or D1_FP16); out may be data. */
 int d1_scale(const void *data, void *out, int type, int64_t n, const float *by, void *stream);
+/* The same of fp32 data, rounded to `type` once, after the product; out must not overlap data unless type is D1_FP32. */
+int d1_scale_to(const float *data, void *out, int type, int64_t n, const float *by, void *stream);
 
 /* h[t] = (1 - z[t]) m[t] h[t-1] + z[t] x[t] with z = sigmoid(gate), for `rows` sequences of `steps` steps of `width`
  * channels; m[t] is 0 where reset[t * reset_t + row * reset_n] is not (what was before is dropped, whatever it holds),
