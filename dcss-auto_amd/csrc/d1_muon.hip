@@ -4,7 +4,7 @@
 // pull every singular value towards 1:
 //   A = X X^T;  B = a I + b A + c A A;  X = B X
 // Matrix instructions take 16-bit operands. A value is held as fp16 (one term: for results in 16 bits, 11 bits of
-// mantissa where bf16 would leave 8), or as the sum of two fp16 halves (for results in 32 bits): hi = fp16(v),
+// mantissa where bf16 would leave 8), or as the sum of two fp16 halves (for results in 32 bits, and of a short side under 16): hi = fp16(v),
 // lo = fp16(v - hi), 22 bits, and a product is hi hi + hi lo + lo hi in one fp32 accumulator, three instructions for one.
 // X, A and B are held 2^12 times as large, which keeps both halves of entries down to 2^-14 of the largest out of fp16's
 // subnormal range; entries stay under 2^4, checked on the host from the coefficients.
@@ -697,7 +697,14 @@ inline int64_t tiles_of(int mode, const Shape &h, int side) {
     const int64_t m = ((int64_t)h.m64 * 64 + side - 1) / side, n = ((int64_t)h.n64 * 64 + side - 1) / side;
     return mode == GRAM || mode == POLY ? m * (m + 1) / 2 : m * n;
 }
-inline int terms_of(const D1MuonTensor &t, const D1Muon *h) { return h->terms ? h->terms : t.type == D1_FP32 ? 3 : 1; }
+// With a short side under 16 an entry of A weighs a whole row or more, and its rounding moves all of it: in 16-bit operands the worst of
+// 300 random 2 x 2 matrices is 4.4% off, of 4 x 300 0.7% (32 x 32 0.25%; bf16's own rounding of the result 0.16%). Two halves take that away,
+// for 8 x 256 90 us in place of 78 and 15 x 131,072 618 for 267; in a list with others that stay in 16 bits, a second row of
+// launches (eight 8 x 256 beside eight 1,024 x 1,024 538 us, 453).
+inline int terms_of(const D1MuonTensor &t, const D1Muon *h) {
+    if (h->terms) return h->terms;
+    return t.type == D1_FP32 || t.rows < 16 || t.cols < 16 ? 3 : 1;
+}
 // The matrices at[from..to) that one row of launches takes: alike in terms, as many as fit its arguments and 4 GB
 inline int group_end(const D1MuonTensor *t, const int *at, int count, int from, const D1Muon *h) {
     const int terms = terms_of(t[at[from]], h);

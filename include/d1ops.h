@@ -203,7 +203,8 @@ typedef struct D1Muon {
     double a, b, c;           /* of the quintic a s + b s^3 + c s^5 */
     double eps, momentum;
     int32_t steps, nesterov;
-    int32_t terms;            /* operands of the products: 1: fp16, 3: two fp16 halves (22 bits), 0: 3 for fp32 results, 1 for others */
+    int32_t terms;            /* operands of the products: 1: fp16, 3: two fp16 halves (22 bits), 0: 3 for fp32 results
+                                 and matrices with a side under 16, 1 for others */
     int32_t pad;
 } D1Muon;
 
