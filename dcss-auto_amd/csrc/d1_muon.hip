@@ -33,7 +33,7 @@ typedef d1f::floatx16 acc_t;
 typedef d1f::u32x4 u32x4;
 
 constexpr int GROUP = 32;                  // matrices of a launch
-constexpr int NORM_PARTS = 1024;           // workgroups that sum a matrix's squares
+constexpr int NORM_PARTS = 1024;           // workgroups that sum a matrix's squares (their sums' numbers pass 32 bits from 2^21 matrices on)
 constexpr float SCALE = 4096.f;            // of X, A and B as they are held
 enum { GRAM, POLY, APPLY, LAST };
 enum { C_STEP, C_SKIPPED, C_GO = 6 };
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(1024) void k_muon_begin(const double *__restrict__ 
     __syncthreads();
     for (int k = threadIdx.x >> 6; k < count; k += 16) {
         double sum = 0.0;
-        for (int i = threadIdx.x & 63; i < parts[k]; i += 64) sum += sums[k * NORM_PARTS + i];
+        for (int i = threadIdx.x & 63; i < parts[k]; i += 64) sum += sums[(int64_t)k * NORM_PARTS + i];
         for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
         if ((threadIdx.x & 63) == 0) {
             scales[k] = (double)SCALE / (sqrt(sum) + eps);
