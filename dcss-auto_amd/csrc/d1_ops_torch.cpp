@@ -701,6 +701,14 @@ void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momen
     std::sort(places.begin(), places.end());
     for (size_t i = 1; i < places.size(); i++)
         if (places[i].first < places[i - 1].second) refuse("parameters, momenta and copies must not overlap");
+    // and a gradient on one of them would be read after it is written (what was copied to be contiguous lies elsewhere)
+    for (size_t i = 0; i < count; i++) {
+        if (!held[i].numel()) continue;
+        const char *begin = (const char *)ptr(held[i]), *end = begin + held[i].nbytes();
+        const auto behind = std::lower_bound(places.begin(), places.end(), std::make_pair(end, (const char *)nullptr));
+        if (behind != places.begin() && (behind - 1)->second > begin)
+            refuse("matrix " + std::to_string(i) + ": its gradient must not overlap parameters, momenta or copies");
+    }
     muon_launch(table, h, (int32_t *)ptr(step), step, stream);
     for (size_t i = 0; i < count; i++) {
         written(params[i]);
