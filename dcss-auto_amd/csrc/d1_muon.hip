@@ -1056,7 +1056,8 @@ int d1_muon_step(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl
     const int live = muon_order(t, count, h, at);
     const MuonWork w = muon_work(t, count, h, at, live);
     int code = D1_E_ARG;
-    if (work && work_bytes >= w.total && !((uintptr_t)work & 255)) code = muon_run(t, h, ctl, (char *)work, w, at, live, (hipStream_t)stream);
+    if (!w.total || (work && work_bytes >= w.total && !((uintptr_t)work & 255)))      // none for no matrices
+        code = muon_run(t, h, ctl, (char *)work, w, at, live, (hipStream_t)stream);
     delete[] at;
     return code;
 }
