@@ -285,6 +285,7 @@ class Muon(torch.optim.Optimizer):
         super().add_param_group(param_group)
         for p in self.param_groups[-1]['params']:
             if p.dim() < 2:
+                del self.param_groups[-1]            # the optimizer stays as it was
                 raise ValueError(f'a parameter must have two dimensions or more, not {list(p.shape)}')
 
     def __getstate__(self):
