@@ -21,7 +21,7 @@ LEARN_SYMBOLS = ('learn_turn_cost', 'learn_return_gamma', 'learn_state_bytes', '
                  'learn_action_size', 'learn_out_size', 'learn_config_bytes', 'learn_init', 'learn_step',
                  'learn_step_active', 'learn_heuristic')
 OPS_SYMBOLS = ('d1_tokens_work_bytes', 'd1_tokens_fwd', 'd1_tokens_bwd', 'd1_norm_fwd', 'd1_norm_work_bytes',
-               'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_read', 'd1_policy_loss_work_bytes',
+               'd1_norm_bwd', 'd1_adamw_work_bytes', 'd1_adamw_step', 'd1_adamw_step_with', 'd1_adamw_read', 'd1_policy_loss_work_bytes',
                'd1_policy_loss', 'd1_scale', 'd1_scale_to', 'd1_scan_marks', 'd1_scan_work_bytes', 'd1_scan_fwd', 'd1_scan_bwd',
                'd1_muon_check', 'd1_muon_work_bytes', 'd1_muon_step')
 _LEARN = {}
@@ -131,7 +131,7 @@ class D1MuonTensor(C.Structure):
 class D1Muon(C.Structure):
     """The D1Muon struct of include/d1ops.h."""
     _fields_ = [*((name, C.c_double) for name in ('a', 'b', 'c', 'eps', 'momentum')),
-                *((name, C.c_int32) for name in ('steps', 'nesterov', 'terms', 'pad'))]
+                *((name, C.c_int32) for name in ('steps', 'nesterov', 'terms', 'part'))]
 
 
 def load_ops():
@@ -152,6 +152,7 @@ def load_ops():
         L.d1_norm_bwd.argtypes = [p, n, p, i, n, i, n, p, i, p, p, p, p, p, p, n, p]
         L.d1_adamw_work_bytes.argtypes = [p, i, p]
         L.d1_adamw_step.argtypes = [p, i, p, p, p, n, p]
+        L.d1_adamw_step_with.argtypes = [p, i, p, p, p, p, n, p]
         L.d1_adamw_read.argtypes = [p, p, n, i, p, p]
         L.d1_policy_loss_work_bytes.argtypes = [p]
         L.d1_policy_loss.argtypes = [p, p, p, p, p, p, n, p]

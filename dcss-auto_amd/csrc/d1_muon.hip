@@ -36,7 +36,7 @@ constexpr int GROUP = 32;                  // matrices of a launch
 constexpr int NORM_PARTS = 1024;           // workgroups that sum a matrix's squares (their sums' numbers pass 32 bits from 2^21 matrices on)
 constexpr float SCALE = 4096.f;            // of X, A and B as they are held
 enum { GRAM, POLY, APPLY, LAST };
-enum { C_STEP, C_SKIPPED, C_GO = 6 };
+enum { C_STEP, C_SKIPPED, C_GO = CTL_GO };
 
 // a matrix as the products see it: m <= n after the turn, M and N their multiples of 64
 struct Mat {
@@ -826,7 +826,7 @@ static double reach_of(const D1Muon *h) {
 }
 
 static bool muon_args(const D1MuonTensor *t, int count, const D1Muon *h) {
-    if (count < 0 || (count && !t) || !h || (h->terms != 0 && h->terms != 1 && h->terms != 3)) return false;
+    if (count < 0 || (count && !t) || !h || (h->terms != 0 && h->terms != 1 && h->terms != 3) || h->part < 0 || h->part > 2) return false;
     if (h->steps < 1 || h->steps > D1_MUON_MAX_STEPS || !(h->eps >= 0) || !(h->momentum >= 0 && h->momentum < 1)) return false;
     for (int i = 0; i < count; i++) {
         const D1MuonTensor &a = t[i];
@@ -947,14 +947,17 @@ static int muon_run(const D1MuonTensor *t, const D1Muon *h, int32_t *ctl, char *
         }
         return tiles;
     };
-    for (int from = 0; from < live;) {
-        const int to = live - from < GROUP ? live : from + GROUP;
-        Sources s;
-        const int64_t tiles = sources(from, to, false, s);
-        hipLaunchKernelGGL(k_muon_norm, dim3((unsigned)tiles), dim3(256), 0, stream, s);
-        from = to;
+    if (h->part != 2) {
+        for (int from = 0; from < live;) {
+            const int to = live - from < GROUP ? live : from + GROUP;
+            Sources s;
+            const int64_t tiles = sources(from, to, false, s);
+            hipLaunchKernelGGL(k_muon_norm, dim3((unsigned)tiles), dim3(256), 0, stream, s);
+            from = to;
+        }
+        hipLaunchKernelGGL(k_muon_begin, dim3(1), dim3(1024), 0, stream, sums, scales, parts, live, h->eps, ctl);
     }
-    hipLaunchKernelGGL(k_muon_begin, dim3(1), dim3(1024), 0, stream, sums, scales, parts, live, h->eps, ctl);
+    if (h->part == 1) return (int)hipGetLastError();
     for (int from = 0; from < live;) {
         const int to = group_end(t, at, live, from, h), terms = terms_of(t[at[from]], h);
         Sources s;
@@ -1049,7 +1052,7 @@ int64_t d1_muon_work_bytes(const D1MuonTensor *t, int count, const D1Muon *h) {
 int d1_muon_check(const D1Muon *h) { return muon_args(nullptr, 0, h) && reach_of(h) < 3.8 ? 0 : D1_E_ARG; }
 
 int d1_muon_step(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl, void *work, int64_t work_bytes, void *stream) {
-    if (!muon_args(t, count, h) || ((uintptr_t)ctl & 3)) return D1_E_ARG;
+    if (!muon_args(t, count, h) || ((uintptr_t)ctl & 3) || (h->part && !ctl)) return D1_E_ARG;
     if (d1_muon_check(h)) return D1_E_ARG;
     int *at = new (std::nothrow) int[count + 1];
     if (!at) return (int)hipErrorOutOfMemory;

@@ -236,7 +236,7 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
                 const std::vector<double> &lr, const std::vector<double> &weight_decay, double beta1, double beta2, double eps,
                 double max_norm, const std::optional<std::vector<Maybe>> &copies, const std::optional<Tensors> &m_exps,
                 const std::optional<Tensors> &v_exps, const std::optional<std::vector<int64_t>> &counters,
-                const std::optional<std::vector<int64_t>> &lags, uint64_t seed, int64_t stream) {
+                const std::optional<std::vector<int64_t>> &lags, uint64_t seed, const Maybe &other, int64_t stream) {
     no_trace("adamw_step");
     const size_t count = params.size();
     const bool eight = m_exps.has_value();
@@ -259,6 +259,9 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
         refuse("betas must be in [0, 1), eps and max_grad_norm not negative");
     if (step.scalar_type() != at::kInt || step.dim() != 1 || step.size(0) != 8 || !step.is_cuda() || !step.is_contiguous())
         refuse("step must be a contiguous int32 CUDA tensor of 8 elements");
+    if (other && (other->scalar_type() != at::kInt || other->dim() != 1 || other->size(0) != 8 || !other->is_contiguous() ||
+                  other->device() != step.device()))
+        refuse("the other step's counts must be a contiguous int32 tensor of 8 elements on " + step.device().str());
     const at::ScalarType moment = eight ? at::kByte : at::kFloat;
     std::vector<D1AdamWTensor> table(count);
     Tensors held;            // contiguous gradients, until the launches that read them are queued
@@ -324,7 +327,8 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
     check(need < 0 ? (int)need : 0, "d1_adamw_work_bytes");
     Maybe work;
     if (need) work = scratch(need, step);
-    check(d1_adamw_step(table.data(), (int)count, &h, (int32_t *)ptr(step), ptr(work), need, (void *)stream), "d1_adamw_step");
+    check(d1_adamw_step_with(table.data(), (int)count, &h, (int32_t *)ptr(step), (int32_t *)ptr(other), ptr(work), need, (void *)stream),
+          "d1_adamw_step_with");
     for (size_t i = 0; i < count; i++) {
         for (const Tensor *t : {&params[i], &exp_avg[i], &exp_avg_sq[i]}) written(*t);
         if (copies && (*copies)[i]) written(*(*copies)[i]);
@@ -334,6 +338,7 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
         }
     }
     written(step);
+    if (other) written(*other);
 }
 
 Tensor adamw_read(const Tensor &code, const Tensor &exp, bool is_signed, const Maybe &out_, int64_t stream) {
@@ -594,11 +599,14 @@ D1Muon muon_settings(double a, double b, double c, double eps, int64_t steps, in
     return h;
 }
 
-void muon_launch(const std::vector<D1MuonTensor> &table, const D1Muon &h, int32_t *ctl, const Tensor &on, int64_t stream) {
+Tensor muon_launch(const std::vector<D1MuonTensor> &table, const D1Muon &h, int32_t *ctl, const Maybe &work_, const Tensor &on,
+                   int64_t stream) {
     const int64_t need = d1_muon_work_bytes(table.data(), (int)table.size(), &h);
     check(need < 0 ? (int)need : 0, "d1_muon_work_bytes");
-    const Tensor work = scratch(need, on);
+    const Tensor work = work_ ? *work_ : scratch(need, on);
+    if (work.nbytes() != (size_t)need) refuse("the second part of a step takes the same matrices as its first");
     check(d1_muon_step(table.data(), (int)table.size(), &h, ctl, ptr(work), need, (void *)stream), "d1_muon_step");
+    return work;
 }
 
 // matrices [..., rows, cols] -> the same, orthogonalised, contiguous and of their types
@@ -627,15 +635,18 @@ Tensors orthogonalize(const Tensors &updates, double a, double b, double c, doub
             table.push_back(t);
         }
     }
-    if (!table.empty()) muon_launch(table, h, nullptr, updates[0], stream);
+    if (!table.empty()) muon_launch(table, h, nullptr, {}, updates[0], stream);
     return out;
 }
 
-void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momenta, const Tensor &step, const std::vector<double> &lr,
+// part 0: a whole step; 1: its norms and whether it is made, -> what part 2 needs; 2: the rest of it
+Maybe muon_step(const Tensors &params, const Tensors &grads, const Tensors &momenta, const Tensor &step, const std::vector<double> &lr,
                const std::vector<double> &scale, const std::vector<double> &weight_decay, const std::optional<std::vector<Maybe>> &copies,
-               double momentum, bool nesterov, double a, double b, double c, double eps, int64_t steps, int64_t terms, int64_t stream) {
+               double momentum, bool nesterov, double a, double b, double c, double eps, int64_t steps, int64_t terms, int64_t part,
+               const Maybe &work_, int64_t stream) {
     no_trace("muon_step");
-    const D1Muon h = muon_settings(a, b, c, eps, steps, terms, momentum, nesterov);
+    D1Muon h = muon_settings(a, b, c, eps, steps, terms, momentum, nesterov);
+    h.part = (int32_t)part;
     const size_t count = params.size();
     auto same = [&](size_t n, const char *name) {
         if (n != count) refuse(std::string(name) + ": " + std::to_string(n) + " for " + std::to_string(count) + " parameters");
@@ -709,13 +720,15 @@ void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momen
         if (behind != places.begin() && (behind - 1)->second > begin)
             refuse("matrix " + std::to_string(i) + ": its gradient must not overlap parameters, momenta or copies");
     }
-    muon_launch(table, h, (int32_t *)ptr(step), step, stream);
+    const Tensor work = muon_launch(table, h, (int32_t *)ptr(step), work_, step, stream);
+    written(step);
+    if (part == 1) return work;
     for (size_t i = 0; i < count; i++) {
         written(params[i]);
         written(momenta[i]);
         if (copies && (*copies)[i]) written(*(*copies)[i]);
     }
-    written(step);
+    return {};
 }
 
 }  // namespace

@@ -27,7 +27,7 @@ namespace d1o {
 
 constexpr int CHUNK = 4096, SMALL_CHUNK = 1024, MAX_TENSORS = 40, NORM_GRID = 2048, JOIN_PARTS = 1024;
 // of ctl
-constexpr int STEP = 0, SKIPPED = 1, COEF = 2, INV_BC1 = 3, INV_BC2 = 4, NORM = 5, GO = 6, BEFORE = 7;
+constexpr int STEP = 0, SKIPPED = 1, COEF = 2, INV_BC1 = 3, INV_BC2 = 4, NORM = 5, GO = CTL_GO, BEFORE = 7;
 
 struct Tensors {
     void *p[MAX_TENSORS];
@@ -143,8 +143,10 @@ __global__ __launch_bounds__(256) void k_adamw_norm(const Tensors t, int per, do
     if (threadIdx.x == 0) parts[blockIdx.x] = s[0];
 }
 
-__global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl, const double *__restrict__ parts, int nparts,
-                                                      double max_norm, double log_b1, double log_b2) {
+// other: the counts of a step that is made or skipped with this one, as it has decided by itself
+__global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl, int32_t *__restrict__ other,
+                                                      const double *__restrict__ parts, int nparts, double max_norm, double log_b1,
+                                                      double log_b2) {
     __shared__ double s[1024];
     double coef = 1.0;
     bool go = true;
@@ -163,6 +165,12 @@ __global__ __launch_bounds__(1024) void k_adamw_begin(int32_t *__restrict__ ctl,
     }
     if (threadIdx.x) return;
     if (!parts && max_norm > 0.0) ctl[NORM] = 0;       // a clip of no elements
+    if (other && !go && other[GO]) {
+        other[GO] = 0;
+        other[STEP]--;
+        other[SKIPPED]++;
+    }
+    if (other) go = other[GO];
     ctl[GO] = go;
     if (!go) {
         ctl[SKIPPED]++;
@@ -464,17 +472,17 @@ extern "C" int64_t d1_adamw_work_bytes(const D1AdamWTensor *t, int count, const 
     return parts * (int64_t)sizeof(double);
 }
 
-extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, void *work, int64_t work_bytes,
-                             void *stream) {
+extern "C" int d1_adamw_step_with(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, int32_t *other, void *work,
+                                  int64_t work_bytes, void *stream) {
     const int64_t need = d1_adamw_work_bytes(t, count, h);
-    if (need < 0 || !ctl || (need && (!work || work_bytes < need || ((uintptr_t)work & 7)))) return D1_E_ARG;
+    if (need < 0 || !ctl || ctl == other || ((uintptr_t)other & 3) || (need && (!work || work_bytes < need || ((uintptr_t)work & 7)))) return D1_E_ARG;
     hipStream_t s = (hipStream_t)stream;
     const double log_b1 = h->beta1 > 0 ? log(h->beta1) : -INFINITY, log_b2 = h->beta2 > 0 ? log(h->beta2) : -INFINITY;
     const int chunk = chunk_of(t, count);
     Tensors l;
     double *parts = h->max_norm > 0 ? (double *)work : nullptr;
     int nparts = 0, e;
-    const bool join = parts && need <= JOIN_PARTS * (int64_t)sizeof(double) && need;
+    const bool join = parts && need <= JOIN_PARTS * (int64_t)sizeof(double) && need && !other;
     if (parts)
         for (int at = 0; at < count;) {
             at = take(t, count, chunk, at, l);
@@ -484,7 +492,7 @@ extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h
             nparts += norm_blocks(l);
         }
     if (!join) {
-        k_adamw_begin<<<1, parts ? 1024 : 64, 0, s>>>(ctl, nparts ? parts : nullptr, nparts, h->max_norm, log_b1, log_b2);
+        k_adamw_begin<<<1, parts ? 1024 : 64, 0, s>>>(ctl, other, nparts ? parts : nullptr, nparts, h->max_norm, log_b1, log_b2);
         if ((e = (int)hipGetLastError())) return e;
     }
     Join j{join ? parts : nullptr, nparts, 1, h->max_norm};
@@ -506,6 +514,11 @@ extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h
         j.first = 0;
     }
     return 0;
+}
+
+extern "C" int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, void *work, int64_t work_bytes,
+                             void *stream) {
+    return d1_adamw_step_with(t, count, h, ctl, nullptr, work, work_bytes, stream);
 }
 
 extern "C" int d1_adamw_read(const uint8_t *code, const uint8_t *exp, int64_t n, int is_signed, float *out, void *stream) {

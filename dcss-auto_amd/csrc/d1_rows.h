@@ -120,6 +120,9 @@ __device__ __forceinline__ float lanes_max(float x) {
     return lanes_f<LANES>(x, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// the word of a step's counts that says whether it is made, of AdamW's and of the orthogonalised updates' alike
+constexpr int CTL_GO = 6;
+
 inline bool is_type(int t) { return t == D1_FP32 || t == D1_BF16 || t == D1_FP16; }
 
 }  // namespace d1o

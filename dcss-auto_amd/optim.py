@@ -36,7 +36,7 @@ def _each(value, count):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-               max_grad_norm=0.0, copies=None, exps=None, counters=None, seed=0, lags=None):
+               max_grad_norm=0.0, copies=None, exps=None, counters=None, seed=0, lags=None, other=None):
     """One AdamW step in place over lists of tensors.
 
     params: fp32 or bf16, contiguous. grads: fp32 or bf16 of the same sizes. exp_avg, exp_avg_sq:
@@ -47,7 +47,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     counts the steps made, [1] those skipped. copies: bf16 tensors that get the new fp32 parameters
     (None in the list: no copy). What the call changes gets a new version, as from torch's operations in
     place; the replay of a captured call cannot give it one. lr and weight_decay: one value or one for each tensor. lags: steps
-    that each tensor has missed.
+    that each tensor has missed. other: the `step` of another step that has decided whether it is made and
+    waits for this one (Muon.begin): both are made, or neither.
 
     With max_grad_norm > 0 the gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with
     the norm over all of them, and a step whose norm is not finite changes nothing and is counted.
@@ -56,7 +57,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     count = len(params)
     m_exps, v_exps = exps if exps is not None else (None, None)
     call('adamw_step', step, params, grads, exp_avg, exp_avg_sq, step, _each(lr, count), _each(weight_decay, count), betas[0],
-         betas[1], eps, max_grad_norm, copies, m_exps, v_exps, counters, lags, seed & 0xFFFFFFFFFFFFFFFF)
+         betas[1], eps, max_grad_norm, copies, m_exps, v_exps, counters, lags, seed & 0xFFFFFFFFFFFFFFFF, other)
 
 
 def read_moment(code, exp, signed, out=None):
@@ -131,6 +132,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._step(None)
+        return loss
+
+    def _step(self, other):
         params, states, lr, decay = [], [], [], []
         for group in self.param_groups:
             for p in group['params']:
@@ -143,7 +148,7 @@ class AdamW(torch.optim.Optimizer):
                     self._not_captured()
                     self.state[p]['left'] = self.ctl[:1].clone()
         if not params:
-            return loss
+            return
         if self.ctl is None:
             self.ctl = torch.zeros(8, dtype=torch.int32, device=params[0].device)
         eight = self.state_bits == 8
@@ -153,8 +158,7 @@ class AdamW(torch.optim.Optimizer):
                    copies=[self.copies.get(p) for p in params] if self.copies else None,
                    exps=(column('exp_avg_exp'), column('exp_avg_sq_exp')) if eight else None,
                    counters=column('counter') if eight else None, seed=self.seed,
-                   lags=column('lag'))
-        return loss
+                   lags=column('lag'), other=other)
 
     def skipped_steps(self):
         """Steps left out because the gradients' norm was not finite (waits for the device)."""
@@ -249,11 +253,17 @@ def muon_step(params, grads, momenta, step, lr=0.02, momentum=0.95, nesterov=Tru
     [1] those skipped: a step with a matrix whose u has no finite norm changes nothing else. scales: one for each matrix
     (None: muon_scale of its shape). copies: bf16 tensors that get the new fp32 parameters (None in the list: no copy).
     lr and weight_decay: one value or one for each matrix. product_bits: as in orthogonalize, None by the parameters' types and sides."""
+    _muon(params, grads, momenta, step, lr, momentum, nesterov, weight_decay, steps, coefficients, eps, scales, copies, product_bits)
+
+
+def _muon(params, grads, momenta, step, lr, momentum, nesterov, weight_decay, steps, coefficients, eps, scales, copies, product_bits,
+          part=0, work=None):
+    """part 0: muon_step; 1: its norms and whether it is made -> the `work` of part 2, which is the rest."""
     count = len(params)
     a, b, c = coefficients
     scales = [muon_scale(p.shape) for p in params] if scales is None else scales
-    call('muon_step', step, params, grads, momenta, step, _each(lr, count), scales, _each(weight_decay, count), copies,
-         momentum, nesterov, a, b, c, eps, steps, _terms(product_bits))
+    return call('muon_step', step, params, grads, momenta, step, _each(lr, count), scales, _each(weight_decay, count), copies,
+                momentum, nesterov, a, b, c, eps, steps, _terms(product_bits), part, work)
 
 
 class Muon(torch.optim.Optimizer):
@@ -297,6 +307,24 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        given = self._given()
+        if given is not None:
+            _muon(**given)
+        return loss
+
+    def begin(self):
+        """The first part of a step that another one takes part in: the norms, and whether it is made, on the device (ctl). -> what
+        `finish` takes after the other (adamw_step's `other`) has had its say; None where no parameter has a gradient."""
+        with torch.no_grad():
+            given = self._given()
+            return None if given is None else (given, _muon(**given, part=1))
+
+    @staticmethod
+    def finish(begun):
+        with torch.no_grad():
+            _muon(**begun[0], part=2, work=begun[1])
+
+    def _given(self):
         params, lr, decay = [], [], []
         for group in self.param_groups:
             for p in group['params']:
@@ -309,13 +337,12 @@ class Muon(torch.optim.Optimizer):
                 lr.append(group['lr'])
                 decay.append(group['weight_decay'])
         if not params:
-            return loss
+            return None
         if self.ctl is None:
             self.ctl = torch.zeros(8, dtype=torch.int32, device=params[0].device)
-        muon_step(params, [p.grad for p in params], [self.state[p]['momentum'] for p in params], self.ctl, lr=lr, weight_decay=decay,
-                  scales=[muon_scale(p.shape, self.rms) for p in params],
-                  copies=[self.copies.get(p) for p in params] if self.copies else None, **self.settings)
-        return loss
+        return dict(params=params, grads=[p.grad for p in params], momenta=[self.state[p]['momentum'] for p in params], step=self.ctl,
+                    lr=lr, weight_decay=decay, scales=[muon_scale(p.shape, self.rms) for p in params],
+                    copies=[self.copies.get(p) for p in params] if self.copies else None, **self.settings)
 
     def skipped_steps(self):
         """Steps left out because an update's norm was not finite (waits for the device)."""
@@ -343,7 +370,9 @@ class Muon(torch.optim.Optimizer):
 class MuonAdamW:
     """Muon for the matrices of a model's trunk and AdamW for the rest, stepped together. `named`: the model's
     named_parameters(); those of two dimensions or more are Muon's, but for heads and embeddings (a name with 'head' or
-    'embed'). muon, adamw: further arguments of each. Each skips a step by the norms of its own gradients."""
+    'embed'). muon, adamw: further arguments of each. A step with a trunk's matrix whose update has no finite norm, or (with
+    adamw's max_grad_norm, which clips by the norm of its own gradients alone: a trunk's step has its size whatever the gradient's) with
+    other gradients without one, changes nothing at all."""
 
     def __init__(self, named, muon=None, adamw=None):
         named = list(named)
@@ -362,12 +391,19 @@ class MuonAdamW:
         for o in self.both:
             o.zero_grad(set_to_none=set_to_none)
 
+    @torch.no_grad()
     def step(self):
-        for o in self.both:
-            o.step()
+        for group in self.adamw.param_groups if self.adamw is not None else ():
+            _check_group(group)
+        begun = None if self.muon is None else self.muon.begin()
+        if self.adamw is not None:
+            self.adamw._step(None if begun is None else self.muon.ctl)
+        if begun is not None:
+            self.muon.finish(begun)
 
     def skipped_steps(self):
-        return sum(o.skipped_steps() for o in self.both)
+        """Steps left out because a norm was not finite (waits for the device)."""
+        return max(o.skipped_steps() for o in self.both)
 
     def state_dict(self):
         return dict(muon=self.muon and self.muon.state_dict(), adamw=self.adamw and self.adamw.state_dict())

@@ -89,7 +89,7 @@ class ModulePPO(PPO):
     NormPolicy and ARPolicy: the module's layers by autograd, its log probabilities, layer norms, the loss and the
     update itself by this package's kernels. Interface and loss are PPO's; the optimizer is AdamW over all
     tensors at once (state_bits: 32 or 8) with the gradient clip in the same call, or with optimizer='muon' Muon (lr muon_lr) for
-    the trunk's matrices and AdamW for the rest (MuonAdamW). clip may be a pair (low, high), value_clip holds the new value
+    the trunk's matrices and AdamW for the rest (MuonAdamW; the clip is then by the norm of the rest's gradients). clip may be a pair (low, high), value_clip holds the new value
     within that much of the old one; with `reference`, a policy that is left as it is, kl_coef times the KL to
     it is added to the loss. `terms`: the last minibatch's loss in its parts (losses.PolicyLoss). Nothing waits
     for the device between minibatches: a minibatch whose gradient norm is not finite changes nothing,

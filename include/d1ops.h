@@ -121,6 +121,11 @@ typedef struct D1AdamW {
 int64_t d1_adamw_work_bytes(const D1AdamWTensor *t, int count, const D1AdamW *h);
 int d1_adamw_step(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, void *work, int64_t work_bytes,
                   void *stream);
+/* The same, made or skipped together with another step that has decided but changed nothing yet: `other` is the ctl of a
+ * d1_muon_step with part 1 before this call on the stream. Where that one is skipped so is this; where this one's norm is not finite
+ * (max_norm > 0) that one's decision is taken back, and its part 2 changes nothing. */
+int d1_adamw_step_with(const D1AdamWTensor *t, int count, const D1AdamW *h, int32_t *ctl, int32_t *other, void *work,
+                       int64_t work_bytes, void *stream);
 /* out[i] (fp32) = the value that an 8-bit moment's code stands for; is_signed 1 for m, 0 for v. */
 int d1_adamw_read(const uint8_t *code, const uint8_t *exp, int64_t n, int is_signed, float *out, void *stream);
 
@@ -205,7 +210,7 @@ typedef struct D1Muon {
     int32_t steps, nesterov;
     int32_t terms;            /* operands of the products: 1: fp16, 3: two fp16 halves (22 bits), 0: 3 for fp32 results
                                  and matrices with a side under 16, 1 for others */
-    int32_t pad;
+    int32_t part;             /* 0: the whole step; 1: its norms and whether it is made, in ctl; 2: the rest of it */
 } D1Muon;
 
 /* 0 where the coefficients can be used: `steps` times the quintic, from singular values in [0, 1], stays under 3.8 and its
@@ -214,7 +219,8 @@ int d1_muon_check(const D1Muon *h);
 /* O(U): X = U / (|U|_F + eps), then `steps` times X = a X + (b A + c A A) X with A = X X^T (on the smaller side).
  * Of a step: m = momentum m + g;  U = nesterov ? g + momentum m : m;  p = p (1 - lr weight_decay) - lr scale O(U).
  * ctl as in d1_adamw_step, [0] steps made, [1] steps skipped, or null: with it a step with a U whose norm is not finite
- * changes nothing but ctl[1]. `t` and `h` are host arrays, read before the call returns. Matrices with no elements are left
+ * changes nothing but ctl[1]. Parts 1 and 2 need ctl, and part 2 the `work` that part 1 left, with the same arguments otherwise and
+ * nothing that they name changed between. `t` and `h` are host arrays, read before the call returns. Matrices with no elements are left
  * out. Results must not overlap each other or gradients. The same inputs give the same bits. */
 int64_t d1_muon_work_bytes(const D1MuonTensor *t, int count, const D1Muon *h);
 int d1_muon_step(const D1MuonTensor *t, int count, const D1Muon *h, int32_t *ctl, void *work, int64_t work_bytes, void *stream);
