@@ -367,12 +367,13 @@ class Muon(torch.optim.Optimizer):
         self.ctl = None if own['ctl'] is None else own['ctl'].to(device, copy=True)
 
 
-class MuonAdamW:
+class MuonAdamW(torch.optim.Optimizer):
     """Muon for the matrices of a model's trunk and AdamW for the rest, stepped together. `named`: the model's
     named_parameters(); those of two dimensions or more are Muon's, but for heads and embeddings (a name with 'head' or
     'embed'). muon, adamw: further arguments of each. A step with a trunk's matrix whose update has no finite norm, or (with
     adamw's max_grad_norm, which clips by the norm of its own gradients alone: a trunk's step has its size whatever the gradient's) with
-    other gradients without one, changes nothing at all."""
+    other gradients without one, changes nothing at all. Its groups and states are those of the two, to which (`muon`, `adamw`)
+    further groups are added."""
 
     def __init__(self, named, muon=None, adamw=None):
         named = list(named)
@@ -382,24 +383,50 @@ class MuonAdamW:
         self.muon = Muon(trunk, **(muon or {})) if trunk else None
         self.adamw = AdamW(rest, **(adamw or {})) if rest else None
         self.both = [o for o in (self.muon, self.adamw) if o is not None]
+        super().__init__(self.param_groups, {})
 
+    # the base class's own lists stay unused
     @property
     def param_groups(self):
         return [g for o in self.both for g in o.param_groups]
+
+    @param_groups.setter
+    def param_groups(self, groups):
+        pass
+
+    @property
+    def state(self):
+        return {p: s for o in self.both for p, s in o.state.items()}
+
+    @state.setter
+    def state(self, state):
+        pass
+
+    def add_param_group(self, param_group):
+        if not any(param_group is g for g in self.param_groups):
+            raise ValueError('a group is added to .muon or to .adamw')
+
+    def __getstate__(self):
+        return dict(muon=self.muon, adamw=self.adamw, both=self.both, defaults=self.defaults)
 
     def zero_grad(self, set_to_none=True):
         for o in self.both:
             o.zero_grad(set_to_none=set_to_none)
 
     @torch.no_grad()
-    def step(self):
+    def step(self, closure=None):
         for group in self.adamw.param_groups if self.adamw is not None else ():
             _check_group(group)
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         begun = None if self.muon is None else self.muon.begin()
         if self.adamw is not None:
             self.adamw._step(None if begun is None else self.muon.ctl)
         if begun is not None:
             self.muon.finish(begun)
+        return loss
 
     def skipped_steps(self):
         """Steps left out because a norm was not finite (waits for the device)."""
