@@ -27,7 +27,7 @@ FP32 = 8                                 # of _call's grads: gradients in fp32
 
 
 def _pair(clip):
-    return (clip, clip) if isinstance(clip, (int, float)) else clip
+    return clip if isinstance(clip, (tuple, list)) else (clip, clip)
 
 
 def _call(grads, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef, value_coef,

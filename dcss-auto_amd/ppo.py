@@ -11,10 +11,11 @@ autocast while the optimizer keeps fp32 master weights; GAE is the HIP kernel.
 import torch
 
 from . import policy as P
-from .losses import policy_loss
+from .losses import PolicyLoss, policy_loss
 from .optim import AdamW, MuonAdamW
 
 OBS = P.OBS
+KERNEL_TYPES = (torch.float32, torch.bfloat16, torch.float16)        # of losses.policy_loss
 
 
 class RolloutBuffer:
@@ -40,6 +41,29 @@ def ppo_loss(logits, values, actions, old_logp, adv, returns, clip=0.2, vcoef=0.
     vloss = 0.5 * (values.float() - returns).square().mean()
     entropy = -(logp_all.exp() * logp_all).sum(-1).mean()
     return pg + vcoef * vloss - ecoef * entropy, pg.detach(), vloss.detach(), entropy.detach()
+
+
+def broadcast_loss(logp, old_logp, adv, ref_logp, entropy, values, returns, old_values, clip, kl_coef, value_coef, value_clip,
+                   entropy_coef):
+    """losses.policy_loss in elementary operations, for results that are not all of logp's shape and of a type the kernel takes:
+    each term is the mean over what broadcasting makes of it. clip: (low, high)."""
+    gap = logp - old_logp
+    ratio = torch.exp(gap)
+    free, held = ratio * adv, ratio.clamp(1 - clip[0], 1 + clip[1]) * adv
+    policy = -torch.minimum(free, held).mean()
+    far = (values.float() - returns).square()
+    if value_clip:
+        near = old_values + (values.float() - old_values).clamp(-value_clip, value_clip)
+        far = torch.maximum(far, (near - returns).square())
+    value, entropy = 0.5 * far.mean(), entropy.mean()
+    loss, kl = policy + value_coef * value - entropy_coef * entropy, policy.new_zeros(())
+    if ref_logp is not None:
+        x = ref_logp - logp
+        kl = (x.exp() - 1 - x).mean()
+        loss = loss + kl_coef * kl
+    parts = loss, policy, value, entropy, kl, (held < free).float().mean(), (ratio - 1 - gap).mean(), torch.full_like(loss, gap.numel())
+    terms = torch.stack([t.detach().float() for t in parts])
+    return PolicyLoss(loss, *terms.unbind()[1:], terms)
 
 
 class PPO:
@@ -89,7 +113,9 @@ class ModulePPO(PPO):
     NormPolicy and ARPolicy: the module's layers by autograd, its log probabilities, layer norms, the loss and the
     update itself by this package's kernels. Interface and loss are PPO's; the optimizer is AdamW over all
     tensors at once (state_bits: 32 or 8) with the gradient clip in the same call, or with optimizer='muon' Muon (lr muon_lr) for
-    the trunk's matrices and AdamW for the rest (MuonAdamW; the clip is then by the norm of the rest's gradients). clip may be a pair (low, high), value_clip holds the new value
+    the trunk's matrices and AdamW for the rest (MuonAdamW; the clip is then by the norm of the rest's gradients). What `evaluate` gives need
+    not have the same shapes and types: with others than the loss's kernel takes (an entropy that is one number, a value that broadcasts, 64
+    bits) the loss is elementary operations. clip may be a pair (low, high), value_clip holds the new value
     within that much of the old one; with `reference`, a policy that is left as it is, kl_coef times the KL to
     it is added to the loss. `terms`: the last minibatch's loss in its parts (losses.PolicyLoss). Nothing waits
     for the device between minibatches: a minibatch whose gradient norm is not finite changes nothing,
@@ -122,8 +148,12 @@ class ModulePPO(PPO):
 
     def _learn(self, evaluated, ref_logp, old_logp, adv, ret, old_values):
         logp, entropy, value = evaluated
-        r = policy_loss(logp, old_logp, adv, ref_logp=ref_logp, entropy=entropy, values=value, returns=ret, old_values=old_values,
-                        clip=self.clip, kl_coef=self.kl_coef, value_coef=self.vcoef, value_clip=self.value_clip, entropy_coef=self.ecoef)
+        low, high = self.clip if isinstance(self.clip, (tuple, list)) else (self.clip, self.clip)
+        settings = dict(clip=(min(low, 1.0), high), kl_coef=self.kl_coef, value_coef=self.vcoef, value_clip=self.value_clip,
+                        entropy_coef=self.ecoef)                      # a ratio is never under 0
+        alike = [t for t in (logp, entropy, value, ref_logp) if t is not None]
+        loss = policy_loss if all(t.shape == old_logp.shape and t.dtype in KERNEL_TYPES for t in alike) else broadcast_loss
+        r = loss(logp, old_logp, adv, ref_logp=ref_logp, entropy=entropy, values=value, returns=ret, old_values=old_values, **settings)
         self.opt.zero_grad(set_to_none=True)
         r.loss.backward()
         self.opt.step()
