@@ -390,7 +390,8 @@ __global__ __launch_bounds__(256) void k_loss_finish(const Loss a, const double 
 
 // Gradients made for a loss gradient of 1, scaled by the real one. They are kept in fp32 until then (`type` then is D1_FP32) and rounded
 // to their own type here: a weight of 1 / tokens leaves fp16 few bits, or none, which a factor behind the rounding does not bring back (at
-// 2^20 tokens, scaled by 65,536, 1.8% off; 0.02% so).
+// 2^20 tokens, scaled by 65,536, 1.8% off; 0.02% so). It reads and writes every gradient once more: 128 x 65,536 fp32 tokens with
+// every term take 138 us forward and backward through autograd, 99 in the one pass that gives the gradients themselves.
 __global__ __launch_bounds__(256) void k_loss_scale(const void *p, int type, void *out, int out_type, int64_t n, const float *__restrict__ by) {
     const float f = *by;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {

@@ -66,12 +66,13 @@ def policy_loss(logp, old_logp, advantages, ref_logp=None, entropy=None, values=
     old_logp: under the policy that took the tokens. advantages: [..., length], or [...]: one a sequence. clip: the ratio
     exp(logp - old_logp) is held in [1 - clip, 1 + clip], or (low, high) for [1 - low, 1 + high]. ref_logp: under a reference
     policy, for the kl term exp(x) - x - 1 with x = ref_logp - logp. entropy: of each distribution. values and returns:
-    half the squared error, with value_clip the larger of it and that of the value held within value_clip of old_values.
+    half the squared error, with value_clip (None or 0: none) the larger of it and that of the value held within value_clip of old_values.
     mask (bool or uint8): only tokens that are true count, whatever the others hold. level: 'token' weighs all tokens
     alike, 'sequence' the sequences that have one, over their own tokens. All are fp32, bf16 or fp16, each of its own
     type, with any strides; everything is computed in fp32 and summed in fp64. Gradients are kept in fp32 (4 bytes a token
     each) until the backward pass, which multiplies them by the loss's gradient and then rounds them to their input's type, once: a
-    launch each that reads and writes them. Without a token that counts all terms and gradients are 0."""
+    launch each that reads and writes them (policy_loss_grads has no such pass). Without a token that counts all terms and
+    gradients are 0."""
     settings = (clip, kl_coef, value_coef, value_clip, entropy_coef, level)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logp, entropy, values)):
         loss, terms = _PolicyLoss.apply(logp, entropy, values, old_logp, advantages, ref_logp, returns, old_values, mask, settings)

@@ -44,7 +44,8 @@ def gated_scan(x, gate, state=None, reset=None):
     sequences as their transpose(0, 1)). state: fp32 [rows, width] (or [width]), h before the first step (None: zeros).
     reset: bool or uint8 [steps, rows] (or [steps]); where it is true the step starts from zero, whatever was before: an
     episode that begins, or the next of several sequences in a row. h has x's type, last is the fp32 state after the last
-    step. A single step is x[None]. States are fp32 throughout."""
+    step. A single step is x[None]. States are fp32 throughout. A state that is not finite stays so until a reset (an infinite one
+    may become NaN, where the factors of many steps together are under fp32's range)."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
         return _GatedScan.apply(x, gate, state, reset)
     return call('scan_fwd', x, x, gate, state, reset, False)[:2]
