@@ -26,15 +26,20 @@ class PolicyLoss(NamedTuple):
 FP32 = 8                                 # of _call's grads: gradients in fp32
 
 
-def _pair(clip):
-    return clip if isinstance(clip, (tuple, list)) else (clip, clip)
+def clip_pair(clip):
+    """(low, high) of a pair, or of one number for both."""
+    try:
+        low, high = clip
+    except TypeError:
+        low = high = clip
+    return float(low), float(high)
 
 
 def _call(grads, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, clip, kl_coef, value_coef,
           value_clip, entropy_coef, level):
     if level not in ('token', 'sequence'):
         raise ValueError(f"level is 'token' or 'sequence', not {level!r}")
-    low, high = _pair(clip)
+    low, high = clip_pair(clip)
     return call('policy_loss', logp, logp, old_logp, advantages, ref_logp, entropy, values, returns, old_values, mask, low, high,
                 kl_coef, value_coef, value_clip or 0.0, entropy_coef, level == 'sequence', grads)
 

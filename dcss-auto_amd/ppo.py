@@ -11,7 +11,7 @@ autocast while the optimizer keeps fp32 master weights; GAE is the HIP kernel.
 import torch
 
 from . import policy as P
-from .losses import PolicyLoss, policy_loss
+from .losses import PolicyLoss, clip_pair, policy_loss
 from .optim import AdamW, MuonAdamW
 
 OBS = P.OBS
@@ -148,7 +148,7 @@ class ModulePPO(PPO):
 
     def _learn(self, evaluated, ref_logp, old_logp, adv, ret, old_values):
         logp, entropy, value = evaluated
-        low, high = self.clip if isinstance(self.clip, (tuple, list)) else (self.clip, self.clip)
+        low, high = clip_pair(self.clip)
         settings = dict(clip=(min(low, 1.0), high), kl_coef=self.kl_coef, value_coef=self.vcoef, value_clip=self.value_clip,
                         entropy_coef=self.ecoef)                      # a ratio is never under 0
         alike = [t for t in (logp, entropy, value, ref_logp) if t is not None]
