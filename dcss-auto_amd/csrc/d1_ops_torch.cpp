@@ -260,8 +260,8 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
     if (step.scalar_type() != at::kInt || step.dim() != 1 || step.size(0) != 8 || !step.is_cuda() || !step.is_contiguous())
         refuse("step must be a contiguous int32 CUDA tensor of 8 elements");
     if (other && (other->scalar_type() != at::kInt || other->dim() != 1 || other->size(0) != 8 || !other->is_contiguous() ||
-                  other->device() != step.device()))
-        refuse("the other step's counts must be a contiguous int32 tensor of 8 elements on " + step.device().str());
+                  other->device() != step.device() || ptr(*other) == ptr(step)))
+        refuse("the other step's counts must be a contiguous int32 tensor of 8 elements on " + step.device().str() + ", not this one's");
     const at::ScalarType moment = eight ? at::kByte : at::kFloat;
     std::vector<D1AdamWTensor> table(count);
     Tensors held;            // contiguous gradients, until the launches that read them are queued
